@@ -88,6 +88,16 @@ SIGNATURES = {
     "ff_attention_full": [P, P, P, P, I64, I64, I64, I64, F32, P],
     "ff_pos_interp": [P, P, P, P, I64, I64, I64, I64, P],
     "ff_vision_qkv": [P, P, P, P, P, P, I64, I64, I64, I64, P],
+    "ff_quant_weight_fp8_block": [P, P, P, I64, I64, P],
+    "ff_pack_weight_fp8_block": [P, P, I64, I64, I64, I64, P],
+    "ff_unpack_weight_fp8_block": [P, P, I64, I64, I64, I64, P],
+    "ff_quant_rows_fp8_block": [P, I64, P, P, I64, I64, P],
+    "ff_gemm_fp8_block": [P, P, P, P, P, I64, I64, I64, I64, P],
+    "ff_linear_fp8_block_workspace": [I64, I64, I64, PI64],
+    "ff_linear_fp8_block": [P, I64, P, P, P, I64, I64, I64, I64, P, I64, P],
+    "ff_moe_route": [P, I32, I64, P, P, P, I64, I64, I64, I32, I64, I64, I32, F32, P],
+    "ff_moe_experts_workspace": [I64, I64, I64, I64, I64, PI64],
+    "ff_moe_experts": [P, I64, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, P, I64, P],
 }
 
 _lib = None

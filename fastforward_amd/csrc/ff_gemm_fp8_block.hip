@@ -1,0 +1,360 @@
+// Block-scaled FP8 linear for gfx950: setup (weight quantisation, packing), the
+// row quantiser and the products y = x . W^T (ff_block.h states the format).
+//
+// skinny_kernel: few rows. A workgroup of 8 waves owns 16 RI rows x 16 NJ weight
+// rows; its waves take the k steps in turn (wave w: steps w, w + 8, ..), so that
+// even 4096 columns make 256 workgroups that read the weights from every channel
+// of memory, and their sums are added through LDS in wave order.
+#include "ff_block.h"
+
+using namespace ff;
+
+namespace {
+
+constexpr int kSkinnyThreads = 512, kSkinnyWaves = kSkinnyThreads / 64;
+constexpr int kRowsMax = 4;             // rows that the product's own launch quantises
+constexpr int kRowsMaxCodes = 49152;    // their codes' LDS
+
+// ---------------------------------------------------------------- setup
+
+// One workgroup per 128 x 128 block: its largest magnitude, then its codes.
+__global__ __launch_bounds__(256) void quant_weight_block_kernel(const bf16_t* __restrict__ w, uint8_t* __restrict__ q,
+                                                                 float* __restrict__ scales, int64_t n, int64_t k,
+                                                                 int kb) {
+  __shared__ float red[4];
+  const int64_t r0 = (int64_t)(blockIdx.x / kb) * kBlock, c0 = (int64_t)(blockIdx.x % kb) * kBlock;
+  const int rows = (int)min((int64_t)kBlock, n - r0), cols = (int)min((int64_t)kBlock, k - c0);
+  w += r0 * k + c0;
+  float m = 0.f;
+  for (int i = threadIdx.x; i < rows * kBlock; i += 256) {
+    const int r = i / kBlock, c = i % kBlock;
+    if (c < cols) m = fmaxf(m, fabsf(bf16_to_f32(w[r * k + c])));
+  }
+  m = block_max<4>(m, red);
+  const float scale = fmaxf(m, 1e-12f) / 448.0f;
+  q += r0 * k + c0;
+  for (int i = threadIdx.x; i < rows * kBlock; i += 256) {
+    const int r = i / kBlock, c = i % kBlock;
+    if (c < cols) q[r * k + c] = (uint8_t)f32_to_e4m3(clamp448(bf16_to_f32(w[r * k + c]) / scale));
+  }
+  if (threadIdx.x == 0) scales[blockIdx.x] = scale;
+}
+
+// One thread per 16 packed bytes.
+__global__ __launch_bounds__(256) void pack_block_kernel(const uint8_t* __restrict__ w, uint8_t* __restrict__ p,
+                                                         int64_t batch, int64_t n, int64_t k, int64_t nf, int64_t kt_n,
+                                                         int aligned) {
+  const int64_t total = batch * nf * kt_n * 128;
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int l = (int)(i & 63), half = (int)(i >> 6) & 1;
+    const int64_t f = (i >> 7) % nf, kt = (i >> 7) / nf % kt_n, b = (i >> 7) / nf / kt_n;
+    const int64_t row = 16 * f + (l & 15), c = 128 * kt + 32 * (l >> 4) + 16 * half;
+    u32x4 v = {0, 0, 0, 0};
+    if (row < n) {
+      const uint8_t* src = w + (b * n + row) * k + c;
+      if (aligned && c + 16 <= k) {
+        v = *reinterpret_cast<const u32x4*>(src);
+      } else {
+        uint32_t d[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (c + e < k) d[e / 4] |= (uint32_t)src[e] << (8 * (e % 4));
+        v = u32x4{d[0], d[1], d[2], d[3]};
+      }
+    }
+    *reinterpret_cast<u32x4*>(p + 16 * i) = v;
+  }
+}
+
+__global__ __launch_bounds__(256) void unpack_block_kernel(const uint8_t* __restrict__ p, uint8_t* __restrict__ w,
+                                                           int64_t batch, int64_t n, int64_t k, int64_t nf,
+                                                           int64_t kt_n) {
+  const int64_t total = batch * n * k;
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t c = i % k, row = i / k % n, b = i / k / n;
+    const int64_t kt = c / 128, f = row / 16;
+    const int in = (int)(c % 128), l = (in / 32) * 16 + (int)(row % 16);
+    w[i] = p[((b * kt_n + kt) * nf + f) * 2048 + (in / 16 % 2) * 1024 + 16 * l + in % 16];
+  }
+}
+
+// ---------------------------------------------------------------- row quantiser
+
+// 16 lanes per (row, 128 channels): codes q (rows, 128 kt_n) and scales (kt_n,
+// rows), channel blocks slowest, so that the lanes of a product's row tile read
+// neighbouring scales.
+__global__ __launch_bounds__(256) void quant_rows_block_kernel(const bf16_t* __restrict__ x, int64_t ldx,
+                                                               uint8_t* __restrict__ q, float* __restrict__ scales,
+                                                               int64_t rows, int64_t k, int kt_n, int vec) {
+  const int s = threadIdx.x & 15;
+  for (int64_t i = (blockIdx.x * (int64_t)256 + threadIdx.x) >> 4; i < rows * kt_n; i += (int64_t)gridDim.x * 16) {
+    const int64_t row = i / kt_n;
+    const int kt = (int)(i % kt_n);
+    float scale;
+    const u32x2 c = quant_group16(x + row * ldx, k, kt, s, vec, &scale);
+    *reinterpret_cast<u32x2*>(q + i * kBlock + 8 * s) = c;
+    if (s == 0) scales[(int64_t)kt * rows + row] = scale;
+  }
+}
+
+// ---------------------------------------------------------------- few rows
+
+// INLINE: the workgroup quantises the rows (at most kRowsMax) into LDS itself.
+template <int RI, int NJ, bool INLINE>
+__global__ __launch_bounds__(kSkinnyThreads) void skinny_kernel(
+    const bf16_t* __restrict__ x, int64_t ldx, int vec, const uint8_t* __restrict__ q, const float* __restrict__ qs,
+    const uint8_t* __restrict__ wp, const float* __restrict__ ws, bf16_t* __restrict__ y, int64_t ldy, int64_t m,
+    int64_t n, int64_t k, int kt_n, int nf) {
+  constexpr int PF = 4;  // k steps whose loads a wave has in flight
+  constexpr int kSums = kSkinnyWaves * RI * NJ * 256;  // floats of the waves' sums
+  constexpr int kLds = INLINE ? kRowsMaxCodes + 16 * kRowsMaxCodes / kBlock : kSums * 4;
+  static_assert(!INLINE || kSums * 4 <= kLds, "the sums reuse the codes' LDS");
+  __shared__ __align__(16) uint8_t smem[kLds];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r16 = lane & 15, g = lane >> 4;
+  const int f0 = blockIdx.x * NJ;
+  const int64_t m0 = (int64_t)blockIdx.y * 16 * RI;
+  const int mine = (kt_n - wave + kSkinnyWaves - 1) / kSkinnyWaves;  // this wave's k steps
+
+  i32x8 wq[PF][NJ], xq[PF][RI];
+  float xs[PF][RI], wsc[PF][NJ];
+  const uint8_t* frag[NJ];
+  const float* wscale[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    const int f = min(f0 + j, nf - 1);
+    frag[j] = wp + (int64_t)f * 2048;
+    wscale[j] = ws + (int64_t)(f / 8) * kt_n;
+  }
+  int64_t row[RI];
+#pragma unroll
+  for (int i = 0; i < RI; ++i) row[i] = min(m0 + 16 * i + r16, m - 1);
+  auto loadW = [&](int u, int kt) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      wq[u][j] = load_frag(frag[j] + (int64_t)kt * nf * 2048, lane);
+      wsc[u][j] = wscale[j][kt];
+    }
+  };
+  auto loadX = [&](int u, int kt) {
+#pragma unroll
+    for (int i = 0; i < RI; ++i) {
+      if constexpr (INLINE) {
+        const int64_t at = row[i] * kt_n + kt;
+        const i32x4v* p = reinterpret_cast<const i32x4v*>(smem + at * kBlock + 32 * g);
+        xq[u][i] = join(p[0], p[1]);
+        xs[u][i] = reinterpret_cast<const float*>(smem + kRowsMaxCodes)[at];
+      } else {
+        const i32x4v* p = reinterpret_cast<const i32x4v*>(q + (row[i] * kt_n + kt) * kBlock + 32 * g);
+        xq[u][i] = join(p[0], p[1]);
+        xs[u][i] = qs[(int64_t)kt * m + row[i]];
+      }
+    }
+  };
+
+  f32x4 acc[RI][NJ];
+#pragma unroll
+  for (int i = 0; i < RI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  for (int b = 0; b < mine || (INLINE && b == 0); b += PF) {
+#pragma unroll
+    for (int u = 0; u < PF; ++u)
+      if (b + u < mine) loadW(u, wave + kSkinnyWaves * (b + u));
+    if constexpr (INLINE) {
+      if (b == 0) {  // the first weights are in flight meanwhile
+        for (int64_t i = threadIdx.x >> 4; i < m * kt_n; i += kSkinnyThreads / 16) {
+          float scale;
+          const u32x2 c = quant_group16(x + i / kt_n * ldx, k, (int)(i % kt_n), r16, vec, &scale);
+          *reinterpret_cast<u32x2*>(smem + i * kBlock + 8 * r16) = c;
+          if (r16 == 0) reinterpret_cast<float*>(smem + kRowsMaxCodes)[i] = scale;
+        }
+        __syncthreads();
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < PF; ++u)
+      if (b + u < mine) loadX(u, wave + kSkinnyWaves * (b + u));
+#pragma unroll
+    for (int u = 0; u < PF; ++u)
+      if (b + u < mine) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int i = 0; i < RI; ++i) fma4(acc[i][j], mfma_step(wq[u][j], xq[u][i]), xs[u][i] * wsc[u][j]);
+      }
+  }
+
+  if constexpr (INLINE) __syncthreads();  // the codes are no longer read
+  f32x4* red = reinterpret_cast<f32x4*>(smem);
+#pragma unroll
+  for (int i = 0; i < RI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) red[(wave * RI * NJ + i * NJ + j) * 64 + lane] = acc[i][j];
+  __syncthreads();
+  for (int t = threadIdx.x; t < RI * NJ * 64; t += kSkinnyThreads) {
+    f32x4 v = red[t];
+#pragma unroll
+    for (int w = 1; w < kSkinnyWaves; ++w) v += red[w * RI * NJ * 64 + t];
+    const int l = t & 63, i = t / 64 / NJ, j = t / 64 % NJ;
+    const int64_t r = m0 + 16 * i + (l & 15), c = 16 * (int64_t)(f0 + j) + 4 * (l >> 4);
+    if (r < m && c < n) store4_bf16(y + r * ldy + c, v, n - c);
+  }
+}
+
+inline bool rows_vec(const void* x, int64_t ldx) { return ff_aligned(x, 16) && ldx % 8 == 0; }
+
+// Fragments (16 weight rows) per workgroup: one where that leaves at most two workgroups per CU.
+template <int RI, bool INLINE>
+void launch_skinny(const bf16_t* x, int64_t ldx, const uint8_t* q, const float* qs, const uint8_t* wp, const float* ws,
+                   bf16_t* y, int64_t ldy, int64_t m, int64_t n, int64_t k, hipStream_t st) {
+  const int nf = (int)((n + 15) / 16), kt_n = (int)((k + kBlock - 1) / kBlock);
+  const int64_t tiles_m = (m + 16 * RI - 1) / (16 * RI);
+  const int vec = rows_vec(x, ldx);
+  if (tiles_m * nf <= 512)
+    hipLaunchKernelGGL((skinny_kernel<RI, 1, INLINE>), dim3((unsigned)nf, (unsigned)tiles_m), dim3(kSkinnyThreads), 0,
+                       st, x, ldx, vec, q, qs, wp, ws, y, ldy, m, n, k, kt_n, nf);
+  else
+    hipLaunchKernelGGL((skinny_kernel<RI, 2, INLINE>), dim3((unsigned)((nf + 1) / 2), (unsigned)tiles_m),
+                       dim3(kSkinnyThreads), 0, st, x, ldx, vec, q, qs, wp, ws, y, ldy, m, n, k, kt_n, nf);
+}
+
+constexpr int64_t kMaxCodes = 1ll << 31;
+
+}  // namespace
+
+namespace ff {
+
+int quant_rows_block(const void* x, int64_t ldx, void* q, float* scales, int64_t rows, int64_t k, hipStream_t st) {
+  const int64_t kt_n = (k + kBlock - 1) / kBlock;
+  const int64_t grid = (rows * kt_n + 15) / 16;
+  hipLaunchKernelGGL(quant_rows_block_kernel, dim3((unsigned)(grid < (1 << 20) ? grid : (1 << 20))), dim3(256), 0, st, (const bf16_t*)x, ldx,
+                     (uint8_t*)q, scales, rows, k, (int)kt_n, (int)rows_vec(x, ldx));
+  FF_LAUNCH_CHECK("quant_rows_fp8_block");
+  return FF_OK;
+}
+
+}  // namespace ff
+
+extern "C" int ff_quant_weight_fp8_block(const void* w, void* q, float* scales, int64_t n, int64_t k,
+                                         ff_stream_t stream) {
+  FF_REQUIRE(w && q && scales, "ff_quant_weight_fp8_block: null pointer");
+  FF_REQUIRE(n > 0 && k > 0 && n < kMaxCodes && k < kMaxCodes, "ff_quant_weight_fp8_block: bad sizes");
+  const int64_t kb = (k + kBlock - 1) / kBlock, nb = (n + kBlock - 1) / kBlock;
+  FF_REQUIRE(nb * kb < (1 << 24), "ff_quant_weight_fp8_block: bad sizes");
+  hipLaunchKernelGGL(quant_weight_block_kernel, dim3((unsigned)(nb * kb)), dim3(256), 0, (hipStream_t)stream,
+                     (const bf16_t*)w, (uint8_t*)q, scales, n, k, (int)kb);
+  FF_LAUNCH_CHECK("ff_quant_weight_fp8_block");
+  return FF_OK;
+}
+
+extern "C" int ff_pack_weight_fp8_block(const void* w, void* packed, int64_t batch, int64_t n, int64_t k, int64_t n_pad,
+                                        ff_stream_t stream) {
+  FF_REQUIRE(w && packed, "ff_pack_weight_fp8_block: null pointer");
+  FF_REQUIRE(batch > 0 && n > 0 && k > 0 && n_pad >= n && n_pad % 16 == 0 && n_pad < kMaxCodes && k < kMaxCodes,
+             "ff_pack_weight_fp8_block: bad sizes");
+  FF_REQUIRE(ff_aligned(packed, 16), "ff_pack_weight_fp8_block: alignment");
+  const int64_t kt_n = (k + kBlock - 1) / kBlock, nf = n_pad / 16;
+  const int64_t grid = (batch * nf * kt_n * 128 + 255) / 256;
+  hipLaunchKernelGGL(pack_block_kernel, dim3((unsigned)(grid < (1 << 20) ? grid : (1 << 20))), dim3(256), 0,
+                     (hipStream_t)stream, (const uint8_t*)w, (uint8_t*)packed, batch, n, k, nf, kt_n,
+                     (int)(ff_aligned(w, 16) && k % 16 == 0));
+  FF_LAUNCH_CHECK("ff_pack_weight_fp8_block");
+  return FF_OK;
+}
+
+extern "C" int ff_unpack_weight_fp8_block(const void* packed, void* w, int64_t batch, int64_t n, int64_t k,
+                                          int64_t n_pad, ff_stream_t stream) {
+  FF_REQUIRE(w && packed, "ff_unpack_weight_fp8_block: null pointer");
+  FF_REQUIRE(batch > 0 && n > 0 && k > 0 && n_pad >= n && n_pad % 16 == 0 && n_pad < kMaxCodes && k < kMaxCodes,
+             "ff_unpack_weight_fp8_block: bad sizes");
+  const int64_t grid = (batch * n * k + 255) / 256;
+  hipLaunchKernelGGL(unpack_block_kernel, dim3((unsigned)(grid < (1 << 20) ? grid : (1 << 20))), dim3(256), 0,
+                     (hipStream_t)stream, (const uint8_t*)packed, (uint8_t*)w, batch, n, k, n_pad / 16,
+                     (k + kBlock - 1) / kBlock);
+  FF_LAUNCH_CHECK("ff_unpack_weight_fp8_block");
+  return FF_OK;
+}
+
+extern "C" int ff_quant_rows_fp8_block(const void* x, int64_t ldx, void* q, float* scales, int64_t rows, int64_t k,
+                                       ff_stream_t stream) {
+  FF_REQUIRE(rows >= 0 && rows < kMaxCodes && k > 0 && k < kMaxCodes && ldx >= 0, "ff_quant_rows_fp8_block: bad sizes");
+  if (rows == 0) return FF_OK;
+  FF_REQUIRE(x && q && scales, "ff_quant_rows_fp8_block: null pointer");
+  FF_REQUIRE(ff_aligned(x, 2) && ff_aligned(q, 16), "ff_quant_rows_fp8_block: alignment");
+  return quant_rows_block(x, ldx, q, scales, rows, k, (hipStream_t)stream);
+}
+
+static int check_gemm(const char* who, const void* packed, const float* ws, const void* y, int64_t ldy, int64_t m,
+                      int64_t n, int64_t k) {
+  FF_REQUIRE(m >= 0 && m < kMaxCodes && n > 0 && k > 0 && n < kMaxCodes && k < kMaxCodes && ldy >= n &&
+                 ((n + 15) / 16 * 16) * ((k + kBlock - 1) / kBlock * kBlock) < kMaxCodes && m <= 65535ll * 16,
+             "%s: bad sizes m=%lld n=%lld k=%lld", who, (long long)m, (long long)n, (long long)k);
+  if (m == 0) return FF_OK;
+  FF_REQUIRE(packed && ws && y, "%s: null pointer", who);
+  FF_REQUIRE(ff_aligned(packed, 16) && ff_aligned(y, 2), "%s: alignment", who);
+  return FF_OK;
+}
+
+static int gemm_block(const void* q, const float* qs, const void* packed, const float* ws, void* y, int64_t ldy,
+                      int64_t m, int64_t n, int64_t k, hipStream_t st) {
+  auto go = [&](auto RI) {
+    launch_skinny<decltype(RI)::value, false>(nullptr, 0, (const uint8_t*)q, qs, (const uint8_t*)packed, ws,
+                                              (bf16_t*)y, ldy, m, n, k, st);
+  };
+  if (m <= 16) go(std::integral_constant<int, 1>{});
+  else if (m <= 32) go(std::integral_constant<int, 2>{});
+  else go(std::integral_constant<int, 4>{});
+  FF_LAUNCH_CHECK("ff_gemm_fp8_block");
+  return FF_OK;
+}
+
+extern "C" int ff_gemm_fp8_block(const void* q, const float* scales, const void* packed, const float* wscales, void* y,
+                                 int64_t ldy, int64_t m, int64_t n, int64_t k, ff_stream_t stream) {
+  const int rc = check_gemm("ff_gemm_fp8_block", packed, wscales, y, ldy, m, n, k);
+  if (rc != FF_OK || m == 0) return rc;
+  FF_REQUIRE(q && scales, "ff_gemm_fp8_block: null pointer");
+  FF_REQUIRE(ff_aligned(q, 16), "ff_gemm_fp8_block: alignment");
+  return gemm_block(q, scales, packed, wscales, y, ldy, m, n, k, (hipStream_t)stream);
+}
+
+// Whether m rows of k channels are quantised inside the product's launch.
+static bool rows_inline(int64_t m, int64_t k) {
+  return m <= kRowsMax && m * ((k + kBlock - 1) / kBlock * kBlock) <= kRowsMaxCodes;
+}
+
+static int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
+
+extern "C" int ff_linear_fp8_block_workspace(int64_t m, int64_t n, int64_t k, int64_t* bytes) {
+  FF_REQUIRE(bytes, "ff_linear_fp8_block_workspace: null pointer");
+  FF_REQUIRE(m >= 0 && n > 0 && k > 0 && m < kMaxCodes && k < kMaxCodes, "ff_linear_fp8_block_workspace: bad sizes");
+  const int64_t kt_n = (k + kBlock - 1) / kBlock;
+  *bytes = rows_inline(m, k) ? 0 : align256(m * kt_n * kBlock) + m * kt_n * 4;
+  return FF_OK;
+}
+
+extern "C" int ff_linear_fp8_block(const void* x, int64_t ldx, const void* packed, const float* wscales, void* y,
+                                   int64_t ldy, int64_t m, int64_t n, int64_t k, void* workspace,
+                                   int64_t workspace_bytes, ff_stream_t stream) {
+  const int rc = check_gemm("ff_linear_fp8_block", packed, wscales, y, ldy, m, n, k);
+  if (rc != FF_OK || m == 0) return rc;
+  FF_REQUIRE(x, "ff_linear_fp8_block: null pointer");
+  FF_REQUIRE(ff_aligned(x, 2) && ldx >= 0, "ff_linear_fp8_block: alignment");
+  const hipStream_t st = (hipStream_t)stream;
+  if (rows_inline(m, k)) {
+    launch_skinny<1, true>((const bf16_t*)x, ldx, nullptr, nullptr, (const uint8_t*)packed, wscales, (bf16_t*)y, ldy, m,
+                           n, k, st);
+    FF_LAUNCH_CHECK("ff_linear_fp8_block");
+    return FF_OK;
+  }
+  const int64_t codes = align256(m * ((k + kBlock - 1) / kBlock) * kBlock);
+  int64_t need = 0;
+  ff_linear_fp8_block_workspace(m, n, k, &need);
+  FF_REQUIRE(workspace && workspace_bytes >= need && ff_aligned(workspace, 16),
+             "ff_linear_fp8_block: workspace of %lld bytes needed", (long long)need);
+  float* scales = (float*)((uint8_t*)workspace + codes);
+  const int rq = quant_rows_block(x, ldx, workspace, scales, m, k, st);
+  if (rq != FF_OK) return rq;
+  return gemm_block(workspace, scales, packed, wscales, y, ldy, m, n, k, st);
+}

@@ -14,6 +14,10 @@ attributes:
   (_family/night_runtime.py:15-42); symmetric group-128 or the reference's
   asymmetric group-32 quantizer.
 
+A fourth has no counterpart there: ``BlockFP8Linear``, the block-scaled FP8 of
+shipped checkpoints (one weight scale per 128 x 128 block, activation scales per
+row and 128 channels).
+
 Weight quantization runs once on the GPU at construction. All calls allocate
 their outputs with torch.empty and launch on the current stream.
 """
@@ -314,6 +318,131 @@ class RuntimeScaleLinear(StaticFP8Linear):
     gfx950 matrix instruction here sums each block of 32 products with ~13
     significant bits and adds the blocks in fp32, i.e. a promotion every 32
     products, which is at least as exact as either mode."""
+
+
+BLOCK = 128  # rows and channels of a weight block that share a scale
+
+
+def _blocks(n):
+    return -(-n // BLOCK)
+
+
+class BlockCodes(PackedCodes):
+    """``PackedCodes`` of weights packed for the block-scaled kernels: ``shape`` is
+    (N, K), or (batch..., N, K) of as many weights packed one after the other, whose
+    rows were padded to ``n_pad``."""
+
+    def __init__(self, packed, shape, n_pad):
+        super().__init__(packed, shape)
+        self.n_pad = n_pad
+
+    def numel(self):
+        return self.shape.numel()
+
+    def rowmajor(self):
+        n, k = self.shape[-2:]
+        w = torch.empty(self.shape, device=self.device, dtype=E4M3)
+        call("ff_unpack_weight_fp8_block", ptr(self._packed), ptr(w), w.numel() // (n * k), n, k, self.n_pad, stream())
+        return w
+
+
+def pack_blocks(codes, multiple=16):
+    """``BlockCodes`` of row-major codes (..., N, K), the rows of each weight padded to
+    a multiple of ``multiple`` and K to one of 128 with zero codes."""
+    n, k = codes.shape[-2:]
+    batch = codes.numel() // (n * k)
+    n_pad = -(-n // multiple) * multiple
+    packed = torch.empty((batch, n_pad, _blocks(k) * BLOCK), device=codes.device, dtype=E4M3)
+    call("ff_pack_weight_fp8_block", ptr(codes), ptr(packed), batch, n, k, n_pad, stream())
+    return BlockCodes(packed, codes.shape, n_pad)
+
+
+def check_block_codes(codes, scales, dims):
+    """The assertions on codes (..., N, K) of ``dims`` dimensions and their block scales."""
+    assert codes.is_cuda and codes.dtype == E4M3 and codes.dim() == dims and codes.numel() > 0
+    assert scales.device == codes.device and scales.dtype in (torch.float32, BF16)
+    assert scales.shape == (*codes.shape[:-2], _blocks(codes.shape[-2]), _blocks(codes.shape[-1])), \
+        f"block scales of codes {tuple(codes.shape)}: {tuple(scales.shape)}"
+
+
+def check_here(*tensors):
+    """Launches go to the current device's stream: every tensor has to live there."""
+    for t in tensors:
+        assert t.is_cuda, f"tensor on {t.device}"
+        assert t.get_device() == torch._C._cuda_getDevice(), f"tensor on {t.device}, which is not the current device"
+
+
+class BlockFP8Linear:
+    """Block-scaled FP8: e4m3 weights with one fp32 scale for every 128 x 128 block,
+    activations quantised per row and 128 channels (scale = amax / 448), fp32 sums of
+    (codes . codes) * row scale * weight scale, bf16 out. Any N and K.
+
+    ``BlockFP8Linear(weight)`` quantises a bf16 weight (N, K);
+    ``BlockFP8Linear.from_codes(codes, scales)`` takes a checkpoint's codes (N, K) and
+    scales (ceil(N / 128), ceil(K / 128)), value = code * scale. ``weight`` is a
+    ``BlockCodes`` (the fragment-packed copy is the only one kept), ``scale`` the
+    block scales in fp32."""
+
+    def __init__(self, weight):
+        assert weight.is_cuda and weight.ndim == 2 and weight.numel() > 0
+        check_here(weight)
+        w = weight.detach().to(BF16).contiguous()
+        n, k = w.shape
+        codes = torch.empty((n, k), device=w.device, dtype=E4M3)
+        scales = torch.empty((_blocks(n), _blocks(k)), device=w.device, dtype=torch.float32)
+        call("ff_quant_weight_fp8_block", ptr(w), ptr(codes), ptr(scales), n, k, stream())
+        self._take(codes, scales)
+
+    @classmethod
+    def from_codes(cls, codes, scales):
+        check_block_codes(codes, scales, 2)
+        check_here(codes)
+        op = cls.__new__(cls)
+        op._take(codes.contiguous(), scales.float().contiguous())
+        return op
+
+    def _take(self, codes, scales):
+        self.weight = pack_blocks(codes)
+        self.packed, self.scale = self.weight._packed, scales
+
+    def _rows2d(self, x):
+        assert x.dtype == BF16 and x.shape[-1] == self.weight.shape[1]
+        check_here(x, self.scale)
+        flat = x.reshape(-1, x.shape[-1])
+        return flat if flat.stride(-1) == 1 or flat.shape[-1] == 1 else flat.contiguous()
+
+    def quantize(self, x):
+        """e4m3 codes (M, 128 ceil(K / 128)) of x's rows, zeros past K, and their scales
+        (ceil(K / 128), M) fp32."""
+        flat = self._rows2d(x)
+        m, k = flat.shape
+        q = torch.empty((m, _blocks(k) * BLOCK), device=x.device, dtype=E4M3)
+        s = torch.empty((_blocks(k), m), device=x.device, dtype=torch.float32)
+        call("ff_quant_rows_fp8_block", ptr(flat), flat.stride(0), ptr(q), ptr(s), m, k, stream())
+        return q, s
+
+    def gemm(self, q, s):
+        """The product from rows quantised by ``quantize``: the bits of ``op(x)``."""
+        n, k = self.weight.shape
+        m = q.shape[0]
+        assert q.dtype == E4M3 and q.shape[1] == _blocks(k) * BLOCK and q.is_contiguous()
+        assert s.dtype == torch.float32 and s.shape == (_blocks(k), m) and s.is_contiguous()
+        check_here(q, s, self.scale)
+        y = torch.empty((m, n), device=q.device, dtype=BF16)
+        call("ff_gemm_fp8_block", ptr(q), ptr(s), ptr(self.packed), ptr(self.scale), ptr(y), n, m, n, k, stream())
+        return y
+
+    def __call__(self, x):
+        flat = self._rows2d(x)
+        m, k = flat.shape
+        n = self.weight.shape[0]
+        y = torch.empty((*x.shape[:-1], n), device=x.device, dtype=BF16)
+        need = ctypes.c_int64(0)
+        call("ff_linear_fp8_block_workspace", m, n, k, ctypes.byref(need))
+        ws = torch.empty(need.value, device=x.device, dtype=torch.uint8) if need.value else None
+        call("ff_linear_fp8_block", ptr(flat), flat.stride(0), ptr(self.packed), ptr(self.scale), ptr(y), n, m, n, k,
+             ptr(ws), need.value, stream())
+        return y
 
 
 class Int4:

@@ -455,6 +455,75 @@ int ff_scatter_rows(const void* src, void* out, int64_t start, int64_t n, int64_
 int ff_mrope_cos_sin(const int64_t* pos, const float* inv_freq, void* cos, void* sin, int64_t t,
                      int64_t d, int sec_h, int sec_w, ff_stream_t stream);
 
+/* ---------------------------------------------------------------- block-scaled FP8
+ * The format FP8 checkpoints are shipped in (no reference counterpart: the
+ * reference quantises per row or per tensor). A weight (n, k) is e4m3 codes with
+ * one fp32 scale for each 128 x 128 block, scales (ceil(n / 128), ceil(k / 128)):
+ * value = code * scale. A row of activations is e4m3 codes with one fp32 scale for
+ * each 128 channels: scale = max(amax, 1e-12) / 448, code = e4m3(x / scale). The
+ * last block of either side may be partial; n and k are any positive sizes. */
+
+/* Codes and block scales of a bf16 weight w (n, k): scale = max(amax, 1e-12) / 448. */
+int ff_quant_weight_fp8_block(const void* w, void* q, float* scales, int64_t n, int64_t k, ff_stream_t stream);
+/* Setup-time repack of `batch` weights' codes w (batch, n, k) row-major into
+ * MFMA-fragment order, rows padded to n_pad (a multiple of 16) and k to a multiple
+ * of 128 with zero codes: packed holds batch * n_pad * 128 ceil(k / 128) bytes,
+ * 16-byte aligned. ff_unpack_weight_fp8_block is the inverse. */
+int ff_pack_weight_fp8_block(const void* w, void* packed, int64_t batch, int64_t n, int64_t k, int64_t n_pad,
+                             ff_stream_t stream);
+int ff_unpack_weight_fp8_block(const void* packed, void* w, int64_t batch, int64_t n, int64_t k, int64_t n_pad,
+                               ff_stream_t stream);
+/* Rows x (rows, k) bf16, row stride ldx, any alignment: codes q (rows, 128
+ * ceil(k / 128)), zeros past k, 16-byte aligned, and scales (ceil(k / 128), rows). */
+int ff_quant_rows_fp8_block(const void* x, int64_t ldx, void* q, float* scales, int64_t rows, int64_t k,
+                            ff_stream_t stream);
+/* y = bf16(sum over blocks of (codes . codes) * row scale * weight scale) from rows
+ * quantised by ff_quant_rows_fp8_block and a weight packed with n_pad = n rounded
+ * up to 16; sums in fp32. y (m, n), row stride ldy. */
+int ff_gemm_fp8_block(const void* q, const float* scales, const void* packed, const float* wscales, void* y,
+                      int64_t ldy, int64_t m, int64_t n, int64_t k, ff_stream_t stream);
+/* The whole linear from bf16 rows x (row stride ldx): quantisation and product. Up
+ * to four rows run in one launch. workspace: ff_linear_fp8_block_workspace bytes
+ * (0: may be NULL), 16-byte aligned. */
+int ff_linear_fp8_block_workspace(int64_t m, int64_t n, int64_t k, int64_t* bytes);
+int ff_linear_fp8_block(const void* x, int64_t ldx, const void* packed, const float* wscales, void* y, int64_t ldy,
+                        int64_t m, int64_t n, int64_t k, void* workspace, int64_t workspace_bytes,
+                        ff_stream_t stream);
+
+/* ---------------------------------------------------------------- mixture of experts
+ * (no reference counterpart: its models have one MLP per layer). */
+
+/* The experts of each token. logits (t, experts) bf16, or fp32 with logits_f32, row
+ * stride ld; p = softmax over the experts or, with sigmoid, 1 / (1 + exp(-l)); the
+ * choice goes by p + bias[e] (bias (experts) fp32 or NULL). With groups > 1 (equal
+ * runs of experts) only the top_groups best groups stay, a group's score being its
+ * best choice score, with a bias the sum of its two best. The top_k best experts
+ * in falling order, the lowest index first among equals, go to ids (t, top_k) int32
+ * and their p to weights (t, top_k) fp32, divided by their sum with renormalize and
+ * multiplied by scale. A logit of -inf switches its expert off; where fewer than
+ * top_k are left the rest have id -1 and weight 0. A row with a NaN (or +inf under
+ * softmax) has ids 0 .. top_k - 1 and NaN weights. Scores are computed and compared
+ * in 64 bits. experts <= 1024, top_k <= 64, groups <= 64,
+ * top_groups * experts / groups >= top_k. */
+int ff_moe_route(const void* logits, int logits_f32, int64_t ld, const float* bias, float* weights, int* ids,
+                 int64_t t, int64_t experts, int64_t top_k, int sigmoid, int64_t groups, int64_t top_groups,
+                 int renormalize, float scale, ff_stream_t stream);
+
+/* y[t] = bf16(sum_j weights[t, j] D_e bf16(silu(G_e x[t]) * (U_e x[t]))), e = ids[t, j],
+ * with x quantised as by ff_quant_rows_fp8_block, sums in fp32. gate_up: the codes
+ * (experts, 2, i, h) of G and U packed with n_pad = i rounded up to 128 and their
+ * scales (experts, 2, ceil(i / 128), ceil(h / 128)); down: the codes (experts, h, i)
+ * of D packed with n_pad = h rounded up to 16, scales (experts, ceil(h / 128),
+ * ceil(i / 128)). x (t, h) bf16 with row stride ldx, weights (t, top_k) fp32, ids
+ * (t, top_k) int32; an id outside [0, experts) is no expert and adds nothing; an
+ * expert may come twice. workspace: ff_moe_experts_workspace bytes, 256-byte
+ * aligned. The sums' order depends on the sizes alone. experts <= 1024. */
+int ff_moe_experts_workspace(int64_t t, int64_t top_k, int64_t experts, int64_t h, int64_t i, int64_t* bytes);
+int ff_moe_experts(const void* x, int64_t ldx, const float* weights, const int* ids, const void* gate_up,
+                   const float* gate_up_scales, const void* down, const float* down_scales, void* y, int64_t ldy,
+                   int64_t t, int64_t top_k, int64_t experts, int64_t h, int64_t i, void* workspace,
+                   int64_t workspace_bytes, ff_stream_t stream);
+
 #ifdef __cplusplus
 /* ---------------------------------------------------------------- vision tower
  * The reference runs the vision tower as bf16 torch modules inside
