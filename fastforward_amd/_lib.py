@@ -4,6 +4,7 @@ The library is loaded from this package directory; there is no fallback. A
 missing library, a missing symbol or a non-gfx950 device raises.
 """
 import ctypes
+import functools
 import os
 
 import torch
@@ -137,6 +138,20 @@ def call(name, *args):
     st = getattr(lib, name)(*args)
     if st != 0:
         raise RuntimeError(f"{name} failed ({st}): {lib.ff_last_error().decode()}")
+
+
+@functools.lru_cache(maxsize=None)
+def entry(name):
+    """``call`` with the entry point looked up once and pointers passed as integers
+    (``data_ptr()``; 0 is NULL): for ops whose launch is as short as their host code."""
+    lib = load()
+    fn = getattr(lib, name)
+
+    def run(*args):
+        st = fn(*args)
+        if st != 0:
+            raise RuntimeError(f"{name} failed ({st}): {lib.ff_last_error().decode()}")
+    return run
 
 
 def ptr(t):

@@ -99,34 +99,61 @@ __device__ __forceinline__ void store4_bf16(bf16_t* p, const f32x4& v, int64_t l
   }
 }
 
-// Expert, first row and rows of row tile `tile` (bm rows each, every expert's rows
-// starting a tile of their own) among experts whose rows are [off[e], off[e + 1]).
-// False past the last tile. Every lane of a wave calls it and gets the result.
-__device__ __forceinline__ bool find_tile(const int* __restrict__ off, int experts, int bm, int tile, int* expert,
-                                          int* row0, int* rows) {
+// Inclusive prefix sum over the 64 lanes (row shifts, then the row totals broadcast on).
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
+// Logical tile of workgroup b of n: consecutive workgroups go to the 8 XCDs in turn, so
+// that each XCD (one L2) takes a contiguous run of tiles.
+__device__ __forceinline__ int xcd_tile(int b, int n) {
+  const int xcd = b & 7, q = n >> 3, r = n & 7;
+  return xcd * q + min(xcd, r) + (b >> 3);
+}
+
+// This workgroup's tile of a product whose rows are ordered by expert, [off[e], off[e +
+// 1]) the rows of expert e: expert, first row, rows and column tile. Row tiles have bm
+// rows, every expert's rows starting one of their own, tiles_n column tiles each (fastest).
+// The grid holds the most workgroups that any choice of experts can need; those past the
+// actual number get false, and the others share the tiles over the XCDs (dealt out over the
+// whole grid, the unused ones would all fall to the last XCDs). Uniform results.
+struct ExpertTile {
+  int expert, row0, rows, col;
+};
+__device__ __forceinline__ bool find_tile(const int* __restrict__ off, int experts, int bm, int tiles_n,
+                                          ExpertTile* out) {
   const int lane = threadIdx.x & 63;
+  int total = 0;
+  for (int e0 = 0; e0 < experts; e0 += 64) {
+    const int e = min(e0 + lane, experts);
+    total += (off[min(e + 1, experts)] - off[e] + bm - 1) / bm;
+  }
+  total = __builtin_amdgcn_readlane(wave_scan(total), 63) * tiles_n;
+  if ((int)blockIdx.x >= total) return false;
+  const int id = xcd_tile(blockIdx.x, total), tile = id / tiles_n;
   int base = 0;
   for (int e0 = 0; e0 < experts; e0 += 64) {
-    const int e = e0 + lane;
-    const int lo = e < experts ? off[e] : 0, hi = e < experts ? off[e + 1] : 0;
+    const int e = min(e0 + lane, experts);
+    const int lo = off[e], hi = off[min(e + 1, experts)];
     const int n = (hi - lo + bm - 1) / bm;
-    int sum = n;  // inclusive prefix sum over the lanes
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int up = __shfl_up(sum, d);
-      if (lane >= d) sum += up;
-    }
-    const int first = base + sum - n;
+    const int sum = wave_scan(n), first = base + sum - n;
     const uint64_t hit = __ballot(tile >= first && tile < first + n);
     if (hit) {
       const int src = __builtin_ctzll(hit);
-      const int f = __shfl(first, src), l = __shfl(lo, src), h = __shfl(hi, src);
-      *expert = e0 + src;
-      *row0 = l + (tile - f) * bm;
-      *rows = min(bm, h - *row0);
+      const int l = __builtin_amdgcn_readlane(lo, src), at = (tile - __builtin_amdgcn_readlane(first, src)) * bm;
+      out->expert = e0 + src;
+      out->row0 = l + at;
+      out->rows = min(bm, __builtin_amdgcn_readlane(hi, src) - l - at);
+      out->col = id % tiles_n;
       return true;
     }
-    base += __shfl(sum, 63);
+    base += __builtin_amdgcn_readlane(sum, 63);
   }
   return false;
 }

@@ -1,11 +1,13 @@
 // Block-scaled FP8 linear for gfx950: setup (weight quantisation, packing), the
 // row quantiser and the products y = x . W^T (ff_block.h states the format).
 //
-// skinny_kernel: few rows. A workgroup of 8 waves owns 16 RI rows x 16 NJ weight
-// rows; its waves take the k steps in turn (wave w: steps w, w + 8, ..), so that
-// even 4096 columns make 256 workgroups that read the weights from every channel
-// of memory, and their sums are added through LDS in wave order.
-#include "ff_block.h"
+// Few rows (skinny_kernel): a workgroup of 8 waves owns 16 rows x 16 or 32 weight rows and
+// its waves take the k steps in turn (wave w: steps w, w + 8, ..), so that even 4096
+// columns make 256 workgroups that read the weights from every channel of memory; their
+// sums are added through LDS in wave order. Up to four rows are quantised in the same
+// launch.
+// More rows (tile_kernel): tiles of 32 x 64, 64 x 128 or 128 x 128 (ff_block_tile.h).
+#include "ff_block_tile.h"
 
 using namespace ff;
 
@@ -82,17 +84,20 @@ __global__ __launch_bounds__(256) void unpack_block_kernel(const uint8_t* __rest
 
 // 16 lanes per (row, 128 channels): codes q (rows, 128 kt_n) and scales (kt_n,
 // rows), channel blocks slowest, so that the lanes of a product's row tile read
-// neighbouring scales.
+// neighbouring scales. A workgroup takes 16 rows of one channel block at a time,
+// whose scales are one 64-byte line.
 __global__ __launch_bounds__(256) void quant_rows_block_kernel(const bf16_t* __restrict__ x, int64_t ldx,
                                                                uint8_t* __restrict__ q, float* __restrict__ scales,
                                                                int64_t rows, int64_t k, int kt_n, int vec) {
   const int s = threadIdx.x & 15;
-  for (int64_t i = (blockIdx.x * (int64_t)256 + threadIdx.x) >> 4; i < rows * kt_n; i += (int64_t)gridDim.x * 16) {
-    const int64_t row = i / kt_n;
+  const int64_t tiles = (rows + 15) / 16 * kt_n;
+  for (int64_t i = blockIdx.x; i < tiles; i += gridDim.x) {
+    const int64_t row = i / kt_n * 16 + (threadIdx.x >> 4);
     const int kt = (int)(i % kt_n);
+    if (row >= rows) continue;
     float scale;
     const u32x2 c = quant_group16(x + row * ldx, k, kt, s, vec, &scale);
-    *reinterpret_cast<u32x2*>(q + i * kBlock + 8 * s) = c;
+    *reinterpret_cast<u32x2*>(q + (row * kt_n + kt) * kBlock + 8 * s) = c;
     if (s == 0) scales[(int64_t)kt * rows + row] = scale;
   }
 }
@@ -100,24 +105,24 @@ __global__ __launch_bounds__(256) void quant_rows_block_kernel(const bf16_t* __r
 // ---------------------------------------------------------------- few rows
 
 // INLINE: the workgroup quantises the rows (at most kRowsMax) into LDS itself.
-template <int RI, int NJ, bool INLINE>
+template <int NJ, bool INLINE>
 __global__ __launch_bounds__(kSkinnyThreads) void skinny_kernel(
     const bf16_t* __restrict__ x, int64_t ldx, int vec, const uint8_t* __restrict__ q, const float* __restrict__ qs,
     const uint8_t* __restrict__ wp, const float* __restrict__ ws, bf16_t* __restrict__ y, int64_t ldy, int64_t m,
     int64_t n, int64_t k, int kt_n, int nf) {
   constexpr int PF = 4;  // k steps whose loads a wave has in flight
-  constexpr int kSums = kSkinnyWaves * RI * NJ * 256;  // floats of the waves' sums
-  constexpr int kLds = INLINE ? kRowsMaxCodes + 16 * kRowsMaxCodes / kBlock : kSums * 4;
-  static_assert(!INLINE || kSums * 4 <= kLds, "the sums reuse the codes' LDS");
+  constexpr int kSums = kSkinnyWaves * NJ * 64 * 16;  // bytes of the waves' sums
+  constexpr int kLds = INLINE ? kRowsMaxCodes + 4 * kRowsMaxCodes / kBlock : kSums;
+  static_assert(kSums <= kLds, "the sums reuse the codes' LDS");
   __shared__ __align__(16) uint8_t smem[kLds];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r16 = lane & 15, g = lane >> 4;
   const int f0 = blockIdx.x * NJ;
-  const int64_t m0 = (int64_t)blockIdx.y * 16 * RI;
+  const int64_t m0 = (int64_t)blockIdx.y * 16, row = min(m0 + r16, m - 1);
   const int mine = (kt_n - wave + kSkinnyWaves - 1) / kSkinnyWaves;  // this wave's k steps
 
-  i32x8 wq[PF][NJ], xq[PF][RI];
-  float xs[PF][RI], wsc[PF][NJ];
+  i32x8 wq[PF][NJ], xq[PF];
+  float xs[PF], wsc[PF][NJ];
   const uint8_t* frag[NJ];
   const float* wscale[NJ];
 #pragma unroll
@@ -126,9 +131,6 @@ __global__ __launch_bounds__(kSkinnyThreads) void skinny_kernel(
     frag[j] = wp + (int64_t)f * 2048;
     wscale[j] = ws + (int64_t)(f / 8) * kt_n;
   }
-  int64_t row[RI];
-#pragma unroll
-  for (int i = 0; i < RI; ++i) row[i] = min(m0 + 16 * i + r16, m - 1);
   auto loadW = [&](int u, int kt) {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
@@ -137,26 +139,15 @@ __global__ __launch_bounds__(kSkinnyThreads) void skinny_kernel(
     }
   };
   auto loadX = [&](int u, int kt) {
-#pragma unroll
-    for (int i = 0; i < RI; ++i) {
-      if constexpr (INLINE) {
-        const int64_t at = row[i] * kt_n + kt;
-        const i32x4v* p = reinterpret_cast<const i32x4v*>(smem + at * kBlock + 32 * g);
-        xq[u][i] = join(p[0], p[1]);
-        xs[u][i] = reinterpret_cast<const float*>(smem + kRowsMaxCodes)[at];
-      } else {
-        const i32x4v* p = reinterpret_cast<const i32x4v*>(q + (row[i] * kt_n + kt) * kBlock + 32 * g);
-        xq[u][i] = join(p[0], p[1]);
-        xs[u][i] = qs[(int64_t)kt * m + row[i]];
-      }
-    }
+    const int64_t at = row * kt_n + kt;
+    const i32x4v* p = reinterpret_cast<const i32x4v*>((INLINE ? smem : q) + at * kBlock + 32 * g);
+    xq[u] = join(p[0], p[1]);
+    xs[u] = INLINE ? reinterpret_cast<const float*>(smem + kRowsMaxCodes)[at] : qs[(int64_t)kt * m + row];
   };
 
-  f32x4 acc[RI][NJ];
+  f32x4 acc[NJ];
 #pragma unroll
-  for (int i = 0; i < RI; ++i)
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < NJ; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   for (int b = 0; b < mine || (INLINE && b == 0); b += PF) {
 #pragma unroll
@@ -164,9 +155,9 @@ __global__ __launch_bounds__(kSkinnyThreads) void skinny_kernel(
       if (b + u < mine) loadW(u, wave + kSkinnyWaves * (b + u));
     if constexpr (INLINE) {
       if (b == 0) {  // the first weights are in flight meanwhile
-        for (int64_t i = threadIdx.x >> 4; i < m * kt_n; i += kSkinnyThreads / 16) {
+        for (int i = threadIdx.x >> 4; i < (int)m * kt_n; i += kSkinnyThreads / 16) {
           float scale;
-          const u32x2 c = quant_group16(x + i / kt_n * ldx, k, (int)(i % kt_n), r16, vec, &scale);
+          const u32x2 c = quant_group16(x + i / kt_n * ldx, k, i % kt_n, r16, vec, &scale);
           *reinterpret_cast<u32x2*>(smem + i * kBlock + 8 * r16) = c;
           if (r16 == 0) reinterpret_cast<float*>(smem + kRowsMaxCodes)[i] = scale;
         }
@@ -180,44 +171,110 @@ __global__ __launch_bounds__(kSkinnyThreads) void skinny_kernel(
     for (int u = 0; u < PF; ++u)
       if (b + u < mine) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
-#pragma unroll
-          for (int i = 0; i < RI; ++i) fma4(acc[i][j], mfma_step(wq[u][j], xq[u][i]), xs[u][i] * wsc[u][j]);
+        for (int j = 0; j < NJ; ++j) fma4(acc[j], mfma_step(wq[u][j], xq[u]), xs[u] * wsc[u][j]);
       }
   }
 
   if constexpr (INLINE) __syncthreads();  // the codes are no longer read
   f32x4* red = reinterpret_cast<f32x4*>(smem);
 #pragma unroll
-  for (int i = 0; i < RI; ++i)
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) red[(wave * RI * NJ + i * NJ + j) * 64 + lane] = acc[i][j];
+  for (int j = 0; j < NJ; ++j) red[(wave * NJ + j) * 64 + lane] = acc[j];
   __syncthreads();
-  for (int t = threadIdx.x; t < RI * NJ * 64; t += kSkinnyThreads) {
+  for (int t = threadIdx.x; t < NJ * 64; t += kSkinnyThreads) {
     f32x4 v = red[t];
 #pragma unroll
-    for (int w = 1; w < kSkinnyWaves; ++w) v += red[w * RI * NJ * 64 + t];
-    const int l = t & 63, i = t / 64 / NJ, j = t / 64 % NJ;
-    const int64_t r = m0 + 16 * i + (l & 15), c = 16 * (int64_t)(f0 + j) + 4 * (l >> 4);
+    for (int w = 1; w < kSkinnyWaves; ++w) v += red[w * NJ * 64 + t];
+    const int64_t r = m0 + (t & 15), c = 16 * (int64_t)(f0 + t / 64) + 4 * (t % 64 / 16);
     if (r < m && c < n) store4_bf16(y + r * ldy + c, v, n - c);
+  }
+}
+
+// ---------------------------------------------------------------- many rows
+
+// BM x 4 CW tiles, KG groups of 4 waves that share the k steps of a tile. Tile order: groups
+// of 8 row tiles, within a group row tiles fastest, so that the tiles an XCD runs at one
+// time share rows and weights.
+template <int BM, int CW, int P, int D, int KG, int OCC>
+__global__ __launch_bounds__(kTileThreads* KG, OCC) void tile_kernel(
+    const uint8_t* __restrict__ q, const float* __restrict__ qs, const uint8_t* __restrict__ wp,
+    const float* __restrict__ ws, bf16_t* __restrict__ y, int64_t ldy, int64_t m, int64_t n, int kt_n, int nf,
+    int tiles_m, int tiles_n) {
+  constexpr int RA = BM / 16, TJ = CW / 16, GM = 8;
+  constexpr int kStages = KG * tile_smem<BM>(), kSums = (KG - 1) * kTileThreads * RA * TJ * 16;
+  __shared__ __align__(1024) uint8_t smem[kStages > kSums ? kStages : kSums];  // the groups' sums reuse the stages
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r16 = lane & 15, g = lane >> 4, group = wave / 4;
+  const int id = xcd_tile(blockIdx.x, tiles_m * tiles_n);
+  const int first = id / (GM * tiles_n) * GM, in = id % (GM * tiles_n), gm = min(GM, tiles_m - first);
+  const int64_t m0 = (int64_t)(first + in % gm) * BM;
+  const int f0 = in / gm * (4 * TJ) + wave % 4 * TJ;
+  const int per = (kt_n + KG - 1) / KG, k0 = group * per;
+  TileWeights<TJ, 1> w{{wp}, (uint32_t)nf * min(kt_n, k0 + per) * 2048u, (uint32_t)nf * 2048u,
+                       {ws + (int64_t)(min(f0, nf - 1) / 8) * kt_n}, {}};
+#pragma unroll
+  for (int j = 0; j < TJ; ++j) w.frag[j] = (uint32_t)(f0 + j) * 2048u;
+  const int rows = (int)min((int64_t)BM, m - m0);
+  const uint32_t kp = (uint32_t)kt_n * kBlock;
+  f32x4 acc[RA][TJ];
+  tile_mainloop<BM, CW, 1, P, D>(
+      acc, smem + group * tile_smem<BM>(), kt_n, k0, per, q + m0 * kp, (uint32_t)rows * kp,
+      [&](int r) { return (uint32_t)min(r, rows - 1) * kp; }, qs, (uint32_t)(4 * m) * kt_n,
+      [&](int r) { return (uint32_t)m0 + min(r, rows - 1); }, (uint32_t)(4 * m), w);
+  if constexpr (KG > 1) {  // the groups' sums, added in order
+    f32x4* red = reinterpret_cast<f32x4*>(smem);
+    __syncthreads();
+    if (group > 0) {
+#pragma unroll
+      for (int i = 0; i < RA; ++i)
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) red[(i * TJ + j) * (KG - 1) * kTileThreads + threadIdx.x - kTileThreads] = acc[i][j];
+    }
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int i = 0; i < RA; ++i)
+#pragma unroll
+      for (int j = 0; j < TJ; ++j)
+#pragma unroll
+        for (int o = 0; o < KG - 1; ++o)
+          acc[i][j] += red[((i * TJ + j) * (KG - 1) + o) * kTileThreads + threadIdx.x];
+  }
+#pragma unroll
+  for (int i = 0; i < RA; ++i) {
+    const int64_t r = m0 + 16 * i + r16;
+    if (r >= m) continue;
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) {
+      const int64_t c = 16 * (int64_t)(f0 + j) + 4 * g;
+      if (c < n) store4_bf16(y + r * ldy + c, acc[i][j], n - c);
+    }
   }
 }
 
 inline bool rows_vec(const void* x, int64_t ldx) { return ff_aligned(x, 16) && ldx % 8 == 0; }
 
-// Fragments (16 weight rows) per workgroup: one where that leaves at most two workgroups per CU.
-template <int RI, bool INLINE>
+// 16 weight rows per workgroup while that leaves at most two workgroups per CU, else 32.
+template <bool INLINE>
 void launch_skinny(const bf16_t* x, int64_t ldx, const uint8_t* q, const float* qs, const uint8_t* wp, const float* ws,
                    bf16_t* y, int64_t ldy, int64_t m, int64_t n, int64_t k, hipStream_t st) {
   const int nf = (int)((n + 15) / 16), kt_n = (int)((k + kBlock - 1) / kBlock);
-  const int64_t tiles_m = (m + 16 * RI - 1) / (16 * RI);
+  const int64_t tiles_m = (m + 15) / 16;
   const int vec = rows_vec(x, ldx);
   if (tiles_m * nf <= 512)
-    hipLaunchKernelGGL((skinny_kernel<RI, 1, INLINE>), dim3((unsigned)nf, (unsigned)tiles_m), dim3(kSkinnyThreads), 0,
-                       st, x, ldx, vec, q, qs, wp, ws, y, ldy, m, n, k, kt_n, nf);
+    hipLaunchKernelGGL((skinny_kernel<1, INLINE>), dim3((unsigned)nf, (unsigned)tiles_m), dim3(kSkinnyThreads), 0, st, x,
+                       ldx, vec, q, qs, wp, ws, y, ldy, m, n, k, kt_n, nf);
   else
-    hipLaunchKernelGGL((skinny_kernel<RI, 2, INLINE>), dim3((unsigned)((nf + 1) / 2), (unsigned)tiles_m),
+    hipLaunchKernelGGL((skinny_kernel<2, INLINE>), dim3((unsigned)((nf + 1) / 2), (unsigned)tiles_m),
                        dim3(kSkinnyThreads), 0, st, x, ldx, vec, q, qs, wp, ws, y, ldy, m, n, k, kt_n, nf);
+}
+
+template <int BM, int CW, int P, int D, int KG>
+void launch_tile(const void* q, const float* qs, const void* packed, const float* ws, void* y, int64_t ldy, int64_t m,
+                 int64_t n, int kt_n, int nf, hipStream_t st) {
+  const int64_t tm = (m + BM - 1) / BM, tn = (nf + CW / 4 - 1) / (CW / 4);
+  hipLaunchKernelGGL((tile_kernel<BM, CW, P, D, KG, 2>), dim3((unsigned)(tm * tn)), dim3(kTileThreads * KG), 0, st,
+                     (const uint8_t*)q, qs, (const uint8_t*)packed, ws, (bf16_t*)y, ldy, m, n, kt_n, nf, (int)tm,
+                     (int)tn);
 }
 
 constexpr int64_t kMaxCodes = 1ll << 31;
@@ -228,7 +285,7 @@ namespace ff {
 
 int quant_rows_block(const void* x, int64_t ldx, void* q, float* scales, int64_t rows, int64_t k, hipStream_t st) {
   const int64_t kt_n = (k + kBlock - 1) / kBlock;
-  const int64_t grid = (rows * kt_n + 15) / 16;
+  const int64_t grid = (rows + 15) / 16 * kt_n;
   hipLaunchKernelGGL(quant_rows_block_kernel, dim3((unsigned)(grid < (1 << 20) ? grid : (1 << 20))), dim3(256), 0, st, (const bf16_t*)x, ldx,
                      (uint8_t*)q, scales, rows, k, (int)kt_n, (int)rows_vec(x, ldx));
   FF_LAUNCH_CHECK("quant_rows_fp8_block");
@@ -289,7 +346,8 @@ extern "C" int ff_quant_rows_fp8_block(const void* x, int64_t ldx, void* q, floa
 static int check_gemm(const char* who, const void* packed, const float* ws, const void* y, int64_t ldy, int64_t m,
                       int64_t n, int64_t k) {
   FF_REQUIRE(m >= 0 && m < kMaxCodes && n > 0 && k > 0 && n < kMaxCodes && k < kMaxCodes && ldy >= n &&
-                 ((n + 15) / 16 * 16) * ((k + kBlock - 1) / kBlock * kBlock) < kMaxCodes && m <= 65535ll * 16,
+                 ((n + 15) / 16 * 16) * ((k + kBlock - 1) / kBlock * kBlock) < kMaxCodes && m <= 65535ll * 16 &&
+                 m * ((k + kBlock - 1) / kBlock) < (1ll << 30),
              "%s: bad sizes m=%lld n=%lld k=%lld", who, (long long)m, (long long)n, (long long)k);
   if (m == 0) return FF_OK;
   FF_REQUIRE(packed && ws && y, "%s: null pointer", who);
@@ -297,15 +355,45 @@ static int check_gemm(const char* who, const void* packed, const float* ws, cons
   return FF_OK;
 }
 
+// The kernel for quantised rows (us in a graph; columns: few-rows kernel, 32 x 64, 64 x 128,
+// 128 x 128 tiles):
+//   m x n x k             few    32 x 64   64 x 128   128 x 128
+//   7 x 4096 x 4096       3.8      6.8       11.9       19.4
+//   16 x 2048 x 25600    17.6     26.2       59         99
+//   7 x 8192 x 4096       5.9      6.9       12.0       19.4
+//   7 x 12288 x 4096     11.5      8.8       12.3       19.5
+//   32 x 6144 x 4096     11.5      6.9       12.1       20.0
+//   128 x 4096 x 4096    21.9      7.5       12.8       20.6
+//   333 x 1152 x 4304    22.5      8.3       13.5       22.8
+//   7 x 19456 x 2560     11.6     11.8        9.7       13.8
+//   176 x 6144 x 4096    70       16.5       13.1       21.1
+//   300 x 4096 x 4096    70       16.9       13.1       21.0
+//   1000 x 2048 x 1024   33       10.2        6.4        9.7
+//   2000 x 4096 x 512    81       33         14.0       13.7
+//   576 x 6144 x 4096   172       37.7       27.5       24.5
+//   1024 x 25600 x 5120 1390     309        179        162
+// The larger tile reads less for a product and takes longer for a step, so it waits until
+// its tiles fill the GPU.
+static int block_kernel(int64_t m, int64_t n) {
+  const int tune = ff_tuning(FF_TUNE_BLOCK_TILE);
+  if (tune) return tune;
+  if (m <= 16 && n <= 8192) return 1;
+  const auto tiles = [&](int64_t bm, int64_t bn) { return ((m + bm - 1) / bm) * ((n + bn - 1) / bn); };
+  if (tiles(128, 128) >= 224) return 4;
+  return tiles(64, 128) >= 128 ? 3 : 2;
+}
+
 static int gemm_block(const void* q, const float* qs, const void* packed, const float* ws, void* y, int64_t ldy,
                       int64_t m, int64_t n, int64_t k, hipStream_t st) {
-  auto go = [&](auto RI) {
-    launch_skinny<decltype(RI)::value, false>(nullptr, 0, (const uint8_t*)q, qs, (const uint8_t*)packed, ws,
-                                              (bf16_t*)y, ldy, m, n, k, st);
-  };
-  if (m <= 16) go(std::integral_constant<int, 1>{});
-  else if (m <= 32) go(std::integral_constant<int, 2>{});
-  else go(std::integral_constant<int, 4>{});
+  const int nf = (int)((n + 15) / 16), kt_n = (int)((k + kBlock - 1) / kBlock);
+  switch (block_kernel(m, n)) {
+    case 1:
+      launch_skinny<false>(nullptr, 0, (const uint8_t*)q, qs, (const uint8_t*)packed, ws, (bf16_t*)y, ldy, m, n, k, st);
+      break;
+    case 2: launch_tile<32, 16, 4, 2, 2>(q, qs, packed, ws, y, ldy, m, n, kt_n, nf, st); break;
+    case 3: launch_tile<64, 32, 3, 1, 1>(q, qs, packed, ws, y, ldy, m, n, kt_n, nf, st); break;
+    default: launch_tile<128, 32, 3, 1, 1>(q, qs, packed, ws, y, ldy, m, n, kt_n, nf, st); break;
+  }
   FF_LAUNCH_CHECK("ff_gemm_fp8_block");
   return FF_OK;
 }
@@ -343,7 +431,7 @@ extern "C" int ff_linear_fp8_block(const void* x, int64_t ldx, const void* packe
   FF_REQUIRE(ff_aligned(x, 2) && ldx >= 0, "ff_linear_fp8_block: alignment");
   const hipStream_t st = (hipStream_t)stream;
   if (rows_inline(m, k)) {
-    launch_skinny<1, true>((const bf16_t*)x, ldx, nullptr, nullptr, (const uint8_t*)packed, wscales, (bf16_t*)y, ldy, m,
+    launch_skinny<true>((const bf16_t*)x, ldx, nullptr, nullptr, (const uint8_t*)packed, wscales, (bf16_t*)y, ldy, m,
                            n, k, st);
     FF_LAUNCH_CHECK("ff_linear_fp8_block");
     return FF_OK;

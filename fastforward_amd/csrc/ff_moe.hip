@@ -16,7 +16,7 @@
 // More pairs: they are ordered by expert (plan), the rows quantised once, and row
 // tiles that belong to one expert each run both products; the down products of a
 // token's experts are added by a last launch in the order of the token's list.
-#include "ff_block.h"
+#include "ff_block_tile.h"
 
 using namespace ff;
 
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(64 * kRouteRows) void route_kernel(
 // order to list[off[e] ..), off[e] = pairs of lower experts. Every workgroup reads
 // all ids (a few hundred KB from L2 at most) and needs nothing from the others: no
 // counters in memory, no order of arrival. ids outside [0, experts) are in no list.
-constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
+constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64, kPlanBatch = 8;
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* __restrict__ ids, int pairs, int experts,
                                                             int* __restrict__ off, int* __restrict__ list) {
   __shared__ int below[kPlanWaves], equal[kPlanWaves];
@@ -193,10 +193,18 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* __restric
   const int seg = (pairs + kPlanWaves - 1) / kPlanWaves;
   const int lo = min(pairs, wave * seg), hi = min(pairs, lo + seg);
   int nb = 0, ne = 0;
-  for (int i = lo + lane; i < hi; i += 64) {
-    const int id = ids[i];
-    nb += id >= 0 && id < e;
-    ne += id == e;
+  for (int i0 = lo; i0 < hi; i0 += 64 * kPlanBatch) {  // the loads of a batch in flight together
+    int id[kPlanBatch];
+#pragma unroll
+    for (int v = 0; v < kPlanBatch; ++v) {
+      const int i = i0 + 64 * v + lane;
+      id[v] = i < hi ? ids[i] : -1;
+    }
+#pragma unroll
+    for (int v = 0; v < kPlanBatch; ++v) {
+      nb += id[v] >= 0 && id[v] < e;
+      ne += id[v] == e;
+    }
   }
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
@@ -217,16 +225,41 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* __restric
     off[e] = base;
     if (e == experts - 1) off[experts] = all;
   }
-  for (int i0 = lo; i0 < hi; i0 += 64) {
-    const int i = i0 + lane;
-    const bool hit = i < hi && ids[i] == e;
-    const uint64_t b = __ballot(hit);
-    if (hit) list[base + __builtin_popcountll(b & ((1ull << lane) - 1))] = i;
-    base += __builtin_popcountll(b);
+  if (equal[wave] == 0) return;
+  for (int i0 = lo; i0 < hi; i0 += 64 * kPlanBatch) {
+    int id[kPlanBatch];
+#pragma unroll
+    for (int v = 0; v < kPlanBatch; ++v) {
+      const int i = i0 + 64 * v + lane;
+      id[v] = i < hi ? ids[i] : -1;
+    }
+#pragma unroll
+    for (int v = 0; v < kPlanBatch; ++v) {
+      const uint64_t b = __ballot(id[v] == e);
+      if (id[v] == e) list[base + __builtin_popcountll(b & ((1ull << lane) - 1))] = i0 + 64 * v + lane;
+      base += __builtin_popcountll(b);
+    }
   }
 }
 
 // ---------------------------------------------------------------- gate/up + SwiGLU
+
+// g / (1 + exp(-g)) to a few units in the last place of fp32 (its bf16 rounding follows):
+// exp(-g) = 2^(-g log2 e), the product's rounding error added back to first order, and the
+// hardware's exponential and reciprocal (1 ulp each) in place of the library's (some 50
+// instructions a value, a fifth of the gate/up tiles' time).
+__device__ __forceinline__ float silu_fast(float g) {
+  constexpr float kLog2e = 1.44269504f, kLog2eLow = 1.92596299e-8f, kLn2 = 0.693147181f;
+  const float p = -g * kLog2e;
+  const float low = __builtin_fmaf(-g, kLog2e, -p) - g * kLog2eLow;
+  float e = __builtin_amdgcn_exp2f(p);
+  e = e > 0.f && e < __builtin_inff() ? __builtin_fmaf(e, low * kLn2, e) : e;
+  return g * __builtin_amdgcn_rcpf(1.0f + e);
+}
+
+__device__ __forceinline__ u32x2 swiglu4(const f32x4& g, const f32x4& u) {
+  return pack4_bf16(silu_fast(g[0]) * u[0], silu_fast(g[1]) * u[1], silu_fast(g[2]) * u[2], silu_fast(g[3]) * u[3]);
+}
 
 // Adds the waves' sums of slot t (a lane's 4 values of one fragment pair) in wave order.
 template <int SLOTS>
@@ -237,45 +270,29 @@ __device__ __forceinline__ f32x4 sum_waves(const f32x4* red, int t) {
   return v;
 }
 
-// 16 RI rows of one expert x 16 channels: gate and up fragment of the channels,
-// k steps shared by the waves. PAIR: blockIdx.y is the pair itself and the
-// workgroup quantises its row. Weights of an expert: gate then up, each nf
-// fragments x kt_n k steps; scales (2, nf / 8, kt_n).
-template <int RI, bool PAIR>
-__global__ __launch_bounds__(kThreads) void gate_up_kernel(
-    const bf16_t* __restrict__ x, int64_t ldx, int vec, int64_t h_n, const uint8_t* __restrict__ q,
-    const float* __restrict__ qs, const int* __restrict__ ids, const int* __restrict__ off,
-    const int* __restrict__ list, const uint8_t* __restrict__ wp, const float* __restrict__ ws,
-    bf16_t* __restrict__ h, int64_t t_n, int top_k, int experts, int kt_n, int nf) {
-  constexpr int PF = RI == 4 ? 2 : 4;
-  constexpr int kLds = PAIR ? kInlineCodes + 4 * kInlineCodes / kBlock : kWaves * RI * 2 * 64 * 16;
-  __shared__ __align__(16) uint8_t smem[kLds];
+// One pair x 16 channels: gate and up fragment of the channels, k steps shared by the
+// waves; the workgroup quantises the token's row. Weights of an expert: gate then up, each
+// nf fragments x kt_n k steps; scales (2, nf / 8, kt_n).
+__global__ __launch_bounds__(kThreads) void gate_up_pair_kernel(
+    const bf16_t* __restrict__ x, int64_t ldx, int vec, int64_t h_n, const int* __restrict__ ids,
+    const uint8_t* __restrict__ wp, const float* __restrict__ ws, bf16_t* __restrict__ h, int top_k, int experts,
+    int kt_n, int nf) {
+  constexpr int PF = 4;
+  __shared__ __align__(16) uint8_t smem[kInlineCodes + 4 * kInlineCodes / kBlock];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r16 = lane & 15, g = lane >> 4;
-  const int c = blockIdx.x % nf, tile = blockIdx.x / nf;
-  int e, row0, rows;
-  if constexpr (PAIR) {
-    row0 = tile;
-    rows = 1;
-    e = ids[tile];
-    if (e < 0 || e >= experts) return;
-  } else {
-    if (!find_tile(off, experts, 16 * RI, tile, &e, &row0, &rows)) return;
-  }
+  const int pair = blockIdx.x / nf, c = blockIdx.x % nf, e = ids[pair];
+  if (e < 0 || e >= experts) return;
   const int64_t matrix = (int64_t)nf * kt_n * 2048;
   const uint8_t* fg = wp + 2 * e * matrix + (int64_t)c * 2048;
   const float* sg = ws + ((int64_t)2 * e * (nf / 8) + c / 8) * kt_n;
   const int64_t sup = (int64_t)(nf / 8) * kt_n;
-  int64_t row[RI];
-#pragma unroll
-  for (int i = 0; i < RI; ++i) row[i] = PAIR ? 0 : list[row0 + min(16 * i + r16, rows - 1)] / top_k;
-  i32x8 wq[PF][2], xq[PF][RI];
-  float xs[PF][RI], wsc[PF][2];
+  float* scales = reinterpret_cast<float*>(smem + kInlineCodes);
+  i32x8 wq[PF][2];
+  float wsc[PF][2];
   const int mine = (kt_n - wave + kWaves - 1) / kWaves;
-  f32x4 acc[RI][2];
-#pragma unroll
-  for (int i = 0; i < RI; ++i) acc[i][0] = acc[i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int b = 0; b < mine || (PAIR && b == 0); b += PF) {
+  f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+  for (int b = 0; b < mine || b == 0; b += PF) {
 #pragma unroll
     for (int u = 0; u < PF; ++u)
       if (b + u < mine) {
@@ -286,54 +303,35 @@ __global__ __launch_bounds__(kThreads) void gate_up_kernel(
           wsc[u][j] = sg[j * sup + kt];
         }
       }
-    if constexpr (PAIR) {
-      if (b == 0) {
-        const bf16_t* src = x + (int64_t)(tile / top_k) * ldx;
-        for (int kt = threadIdx.x >> 4; kt < kt_n; kt += kThreads / 16) {
-          float scale;
-          const u32x2 code = quant_group16(src, h_n, kt, r16, vec, &scale);
-          *reinterpret_cast<u32x2*>(smem + kt * kBlock + 8 * r16) = code;
-          if (r16 == 0) reinterpret_cast<float*>(smem + kInlineCodes)[kt] = scale;
-        }
-        __syncthreads();
+    if (b == 0) {  // the first weights are in flight meanwhile
+      const bf16_t* src = x + (int64_t)(pair / top_k) * ldx;
+      for (int kt = threadIdx.x >> 4; kt < kt_n; kt += kThreads / 16) {
+        float scale;
+        const u32x2 code = quant_group16(src, h_n, kt, r16, vec, &scale);
+        *reinterpret_cast<u32x2*>(smem + kt * kBlock + 8 * r16) = code;
+        if (r16 == 0) scales[kt] = scale;
       }
+      __syncthreads();
     }
 #pragma unroll
     for (int u = 0; u < PF; ++u)
       if (b + u < mine) {
         const int kt = wave + kWaves * (b + u);
+        const i32x4v* p = reinterpret_cast<const i32x4v*>(smem + kt * kBlock + 32 * g);
+        const i32x8 xq = join(p[0], p[1]);
 #pragma unroll
-        for (int i = 0; i < RI; ++i) {
-          const uint8_t* src = PAIR ? smem + kt * kBlock : q + (row[i] * kt_n + kt) * kBlock;
-          const i32x4v* p = reinterpret_cast<const i32x4v*>(src + 32 * g);
-          xq[u][i] = join(p[0], p[1]);
-          xs[u][i] = PAIR ? reinterpret_cast<const float*>(smem + kInlineCodes)[kt] : qs[(int64_t)kt * t_n + row[i]];
-        }
-      }
-#pragma unroll
-    for (int u = 0; u < PF; ++u)
-      if (b + u < mine) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int i = 0; i < RI; ++i) fma4(acc[i][j], mfma_step(wq[u][j], xq[u][i]), xs[u][i] * wsc[u][j]);
+        for (int j = 0; j < 2; ++j) fma4(acc[j], mfma_step(wq[u][j], xq), scales[kt] * wsc[u][j]);
       }
   }
-  if constexpr (PAIR) __syncthreads();  // the codes are no longer read
-  constexpr int kSlots = RI * 2 * 64;
-  f32x4* red = reinterpret_cast<f32x4*>(smem);
+  __syncthreads();  // the codes are no longer read
+  f32x4* red = reinterpret_cast<f32x4*>(smem);  // every result row is the pair's: one lane of each group keeps it
+  if (r16 == 0)
 #pragma unroll
-  for (int i = 0; i < RI; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) red[wave * kSlots + (i * 2 + j) * 64 + lane] = acc[i][j];
+    for (int j = 0; j < 2; ++j) red[wave * 8 + 4 * j + g] = acc[j];
   __syncthreads();
-  if (threadIdx.x >= RI * 64) return;
-  const int i = threadIdx.x >> 6;
-  const f32x4 gate = sum_waves<kSlots>(red, i * 128 + lane), up = sum_waves<kSlots>(red, i * 128 + 64 + lane);
-  if (16 * i + r16 >= rows) return;
-  bf16_t* out = h + (int64_t)(row0 + 16 * i + r16) * (16 * nf) + 16 * c + 4 * g;
-  *reinterpret_cast<u32x2*>(out) = pack4_bf16(silu(gate[0]) * up[0], silu(gate[1]) * up[1], silu(gate[2]) * up[2],
-                                              silu(gate[3]) * up[3]);
+  if (threadIdx.x < 4)
+    *reinterpret_cast<u32x2*>(h + (int64_t)pair * (16 * nf) + 16 * c + 4 * threadIdx.x) =
+        swiglu4(sum_waves<8>(red, threadIdx.x), sum_waves<8>(red, 4 + threadIdx.x));
 }
 
 // ---------------------------------------------------------------- down
@@ -344,7 +342,7 @@ __device__ __forceinline__ void load_h(u32x4 (&x)[4], const bf16_t* p) {
   for (int u = 0; u < 4; ++u) x[u] = reinterpret_cast<const u32x4*>(p)[u];
 }
 
-// PAIR: one token's y, 16 channels: the k steps of all its experts shared by the
+// One token's y, 16 channels: the k steps of all its experts shared by the
 // waves. All 16 result rows are the token's (every lane group reads the same row).
 __global__ __launch_bounds__(kThreads) void down_pair_kernel(
     const bf16_t* __restrict__ h, const float* __restrict__ weights, const int* __restrict__ ids,
@@ -395,68 +393,80 @@ __global__ __launch_bounds__(kThreads) void down_pair_kernel(
   }
 }
 
-// 16 RI rows of one expert x 16 NJ channels, k steps shared by the waves; fp32
-// products to part[pair] (row stride ldp).
-template <int RI, int NJ>
-__global__ __launch_bounds__(kThreads) void down_kernel(const bf16_t* __restrict__ h, const int* __restrict__ off,
-                                                        const int* __restrict__ list, const uint8_t* __restrict__ wp,
-                                                        const float* __restrict__ ws, float* __restrict__ part,
-                                                        int64_t ldp, int64_t n, int experts, int kt_n, int nf,
-                                                        int tiles_n) {
-  constexpr int PF = 2;
-  constexpr int kSlots = RI * NJ * 64;
-  __shared__ f32x4 red[kWaves * kSlots];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// ---------------------------------------------------------------- row tiles
+
+// BM rows of one expert x 2 CW channels: wave w's fragments alternate gate and up of the
+// same 16 channels, so SwiGLU runs on the lane's own sums.
+template <int BM, int CW, int P>
+__global__ __launch_bounds__(kTileThreads, 2) void gate_up_tile_kernel(
+    const uint8_t* __restrict__ q, const float* __restrict__ qs, const int* __restrict__ off,
+    const int* __restrict__ list, const uint8_t* __restrict__ wp, const float* __restrict__ ws,
+    bf16_t* __restrict__ h, int64_t t_n, int top_k, int experts, int kt_n, int nf, int tiles_n) {
+  constexpr int RA = BM / 16, TJ = CW / 16;
+  static_assert(TJ % 2 == 0, "gate and up");
+  __shared__ __align__(1024) uint8_t smem[tile_smem<BM>()];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, g = lane >> 4;
-  const int f0 = blockIdx.x % tiles_n * NJ, tile = blockIdx.x / tiles_n;
-  int e, row0, rows;
-  if (!find_tile(off, experts, 16 * RI, tile, &e, &row0, &rows)) return;
+  ExpertTile at;
+  if (!find_tile(off, experts, BM, tiles_n, &at)) return;
+  const int e = at.expert, row0 = at.row0, rows = at.rows;
+  const int c0 = (at.col * 4 + wave) * (TJ / 2);  // the wave's first 16-channel block
+  const int64_t matrix = (int64_t)nf * kt_n * 2048;
+  const int64_t nb = nf / 8;
+  const float* scale = ws + (2 * e * nb + min(c0, nf - 1) / 8) * kt_n;
+  const uint8_t* gate = wp + 2 * e * matrix;
+  TileWeights<TJ, 2> w{{gate, gate + matrix}, (uint32_t)matrix, (uint32_t)nf * 2048u, {scale, scale + nb * kt_n}, {}};
+#pragma unroll
+  for (int j = 0; j < TJ; ++j) w.frag[j] = (uint32_t)(c0 + j / 2) * 2048u;
+  const uint32_t kp = (uint32_t)kt_n * kBlock;
+  const auto token = [&](int r) { return (uint32_t)(list[row0 + min(r, rows - 1)] / top_k); };
+  f32x4 acc[RA][TJ];
+  tile_mainloop<BM, CW, 2, P, 1>(
+      acc, smem, kt_n, 0, kt_n, q, (uint32_t)t_n * kp, [&](int r) { return token(r) * kp; }, qs, (uint32_t)(4 * t_n) * kt_n,
+      token, (uint32_t)(4 * t_n), w);
+#pragma unroll
+  for (int i = 0; i < RA; ++i) {
+    if (16 * i + r16 >= rows) continue;
+    bf16_t* out = h + (int64_t)(row0 + 16 * i + r16) * (16 * nf) + 4 * g;
+#pragma unroll
+    for (int j = 0; j < TJ; j += 2)
+      if (c0 + j / 2 < nf) *reinterpret_cast<u32x2*>(out + 16 * (c0 + j / 2)) = swiglu4(acc[i][j], acc[i][j + 1]);
+  }
+}
+
+// BM rows of one expert x 4 CW channels of the down product; fp32 to part[pair].
+template <int BM, int CW, int P>
+__global__ __launch_bounds__(kTileThreads, 2) void down_tile_kernel(
+    const bf16_t* __restrict__ h, const int* __restrict__ off, const int* __restrict__ list,
+    const uint8_t* __restrict__ wp, const float* __restrict__ ws, float* __restrict__ part, int64_t ldp, int64_t n,
+    int experts, int kt_n, int nf, int tiles_n) {
+  constexpr int RA = BM / 16, TJ = CW / 16;
+  __shared__ __align__(1024) uint8_t smem[tile_smem_bf16<BM>()];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r16 = lane & 15, g = lane >> 4;
+  ExpertTile at;
+  if (!find_tile(off, experts, BM, tiles_n, &at)) return;
+  const int e = at.expert, row0 = at.row0, rows = at.rows;
+  const int f0 = (at.col * 4 + wave) * TJ;
   const int64_t matrix = (int64_t)nf * kt_n * 2048;
   const int64_t nb = (n + kBlock - 1) / kBlock;
-  const int mine = (kt_n - wave + kWaves - 1) / kWaves;
-  f32x4 acc[RI][NJ];
+  TileWeights<TJ, 1> w{{wp + e * matrix}, (uint32_t)matrix, (uint32_t)nf * 2048u,
+                       {ws + (e * nb + min(f0, nf - 1) / 8) * kt_n}, {}};
 #pragma unroll
-  for (int i = 0; i < RI; ++i)
+  for (int j = 0; j < TJ; ++j) w.frag[j] = (uint32_t)(f0 + j) * 2048u;
+  const uint32_t kp = (uint32_t)kt_n * (2 * kBlock);
+  f32x4 acc[RA][TJ];
+  tile_mainloop_bf16<BM, CW, P>(acc, smem, kt_n, reinterpret_cast<const uint8_t*>(h) + (int64_t)row0 * kp,
+                                (uint32_t)rows * kp, [&](int r) { return (uint32_t)min(r, rows - 1) * kp; }, w);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int b = 0; b < mine; b += PF) {
-    i32x8 wq[PF][NJ];
-    u32x4 xh[PF][RI][4];
-    float s[PF][NJ];
+  for (int i = 0; i < RA; ++i) {
+    if (16 * i + r16 >= rows) continue;
+    float* out = part + (int64_t)list[row0 + 16 * i + r16] * ldp;
 #pragma unroll
-    for (int u = 0; u < PF; ++u)
-      if (b + u < mine) {
-        const int kt = wave + kWaves * (b + u);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          const int f = min(f0 + j, nf - 1);
-          wq[u][j] = load_frag(wp + e * matrix + ((int64_t)kt * nf + f) * 2048, lane);
-          s[u][j] = ws[((int64_t)e * nb + f / 8) * kt_n + kt];
-        }
-#pragma unroll
-        for (int i = 0; i < RI; ++i)
-          load_h(xh[u][i], h + ((int64_t)(row0 + min(16 * i + r16, rows - 1)) * kt_n + kt) * kBlock + 32 * g);
-      }
-#pragma unroll
-    for (int u = 0; u < PF; ++u)
-      if (b + u < mine) {
-#pragma unroll
-        for (int j = 0; j < NJ; ++j)
-#pragma unroll
-          for (int i = 0; i < RI; ++i) fma4(acc[i][j], mfma_step_bf16(wq[u][j], xh[u][i]), s[u][j]);
-      }
-  }
-#pragma unroll
-  for (int i = 0; i < RI; ++i)
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) red[wave * kSlots + (i * NJ + j) * 64 + lane] = acc[i][j];
-  __syncthreads();
-  for (int t = threadIdx.x; t < kSlots; t += kThreads) {
-    const f32x4 v = sum_waves<kSlots>(red, t);
-    const int l = t & 63, i = t / 64 / NJ, j = t / 64 % NJ;
-    const int r = 16 * i + (l & 15);
-    const int64_t c = 16 * (int64_t)(f0 + j) + 4 * (l >> 4);
-    if (r < rows && c < n) *reinterpret_cast<f32x4*>(part + (int64_t)list[row0 + r] * ldp + c) = v;
+    for (int j = 0; j < TJ; ++j) {
+      const int64_t c = 16 * (int64_t)(f0 + j) + 4 * g;
+      if (c < n) *reinterpret_cast<f32x4*>(out + c) = acc[i][j];
+    }
   }
 }
 
@@ -486,8 +496,12 @@ struct Shape {
   int64_t pairs() const { return t * top_k; }
   int kth() const { return (int)((h + kBlock - 1) / kBlock); }
   int kti() const { return (int)((i + kBlock - 1) / kBlock); }
-  // Up to this many pairs they are taken one by one.
-  bool by_pair() const { return pairs() <= 64 && (int64_t)kth() * kBlock <= kInlineCodes; }
+  // Up to 32 pairs they are taken one by one (128 experts, 8 a token, h 2048, i 768, us: 4 tokens
+  // 36.9 against 40.0 on tiles, 8 tokens 68.8 against 54.0).
+  bool by_pair() const {
+    const int tune = ff_tuning(FF_TUNE_MOE_TILE);
+    return (tune ? tune == 1 && t < (1 << 16) : pairs() <= 32) && (int64_t)kth() * kBlock <= kInlineCodes;
+  }
 };
 
 int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
@@ -515,32 +529,31 @@ struct Layout {
   }
 };
 
-// Bounds under which every grid below stays under 2^32 threads: the row tiles of
+// Bounds under which the rows' codes stay under 2^32 bytes and every grid below stays under 2^32 threads: the row tiles of
 // either product (16 rows at least, one more for each expert) times its columns.
 int check_shape(const char* who, int64_t t, int64_t top_k, int64_t experts, int64_t h, int64_t i) {
   FF_REQUIRE(t >= 0 && top_k > 0 && experts > 0 && experts <= kMaxExperts && h > 0 && i > 0 && h <= (1 << 24) &&
                  i <= (1 << 24) && top_k <= 1024 && t < (1 << 21) &&
-                 (t * top_k / 16 + experts) * ((h > i ? h : i) / 16 + 8) < (1 << 23),
+                 t * ((h + kBlock - 1) / kBlock) < (1 << 25) && (t * top_k / 16 + experts) * ((h > i ? h : i) / 16 + 8) < (1 << 23),
              "%s: bad sizes t=%lld top_k=%lld experts=%lld h=%lld i=%lld", who, (long long)t, (long long)top_k,
              (long long)experts, (long long)h, (long long)i);
   return FF_OK;
 }
 
-template <int RI>
-void launch_experts(const Shape& s, uint8_t* w, const Layout& l, const void* gate_up, const float* gate_up_scales,
-                    const void* down, const float* down_scales, hipStream_t st) {
-  const int64_t tiles = s.pairs() / (16 * RI) + (s.pairs() < s.experts ? s.pairs() : s.experts);
+template <int BM, int CWG, int PG, int CWD, int PD>
+void launch_tiles(const Shape& s, uint8_t* w, const Layout& l, const void* gate_up, const float* gate_up_scales,
+                  const void* down, const float* down_scales, hipStream_t st) {
+  const int tiles = (int)(s.pairs() / BM + (s.pairs() < s.experts ? s.pairs() : s.experts));
   const int nfi = s.kti() * 8, nfh = (int)((s.h + 15) / 16);
   const int* off = (const int*)(w + l.off);
   const int* list = (const int*)(w + l.list);
-  hipLaunchKernelGGL((gate_up_kernel<RI, false>), dim3((unsigned)(tiles * nfi)), dim3(kThreads), 0, st, nullptr, 0, 0,
-                     s.h, w + l.q, (const float*)(w + l.qs), nullptr, off, list, (const uint8_t*)gate_up,
-                     gate_up_scales, (bf16_t*)(w + l.h), s.t, s.top_k, s.experts, s.kth(), nfi);
-  constexpr int NJ = 2;
-  const int tn = (nfh + NJ - 1) / NJ;
-  hipLaunchKernelGGL((down_kernel<RI, NJ>), dim3((unsigned)(tiles * tn)), dim3(kThreads), 0, st,
+  const int tg = (nfi + CWG / 8 - 1) / (CWG / 8), td = (nfh + CWD / 4 - 1) / (CWD / 4);
+  hipLaunchKernelGGL((gate_up_tile_kernel<BM, CWG, PG>), dim3((unsigned)(tiles * tg)), dim3(kTileThreads), 0, st,
+                     w + l.q, (const float*)(w + l.qs), off, list, (const uint8_t*)gate_up, gate_up_scales,
+                     (bf16_t*)(w + l.h), s.t, s.top_k, s.experts, s.kth(), nfi, tg);
+  hipLaunchKernelGGL((down_tile_kernel<BM, CWD, PD>), dim3((unsigned)(tiles * td)), dim3(kTileThreads), 0, st,
                      (const bf16_t*)(w + l.h), off, list, (const uint8_t*)down, down_scales, (float*)(w + l.part),
-                     l.ldp, s.h, s.experts, s.kti(), nfh, tn);
+                     l.ldp, s.h, s.experts, s.kti(), nfh, td);
 }
 
 }  // namespace
@@ -605,9 +618,9 @@ extern "C" int ff_moe_experts(const void* x, int64_t ldx, const float* weights, 
   const int nfi = s.kti() * 8, nfh = (int)((h + 15) / 16);
   const int vec = ff_aligned(x, 16) && ldx % 8 == 0;
   if (s.by_pair()) {
-    hipLaunchKernelGGL((gate_up_kernel<1, true>), dim3((unsigned)(s.pairs() * nfi)), dim3(kThreads), 0, st,
-                       (const bf16_t*)x, ldx, vec, h, nullptr, nullptr, ids, nullptr, nullptr, (const uint8_t*)gate_up,
-                       gate_up_scales, (bf16_t*)(w + l.h), t, (int)top_k, (int)experts, s.kth(), nfi);
+    hipLaunchKernelGGL(gate_up_pair_kernel, dim3((unsigned)(s.pairs() * nfi)), dim3(kThreads), 0, st, (const bf16_t*)x,
+                       ldx, vec, h, ids, (const uint8_t*)gate_up, gate_up_scales, (bf16_t*)(w + l.h), (int)top_k,
+                       (int)experts, s.kth(), nfi);
     hipLaunchKernelGGL(down_pair_kernel, dim3((unsigned)(t * nfh)), dim3(kThreads), 0, st, (const bf16_t*)(w + l.h),
                        weights, ids, (const uint8_t*)down, down_scales, (bf16_t*)y, ldy, h, (int)top_k, (int)experts,
                        s.kti(), nfh);
@@ -618,10 +631,14 @@ extern "C" int ff_moe_experts(const void* x, int64_t ldx, const float* weights, 
                      (int*)(w + l.off), (int*)(w + l.list));
   const int rq = quant_rows_block(x, ldx, w + l.q, (float*)(w + l.qs), t, h, st);
   if (rq != FF_OK) return rq;
-  const int64_t per = s.pairs() / experts;  // rows of an expert on average
-  if (per <= 16) launch_experts<1>(s, w, l, gate_up, gate_up_scales, down, down_scales, st);
-  else if (per <= 32) launch_experts<2>(s, w, l, gate_up, gate_up_scales, down, down_scales, st);
-  else launch_experts<4>(s, w, l, gate_up, gate_up_scales, down, down_scales, st);
+  // Rows of an expert on average: with few, tiles of 32 rows (us on 32- and 64-row tiles, 128
+  // experts, 8 a token, h 2048, i 768: 8 tokens 54.0 and 61.7, 32 tokens 101 and 111, 128 tokens
+  // 122 and 121, 512 tokens 163 and 155, 4096 tokens 581 and 429).
+  const int tune = ff_tuning(FF_TUNE_MOE_TILE);
+  if (tune ? tune == 2 : s.pairs() / experts < 8)
+    launch_tiles<32, 32, 3, 32, 2>(s, w, l, gate_up, gate_up_scales, down, down_scales, st);
+  else
+    launch_tiles<64, 64, 3, 64, 1>(s, w, l, gate_up, gate_up_scales, down, down_scales, st);
   const int64_t grid = (t * (l.ldp / 4) + 255) / 256;
   hipLaunchKernelGGL(combine_kernel, dim3((unsigned)(grid < (1 << 20) ? grid : (1 << 20))), dim3(256), 0, st,
                      (const float*)(w + l.part), l.ldp, weights,

@@ -22,11 +22,12 @@ Weight quantization runs once on the GPU at construction. All calls allocate
 their outputs with torch.empty and launch on the current stream.
 """
 import ctypes
+import functools
 import types
 
 import torch
 
-from ._lib import call, ptr, stream
+from ._lib import call, entry, ptr, stream
 
 E4M3 = torch.float8_e4m3fn
 BF16 = torch.bfloat16
@@ -368,8 +369,16 @@ def check_block_codes(codes, scales, dims):
 def check_here(*tensors):
     """Launches go to the current device's stream: every tensor has to live there."""
     for t in tensors:
-        assert t.is_cuda, f"tensor on {t.device}"
-        assert t.get_device() == torch._C._cuda_getDevice(), f"tensor on {t.device}, which is not the current device"
+        assert t.is_cuda and t.get_device() == torch._C._cuda_getDevice(), \
+            f"tensor on {t.device}, which is not the current GPU"
+
+
+@functools.lru_cache(maxsize=1024)
+def block_workspace(m, n, k):
+    """Bytes of workspace ff_linear_fp8_block needs (0: none)."""
+    need = ctypes.c_int64(0)
+    call("ff_linear_fp8_block_workspace", m, n, k, ctypes.byref(need))
+    return need.value
 
 
 class BlockFP8Linear:
@@ -408,7 +417,7 @@ class BlockFP8Linear:
     def _rows2d(self, x):
         assert x.dtype == BF16 and x.shape[-1] == self.weight.shape[1]
         check_here(x, self.scale)
-        flat = x.reshape(-1, x.shape[-1])
+        flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
         return flat if flat.stride(-1) == 1 or flat.shape[-1] == 1 else flat.contiguous()
 
     def quantize(self, x):
@@ -422,7 +431,8 @@ class BlockFP8Linear:
         return q, s
 
     def gemm(self, q, s):
-        """The product from rows quantised by ``quantize``: the bits of ``op(x)``."""
+        """The product from rows quantised by ``quantize``: the bits of ``op(x)`` for more rows
+        than run in one launch (four)."""
         n, k = self.weight.shape
         m = q.shape[0]
         assert q.dtype == E4M3 and q.shape[1] == _blocks(k) * BLOCK and q.is_contiguous()
@@ -436,13 +446,12 @@ class BlockFP8Linear:
         flat = self._rows2d(x)
         m, k = flat.shape
         n = self.weight.shape[0]
-        y = torch.empty((*x.shape[:-1], n), device=x.device, dtype=BF16)
-        need = ctypes.c_int64(0)
-        call("ff_linear_fp8_block_workspace", m, n, k, ctypes.byref(need))
-        ws = torch.empty(need.value, device=x.device, dtype=torch.uint8) if need.value else None
-        call("ff_linear_fp8_block", ptr(flat), flat.stride(0), ptr(self.packed), ptr(self.scale), ptr(y), n, m, n, k,
-             ptr(ws), need.value, stream())
-        return y
+        y = x.new_empty((m, n))
+        need = block_workspace(m, n, k)
+        ws = x.new_empty((need,), dtype=torch.uint8) if need else None
+        entry("ff_linear_fp8_block")(flat.data_ptr(), flat.stride(0), self.packed.data_ptr(), self.scale.data_ptr(),
+                                     y.data_ptr(), n, m, n, k, ws.data_ptr() if need else 0, need, stream())
+        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], n)
 
 
 class Int4:

@@ -11,10 +11,11 @@ any launch, outputs are fresh tensors, inputs are never written, launches go to 
 current stream and can be captured (no host sync, no device-dependent grid).
 """
 import ctypes
+import functools
 
 import torch
 
-from ._lib import call, ptr, stream
+from ._lib import call, entry, ptr, stream
 from .linear import BF16, _blocks, check_block_codes, check_here, pack_blocks
 
 F32, I32 = torch.float32, torch.int32
@@ -48,11 +49,20 @@ def route(logits, top_k, score="softmax", bias=None, groups=1, top_groups=None, 
         check_here(bias)
     if logits.stride(-1) != 1 and e > 1:
         logits = logits.contiguous()
-    weights = torch.empty((t, top_k), device=logits.device, dtype=F32)
-    ids = torch.empty((t, top_k), device=logits.device, dtype=I32)
-    call("ff_moe_route", ptr(logits), int(logits.dtype == F32), logits.stride(0), ptr(bias), ptr(weights), ptr(ids), t,
-         e, top_k, int(score == "sigmoid"), groups, top_groups, int(bool(renormalize)), float(scale), stream())
+    weights = logits.new_empty((t, top_k), dtype=F32)
+    ids = logits.new_empty((t, top_k), dtype=I32)
+    entry("ff_moe_route")(logits.data_ptr(), logits.dtype == F32, logits.stride(0), 0 if bias is None else bias.data_ptr(),
+                          weights.data_ptr(), ids.data_ptr(), t, e, top_k, score == "sigmoid", groups, top_groups,
+                          bool(renormalize), scale, stream())
     return weights, ids
+
+
+@functools.lru_cache(maxsize=1024)
+def experts_workspace(t, top_k, experts, h, i):
+    """Bytes of workspace ff_moe_experts needs."""
+    need = ctypes.c_int64(0)
+    call("ff_moe_experts_workspace", t, top_k, experts, h, i, ctypes.byref(need))
+    return need.value
 
 
 class Experts:
@@ -110,13 +120,13 @@ class Experts:
         if x.stride(-1) != 1 and h > 1:
             x = x.contiguous()
         top_k = ids.shape[1]
-        y = torch.empty((t, h), device=x.device, dtype=BF16)
-        need = ctypes.c_int64(0)
-        call("ff_moe_experts_workspace", t, top_k, self.experts, h, self.inter, ctypes.byref(need))
-        ws = torch.empty(need.value, device=x.device, dtype=torch.uint8)
-        call("ff_moe_experts", ptr(x), x.stride(0), ptr(weights), ptr(ids), ptr(self.gate_up._packed),
-             ptr(self.gate_up_scale), ptr(self.down._packed), ptr(self.down_scale), ptr(y), h, t, top_k, self.experts,
-             h, self.inter, ptr(ws), need.value, stream())
+        y = x.new_empty((t, h))
+        need = experts_workspace(t, top_k, self.experts, h, self.inter)
+        ws = x.new_empty((need,), dtype=torch.uint8)
+        entry("ff_moe_experts")(x.data_ptr(), x.stride(0), weights.data_ptr(), ids.data_ptr(),
+                                self.gate_up._packed.data_ptr(), self.gate_up_scale.data_ptr(),
+                                self.down._packed.data_ptr(), self.down_scale.data_ptr(), y.data_ptr(), h, t, top_k,
+                                self.experts, h, self.inter, ws.data_ptr(), need, stream())
         return y
 
 

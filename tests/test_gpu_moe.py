@@ -160,6 +160,26 @@ def test_experts(gpu, t, k, e, h, i):
 
 
 @gpu_test
+@pytest.mark.parametrize("tile", [1, 2, 3])
+@pytest.mark.parametrize("t,k,e,h,i", EXPERT_CASES)
+def test_every_path(gpu, t, k, e, h, i, tile):
+    """Pair by pair, 32- and 64-row tiles, at sizes that another would be chosen for."""
+    from fastforward_amd import moe
+    from fastforward_amd._lib import call
+    codes = _weights(e, h, i)
+    x, w, ids = _tokens(t, k, e, h)
+    op = _experts(codes)
+    call("ff_set_tuning", 13, tile)
+    moe.experts_workspace.cache_clear()
+    try:
+        y = op(x.to(DEV), w.to(DEV), ids.to(DEV))
+    finally:
+        call("ff_set_tuning", 13, 0)
+        moe.experts_workspace.cache_clear()
+    _check(y, x, w, ids, codes)
+
+
+@gpu_test
 @pytest.mark.parametrize("t,k,e,h,i", [(1, 8, 128, 2048, 768), (48, 4, 64, 2560, 1024), (300, 5, 12, 2120, 1000),
                                        (1024, 8, 16, 2048, 768)])
 def test_experts_at_model_sizes(gpu, t, k, e, h, i):
