@@ -14,11 +14,11 @@ Two bundle architectures:
   ``checkpoint_sha256`` (the repair adapter; only the identity -- all-zero --
   adapter the reference's family runtime accepts), ``profile_path`` +
   ``profile_sha256`` (static FP8 calibration), plus ``linear`` to pick the
-  linear format ('fp8' per-token dynamic, 'fp8_static', 'w4a16', 'int4').
+  linear format ('fp8' per-token dynamic, 'fp8_static', 'fp8_block', 'w4a16', 'int4').
 * ``"qwen3_vl_lm"`` -- synthetic weights of a named LM preset, requests as
   token ids (``predict_tokens``): ``{"schema_version": 1, "task":
   "visual_choice", "architecture": "qwen3_vl_lm", "preset": "qwen3vl-8b",
-  "linear": "fp8" | "fp8_static" | "w4a16", "seed": 0, "tokens": 576,
+  "linear": "fp8" | "fp8_static" | "fp8_block" | "w4a16", "seed": 0, "tokens": 576,
   "image_grid": [16, 32], "prefix_tokens": 4, "buckets": [576]}``;
   ``buckets`` defaults to ``[tokens]``. With ``linear: "fp8_static"`` a bundle
   may name a calibration profile (``profile_path``, ``profile_sha256``,
@@ -31,7 +31,7 @@ import threading
 from pathlib import Path
 
 BACKENDS = ("fast", "native", "established")
-LINEAR_MODES = ("fp8", "fp8_static", "w4a16", "int4")
+LINEAR_MODES = ("fp8", "fp8_static", "fp8_block", "w4a16", "int4")
 ARCHITECTURES = ("qwen3_vl_lm", "qwen3_vl_family")
 
 

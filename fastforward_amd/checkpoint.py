@@ -8,7 +8,10 @@ into four FP8 linears -- q/k/v and gate/up concatenated row-wise -- and
 releases the bf16 copies. Here the tensors are read one at a time from the
 safetensors files (one file or an index of shards), moved to the GPU in bf16
 and quantised there by the linear ops (``FP8Linear`` / ``RuntimeScaleLinear``
-/ ``Int4``); no bf16 copy of a linear outlives its quantisation. The vision
+/ ``Int4`` / ``BlockFP8Linear``); no bf16 copy of a linear outlives its
+quantisation. Block-scaled FP8 checkpoints (e4m3 weights with a
+``weight_scale_inv`` of one scale per 128 x 128 block beside them) load as they
+are in the ``fp8_block`` mode and dequantised in the others. The vision
 tower keeps bf16 weights (its MLP intermediate zero-padded to a multiple of
 64). The choice head is the rows of ``lm_head`` (or of the tied embedding)
 at the option token ids, as the reference slices it
@@ -19,7 +22,7 @@ import os
 
 import torch
 
-from .linear import MIXED_MODES, FP8Linear, Int4, RuntimeScaleLinear, bank_of
+from .linear import BLOCK, E4M3, MIXED_MODES, BlockFP8Linear, FP8Linear, Int4, RuntimeScaleLinear, bank_of
 from .ops import RMSNorm
 from .runtime import LayerWeights, LMConfig, ModelWeights
 from .vision import Lin, Norm, VBlock, VisionConfig, VisionWeights, VMerger, pad_mlp
@@ -49,13 +52,32 @@ class Tensors:
     def __contains__(self, name):
         return name in self.where
 
-    def get(self, name, device="cuda"):
+    def raw(self, name, device="cuda"):
+        """The tensor in its own type."""
         if name not in self.where:
             raise KeyError(f"checkpoint has no tensor {name!r}")
         fn = self.where[name]
         if fn not in self._files:
             self._files[fn] = self._open(fn, "pt")
-        return self._files[fn].get_tensor(name).to(device=device, dtype=BF16).contiguous()
+        return self._files[fn].get_tensor(name).to(device=device).contiguous()
+
+    def blocks(self, name, device="cuda"):
+        """(codes, block scales fp32) of a block-scaled FP8 weight, None for another."""
+        if name + "_scale_inv" not in self.where:
+            return None
+        codes, scales = self.raw(name, device), self.raw(name + "_scale_inv", device).float()
+        want = tuple(-(-n // BLOCK) for n in codes.shape)
+        if codes.dtype != E4M3 or tuple(scales.shape) != want:
+            raise ValueError(f"{name}: {codes.dtype} with scales {tuple(scales.shape)}, expected e4m3 with {want}")
+        return codes, scales
+
+    def get(self, name, device="cuda"):
+        block = self.blocks(name, device)
+        if block is None:
+            return self.raw(name, device).to(BF16)
+        codes, scales = block
+        n, k = codes.shape
+        return (codes.float() * scales.repeat_interleave(BLOCK, 0)[:n].repeat_interleave(BLOCK, 1)[:, :k]).to(BF16)
 
 
 def read_config(path):
@@ -99,11 +121,24 @@ def _linear(w, mode, static_bound, oracle=False):
         return FP8Linear(w)
     if mode == "fp8_static":
         return RuntimeScaleLinear(w, 448.0 / static_bound)
+    if mode == "fp8_block":
+        return BlockFP8Linear(w)
     if mode == "w4a16":
         return Int4(w, oracle=oracle)
     if mode == "int4":      # the reference's asymmetric group-32 quantizer
         return Int4(w, group=32, symmetric=False, oracle=oracle)
     raise ValueError(f"unknown linear mode {mode!r}")
+
+
+def _block_linear(ts, names, device):
+    """BlockFP8Linear of the row-wise concatenation of a checkpoint's block-scaled weights
+    as they are; None where one is not block-scaled, or its rows end inside a block and
+    another follows (its blocks would not be blocks of the concatenation)."""
+    parts = [ts.blocks(name, device) for name in names]
+    if any(p is None for p in parts) or any(codes.shape[0] % BLOCK for codes, _ in parts[:-1]):
+        return None
+    return BlockFP8Linear.from_codes(torch.cat([c.view(torch.uint8) for c, _ in parts]).view(E4M3),
+                                     torch.cat([s for _, s in parts]))
 
 
 def load_lm(path, cfg, option_ids, mode="fp8", device="cuda", static_bound=8.0, tensors=None, fp8_bank="fp8"):
@@ -117,25 +152,24 @@ def load_lm(path, cfg, option_ids, mode="fp8", device="cuda", static_bound=8.0, 
     embed = ts.get(p + "embed_tokens.weight", device)
     layers = []
 
-    def lin(w, j, role):
+    def lin(names, j, role):
         # the middle layer's int4 QKV carries the operator check, as pack_release
         # builds it (_family/night_runtime.py:77)
         oracle = j == cfg.layers // 2 and role == "qkv"
+        op = _block_linear(ts, names, device) if mode == "fp8_block" else None
+        if op is not None:
+            return op
+        w = [ts.get(name, device) for name in names]
+        w = torch.cat(w) if len(w) > 1 else w[0]
         if mode in MIXED_MODES:
             bank = "int4" if bank_of(mode, j, cfg.layers, role) == "int4" else fp8_bank
             return _linear(w, bank, static_bound, oracle)
         return _linear(w, mode, static_bound, oracle)
     for j in range(cfg.layers):
         q = f"{p}layers.{j}."
-        ops = {}
-        w = torch.cat([ts.get(q + f"self_attn.{x}_proj.weight", device) for x in "qkv"])
-        ops["qkv"] = lin(w, j, "qkv")
-        del w
-        ops["o"] = lin(ts.get(q + "self_attn.o_proj.weight", device), j, "o")
-        w = torch.cat([ts.get(q + f"mlp.{x}_proj.weight", device) for x in ("gate", "up")])
-        ops["gateup"] = lin(w, j, "gateup")
-        del w
-        ops["down"] = lin(ts.get(q + "mlp.down_proj.weight", device), j, "down")
+        names = {"qkv": [q + f"self_attn.{x}_proj.weight" for x in "qkv"], "o": [q + "self_attn.o_proj.weight"],
+                 "gateup": [q + f"mlp.{x}_proj.weight" for x in ("gate", "up")], "down": [q + "mlp.down_proj.weight"]}
+        ops = {role: lin(names[role], j, role) for role in names}
         layers.append(LayerWeights(
             input_norm=RMSNorm(ts.get(q + "input_layernorm.weight", device), cfg.eps),
             post_norm=RMSNorm(ts.get(q + "post_attention_layernorm.weight", device), cfg.eps),

@@ -28,155 +28,193 @@ constexpr int kInlineCodes = 49152;  // codes of the row that a gate_up workgrou
 
 // ---------------------------------------------------------------- routing
 
-constexpr int kRouteRows = 4;  // rows (one wave each) per workgroup
+constexpr int kRouteWaves = 4;
 
-template <int CTRL>
-__device__ __forceinline__ double dpp64(double x) {
-  const uint64_t u = __builtin_bit_cast(uint64_t, x);
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xF, 0xF, false);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, false);
-  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+template <int CTRL, typename T>
+__device__ __forceinline__ T dpp_of(T x) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(
+        T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xF, 0xF, false));
+  } else {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xF, 0xF, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, false);
+    return __builtin_bit_cast(T, (uint64_t)hi << 32 | lo);
+  }
 }
 
-// f over the 64 lanes, the same bits in every lane (each step combines a lane with its partner).
-template <typename F>
-__device__ __forceinline__ double wave_reduce64(double v, F&& f) {
-  v = f(v, dpp64<kDppXor1>(v));
-  v = f(v, dpp64<kDppXor2>(v));
-  v = f(v, dpp64<kDppHalfMirror>(v));
-  v = f(v, dpp64<kDppRowMirror>(v));
-  v = f(v, __shfl_xor(v, 16));
-  return f(v, __shfl_xor(v, 32));
+// The value of lane l ^ D, D 16 or 32: both results of a row swap, of which one is the lane's own.
+template <int D>
+__device__ __forceinline__ uint32_t swap32(uint32_t x) {
+  if constexpr (D == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return (threadIdx.x & 32) ? r[0] : r[1];
+  } else {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return (threadIdx.x & 16) ? r[0] : r[1];
+  }
+}
+template <int D, typename T>
+__device__ __forceinline__ T swap_of(T x) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, swap32<D>(__builtin_bit_cast(uint32_t, x)));
+  } else {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    return __builtin_bit_cast(T, (uint64_t)swap32<D>((uint32_t)(u >> 32)) << 32 | swap32<D>((uint32_t)u));
+  }
 }
 
-// One wave per row; lane l holds experts l, l + 64, ... Scores, sums and the
-// comparisons between experts are 64-bit: in 32 bits, scores that lie next to
-// each other change places with the last bit of exp().
-template <int EPL, bool F32>
-__global__ __launch_bounds__(64 * kRouteRows) void route_kernel(
+// f over LPR (16 or 64) lanes, the same bits in each (every step combines a lane with its partner).
+template <int LPR, typename T, typename F>
+__device__ __forceinline__ T reduce(T v, F&& f) {
+  v = f(v, dpp_of<kDppXor1>(v));
+  v = f(v, dpp_of<kDppXor2>(v));
+  v = f(v, dpp_of<kDppHalfMirror>(v));
+  v = f(v, dpp_of<kDppRowMirror>(v));
+  if constexpr (LPR == 64) {
+    v = f(v, swap_of<16>(v));
+    v = f(v, swap_of<32>(v));
+  }
+  return v;
+}
+
+// exp(x) to about 1e-14 of its value: 2^k exp(r), k = rint(x / ln 2), |r| <= ln 2 / 2, and
+// the Taylor polynomial of degree 11 (its next term is below 7e-15).
+__device__ __forceinline__ double exp64(double x) {
+  if (x < -746.0) return 0.0;
+  if (x > 710.0) return __builtin_inf();
+  const double k = __builtin_rint(x * 1.4426950408889634);
+  double r = __builtin_fma(-k, 6.93147180369123816490e-01, x);  // ln 2: the leading 33 bits, then the rest
+  r = __builtin_fma(-k, 1.90821492927058770002e-10, r);
+  double p = 1.0 / 39916800;
+  constexpr double kInv[11] = {1.0, 1.0, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320,
+                               1.0 / 362880, 1.0 / 3628800};
+#pragma unroll
+  for (int i = 10; i >= 0; --i) p = __builtin_fma(p, r, kInv[i]);
+  return __builtin_ldexp(p, (int)k);
+}
+
+// LPR lanes per row; lane l of them holds experts l, l + LPR, ... Without a bias experts are
+// compared by their logits (scores rise with them); with one by score + bias in 64 bits: in 32,
+// scores that lie next to each other would change places with the last bit of exp(). Sums and
+// weights are 64-bit until their one rounding.
+// Bound by instructions, not by its few bytes. 16 lanes for many rows (16387 x 160, softmax, 5
+// groups: 31 us with 64 lanes and library exponentials for every comparison), 64 for few.
+template <int LPR, int EPL, bool F32, bool BIAS>
+__global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(
     const void* __restrict__ logits, int64_t ld, const float* __restrict__ bias, float* __restrict__ weights,
     int* __restrict__ ids, int64_t t, int experts, int top_k, int sigmoid, int groups, int top_groups, int renormalize,
     float scale) {
-  __shared__ double sc[kRouteRows][EPL * 64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t row = blockIdx.x * (int64_t)kRouteRows + wave;
-  if (row >= t) return;  // waves share nothing: LDS rows are per wave
-  const double kNone = -__builtin_inf();
-  const auto maximum = [](double a, double b) { return a > b ? a : b; };
-  double p[EPL], c[EPL];
+  using Key = std::conditional_t<BIAS, double, float>;
+  constexpr int kRows = 64 / LPR;  // rows of a wave
+  __shared__ Key sc[kRouteWaves * kRows][LPR * EPL];
+  __shared__ Key best_of[kRouteWaves * kRows][64];
+  const int lane = threadIdx.x & 63, li = lane % LPR, slot = threadIdx.x / LPR;
+  const int64_t row = blockIdx.x * (int64_t)(kRouteWaves * kRows) + slot;
+  const bool live = row < t;  // rows past the end are worked on as all-off ones: every lane takes part in every step
+  const Key kNone = -(Key)__builtin_inf();
+  const auto larger = [](auto a, auto b) { return a > b ? a : b; };
+  const auto load = [&](int e) {
+    if constexpr (F32) return reinterpret_cast<const float*>(logits)[row * ld + e];
+    else return bf16_to_f32(reinterpret_cast<const bf16_t*>(logits)[row * ld + e]);
+  };
+  float l[EPL];
   bool bad = false;
-  double top = kNone;
+  float top = -__builtin_inff();
 #pragma unroll
   for (int v = 0; v < EPL; ++v) {
-    const int e = lane + 64 * v;
-    float l = -__builtin_inff();
-    if (e < experts) {
-      if constexpr (F32) l = reinterpret_cast<const float*>(logits)[row * ld + e];
-      else l = bf16_to_f32(reinterpret_cast<const bf16_t*>(logits)[row * ld + e]);
-    }
-    bad |= l != l || (!sigmoid && l == __builtin_inff());
-    p[v] = (double)l;
-    top = maximum(top, p[v]);
+    const int e = li + LPR * v;
+    l[v] = live && e < experts ? load(e) : -__builtin_inff();
+    bad |= l[v] != l[v] || (!sigmoid && l[v] == __builtin_inff());
+    top = larger(top, l[v]);
   }
-  if (sigmoid) {
-#pragma unroll
-    for (int v = 0; v < EPL; ++v) {
-      c[v] = p[v];
-      p[v] = 1.0 / (1.0 + exp(-p[v]));
-    }
-  } else {
-    top = wave_reduce64(top, maximum);
+  double inv = 0;  // 1 / the softmax's sum
+  if (!sigmoid) {
+    top = reduce<LPR>(top, larger);
     double sum = 0;
 #pragma unroll
-    for (int v = 0; v < EPL; ++v) {
-      c[v] = p[v];
-      p[v] = p[v] == kNone ? 0.0 : exp(p[v] - top);
-      sum += p[v];
-    }
-    sum = wave_reduce64(sum, [](double a, double b) { return a + b; });
-#pragma unroll
-    for (int v = 0; v < EPL; ++v) p[v] = sum > 0 ? p[v] / sum : 0.0;
+    for (int v = 0; v < EPL; ++v)
+      if (LPR * v < experts) sum += l[v] == -__builtin_inff() ? 0.0 : exp64((double)l[v] - (double)top);
+    sum = reduce<LPR>(sum, [](double a, double b) { return a + b; });
+    inv = sum > 0 ? 1.0 / sum : 0.0;
   }
-  // choice score: -inf for experts that are switched off
+  const auto score = [&](float x) {
+    return sigmoid ? 1.0 / (1.0 + exp64(-(double)x)) : exp64((double)x - (double)top) * inv;
+  };
+  Key c[EPL];  // what experts are compared by; -inf for those switched off
 #pragma unroll
   for (int v = 0; v < EPL; ++v) {
-    const int e = lane + 64 * v;
-    const bool off = c[v] == kNone;
-    const double b = bias && e < experts ? (double)bias[e] : 0.0;
-    bad |= b != b;
-    c[v] = off ? kNone : p[v] + b;
-  }
-  int* out_id = ids + row * top_k;
-  float* out_w = weights + row * top_k;
-  if (__ballot(bad)) {  // a NaN (or a softmax over +inf) shows in every weight of the row
-    for (int j = lane; j < top_k; j += 64) {
-      out_id[j] = j;
-      out_w[j] = __builtin_nanf("");
+    if constexpr (BIAS) {
+      const int e = li + LPR * v;
+      const double b = e < experts ? (double)bias[e] : 0.0;
+      bad |= b != b;
+      c[v] = l[v] == -__builtin_inff() ? kNone : score(l[v]) + b;
+    } else {
+      c[v] = l[v];
     }
-    return;
   }
+  const uint64_t row_lanes = LPR == 64 ? ~0ull : ((1ull << (LPR & 63)) - 1) << (lane - li);
   if (groups > 1) {
     const int per = experts / groups;
 #pragma unroll
-    for (int v = 0; v < EPL; ++v) sc[wave][lane + 64 * v] = c[v];
+    for (int v = 0; v < EPL; ++v) sc[slot][li + LPR * v] = c[v];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    double best = kNone, second = kNone;
-    if (lane < groups)
-      for (int m = 0; m < per; ++m) {
-        const double s = sc[wave][lane * per + m];
-        if (s > best) {
-          second = best;
-          best = s;
-        } else if (s > second) {
-          second = s;
+    int share = 1;  // lanes of a group, a power of two
+    while (2 * share * groups <= LPR) share *= 2;
+    for (int g0 = 0; g0 < groups; g0 += LPR / share) {
+      const int g = g0 + li / share;
+      Key best = kNone, second = kNone;
+      if (g < groups)
+        for (int m = li % share; m < per; m += share) {
+          const Key s = sc[slot][g * per + m];
+          second = larger(second, s < best ? s : best);
+          best = larger(best, s);
         }
+      for (int d = 1; d < share; d *= 2) {
+        const Key ob = __shfl_xor(best, d), os = __shfl_xor(second, d);
+        second = larger(larger(second, os), best < ob ? best : ob);
+        best = larger(best, ob);
       }
-    if (bias && second != kNone) best += second;
+      if (BIAS && second != kNone) best += second;
+      if (g < groups && li % share == 0) best_of[slot][g] = best;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const Key mine = li < groups ? best_of[slot][li] : kNone;
     int rank = 0;  // groups ahead of this lane's
     for (int o = 0; o < groups; ++o) {
-      const double s = __shfl(best, o);
-      rank += s > best || (s == best && o < lane);
+      const Key s = best_of[slot][o];
+      rank += s > mine || (s == mine && o < li);
     }
-    const uint64_t keep = __ballot(lane < groups && rank < top_groups);
+    const uint64_t keep = __ballot(li < groups && rank < top_groups) >> (lane - li);
 #pragma unroll
     for (int v = 0; v < EPL; ++v) {
-      const int e = lane + 64 * v;
+      const int e = li + LPR * v;
       if (e < experts && !(keep >> (e / per) & 1)) c[v] = kNone;
     }
   }
-  double total = 0, mine_w = 0;
-  int mine_id = -1;
+  int mine_id = -1;  // lane j's: the j-th chosen
   for (int j = 0; j < top_k; ++j) {
-    double best = kNone;
+    Key best = kNone;
 #pragma unroll
-    for (int v = 0; v < EPL; ++v) best = maximum(best, c[v]);
-    best = wave_reduce64(best, maximum);
-    int id = -1;
-    double w = 0;
-    if (best != kNone) {  // the lowest expert with that score: experts of one v lie below those of the next
+    for (int v = 0; v < EPL; ++v) best = larger(best, c[v]);
+    best = reduce<LPR>(best, larger);
+    int id = 1 << 30;  // the lowest expert with that score
 #pragma unroll
-      for (int v = EPL - 1; v >= 0; --v) {
-        const uint64_t hit = __ballot(c[v] == best);
-        if (hit) id = 64 * v + __builtin_ctzll(hit);
-      }
+    for (int v = EPL - 1; v >= 0; --v)
+      if (c[v] == best) id = li + LPR * v;
+    id = reduce<LPR>(id, [](int a, int b) { return a < b ? a : b; });
 #pragma unroll
-      for (int v = 0; v < EPL; ++v)
-        if (id / 64 == v) {
-          w = __shfl(p[v], id % 64);
-          if (lane == id % 64) c[v] = kNone;
-        }
-    }
-    total += w;
-    if (lane == j) {
-      mine_w = w;
-      mine_id = id;
-    }
+    for (int v = 0; v < EPL; ++v)
+      if (li + LPR * v == id) c[v] = kNone;
+    if (li == j && best != kNone) mine_id = id;
   }
-  if (lane < top_k) {
-    if (renormalize) mine_w = total > 0 ? mine_w / total : 0.0;
-    out_id[lane] = mine_id;
-    out_w[lane] = (float)(mine_w * (double)scale);
-  }
+  const bool poisoned = (__ballot(bad) & row_lanes) != 0;  // a NaN (or a softmax over +inf) shows in every weight
+  double w = live && li < top_k && mine_id >= 0 && !poisoned ? score(load(mine_id)) : 0.0;
+  const double total = reduce<LPR>(w, [](double a, double b) { return a + b; });
+  if (!live || li >= top_k) return;
+  if (renormalize) w = total > 0 ? w / total : 0.0;
+  ids[row * top_k + li] = poisoned ? li : mine_id;
+  weights[row * top_k + li] = poisoned ? __builtin_nanf("") : (float)(w * (double)scale);
 }
 
 // ---------------------------------------------------------------- pairs by expert
@@ -561,7 +599,7 @@ void launch_tiles(const Shape& s, uint8_t* w, const Layout& l, const void* gate_
 extern "C" int ff_moe_route(const void* logits, int logits_f32, int64_t ld, const float* bias, float* weights, int* ids,
                             int64_t t, int64_t experts, int64_t top_k, int sigmoid, int64_t groups, int64_t top_groups,
                             int renormalize, float scale, ff_stream_t stream) {
-  FF_REQUIRE(t >= 0 && t < (1ll << 31) && experts > 0 && experts <= kMaxExperts && ld >= 0 && top_k > 0 &&
+  FF_REQUIRE(t >= 0 && t < (1ll << 26) && experts > 0 && experts <= kMaxExperts && ld >= 0 && top_k > 0 &&
                  top_k <= 64 && top_k <= experts && groups > 0 && groups <= 64 && experts % groups == 0 &&
                  top_groups > 0 && top_groups <= groups && top_groups * (experts / groups) >= top_k,
              "ff_moe_route: bad sizes t=%lld experts=%lld top_k=%lld groups=%lld top_groups=%lld", (long long)t,
@@ -569,22 +607,39 @@ extern "C" int ff_moe_route(const void* logits, int logits_f32, int64_t ld, cons
   if (t == 0) return FF_OK;
   FF_REQUIRE(logits && weights && ids, "ff_moe_route: null pointer");
   FF_REQUIRE(ff_aligned(logits, logits_f32 ? 4 : 2), "ff_moe_route: alignment");
-  const dim3 grid((unsigned)((t + kRouteRows - 1) / kRouteRows)), block(64 * kRouteRows);
   const hipStream_t st = (hipStream_t)stream;
-  const auto go = [&](auto EPL_) {
-    constexpr int EPL = decltype(EPL_)::value;
-    if (logits_f32)
-      hipLaunchKernelGGL((route_kernel<EPL, true>), grid, block, 0, st, logits, ld, bias, weights, ids, t, (int)experts,
-                         (int)top_k, sigmoid, (int)groups, (int)top_groups, renormalize, scale);
-    else
-      hipLaunchKernelGGL((route_kernel<EPL, false>), grid, block, 0, st, logits, ld, bias, weights, ids, t,
-                         (int)experts, (int)top_k, sigmoid, (int)groups, (int)top_groups, renormalize, scale);
+  const auto go = [&](auto LPR_, auto EPL_) {
+    constexpr int LPR = decltype(LPR_)::value, EPL = decltype(EPL_)::value, rows = kRouteWaves * 64 / LPR;
+    const dim3 grid((unsigned)((t + rows - 1) / rows)), block(64 * kRouteWaves);
+    const auto run = [&](auto F32_, auto BIAS_) {
+      hipLaunchKernelGGL((route_kernel<LPR, EPL, decltype(F32_)::value, decltype(BIAS_)::value>), grid, block, 0, st,
+                         logits, ld, bias, weights, ids, t, (int)experts, (int)top_k, sigmoid, (int)groups,
+                         (int)top_groups, renormalize, scale);
+    };
+    using Yes = std::true_type;
+    using No = std::false_type;
+    if (logits_f32) bias ? run(Yes{}, Yes{}) : run(Yes{}, No{});
+    else bias ? run(No{}, Yes{}) : run(No{}, No{});
   };
-  if (experts <= 64) go(std::integral_constant<int, 1>{});
-  else if (experts <= 128) go(std::integral_constant<int, 2>{});
-  else if (experts <= 256) go(std::integral_constant<int, 4>{});
-  else if (experts <= 512) go(std::integral_constant<int, 8>{});
-  else go(std::integral_constant<int, 16>{});
+  using std::integral_constant;
+  using L16 = integral_constant<int, 16>;
+  using L64 = integral_constant<int, 64>;
+  if (t >= 1024 && experts <= 256 && groups <= 16 && top_k <= 16) {
+    if (experts <= 64) go(L16{}, integral_constant<int, 4>{});
+    else if (experts <= 128) go(L16{}, integral_constant<int, 8>{});
+    else if (experts <= 192) go(L16{}, integral_constant<int, 12>{});
+    else go(L16{}, integral_constant<int, 16>{});
+  } else if (experts <= 64) {
+    go(L64{}, integral_constant<int, 1>{});
+  } else if (experts <= 128) {
+    go(L64{}, integral_constant<int, 2>{});
+  } else if (experts <= 256) {
+    go(L64{}, integral_constant<int, 4>{});
+  } else if (experts <= 512) {
+    go(L64{}, integral_constant<int, 8>{});
+  } else {
+    go(L64{}, integral_constant<int, 16>{});
+  }
   FF_LAUNCH_CHECK("ff_moe_route");
   return FF_OK;
 }

@@ -48,7 +48,7 @@ class FamilyRuntime:
     config.json, safetensors and tokenizer.json), ``buckets`` (token counts),
     and optionally ``variant`` (canvas policy, default 'square256'),
     ``prompt_style`` ('short' / 'minimal' / 'standard'), ``linear`` ('fp8',
-    'fp8_static', 'w4a16', 'int4'), ``execution_mode``, ``expected_dimensions``
+    'fp8_static', 'fp8_block', 'w4a16', 'int4'), ``execution_mode``, ``expected_dimensions``
     ([LM layers, LM width, vision blocks]).
     """
 

@@ -36,7 +36,8 @@ def route(logits, top_k, score="softmax", bias=None, groups=1, top_groups=None, 
 
     A logit of -inf switches its expert off; where fewer than ``top_k`` are left, the
     rest have id -1 and weight 0. A row with a NaN (or +inf under softmax) has NaN
-    weights. Scores are computed and compared in 64 bits."""
+    weights. Scores are computed in 64 bits; without a bias experts are compared by their
+    logits (scores rise with them), with one by score + bias in 64 bits."""
     assert logits.dim() == 2 and logits.dtype in (BF16, F32) and score in ("softmax", "sigmoid")
     t, e = logits.shape
     top_groups = groups if top_groups is None else top_groups
@@ -130,9 +131,32 @@ class Experts:
         return y
 
 
+class Router:
+    """The router's linear: logits (T, E) bf16 = bf16(x . weight^T) from a bf16 weight (E, H),
+    E % 4 == 0 and H % 64 == 0."""
+
+    def __init__(self, weight):
+        assert weight.dim() == 2 and weight.dtype == BF16 and weight.shape[0] % 4 == weight.shape[1] % 64 == 0
+        check_here(weight)
+        self.weight = weight.contiguous()
+        self.zero = torch.zeros(weight.shape[0], device=weight.device, dtype=BF16)     # ff_gemm_bf16 takes a bias
+
+    def __call__(self, x):
+        assert x.dim() == 2 and x.dtype == BF16 and x.shape[1] == self.weight.shape[1] and x.stride(1) == 1
+        check_here(x, self.weight)
+        m, k = x.shape
+        n = self.weight.shape[0]
+        y = x.new_empty((m, n))
+        if m:
+            call("ff_gemm_bf16", ptr(x), x.stride(0), ptr(self.weight), ptr(self.zero), ptr(y), n, None, 0, m, n, k, 0,
+                 stream())
+        return y
+
+
 class MoE:
-    """A layer's mixture-of-experts MLP: ``router`` (a linear op to E logits), ``experts``
-    and the arguments of ``route``. ``moe(x)``: x (..., H) bf16 -> (..., H) bf16."""
+    """A layer's mixture-of-experts MLP: ``router`` (a callable to logits (T, E), e.g.
+    ``Router``), ``experts`` and the arguments of ``route``. ``moe(x)``: x (..., H) bf16 ->
+    (..., H) bf16."""
 
     def __init__(self, router, experts, top_k, **routing):
         self.router, self.experts, self.top_k, self.routing = router, experts, top_k, routing
@@ -143,4 +167,4 @@ class MoE:
         return self.experts(flat, weights, ids).reshape(x.shape)
 
 
-__all__ = ["route", "Experts", "MoE"]
+__all__ = ["route", "Experts", "Router", "MoE"]

@@ -12,8 +12,9 @@ Two step bodies produce identical numbers:
   the kernel that produces it (add_rms, fast_norm, swiglu), and V is written
   transposed by the QKV GEMM's epilogue; the down projection's split-K partials
   are added by the next add_rms launch. 9 launches per layer.
-* ``generic`` (any linear op): the reference's own op sequence through the
-  drop-in ops of ``fastforward_amd.ops`` and ``Linear.apply``.
+* ``generic`` (any linear op, and layers whose MLP is a mixture of experts): the
+  reference's own op sequence through the drop-in ops of ``fastforward_amd.ops``
+  and ``Linear.apply``, with ``moe.MoE`` in the MLP's place.
 
 Inputs are a bucket-sized token id buffer (zero padded), M-RoPE positions
 (3, T) and the picked row; the step writes the choice logits (n_options,) fp32.
@@ -47,6 +48,8 @@ class LMConfig:
     theta: float = 5e6
     sections: tuple = (24, 20, 20)
     tie_embed: bool = False
+    experts: int = 0          # > 0: every layer's MLP is a mixture of experts (moe.MoE), ``inter`` wide each
+    top_k: int = 0
 
     @property
     def scaling(self):
@@ -99,8 +102,14 @@ class LayerWeights:
     k_norm: ops.RMSNorm
     qkv: object
     o: object
-    gateup: object
+    gateup: object            # None, like down, where the layer has a mixture of experts
     down: object
+    moe: object = None        # moe.MoE
+
+    @property
+    def linears(self):
+        """The layer's linear ops."""
+        return [op for op in (self.qkv, self.o, self.gateup, self.down) if op is not None]
 
 
 @dataclass
@@ -234,7 +243,7 @@ class Runtime:
                 L.down.pack()
         else:
             for L in weights.layers:  # fragment copies of the int4 weights for the packed W4A16 kernels
-                for op in (L.qkv, L.o, L.gateup, L.down):
+                for op in L.linears:
                     if isinstance(op, Int4):
                         op.pack()
         T, H, D = tokens, cfg.hidden, cfg.head_dim
@@ -265,8 +274,11 @@ class Runtime:
         """"fused" when every linear is an FP8Linear (per-token / per-channel),
         "fused_static" when every linear is a StaticFP8Linear /
         RuntimeScaleLinear (calibrated per-tensor scales), else "generic" (the
-        reference's op sequence through the drop-in ops)."""
-        ops_ = [op for L in weights.layers for op in (L.qkv, L.o, L.gateup, L.down)]
+        reference's op sequence through the drop-in ops), as with any layer whose
+        MLP is a mixture of experts."""
+        if any(L.moe is not None for L in weights.layers):
+            return "generic"
+        ops_ = [op for L in weights.layers for op in L.linears]
         if all(isinstance(op, FP8Linear) for op in ops_):
             return "fused"
         if all(isinstance(op, StaticFP8Linear) for op in ops_):
@@ -493,9 +505,12 @@ class Runtime:
             attn = self._attention_generic(lw, normalized, cos, sin)
             residual, post = self._linear_add_rms(attn, lw.o, h, None, lw.post_norm)
             deep = self.deep[j] if j < len(self.deep) else None
-            h, normalized = self._linear_add_rms(self._swiglu(post, lw.gateup), lw.down, residual, deep,
-                                                 L[j + 1].input_norm, self.image_start,
-                                                 self.nv if deep is not None else 0)
+            norm, start, nv = L[j + 1].input_norm, self.image_start, self.nv if deep is not None else 0
+            if lw.moe is not None:
+                h, normalized = ops.add_rms(residual, lw.moe(post), deep, norm, start, nv)
+            else:
+                h, normalized = self._linear_add_rms(self._swiglu(post, lw.gateup), lw.down, residual, deep, norm,
+                                                     start, nv)
             if trace is not None:
                 trace.append(h[0].clone())
         lw = L[-1]
@@ -518,7 +533,7 @@ class Runtime:
         value = Linear.apply(out.reshape(1, 1, -1), lw.o)
         hp = self._index_rows(h[0], self.pick, dim1=True)           # h.index_select(1, pick)
         residual, post = ops.add_rms(hp, value, None, lw.post_norm)
-        mlp = Linear.apply(self._swiglu(post[0], lw.gateup), lw.down)
+        mlp = lw.moe(post[0]) if lw.moe is not None else Linear.apply(self._swiglu(post[0], lw.gateup), lw.down)
         y = torch.empty((1, w.head.shape[0]), device=self.dev, dtype=torch.float32)
         call("ff_lm_readout", ptr(residual), ptr(mlp), ptr(w.norm.weight), ptr(w.head), ptr(y), cfg.hidden,
              w.head.shape[0], float(w.norm.variance_epsilon), stream())

@@ -9,7 +9,8 @@ concatenated row-wise as the reference packs them.
 """
 import torch
 
-from .linear import MIXED_MODES, FP8Linear, Int4, RuntimeScaleLinear, bank_of
+from .linear import MIXED_MODES, BlockFP8Linear, FP8Linear, Int4, RuntimeScaleLinear, bank_of
+from .moe import Experts, MoE, Router
 from .ops import RMSNorm
 from .runtime import LayerWeights, ModelWeights, mrope_positions
 
@@ -52,17 +53,28 @@ def _norm(n, jitter, device, seed):
     return (1 + jitter * torch.randn(n, generator=g, device=device)).to(BF16)
 
 
+def _moe(cfg, seed, device):
+    """A layer's mixture of experts: N(0, 0.02) router and experts."""
+    e, h, i = cfg.experts, cfg.hidden, cfg.inter
+    g = _gen(device, seed)
+    w = lambda *shape: (torch.randn(shape, generator=g, device=device) * 0.02).to(BF16)  # noqa: E731
+    return MoE(Router(w(e, h)), Experts(w(e, 2, i, h), w(e, h, i)), cfg.top_k)
+
+
 def make_model(cfg, mode="fp8", seed=0, device="cuda", n_options=8, norm_jitter=0.0,
                static_bound=8.0, int4_group=128, int4_symmetric=True, keep_bf16=None, fp8_bank="fp8_static"):
     """Build ModelWeights for ``cfg``.
 
     mode: "fp8" (FP8Linear: per-token / per-channel), "fp8_static"
-    (RuntimeScaleLinear with activation bound ``static_bound``), "w4a16" (Int4,
+    (RuntimeScaleLinear with activation bound ``static_bound``), "fp8_block"
+    (BlockFP8Linear), "w4a16" (Int4,
     ``int4_group`` / ``int4_symmetric``), "int4" (Int4, asymmetric group 32),
     "int4_half" / "int4_ffn" (the reference's mixed execution modes: the
     asymmetric group-32 int4 bank in the interior layers by ``bank_of``, the
     ``fp8_bank`` format elsewhere).
     ``keep_bf16`` (a dict) receives the bf16 weights by (layer, role) on the CPU.
+    With ``cfg.experts`` the MLP of every layer is a mixture of block-scaled FP8
+    experts (softmax routing, weights renormalised) whatever the mode.
     """
     H, D = cfg.hidden, cfg.head_dim
     g = _gen(device, _seed(seed, 10 ** 6))
@@ -71,6 +83,9 @@ def make_model(cfg, mode="fp8", seed=0, device="cuda", n_options=8, norm_jitter=
     for j in range(cfg.layers):
         ops = {}
         for role in ROLES:
+            if cfg.experts and role in ("gateup", "down"):
+                ops[role] = None
+                continue
             w = linear_weight(cfg, j, role, seed, device)
             if keep_bf16 is not None:
                 keep_bf16[(j, role)] = w.cpu()
@@ -81,6 +96,8 @@ def make_model(cfg, mode="fp8", seed=0, device="cuda", n_options=8, norm_jitter=
                 ops[role] = FP8Linear(w)
             elif m == "fp8_static":
                 ops[role] = RuntimeScaleLinear(w, 448.0 / static_bound)
+            elif m == "fp8_block":
+                ops[role] = BlockFP8Linear(w)
             elif m == "w4a16":
                 ops[role] = Int4(w, group=int4_group, symmetric=int4_symmetric)
             elif m == "int4":       # the reference's asymmetric group-32 quantizer
@@ -89,6 +106,8 @@ def make_model(cfg, mode="fp8", seed=0, device="cuda", n_options=8, norm_jitter=
                 raise ValueError(mode)
             del w
         ns = lambda k: _seed(seed, j, 100 + k)  # noqa: E731
+        if cfg.experts:
+            ops["moe"] = _moe(cfg, ns(4), device)
         layers.append(LayerWeights(
             input_norm=RMSNorm(_norm(H, norm_jitter, device, ns(0)), cfg.eps),
             post_norm=RMSNorm(_norm(H, norm_jitter, device, ns(1)), cfg.eps),

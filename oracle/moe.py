@@ -84,7 +84,8 @@ def route(logits, top_k, score="softmax", bias=None, groups=1, top_groups=None, 
             p = {j: math.exp(l[j] - top) / z for j in on}
         else:
             p = {j: 1 / (1 + math.exp(-l[j])) if l[j] > -700 else 0.0 for j in on}
-        c = {j: p[j] + b[j] for j in on}
+        # without a bias by logit: scores rise with it, and those that round to the same number keep their order
+        c = {j: l[j] if bias is None else p[j] + b[j] for j in on}
         if groups > 1:
             per, best = e // groups, []
             for g in range(groups):

@@ -37,7 +37,8 @@ def _check_route(logits, top_k, **kw):
 
 @gpu_test
 @pytest.mark.parametrize("t,e,k", [(1, 1, 1), (1, 128, 8), (3, 5, 5), (7, 60, 6), (33, 64, 1), (65, 65, 4),
-                                   (130, 160, 6), (64, 256, 8), (9, 512, 16), (5, 1000, 64), (2, 1024, 10)])
+                                   (130, 160, 6), (64, 256, 8), (9, 512, 16), (5, 1000, 64), (2, 1024, 10),
+                                   (1025, 60, 4), (1030, 128, 8), (1024, 150, 6), (1027, 256, 16), (1026, 9, 3)])
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_route(gpu, t, e, k, score):
     for dtype in (BF16, torch.float32):
@@ -49,7 +50,8 @@ def test_route(gpu, t, e, k, score):
 
 @gpu_test
 @pytest.mark.parametrize("t,e,k,groups,top", [(40, 256, 8, 8, 4), (9, 160, 6, 5, 1), (33, 64, 8, 64, 8), (5, 12, 4, 2, 2),
-                                              (21, 96, 3, 3, 2), (4, 1024, 32, 32, 3)])
+                                              (21, 96, 3, 3, 2), (4, 1024, 32, 32, 3),
+                                                  (1029, 160, 6, 5, 2), (1024, 256, 8, 16, 3)])
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_route_groups(gpu, t, e, k, groups, top, score):
     l = torch.randn(t, e, generator=_g(e + groups))
@@ -79,6 +81,7 @@ def test_route_special_rows(gpu, score):
     for kw in (dict(), dict(renormalize=False), dict(groups=4, top_groups=2),
                dict(bias=torch.randn(40, generator=_g(5)) * 0.1, groups=4, top_groups=3)):
         _check_route(l, 6, score=score, **kw)
+        _check_route(l.repeat(74, 1), 6, score=score, **kw)     # many rows: 16 lanes each
     bias = torch.zeros(40)
     bias[3], bias[4], bias[5] = -inf, inf, 1e30
     _check_route(l, 6, score=score, bias=bias)
