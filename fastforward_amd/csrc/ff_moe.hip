@@ -300,11 +300,11 @@ __device__ __forceinline__ u32x2 swiglu4(const f32x4& g, const f32x4& u) {
 }
 
 // Adds the waves' sums of slot t (a lane's 4 values of one fragment pair) in wave order.
-template <int SLOTS>
+template <int SLOTS, int WAVES = kWaves>
 __device__ __forceinline__ f32x4 sum_waves(const f32x4* red, int t) {
   f32x4 v = red[t];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) v += red[w * SLOTS + t];
+  for (int w = 1; w < WAVES; ++w) v += red[w * SLOTS + t];
   return v;
 }
 
@@ -380,52 +380,54 @@ __device__ __forceinline__ void load_h(u32x4 (&x)[4], const bf16_t* p) {
   for (int u = 0; u < 4; ++u) x[u] = reinterpret_cast<const u32x4*>(p)[u];
 }
 
-// One token's y, 16 channels: the k steps of all its experts shared by the
-// waves. All 16 result rows are the token's (every lane group reads the same row).
-__global__ __launch_bounds__(kThreads) void down_pair_kernel(
+// One token's y, 16 channels: the k steps of all its experts shared by 16 waves (few
+// workgroups: with three steps each, all of 128 x 768 x 8 experts is in flight at once). All
+// 16 result rows are the token's (every lane group reads the same row). A slot without an
+// expert reads expert 0's weights and is not added (its row of h was not written); every
+// id is read before the first use of one, so the loads do not wait for each other.
+constexpr int kDownThreads = 1024, kDownWaves = kDownThreads / 64;
+__global__ __launch_bounds__(kDownThreads) void down_pair_kernel(
     const bf16_t* __restrict__ h, const float* __restrict__ weights, const int* __restrict__ ids,
     const uint8_t* __restrict__ wp, const float* __restrict__ ws, bf16_t* __restrict__ y, int64_t ldy, int64_t n,
     int top_k, int experts, int kt_n, int nf) {
-  constexpr int PF = 4;
-  __shared__ f32x4 red[kWaves * 4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int PF = 3;
+  __shared__ f32x4 red[kDownWaves * 4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, g = lane >> 4;
   const int f = blockIdx.x % nf, tok = blockIdx.x / nf;
   const int64_t matrix = (int64_t)nf * kt_n * 2048;
   const int64_t nb = (n + kBlock - 1) / kBlock;
   const int steps = top_k * kt_n;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int b = wave; b < steps; b += kWaves * PF) {
+  for (int b = wave; b < steps; b += kDownWaves * PF) {
+    int id[PF];
+    float wt[PF], s[PF];
     i32x8 wq[PF];
     u32x4 xh[PF][4];
-    float s[PF];
 #pragma unroll
     for (int u = 0; u < PF; ++u) {
-      const int at = b + kWaves * u;
-      s[u] = 0.f;
-      if (at < steps) {
-        const int pair = tok * top_k + at / kt_n, kt = at % kt_n;
-        const int e = ids[pair];
-        if (e >= 0 && e < experts) {
-          wq[u] = load_frag(wp + e * matrix + ((int64_t)kt * nf + f) * 2048, lane);
-          load_h(xh[u], h + ((int64_t)pair * kt_n + kt) * kBlock + 32 * g);
-          s[u] = weights[pair] * ws[((int64_t)e * nb + f / 8) * kt_n + kt];
-        }
-      }
+      const int pair = tok * top_k + min(b + kDownWaves * u, steps - 1) / kt_n;
+      id[u] = ids[pair];
+      wt[u] = weights[pair];
     }
 #pragma unroll
     for (int u = 0; u < PF; ++u) {
-      const int at = b + kWaves * u;
-      if (at < steps) {
-        const int e = ids[tok * top_k + at / kt_n];
-        if (e >= 0 && e < experts) fma4(acc, mfma_step_bf16(wq[u], xh[u]), s[u]);
-      }
+      const int at = min(b + kDownWaves * u, steps - 1), pair = tok * top_k + at / kt_n, kt = at % kt_n;
+      const bool on = id[u] >= 0 && id[u] < experts && b + kDownWaves * u < steps;
+      const int e = on ? id[u] : 0;
+      id[u] = on;
+      wq[u] = load_frag(wp + e * matrix + ((int64_t)kt * nf + f) * 2048, lane);
+      load_h(xh[u], h + ((int64_t)pair * kt_n + kt) * kBlock + 32 * g);
+      s[u] = ws[((int64_t)e * nb + f / 8) * kt_n + kt];
     }
+#pragma unroll
+    for (int u = 0; u < PF; ++u)
+      if (id[u]) fma4(acc, mfma_step_bf16(wq[u], xh[u]), wt[u] * s[u]);
   }
   if (r16 == 0) red[wave * 4 + g] = acc;
   __syncthreads();
   if (threadIdx.x < 4) {
-    const f32x4 v = sum_waves<4>(red, threadIdx.x);
+    const f32x4 v = sum_waves<4, kDownWaves>(red, threadIdx.x);
     const int64_t c = 16 * (int64_t)f + 4 * threadIdx.x;
     if (c < n) store4_bf16(y + tok * ldy + c, v, n - c);
   }
@@ -676,7 +678,7 @@ extern "C" int ff_moe_experts(const void* x, int64_t ldx, const float* weights, 
     hipLaunchKernelGGL(gate_up_pair_kernel, dim3((unsigned)(s.pairs() * nfi)), dim3(kThreads), 0, st, (const bf16_t*)x,
                        ldx, vec, h, ids, (const uint8_t*)gate_up, gate_up_scales, (bf16_t*)(w + l.h), (int)top_k,
                        (int)experts, s.kth(), nfi);
-    hipLaunchKernelGGL(down_pair_kernel, dim3((unsigned)(t * nfh)), dim3(kThreads), 0, st, (const bf16_t*)(w + l.h),
+    hipLaunchKernelGGL(down_pair_kernel, dim3((unsigned)(t * nfh)), dim3(kDownThreads), 0, st, (const bf16_t*)(w + l.h),
                        weights, ids, (const uint8_t*)down, down_scales, (bf16_t*)y, ldy, h, (int)top_k, (int)experts,
                        s.kti(), nfh);
     FF_LAUNCH_CHECK("ff_moe_experts");
