@@ -48,6 +48,24 @@ __device__ __forceinline__ u32x2 quant_group16(const bf16_t* __restrict__ row, i
   return quant8(v, sc, 1.0f / sc);
 }
 
+// Codes q (rows, 128 kt_n) and scales (kt_n, rows) of ROWS rows x 128 channels by 16 ROWS
+// threads, tile `i` of (rows / ROWS rounded up) x kt_n, channel blocks fastest. Scales have
+// channel blocks slowest: the lanes of a product's row tile read neighbouring ones, and a
+// tile's are whole 64-byte lines here.
+template <int ROWS>
+__device__ __forceinline__ void quant_rows_tile(const bf16_t* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q,
+                                                float* __restrict__ scales, int64_t rows, int64_t k, int kt_n, int vec,
+                                                int64_t i) {
+  const int s = threadIdx.x & 15;
+  const int64_t row = i / kt_n * ROWS + (threadIdx.x >> 4);
+  const int kt = (int)(i % kt_n);
+  if (row >= rows) return;
+  float scale;
+  const u32x2 c = quant_group16(x + row * ldx, k, kt, s, vec, &scale);
+  *reinterpret_cast<u32x2*>(q + (row * kt_n + kt) * kBlock + 8 * s) = c;
+  if (s == 0) scales[(int64_t)kt * rows + row] = scale;
+}
+
 // The 128 products of one k step, from zero.
 __device__ __forceinline__ f32x4 mfma_step(const i32x8& w, const i32x8& x) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
@@ -157,9 +175,5 @@ __device__ __forceinline__ bool find_tile(const int* __restrict__ off, int exper
   }
   return false;
 }
-
-// Launch of the row quantiser (defined with the linear): q (rows, 128 ceil(k / 128))
-// 16-byte aligned, scales (ceil(k / 128), rows).
-int quant_rows_block(const void* x, int64_t ldx, void* q, float* scales, int64_t rows, int64_t k, hipStream_t st);
 
 }  // namespace ff

@@ -82,24 +82,11 @@ __global__ __launch_bounds__(256) void unpack_block_kernel(const uint8_t* __rest
 
 // ---------------------------------------------------------------- row quantiser
 
-// 16 lanes per (row, 128 channels): codes q (rows, 128 kt_n) and scales (kt_n,
-// rows), channel blocks slowest, so that the lanes of a product's row tile read
-// neighbouring scales. A workgroup takes 16 rows of one channel block at a time,
-// whose scales are one 64-byte line.
 __global__ __launch_bounds__(256) void quant_rows_block_kernel(const bf16_t* __restrict__ x, int64_t ldx,
                                                                uint8_t* __restrict__ q, float* __restrict__ scales,
                                                                int64_t rows, int64_t k, int kt_n, int vec) {
-  const int s = threadIdx.x & 15;
   const int64_t tiles = (rows + 15) / 16 * kt_n;
-  for (int64_t i = blockIdx.x; i < tiles; i += gridDim.x) {
-    const int64_t row = i / kt_n * 16 + (threadIdx.x >> 4);
-    const int kt = (int)(i % kt_n);
-    if (row >= rows) continue;
-    float scale;
-    const u32x2 c = quant_group16(x + row * ldx, k, kt, s, vec, &scale);
-    *reinterpret_cast<u32x2*>(q + (row * kt_n + kt) * kBlock + 8 * s) = c;
-    if (s == 0) scales[(int64_t)kt * rows + row] = scale;
-  }
+  for (int64_t i = blockIdx.x; i < tiles; i += gridDim.x) quant_rows_tile<16>(x, ldx, q, scales, rows, k, kt_n, vec, i);
 }
 
 // ---------------------------------------------------------------- few rows
@@ -281,18 +268,15 @@ constexpr int64_t kMaxCodes = 1ll << 31;
 
 }  // namespace
 
-namespace ff {
-
-int quant_rows_block(const void* x, int64_t ldx, void* q, float* scales, int64_t rows, int64_t k, hipStream_t st) {
+static int quant_rows_block(const void* x, int64_t ldx, void* q, float* scales, int64_t rows, int64_t k,
+                            hipStream_t st) {
   const int64_t kt_n = (k + kBlock - 1) / kBlock;
   const int64_t grid = (rows + 15) / 16 * kt_n;
-  hipLaunchKernelGGL(quant_rows_block_kernel, dim3((unsigned)(grid < (1 << 20) ? grid : (1 << 20))), dim3(256), 0, st, (const bf16_t*)x, ldx,
-                     (uint8_t*)q, scales, rows, k, (int)kt_n, (int)rows_vec(x, ldx));
+  hipLaunchKernelGGL(quant_rows_block_kernel, dim3((unsigned)(grid < (1 << 20) ? grid : (1 << 20))), dim3(256), 0, st,
+                     (const bf16_t*)x, ldx, (uint8_t*)q, scales, rows, k, (int)kt_n, (int)rows_vec(x, ldx));
   FF_LAUNCH_CHECK("quant_rows_fp8_block");
   return FF_OK;
 }
-
-}  // namespace ff
 
 extern "C" int ff_quant_weight_fp8_block(const void* w, void* q, float* scales, int64_t n, int64_t k,
                                          ff_stream_t stream) {

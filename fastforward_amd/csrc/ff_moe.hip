@@ -219,13 +219,23 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(
 
 // ---------------------------------------------------------------- pairs by expert
 
-// One workgroup per expert: pairs p = token * top_k + slot of the expert in rising
-// order to list[off[e] ..), off[e] = pairs of lower experts. Every workgroup reads
-// all ids (a few hundred KB from L2 at most) and needs nothing from the others: no
-// counters in memory, no order of arrival. ids outside [0, experts) are in no list.
+// The first `experts` workgroups order the pairs, one expert each: its pairs p = token *
+// top_k + slot in rising order to list[off[e] ..), off[e] = pairs of lower experts. Every
+// workgroup reads all ids (a few hundred KB from L2 at most) and needs nothing from the
+// others: no counters in memory, no order of arrival. ids outside [0, experts) are in no
+// list. The other workgroups quantise the rows.
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64, kPlanBatch = 8;
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* __restrict__ ids, int pairs, int experts,
-                                                            int* __restrict__ off, int* __restrict__ list) {
+                                                            int* __restrict__ off, int* __restrict__ list,
+                                                            const bf16_t* __restrict__ x, int64_t ldx, int vec,
+                                                            int64_t t, int64_t h, int kt_n, uint8_t* __restrict__ q,
+                                                            float* __restrict__ qs) {
+  if ((int)blockIdx.x >= experts) {
+    const int64_t tiles = (t + kPlanThreads / 16 - 1) / (kPlanThreads / 16) * kt_n;
+    for (int64_t i = blockIdx.x - experts; i < tiles; i += gridDim.x - experts)
+      quant_rows_tile<kPlanThreads / 16>(x, ldx, q, qs, t, h, kt_n, vec, i);
+    return;
+  }
   __shared__ int below[kPlanWaves], equal[kPlanWaves];
   const int e = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int seg = (pairs + kPlanWaves - 1) / kPlanWaves;
@@ -684,10 +694,10 @@ extern "C" int ff_moe_experts(const void* x, int64_t ldx, const float* weights, 
     FF_LAUNCH_CHECK("ff_moe_experts");
     return FF_OK;
   }
-  hipLaunchKernelGGL(plan_kernel, dim3((unsigned)experts), dim3(kPlanThreads), 0, st, ids, (int)s.pairs(), (int)experts,
-                     (int*)(w + l.off), (int*)(w + l.list));
-  const int rq = quant_rows_block(x, ldx, w + l.q, (float*)(w + l.qs), t, h, st);
-  if (rq != FF_OK) return rq;
+  const int64_t quant = (t + kPlanThreads / 16 - 1) / (kPlanThreads / 16) * s.kth();
+  hipLaunchKernelGGL(plan_kernel, dim3((unsigned)(experts + (quant < (1 << 20) ? quant : (1 << 20)))),
+                     dim3(kPlanThreads), 0, st, ids, (int)s.pairs(), (int)experts, (int*)(w + l.off), (int*)(w + l.list),
+                     (const bf16_t*)x, ldx, vec, t, h, s.kth(), w + l.q, (float*)(w + l.qs));
   // Rows of an expert on average: with few, tiles of 32 rows (us on 32- and 64-row tiles, 128
   // experts, 8 a token, h 2048, i 768: 8 tokens 54.0 and 61.7, 32 tokens 101 and 111, 128 tokens
   // 122 and 121, 512 tokens 163 and 155, 4096 tokens 581 and 429).
