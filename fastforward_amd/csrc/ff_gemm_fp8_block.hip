@@ -327,11 +327,14 @@ extern "C" int ff_quant_rows_fp8_block(const void* x, int64_t ldx, void* q, floa
   return quant_rows_block(x, ldx, q, scales, rows, k, (hipStream_t)stream);
 }
 
+// Sizes under which 32-bit offsets hold: the packed weight, with the loads of some steps past
+// its end, the codes of a row tile, the rows' scales, and the threads of a grid.
 static int check_gemm(const char* who, const void* packed, const float* ws, const void* y, int64_t ldy, int64_t m,
                       int64_t n, int64_t k) {
-  FF_REQUIRE(m >= 0 && m < kMaxCodes && n > 0 && k > 0 && n < kMaxCodes && k < kMaxCodes && ldy >= n &&
-                 ((n + 15) / 16 * 16) * ((k + kBlock - 1) / kBlock * kBlock) < kMaxCodes && m <= 65535ll * 16 &&
-                 m * ((k + kBlock - 1) / kBlock) < (1ll << 30),
+  const int64_t n16 = (n + 15) / 16 * 16, kt_n = (k + kBlock - 1) / kBlock;
+  FF_REQUIRE(m >= 0 && m < kMaxCodes && n > 0 && k > 0 && n < kMaxCodes && k < (1 << 24) && ldy >= n &&
+                 n16 * kt_n * kBlock < kMaxCodes && n16 * (kt_n + 8) * kBlock < 2 * kMaxCodes &&
+                 m * kt_n < (1ll << 30) && m * n < (1ll << 38),
              "%s: bad sizes m=%lld n=%lld k=%lld", who, (long long)m, (long long)n, (long long)k);
   if (m == 0) return FF_OK;
   FF_REQUIRE(packed && ws && y, "%s: null pointer", who);
@@ -360,7 +363,7 @@ static int check_gemm(const char* who, const void* packed, const float* ws, cons
 // its tiles fill the GPU.
 static int block_kernel(int64_t m, int64_t n) {
   const int tune = ff_tuning(FF_TUNE_BLOCK_TILE);
-  if (tune) return tune;
+  if (tune && m <= 65535 * 16 && m * n < (1ll << 31)) return tune;
   if (m <= 16 && n <= 8192) return 1;
   const auto tiles = [&](int64_t bm, int64_t bn) { return ((m + bm - 1) / bm) * ((n + bn - 1) / bn); };
   if (tiles(128, 128) >= 224) return 4;

@@ -13,9 +13,9 @@
 // channels, the row quantised in the workgroup; down: a workgroup per token and 16
 // channels, its waves sharing the k steps of all the token's experts, so the
 // weighted sum over experts needs no launch of its own.
-// More pairs: they are ordered by expert (plan), the rows quantised once, and row
-// tiles that belong to one expert each run both products; the down products of a
-// token's experts are added by a last launch in the order of the token's list.
+// More pairs: one launch orders them by expert and quantises the rows, row tiles that
+// belong to one expert each run both products, and the down products of a token's experts
+// are added by a last launch in the order of the token's list.
 #include "ff_block_tile.h"
 
 using namespace ff;
@@ -548,9 +548,11 @@ struct Shape {
   int kti() const { return (int)((i + kBlock - 1) / kBlock); }
   // Up to 32 pairs they are taken one by one (128 experts, 8 a token, h 2048, i 768, us: 4 tokens
   // 36.9 against 40.0 on tiles, 8 tokens 68.8 against 54.0).
+  // The row has to fit in LDS and either grid's threads in 32 bits.
   bool by_pair() const {
     const int tune = ff_tuning(FF_TUNE_MOE_TILE);
-    return (tune ? tune == 1 && t < (1 << 16) : pairs() <= 32) && (int64_t)kth() * kBlock <= kInlineCodes;
+    return (tune ? tune == 1 : pairs() <= 32) && (int64_t)kth() * kBlock <= kInlineCodes &&
+           pairs() * 8 * (kth() > kti() ? kth() : kti()) < (1 << 22);
   }
 };
 
@@ -579,12 +581,19 @@ struct Layout {
   }
 };
 
-// Bounds under which the rows' codes stay under 2^32 bytes and every grid below stays under 2^32 threads: the row tiles of
-// either product (16 rows at least, one more for each expert) times its columns.
+// Sizes under which 32-bit offsets hold: one matrix of an expert, with the loads of some
+// steps past its end, the rows' codes, and the threads of every grid (32 rows x 64 channels
+// a workgroup at the least).
 int check_shape(const char* who, int64_t t, int64_t top_k, int64_t experts, int64_t h, int64_t i) {
+  constexpr int64_t kMax = 1ll << 32;
   FF_REQUIRE(t >= 0 && top_k > 0 && experts > 0 && experts <= kMaxExperts && h > 0 && i > 0 && h <= (1 << 24) &&
-                 i <= (1 << 24) && top_k <= 1024 && t < (1 << 21) &&
-                 t * ((h + kBlock - 1) / kBlock) < (1 << 25) && (t * top_k / 16 + experts) * ((h > i ? h : i) / 16 + 8) < (1 << 23),
+                 i <= (1 << 24) && top_k <= 1024 && t < (1 << 24),
+             "%s: bad sizes t=%lld top_k=%lld experts=%lld h=%lld i=%lld", who, (long long)t, (long long)top_k,
+             (long long)experts, (long long)h, (long long)i);
+  const int64_t hb = (h + kBlock - 1) / kBlock, ib = (i + kBlock - 1) / kBlock;
+  FF_REQUIRE(hb * ib * kBlock * kBlock < kMax / 2 && ib * kBlock * (hb + 8) * kBlock < kMax &&
+                 hb * kBlock * (ib + 8) * kBlock < kMax && t * (hb + 8) * kBlock < kMax &&
+                 (t * top_k / 32 + experts) * ((h > i ? h : i) / 64 + 2) < (1 << 24),
              "%s: bad sizes t=%lld top_k=%lld experts=%lld h=%lld i=%lld", who, (long long)t, (long long)top_k,
              (long long)experts, (long long)h, (long long)i);
   return FF_OK;
@@ -611,7 +620,7 @@ void launch_tiles(const Shape& s, uint8_t* w, const Layout& l, const void* gate_
 extern "C" int ff_moe_route(const void* logits, int logits_f32, int64_t ld, const float* bias, float* weights, int* ids,
                             int64_t t, int64_t experts, int64_t top_k, int sigmoid, int64_t groups, int64_t top_groups,
                             int renormalize, float scale, ff_stream_t stream) {
-  FF_REQUIRE(t >= 0 && t < (1ll << 26) && experts > 0 && experts <= kMaxExperts && ld >= 0 && top_k > 0 &&
+  FF_REQUIRE(t >= 0 && t < (1ll << 25) && experts > 0 && experts <= kMaxExperts && ld >= 0 && top_k > 0 &&
                  top_k <= 64 && top_k <= experts && groups > 0 && groups <= 64 && experts % groups == 0 &&
                  top_groups > 0 && top_groups <= groups && top_groups * (experts / groups) >= top_k,
              "ff_moe_route: bad sizes t=%lld experts=%lld top_k=%lld groups=%lld top_groups=%lld", (long long)t,

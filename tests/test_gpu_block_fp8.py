@@ -175,6 +175,39 @@ def test_graph_and_stream(gpu, m):
         assert torch.equal(got, op(xi))
 
 
+@gpu_test
+def test_offsets_past_32_bits(gpu):
+    """More than 2^32 codes of activations: equal rows of x give equal rows of y."""
+    from fastforward_amd.linear import BlockFP8Linear
+    rows, times, n, k = 1024, 64, 128, 65792
+    g = torch.Generator(device=DEV).manual_seed(0)
+    op = BlockFP8Linear((torch.randn(n, k, generator=g, device=DEV) * 0.02).to(BF16))
+    base = torch.randn(rows, k, generator=g, device=DEV).to(BF16)
+    y = op(base.repeat(times, 1)).view(times, rows, n)
+    assert (y == y[:1]).all()
+    want = op(base).float()     # another tile's order of sums: two bf16 roundings apart at most
+    assert float((y[0].float() - want).norm() / want.norm()) <= 2 ** -7
+
+
+@gpu_test
+def test_two_streams(gpu):
+    """Calls that overlap on two streams share nothing."""
+    from fastforward_amd.linear import BlockFP8Linear
+    g = torch.Generator(device=DEV).manual_seed(1)
+    op = BlockFP8Linear((torch.randn(512, 1024, generator=g, device=DEV) * 0.02).to(BF16))
+    xs = [torch.randn(m, 1024, generator=g, device=DEV).to(BF16) for m in (40, 300)]
+    want = [op(x) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[], []]
+    for _ in range(20):
+        for j, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[j].append(op(xs[j]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, w) for ys, w in zip(got, want) for y in ys)
+
+
 def test_refusals_python():
     """Checked before any launch: no GPU is touched."""
     from fastforward_amd.linear import BlockFP8Linear
@@ -195,6 +228,9 @@ def test_refusals_c():
     bad = [("ff_linear_fp8_block", (p, 8, p, p, p, 8, 1, 0, 8, None, 0, None), "bad sizes"),
            ("ff_linear_fp8_block", (p, 8, p, p, p, 7, 1, 8, 8, None, 0, None), "bad sizes"),
            ("ff_linear_fp8_block", (p, 8, p, p, p, 1 << 20, 1, 1 << 20, 1 << 20, None, 0, None), "bad sizes"),
+           ("ff_linear_fp8_block", (p, 8, p, p, p, 1 << 23, 1, 1 << 23, 64, None, 0, None), "bad sizes"),
+           ("ff_linear_fp8_block", (p, 8, p, p, p, 8, 17, 8, 1 << 24, None, 0, None), "bad sizes"),
+           ("ff_linear_fp8_block", (p, 8, p, p, p, 8, 1 << 24, 8, 128 * 64, None, 0, None), "bad sizes"),
            ("ff_linear_fp8_block", (p, 8, p, p, p, 8, 9, 8, 8, None, 0, None), "workspace"),
            ("ff_linear_fp8_block", (p, 8, p, p, p, 8, 9, 8, 8, p, 16, None), "workspace"),
            ("ff_linear_fp8_block", (None, 8, p, p, p, 8, 1, 8, 8, None, 0, None), "null"),

@@ -273,6 +273,34 @@ def test_experts_graph_and_stream(gpu, t):
 
 
 @gpu_test
+def test_experts_offsets_past_32_bits(gpu):
+    """Down products of more than 2^32 bytes: equal tokens give equal rows."""
+    rows, times, k, e, h, i = 1050, 64, 8, 16, 2048, 128
+    op = _experts(_weights(e, h, i))
+    x, w, ids = (v.to(DEV) for v in _tokens(rows, k, e, h))
+    y = op(x.repeat(times, 1), w.repeat(times, 1), ids.repeat(times, 1)).view(times, rows, h)
+    assert torch.equal(y[0], op(x, w, ids)) and (y == y[:1]).all()      # 64-row tiles both times
+
+
+@gpu_test
+def test_experts_two_streams(gpu):
+    """Calls that overlap on two streams share nothing."""
+    k, e, h, i = 4, 8, 256, 128
+    op = _experts(_weights(e, h, i))
+    args = [[v.to(DEV) for v in _tokens(t, k, e, h, t)] for t in (20, 130)]
+    want = [op(*a) for a in args]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in args]
+    got = [[], []]
+    for _ in range(20):
+        for j, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[j].append(op(*args[j]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, v) for ys, v in zip(got, want) for y in ys)
+
+
+@gpu_test
 def test_experts_from_bf16(gpu):
     from fastforward_amd.moe import Experts
     e, h, i = 3, 136, 200
@@ -322,7 +350,8 @@ def test_refusals_c():
     def experts(x=p, gu=p, t=1, k=2, e=4, h=8, i=8, ldy=8, ws=p, nbytes=4096):
         _lib.call("ff_moe_experts", x, h, p, p, gu, p, p, p, p, ldy, t, k, e, h, i, ws, nbytes, None)
 
-    for kw in (dict(k=0), dict(e=0), dict(e=1025), dict(h=0, ldy=8), dict(i=0), dict(t=-1), dict(t=1 << 22)):
+    for kw in (dict(k=0), dict(e=0), dict(e=1025), dict(h=0, ldy=8), dict(i=0), dict(t=-1), dict(t=1 << 24),
+               dict(t=1 << 21, h=2048, ldy=2048), dict(h=1 << 16, i=1 << 15, ldy=1 << 16), dict(t=1 << 20, k=1000)):
         with pytest.raises(RuntimeError, match="bad sizes"):
             experts(**kw)
     for kw, message in ((dict(ldy=7), "strides"), (dict(x=None), "null"), (dict(x=p + 1), "alignment"),
