@@ -343,43 +343,55 @@ static int check_gemm(const char* who, const void* packed, const float* ws, cons
 }
 
 // The kernel for quantised rows (us in a graph; columns: few-rows kernel, 32 x 64, 64 x 128,
-// 128 x 128 tiles):
-//   m x n x k             few    32 x 64   64 x 128   128 x 128
+// 128 x 128 tiles, 128 x 128 with two k groups):
+//   m x n x k             few    32 x 64   64 x 128   128 x 128   two groups
 //   7 x 4096 x 4096       3.8      6.8       11.9       19.4
 //   16 x 2048 x 25600    17.6     26.2       59         99
 //   7 x 8192 x 4096       5.9      6.9       12.0       19.4
 //   7 x 12288 x 4096     11.5      8.8       12.3       19.5
 //   32 x 6144 x 4096     11.5      6.9       12.1       20.0
 //   128 x 4096 x 4096    21.9      7.5       12.8       20.6
-//   333 x 1152 x 4304    22.5      8.3       13.5       22.8
-//   7 x 19456 x 2560     11.6     11.8        9.7       13.8
-//   176 x 6144 x 4096    70       16.5       13.1       21.1
-//   300 x 4096 x 4096    70       16.9       13.1       21.0
-//   1000 x 2048 x 1024   33       10.2        6.4        9.7
-//   2000 x 4096 x 512    81       33         14.0       13.7
-//   576 x 6144 x 4096   172       37.7       27.5       24.5
+//   333 x 1152 x 4304    22.5      7.8       13.1       22.8        19.4
+//   7 x 19456 x 2560     11.6     12.0        9.8       13.8        13.9
+//   176 x 6144 x 4096    70       16.2       13.1       21.4        20.4
+//   300 x 4096 x 4096    70       16.4       13.1       20.6        20.2
+//   1000 x 2048 x 1024   33       10.0        6.4        9.5        10.9
+//   576 x 4096 x 4096             26.8       24.7       21.3        21.5
+//   576 x 6144 x 4096   172       40.1       27.5       25.5        23.9
+//   1280 x 2560 x 2560                       15.9       16.2        16.8
+//   576 x 4096 x 12288            70.7       65.2       52.9        47.6
+//   500 x 5120 x 25600                      111        105          88
+//   1024 x 6144 x 4096            59.8       35.3       38.0        43.9
+//   800 x 6144 x 4096                        33.8       37.6        42.7
+//   1000 x 8192 x 4096                       45.4       42.4        46.6
+//   576 x 24576 x 4096           140.6       94.5       79.2        89.8
 //   1024 x 25600 x 5120 1390     309        179        162
-// The larger tile reads less for a product and takes longer for a step, so it waits until
-// its tiles fill the GPU.
-static int block_kernel(int64_t m, int64_t n) {
+// The larger tile reads less for a product and takes longer for a step. Both large ones take
+// about the same time for every 256 tiles (a CU's share of one), the smaller 0.58 of the
+// larger's: whichever needs less of it for the whole product. Two k groups put two waves on a
+// SIMD where there is one 128 x 128 tile for a CU at most; at 32 k steps the exchange of
+// their sums costs what that gains.
+static int block_kernel(int64_t m, int64_t n, int64_t kt_n) {
   const int tune = ff_tuning(FF_TUNE_BLOCK_TILE);
   if (tune && m <= 65535 * 16 && m * n < (1ll << 31)) return tune;
   if (m <= 16 && n <= 8192) return 1;
   const auto tiles = [&](int64_t bm, int64_t bn) { return ((m + bm - 1) / bm) * ((n + bn - 1) / bn); };
-  if (tiles(128, 128) >= 224) return 4;
-  return tiles(64, 128) >= 128 ? 3 : 2;
+  const int64_t small = tiles(64, 128), large = tiles(128, 128);
+  if (58 * ((small + 255) / 256) > 100 * ((large + 255) / 256)) return large <= 256 && kt_n >= 64 ? 5 : 4;
+  return small >= 128 ? 3 : 2;
 }
 
 static int gemm_block(const void* q, const float* qs, const void* packed, const float* ws, void* y, int64_t ldy,
                       int64_t m, int64_t n, int64_t k, hipStream_t st) {
   const int nf = (int)((n + 15) / 16), kt_n = (int)((k + kBlock - 1) / kBlock);
-  switch (block_kernel(m, n)) {
+  switch (block_kernel(m, n, kt_n)) {
     case 1:
       launch_skinny<false>(nullptr, 0, (const uint8_t*)q, qs, (const uint8_t*)packed, ws, (bf16_t*)y, ldy, m, n, k, st);
       break;
     case 2: launch_tile<32, 16, 4, 2, 2>(q, qs, packed, ws, y, ldy, m, n, kt_n, nf, st); break;
     case 3: launch_tile<64, 32, 3, 1, 1>(q, qs, packed, ws, y, ldy, m, n, kt_n, nf, st); break;
-    default: launch_tile<128, 32, 3, 1, 1>(q, qs, packed, ws, y, ldy, m, n, kt_n, nf, st); break;
+    case 4: launch_tile<128, 32, 3, 1, 1>(q, qs, packed, ws, y, ldy, m, n, kt_n, nf, st); break;
+    default: launch_tile<128, 32, 3, 1, 2>(q, qs, packed, ws, y, ldy, m, n, kt_n, nf, st); break;
   }
   FF_LAUNCH_CHECK("ff_gemm_fp8_block");
   return FF_OK;

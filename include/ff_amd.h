@@ -54,7 +54,8 @@ int ff_device_check(void);
 #define FF_TUNE_BF16_PK_SPLIT 10  /* ff_gemm_bf16_pk_ws / _ln: 1 no k split, 2..8 the split count */
 #define FF_TUNE_FP8_PK_SPLIT_SHORT_K 11 /* as FF_TUNE_FP8_PK_SPLIT, for k <= 4096 only (ahead of it there) */
 #define FF_TUNE_BLOCK_TILE 12 /* ff_gemm_fp8_block / ff_linear_fp8_block past the rows of one launch: 1 few rows,
-                                 2 32x64, 3 64x128, 4 128x128 tiles */
+                                 2 32x64, 3 64x128, 4 128x128 tiles, 5 those
+                                 on two k groups */
 #define FF_TUNE_MOE_TILE 13   /* ff_moe_experts: 1 pair by pair, 2 32-row, 3 64-row tiles (set it before the
                                  workspace is asked for) */
 int ff_set_tuning(int knob, int value);

@@ -59,7 +59,7 @@ def test_linear(gpu, m, n, k):
 
 
 @gpu_test
-@pytest.mark.parametrize("tile", [1, 2, 3, 4])
+@pytest.mark.parametrize("tile", [1, 2, 3, 4, 5])
 @pytest.mark.parametrize("m,n,k", SHAPES)
 def test_every_kernel(gpu, m, n, k, tile):
     """Each kernel of the product at sizes that another would be chosen for."""
@@ -77,7 +77,7 @@ def test_every_kernel(gpu, m, n, k, tile):
 
 @gpu_test
 @pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (7, 19456, 2560), (48, 2048, 6144), (176, 6144, 4096),
-                                   (576, 4096, 2048), (1024, 2560, 9728), (700, 1152, 4304)])
+                                   (576, 4096, 2048), (500, 5120, 8200), (1024, 2560, 9728), (700, 1152, 4304)])
 def test_linear_at_model_sizes(gpu, m, n, k):
     """Relative RMS against float64 on the GPU: one bf16 rounding is at most 2^-8 / sqrt(3)
     = 2.3e-3; the sums' error adds less than a tenth of that."""
