@@ -154,7 +154,7 @@ __device__ __forceinline__ bool find_tile(const int* __restrict__ off, int exper
   }
   total = __builtin_amdgcn_readlane(wave_scan(total), 63) * tiles_n;
   if ((int)blockIdx.x >= total) return false;
-  const int id = xcd_tile(blockIdx.x, total), tile = id / tiles_n;
+  const int id = xcd_tile(blockIdx.x, total), tile = id / tiles_n;  // of a list with columns fastest: the right expert
   int base = 0;
   for (int e0 = 0; e0 < experts; e0 += 64) {
     const int e = min(e0 + lane, experts);
@@ -164,11 +164,12 @@ __device__ __forceinline__ bool find_tile(const int* __restrict__ off, int exper
     const uint64_t hit = __ballot(tile >= first && tile < first + n);
     if (hit) {
       const int src = __builtin_ctzll(hit);
-      const int l = __builtin_amdgcn_readlane(lo, src), at = (tile - __builtin_amdgcn_readlane(first, src)) * bm;
+      const int l = __builtin_amdgcn_readlane(lo, src), tiles = __builtin_amdgcn_readlane(n, src);
+      const int in = id - __builtin_amdgcn_readlane(first, src) * tiles_n, at = in % tiles * bm;
       out->expert = e0 + src;
       out->row0 = l + at;
       out->rows = min(bm, __builtin_amdgcn_readlane(hi, src) - l - at);
-      out->col = id % tiles_n;
+      out->col = in / tiles;
       return true;
     }
     base += __builtin_amdgcn_readlane(sum, 63);
