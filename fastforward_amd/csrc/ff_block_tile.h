@@ -19,8 +19,8 @@ constexpr int kTileThreads = 256;
 // The weights a wave multiplies its tile's rows with. base, bytes: the packed weight; frag[j]:
 // byte offset of fragment row j at k step 0 (uniform), `stride` bytes for the next k step;
 // reads past the last fragment stay in the weight or give zeros (their sums are not stored).
-// scale[s]: block scales of the fragments j with j % NS == s, one per k step.
-// base[s], likewise, the packed weight itself.
+// scale[s]: block scales of the fragments j with j % NS == s, one per k step; base[s],
+// likewise, the packed weight itself.
 template <int TJ, int NS>
 struct TileWeights {
   const uint8_t* base[NS];
@@ -29,15 +29,15 @@ struct TileWeights {
   uint32_t frag[TJ];
 };
 
-// LDS of the three stages: codes, then the rows' scales.
+// LDS of the three stages: codes, then the rows' scales and a place for values that are none.
 template <int BM>
 constexpr int tile_smem() {
-  return 3 * BM * (kBlock + 4);
+  return 3 * (BM * (kBlock + 4) + 16);
 }
 
-// acc = rows . weights^T with e4m3 rows. abase, abytes: the rows' codes; aoff(r): byte offset of row r of the tile at k step 0 (rows past the end take
-// a valid one); sbase, sbytes: the rows' scales; soff(r): index of row r's at k step 0, the
-// next step's sstride bytes on.
+// acc = rows . weights^T with e4m3 rows. abase, abytes: the rows' codes; aoff(r): byte offset of
+// row r of the tile at k step 0 (rows past the end take a valid one); sbase, sbytes (below 2^31):
+// the rows' scales; soff(r): index of row r's at k step 0, the next step's sstride bytes on.
 // A step of 128 channels is one matrix instruction per 16 x 16 products on a zero
 // accumulator and four fused multiply-adds into the running sums, which stay in ordinary
 // registers: the adds of one instruction's result run while the next instruction does.
@@ -62,18 +62,24 @@ __device__ __forceinline__ void tile_mainloop(f32x4 (&acc)[BM / 16][CW / 16], ui
 #pragma unroll
   for (int s = 0; s < NS; ++s) rW[s] = make_rsrc(w.base[s], w.bytes);
   i32x8 wq[P][TJ];
-  uint32_t wat = k0 * w.stride, wk = 4 * k0;  // offset of the next weights' k step, and of their scales
-  // The scales come as vector loads too: scalar ones return in no order with LDS reads, and
-  // waiting for them would drain those.
-  __amdgpu_buffer_rsrc_t rWS[NS];
-#pragma unroll
-  for (int s = 0; s < NS; ++s) rWS[s] = make_rsrc(w.scale[s], 4 * kt_n);
-  uint32_t wsc[P][NS];
+  uint32_t wat = k0 * w.stride;  // offset of the next weights' k step
   auto loadW = [&](int slot, int j) {
     wq[slot][j] = join(bload16(rW[j % NS], 16 * lane, w.frag[j] + wat),
                        bload16(rW[j % NS], 1024 + 16 * lane, w.frag[j] + wat));
-    if (j < NS) wsc[slot][j] = bload4(rWS[j], 0, wk);
   };
+  // Block scales: lane l has those of step l of CHUNK steps (zeros past the last); the next
+  // chunk's are loaded a chunk ahead. As vector loads: scalar ones return in no order with LDS
+  // reads, and waiting for them would drain those.
+  constexpr int CHUNK = 64 / P * P;
+  __amdgpu_buffer_rsrc_t rWS[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) rWS[s] = make_rsrc(w.scale[s], 4 * kt_n);
+  uint32_t wsc[NS], wsn[NS];
+  auto loadWS = [&](uint32_t (&to)[NS], int k) {
+#pragma unroll
+    for (int s = 0; s < NS; ++s) to[s] = bload4(rWS[s], 4 * lane, 4 * (k0 + k));
+  };
+  loadWS(wsc, 0);
 
   // LDS stage: 1 KB blocks of 8 rows, chunk c of row r at slot c ^ (r % 8) ^ (r / 8 % 2): the
   // 16 rows x 2 chunks of a fragment read fall on distinct banks per 8 and 16 lanes.
@@ -87,8 +93,12 @@ __device__ __forceinline__ void tile_mainloop(f32x4 (&acc)[BM / 16][CW / 16], ui
     adst[i] = (row >> 3) * 1024 + 128 * (row & 7) + 16 * (ch ^ (row & 7) ^ ((row >> 3) & 1));
   }
   const __amdgpu_buffer_rsrc_t rS = make_rsrc(sbase, sbytes);
-  // every thread takes a scale (a row's several threads the same one): no branch in the loop
-  const uint32_t ssrc = 4 * soff(tid % BM);
+  // A wave takes the scales of BM / 4 rows, its other lanes an offset out of range: no branch in
+  // the loop, and no line is asked for twice.
+  const int srow = tid / 64 * (BM / 4) + lane;
+  const uint32_t ssrc = lane < BM / 4 ? 4 * soff(srow) : 0x80000000u;
+  constexpr int SSTAGE = 4 * BM + 16;
+  const int sdst = lane < BM / 4 ? 4 * srow : 4 * BM;
   i32x4v ast[D][NA];
   uint32_t sst[D];
   int ak = min(k0, kt_n - 1);  // k step of the next activations
@@ -101,7 +111,7 @@ __device__ __forceinline__ void tile_mainloop(f32x4 (&acc)[BM / 16][CW / 16], ui
   auto writeA = [&](int slot, int stage) {
 #pragma unroll
     for (int i = 0; i < NA; ++i) *reinterpret_cast<i32x4v*>(smem + stage * STAGE + adst[i]) = ast[slot][i];
-    *reinterpret_cast<uint32_t*>(sc_lds + stage * (4 * BM) + 4 * (tid % BM)) = sst[slot];
+    *reinterpret_cast<uint32_t*>(sc_lds + stage * SSTAGE + sdst) = sst[slot];
   };
   const int frag = 128 * (r16 & 7) + 1024 * (r16 >> 3);
   const int sw = (r16 & 7) ^ (r16 >> 3);
@@ -111,7 +121,7 @@ __device__ __forceinline__ void tile_mainloop(f32x4 (&acc)[BM / 16][CW / 16], ui
   auto readA = [&](int stage, int i) {
     const uint8_t* st = smem + stage * STAGE + 2048 * i;
     xq[i] = join(*reinterpret_cast<const i32x4v*>(st + c0), *reinterpret_cast<const i32x4v*>(st + c1));
-    xs[i] = *reinterpret_cast<const float*>(sc_lds + stage * (4 * BM) + 64 * i + 4 * r16);
+    xs[i] = *reinterpret_cast<const float*>(sc_lds + stage * SSTAGE + 64 * i + 4 * r16);
   };
 #pragma unroll
   for (int i = 0; i < RA; ++i)
@@ -133,7 +143,6 @@ __device__ __forceinline__ void tile_mainloop(f32x4 (&acc)[BM / 16][CW / 16], ui
 #pragma unroll
     for (int j = 0; j < TJ; ++j) loadW(p, j);
     wat += w.stride;
-    wk += 4;
     __builtin_amdgcn_sched_barrier(0);
   });
   __syncthreads();
@@ -151,11 +160,11 @@ __device__ __forceinline__ void tile_mainloop(f32x4 (&acc)[BM / 16][CW / 16], ui
   for (int n = 0; n < RING; ++n) t[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int n = 0; n < LAG; ++n) sp[n] = 0.f;
-  auto step = [&](int u) {
+  auto step = [&](int u, int at) {  // at: the step's place in its chunk
     const int wr = rd == 2 ? 0 : rd + 1;
     float ws[NS];
 #pragma unroll
-    for (int v = 0; v < NS; ++v) ws[v] = __uint_as_float(wsc[u][v]);
+    for (int v = 0; v < NS; ++v) ws[v] = __uint_as_float(__builtin_amdgcn_readlane(wsc[v], at));
     // Instruction n = i TJ + j is followed by the adds of instruction n - LAG, the first LAG
     // of a step by those of the last step's last. A result is there some 40 clocks after its
     // instruction's start: with LAG 3 the matrix unit is busy 83 % of the time (one wave; 89 %
@@ -185,15 +194,20 @@ __device__ __forceinline__ void tile_mainloop(f32x4 (&acc)[BM / 16][CW / 16], ui
 #pragma unroll
     for (int n = 0; n < LAG; ++n) sp[n] = s[(ALL - LAG + n) / TJ][(ALL - LAG + n) % TJ % NS];
     wat += w.stride;
-    wk += 4;
     rd = wr;
   };
   // Whole rounds of P steps: a way out of the loop, or past some of its loads, inside a round
   // would cost every round the wait counts of the shorter way. The weights of steps past the
   // last lie past their end (w.bytes), where loads give zeros; the activations are the row's
   // own, so a NaN stays in its row.
-  for (int kt = 0; kt < steps; kt += P)
-    static_for<0, P>([&](auto U_) { step(decltype(U_)::value); });
+  for (int c = 0; c < steps; c += CHUNK) {
+    loadWS(wsn, c + CHUNK);
+    const int n = min(CHUNK, steps - c);
+    for (int at = 0; at < n; at += P)
+      static_for<0, P>([&](auto U_) { step(decltype(U_)::value, at + decltype(U_)::value); });
+#pragma unroll
+    for (int s = 0; s < NS; ++s) wsc[s] = wsn[s];
+  }
 #pragma unroll
   for (int n = 0; n < LAG; ++n) fma4(acc[(ALL - LAG + n) / TJ][(ALL - LAG + n) % TJ], t[(ALL - LAG + n) % RING], sp[n]);
 }

@@ -334,7 +334,7 @@ static int check_gemm(const char* who, const void* packed, const float* ws, cons
   const int64_t n16 = (n + 15) / 16 * 16, kt_n = (k + kBlock - 1) / kBlock;
   FF_REQUIRE(m >= 0 && m < kMaxCodes && n > 0 && k > 0 && n < kMaxCodes && k < (1 << 24) && ldy >= n &&
                  n16 * kt_n * kBlock < kMaxCodes && n16 * (kt_n + 8) * kBlock < 2 * kMaxCodes &&
-                 m * kt_n < (1ll << 30) && m * n < (1ll << 38),
+                 m * kt_n < (1ll << 29) && m * n < (1ll << 38),
              "%s: bad sizes m=%lld n=%lld k=%lld", who, (long long)m, (long long)n, (long long)k);
   if (m == 0) return FF_OK;
   FF_REQUIRE(packed && ws && y, "%s: null pointer", who);
