@@ -82,6 +82,9 @@ __global__ __launch_bounds__(256) void unpack_block_kernel(const uint8_t* __rest
 
 // ---------------------------------------------------------------- row quantiser
 
+// 16 lanes a row and 128 channels: the block is read once and kept in registers between its
+// maximum and its codes. Bound by memory: 4096 x 25600 in 66 us, 4.8 TB/s (a large copy:
+// 5.2); 576 x 4096 3.5 us, about the shortest a launch takes.
 __global__ __launch_bounds__(256) void quant_rows_block_kernel(const bf16_t* __restrict__ x, int64_t ldx,
                                                                uint8_t* __restrict__ q, float* __restrict__ scales,
                                                                int64_t rows, int64_t k, int kt_n, int vec) {
@@ -91,7 +94,10 @@ __global__ __launch_bounds__(256) void quant_rows_block_kernel(const bf16_t* __r
 
 // ---------------------------------------------------------------- few rows
 
-// INLINE: the workgroup quantises the rows (at most kRowsMax) into LDS itself.
+// INLINE: the workgroup quantises the rows (at most kRowsMax) into LDS itself, while its first
+// weights are on the way: a launch of its own would take longer than the whole product. Bound
+// by the weights' bytes and the launch: 1 x 4096 x 4096 in 4.3 us (16.9 MB at 3.9 TB/s), 8 waves
+// with four steps in flight each.
 template <int NJ, bool INLINE>
 __global__ __launch_bounds__(kSkinnyThreads) void skinny_kernel(
     const bf16_t* __restrict__ x, int64_t ldx, int vec, const uint8_t* __restrict__ q, const float* __restrict__ qs,
@@ -181,6 +187,13 @@ __global__ __launch_bounds__(kSkinnyThreads) void skinny_kernel(
 // BM x 4 CW tiles, KG groups of 4 waves that share the k steps of a tile. Tile order: groups
 // of 8 row tiles, within a group row tiles fastest, so that the tiles an XCD runs at one
 // time share rows and weights.
+// 4096 x 5120 x 25600 on 128 x 128 tiles: 535 us, 2.0 PFLOP/s (a library product without block
+// scales: 2.8). The matrix unit is busy 52 % of the time: the waves' fragments from LDS (64 KB a
+// step and CU, 512 clocks, as long as its matrix instructions), the loads (32 KB, 512 clocks of
+// the return path) and the adds (256 clocks) run beside it, not wholly overlapped. One tile of 128 x
+// 64 a wave would halve the first, but leaves one wave a SIMD: 1.98 PFLOP/s. Short products
+// are a chain of steps on few CUs: 333 x 1152 x 4304 on 32 x 64 tiles in two k groups 8.2 us,
+// 576 x 6144 x 4096 24.6 us (240 tiles of 128 x 128).
 template <int BM, int CW, int P, int D, int KG, int OCC>
 __global__ __launch_bounds__(kTileThreads* KG, OCC) void tile_kernel(
     const uint8_t* __restrict__ q, const float* __restrict__ qs, const uint8_t* __restrict__ wp,
