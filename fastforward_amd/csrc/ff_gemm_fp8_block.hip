@@ -4,7 +4,7 @@
 // Few rows (skinny_kernel): a workgroup of 8 waves owns 16 rows x 16 or 32 weight rows and
 // its waves take the k steps in turn (wave w: steps w, w + 8, ..), so that even 4096
 // columns make 256 workgroups that read the weights from every channel of memory; their
-// sums are added through LDS in wave order. Up to four rows are quantised in the same
+// sums are added through LDS in wave order. A few short rows are quantised in the same
 // launch.
 // More rows (tile_kernel): tiles of 32 x 64, 64 x 128 or 128 x 128 (ff_block_tile.h).
 #include "ff_block_tile.h"
@@ -14,8 +14,7 @@ using namespace ff;
 namespace {
 
 constexpr int kSkinnyThreads = 512, kSkinnyWaves = kSkinnyThreads / 64;
-constexpr int kRowsMax = 4;             // rows that the product's own launch quantises
-constexpr int kRowsMaxCodes = 49152;    // their codes' LDS
+constexpr int kRowsMaxCodes = 128 * kBlock;  // codes that the product's own launch quantises
 
 // ---------------------------------------------------------------- setup
 
@@ -94,7 +93,7 @@ __global__ __launch_bounds__(256) void quant_rows_block_kernel(const bf16_t* __r
 
 // ---------------------------------------------------------------- few rows
 
-// INLINE: the workgroup quantises the rows (at most kRowsMax) into LDS itself, while its first
+// INLINE: the workgroup quantises the rows (at most 16) into LDS itself, while its first
 // weights are on the way: a launch of its own would take longer than the whole product. Bound
 // by the weights' bytes and the launch: 1 x 4096 x 4096 in 4.3 us (16.9 MB at 3.9 TB/s), 8 waves
 // with four steps in flight each.
@@ -419,9 +418,14 @@ extern "C" int ff_gemm_fp8_block(const void* q, const float* scales, const void*
   return gemm_block(q, scales, packed, wscales, y, ldy, m, n, k, (hipStream_t)stream);
 }
 
-// Whether m rows of k channels are quantised inside the product's launch.
-static bool rows_inline(int64_t m, int64_t k) {
-  return m <= kRowsMax && m * ((k + kBlock - 1) / kBlock * kBlock) <= kRowsMaxCodes;
+// Whether m rows of k channels are quantised inside the product's launch. Each workgroup then
+// does that work, so it is bounded per CU: 8192 columns are a workgroup or two for each. In a graph,
+// weights from memory, us (in the launch / in one of their own): 4 x 4096 x 4096 8.2 / 8.4, 3 x
+// 6144 x 4096 10.0 / 10.4, 4 x 4096 x 12288 19.7 / 15.3, 1 x 24576 x 4096 22.0 / 21.5, 2 x 24576 x
+// 4096 24.0 / 21.5, 3 x 5120 x 8192 16.3 / 15.5; 6 x 2560 x 2560 6.1 / 6.4. A launch saved is also
+// two to three us of the host's.
+static bool rows_inline(int64_t m, int64_t n, int64_t k) {
+  return m <= 16 && m * ((k + kBlock - 1) / kBlock) * ((n + 8191) / 8192) <= kRowsMaxCodes / kBlock;
 }
 
 static int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
@@ -430,7 +434,7 @@ extern "C" int ff_linear_fp8_block_workspace(int64_t m, int64_t n, int64_t k, in
   FF_REQUIRE(bytes, "ff_linear_fp8_block_workspace: null pointer");
   FF_REQUIRE(m >= 0 && n > 0 && k > 0 && m < kMaxCodes && k < kMaxCodes, "ff_linear_fp8_block_workspace: bad sizes");
   const int64_t kt_n = (k + kBlock - 1) / kBlock;
-  *bytes = rows_inline(m, k) ? 0 : align256(m * kt_n * kBlock) + m * kt_n * 4;
+  *bytes = rows_inline(m, n, k) ? 0 : align256(m * kt_n * kBlock) + m * kt_n * 4;
   return FF_OK;
 }
 
@@ -442,7 +446,7 @@ extern "C" int ff_linear_fp8_block(const void* x, int64_t ldx, const void* packe
   FF_REQUIRE(x, "ff_linear_fp8_block: null pointer");
   FF_REQUIRE(ff_aligned(x, 2) && ldx >= 0, "ff_linear_fp8_block: alignment");
   const hipStream_t st = (hipStream_t)stream;
-  if (rows_inline(m, k)) {
+  if (rows_inline(m, n, k)) {
     launch_skinny<true>((const bf16_t*)x, ldx, nullptr, nullptr, (const uint8_t*)packed, wscales, (bf16_t*)y, ldy, m,
                            n, k, st);
     FF_LAUNCH_CHECK("ff_linear_fp8_block");

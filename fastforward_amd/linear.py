@@ -431,8 +431,8 @@ class BlockFP8Linear:
         return q, s
 
     def gemm(self, q, s):
-        """The product from rows quantised by ``quantize``: the bits of ``op(x)`` for more rows
-        than run in one launch (four)."""
+        """The product from rows quantised by ``quantize``: the bits of ``op(x)`` for more than
+        16 rows (fewer may run in one launch, with another order of the sums)."""
         n, k = self.weight.shape
         m = q.shape[0]
         assert q.dtype == E4M3 and q.shape[1] == _blocks(k) * BLOCK and q.is_contiguous()

@@ -487,8 +487,8 @@ int ff_quant_rows_fp8_block(const void* x, int64_t ldx, void* q, float* scales, 
  * up to 16; sums in fp32. y (m, n), row stride ldy. */
 int ff_gemm_fp8_block(const void* q, const float* scales, const void* packed, const float* wscales, void* y,
                       int64_t ldy, int64_t m, int64_t n, int64_t k, ff_stream_t stream);
-/* The whole linear from bf16 rows x (row stride ldx): quantisation and product. Up
- * to four rows run in one launch. workspace: ff_linear_fp8_block_workspace bytes
+/* The whole linear from bf16 rows x (row stride ldx): quantisation and product. A few
+ * short rows (a row of up to 16384 channels, four of 4096) run in one launch. workspace: ff_linear_fp8_block_workspace bytes
  * (0: may be NULL), 16-byte aligned. */
 int ff_linear_fp8_block_workspace(int64_t m, int64_t n, int64_t k, int64_t* bytes);
 int ff_linear_fp8_block(const void* x, int64_t ldx, const void* packed, const float* wscales, void* y, int64_t ldy,
