@@ -16,6 +16,7 @@ P = ctypes.c_void_p
 I64 = ctypes.c_int64
 I32 = ctypes.c_int
 F32 = ctypes.c_float
+F64 = ctypes.c_double
 PI64 = ctypes.POINTER(ctypes.c_int64)
 PI32 = ctypes.POINTER(ctypes.c_int)
 
@@ -96,7 +97,7 @@ SIGNATURES = {
     "ff_gemm_fp8_block": [P, P, P, P, P, I64, I64, I64, I64, P],
     "ff_linear_fp8_block_workspace": [I64, I64, I64, PI64],
     "ff_linear_fp8_block": [P, I64, P, P, P, I64, I64, I64, I64, P, I64, P],
-    "ff_moe_route": [P, I32, I64, P, P, P, I64, I64, I64, I32, I64, I64, I32, F32, P],
+    "ff_moe_route": [P, I32, I64, P, P, P, I64, I64, I64, I32, I64, I64, I32, F64, P],
     "ff_moe_experts_workspace": [I64, I64, I64, I64, I64, PI64],
     "ff_moe_experts": [P, I64, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, P, I64, P],
 }

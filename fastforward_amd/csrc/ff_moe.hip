@@ -105,7 +105,7 @@ template <int LPR, int EPL, bool F32, bool BIAS>
 __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(
     const void* __restrict__ logits, int64_t ld, const float* __restrict__ bias, float* __restrict__ weights,
     int* __restrict__ ids, int64_t t, int experts, int top_k, int sigmoid, int groups, int top_groups, int renormalize,
-    float scale) {
+    double scale) {
   using Key = std::conditional_t<BIAS, double, float>;
   constexpr int kRows = 64 / LPR;  // rows of a wave
   __shared__ Key sc[kRouteWaves * kRows][LPR * EPL];
@@ -215,7 +215,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(
   if (!live || li >= top_k) return;
   if (renormalize) w = total > 0 ? w / total : 0.0;
   ids[row * top_k + li] = poisoned ? li : mine_id;
-  weights[row * top_k + li] = poisoned ? __builtin_nanf("") : (float)(w * (double)scale);
+  weights[row * top_k + li] = poisoned ? __builtin_nanf("") : (float)(w * scale);
 }
 
 // ---------------------------------------------------------------- pairs by expert
@@ -634,7 +634,7 @@ void launch_tiles(const Shape& s, uint8_t* w, const Layout& l, const void* gate_
 
 extern "C" int ff_moe_route(const void* logits, int logits_f32, int64_t ld, const float* bias, float* weights, int* ids,
                             int64_t t, int64_t experts, int64_t top_k, int sigmoid, int64_t groups, int64_t top_groups,
-                            int renormalize, float scale, ff_stream_t stream) {
+                            int renormalize, double scale, ff_stream_t stream) {
   FF_REQUIRE(t >= 0 && t < (1ll << 25) && experts > 0 && experts <= kMaxExperts && ld >= 0 && top_k > 0 &&
                  top_k <= 64 && top_k <= experts && groups > 0 && groups <= 64 && experts % groups == 0 &&
                  top_groups > 0 && top_groups <= groups && top_groups * (experts / groups) >= top_k,

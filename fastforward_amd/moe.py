@@ -36,8 +36,9 @@ def route(logits, top_k, score="softmax", bias=None, groups=1, top_groups=None, 
 
     A logit of -inf switches its expert off; where fewer than ``top_k`` are left, the
     rest have id -1 and weight 0. A row with a NaN (or +inf under softmax) has NaN
-    weights. Scores are computed in 64 bits; without a bias experts are compared by their
-    logits (scores rise with them), with one by score + bias in 64 bits."""
+    weights. Scores and weights are 64-bit until the weights' one rounding; without a bias
+    experts are compared by their logits (scores rise with them), with one by score +
+    bias in 64 bits."""
     assert logits.dim() == 2 and logits.dtype in (BF16, F32) and score in ("softmax", "sigmoid")
     t, e = logits.shape
     top_groups = groups if top_groups is None else top_groups

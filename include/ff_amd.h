@@ -507,13 +507,13 @@ int ff_linear_fp8_block(const void* x, int64_t ldx, const void* packed, const fl
  * and their p to weights (t, top_k) fp32, divided by their sum with renormalize and
  * multiplied by scale. A logit of -inf switches its expert off; where fewer than
  * top_k are left the rest have id -1 and weight 0. A row with a NaN (or +inf under
- * softmax) has ids 0 .. top_k - 1 and NaN weights. Scores are computed in 64 bits;
- * without a bias experts are compared by their logits, with one by score + bias in 64
- * bits. experts <= 1024, top_k <= 64, groups <= 64,
+ * softmax) has ids 0 .. top_k - 1 and NaN weights. Scores and weights are 64-bit until
+ * the weights' one rounding; without a bias experts are compared by their logits, with
+ * one by score + bias in 64 bits. experts <= 1024, top_k <= 64, groups <= 64,
  * top_groups * experts / groups >= top_k. */
 int ff_moe_route(const void* logits, int logits_f32, int64_t ld, const float* bias, float* weights, int* ids,
                  int64_t t, int64_t experts, int64_t top_k, int sigmoid, int64_t groups, int64_t top_groups,
-                 int renormalize, float scale, ff_stream_t stream);
+                 int renormalize, double scale, ff_stream_t stream);
 
 /* y[t] = bf16(sum_j weights[t, j] D_e bf16(silu(G_e x[t]) * (U_e x[t]))), e = ids[t, j],
  * with x quantised as by ff_quant_rows_fp8_block, sums in fp32. gate_up: the codes

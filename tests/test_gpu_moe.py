@@ -113,6 +113,16 @@ def test_route_strides_graph_stream(gpu):
         assert all(torch.equal(a, b) for a, b in zip(out, moe.route(static, 4)))
 
 
+@gpu_test
+@pytest.mark.parametrize("scale", [2.446, 2.827, 1 / 3])
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_route_scale_between_fp32_numbers(gpu, scale, renormalize):
+    """A scale that fp32 does not hold: the weights have one rounding all the same."""
+    l = torch.randn(200, 64, generator=_g(8)) * 2
+    for bias in (None, torch.randn(64, generator=_g(9)) * 0.1):
+        _check_route(l, 8, score="sigmoid", scale=scale, renormalize=renormalize, bias=bias)
+
+
 # ---------------------------------------------------------------- experts
 
 def _weights(e, h, i, seed=0):
