@@ -25,7 +25,8 @@ constexpr int kBlock = 128;  // rows and channels that share a scale
 // k channels, lane s of 16 consecutive lanes holding channels 8 s .. + 7 (zeros
 // past k): scale = max(amax, 1e-12) / 448, code = e4m3(x / scale), both quotients
 // correctly rounded fp32. vec: the row may be read 16 bytes at a time. A NaN
-// keeps its code; a row's infinity makes the scale infinite and its own code NaN.
+// keeps its code and is not in amax; an infinity makes the scale infinite, its own code
+// NaN and the block's other codes 0.
 __device__ __forceinline__ u32x2 quant_group16(const bf16_t* __restrict__ row, int64_t k, int kt, int s, bool vec,
                                                float* scale) {
   const int64_t c = (int64_t)kt * kBlock + 8 * s;
@@ -45,7 +46,9 @@ __device__ __forceinline__ u32x2 quant_group16(const bf16_t* __restrict__ row, i
   a = fmaxf(a, dpp<kDppRowMirror>(a));
   const float sc = fmaxf(a, 1e-12f) / 448.0f;
   *scale = sc;
-  return quant8(v, sc, 1.0f / sc);
+  // an infinite divisor would make the quotient's correction 0 * inf; with 0 in its place
+  // and the reciprocal 0 the quotients are x * 0
+  return quant8(v, sc == __builtin_inff() ? 0.0f : sc, 1.0f / sc);
 }
 
 // Codes q (rows, 128 kt_n) and scales (kt_n, rows) of ROWS rows x 128 channels by 16 ROWS

@@ -479,7 +479,9 @@ int ff_pack_weight_fp8_block(const void* w, void* packed, int64_t batch, int64_t
 int ff_unpack_weight_fp8_block(const void* packed, void* w, int64_t batch, int64_t n, int64_t k, int64_t n_pad,
                                ff_stream_t stream);
 /* Rows x (rows, k) bf16, row stride ldx, any alignment: codes q (rows, 128
- * ceil(k / 128)), zeros past k, 16-byte aligned, and scales (ceil(k / 128), rows). */
+ * ceil(k / 128)), zeros past k, 16-byte aligned, and scales (ceil(k / 128), rows). A
+ * NaN is not in amax and keeps its code; an infinity makes the scale infinite, its own
+ * code NaN and the block's others 0: either way the row's products are NaN. */
 int ff_quant_rows_fp8_block(const void* x, int64_t ldx, void* q, float* scales, int64_t rows, int64_t k,
                             ff_stream_t stream);
 /* y = bf16(sum over blocks of (codes . codes) * row scale * weight scale) from rows

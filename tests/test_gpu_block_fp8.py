@@ -151,6 +151,22 @@ def test_special_values(gpu, m):
 
 
 @gpu_test
+def test_quantise_special_values(gpu):
+    """Beside an infinity x / scale is 0 and its own code NaN; a NaN keeps its code and
+    leaves the others to the largest number."""
+    inf, nan = float("inf"), float("nan")
+    x, codes, scale = _case(8, 16, 300)
+    x[1, 7], x[2, 128:256], x[3, 299], x[4, 0], x[4, 1] = inf, -inf, -inf, inf, -inf
+    x[5, 3], x[6, 128:256], x[7, 298] = nan, nan, nan
+    q, s = _op(codes, scale).quantize(x.to(DEV))
+    q = q.cpu()
+    none = torch.nn.functional.pad(~x.isfinite(), (0, 84))
+    want_q, want_s = M.quant_rows(x.masked_fill(x.isnan(), 0))
+    assert torch.equal(s.cpu(), want_s) and torch.equal(q.float().isnan(), none)
+    assert torch.equal(q.view(torch.uint8)[~none], want_q.view(torch.uint8)[~none])
+
+
+@gpu_test
 @pytest.mark.parametrize("m", [1, 6, 96])
 def test_graph_and_stream(gpu, m):
     """Captured once, replayed on new inputs with eager calls between; on a side stream."""
