@@ -143,13 +143,16 @@ class Router:
         self.zero = torch.zeros(weight.shape[0], device=weight.device, dtype=BF16)     # ff_gemm_bf16 takes a bias
 
     def __call__(self, x):
-        assert x.dim() == 2 and x.dtype == BF16 and x.shape[1] == self.weight.shape[1] and x.stride(1) == 1
+        assert x.dim() == 2 and x.dtype == BF16 and x.shape[1] == self.weight.shape[1]
         check_here(x, self.weight)
         m, k = x.shape
         n = self.weight.shape[0]
+        lda = k if m == 1 else x.stride(0)
+        if x.stride(1) != 1 or lda < k or lda % 8 or x.data_ptr() % 16:     # what ff_gemm_bf16 reads in place
+            x, lda = x.clone(memory_format=torch.contiguous_format), k
         y = x.new_empty((m, n))
         if m:
-            call("ff_gemm_bf16", ptr(x), x.stride(0), ptr(self.weight), ptr(self.zero), ptr(y), n, None, 0, m, n, k, 0,
+            call("ff_gemm_bf16", ptr(x), lda, ptr(self.weight), ptr(self.zero), ptr(y), n, None, 0, m, n, k, 0,
                  stream())
         return y
 

@@ -311,6 +311,21 @@ def test_experts_two_streams(gpu):
 
 
 @gpu_test
+def test_moe_strides(gpu):
+    """The whole MLP, its router's product included, on rows of any stride and alignment."""
+    from fastforward_amd.moe import MoE, Router
+    h, i, e = 128, 72, 8
+    op = MoE(Router((torch.randn(e, h, generator=_g(1)) * 0.1).to(BF16).to(DEV)), _experts(_weights(e, h, i)), 3)
+    base = torch.randn(2 * h + 9, 2 * h + 3, generator=_g(2)).to(BF16).to(DEV)
+    for x in (base[:9, 1:h + 1], base[:9, 8:h + 8], base[:9, :2 * h:2], base[:1, :h].expand(9, h), base[:h, :6].T,
+              base[:h, :1].T, base[:h, :1].contiguous().T, base[None, :4, 3:h + 3], base[0, 5:h + 5], base[:0, :h]):
+        flat = x.reshape(-1, h)
+        copy = torch.empty(flat.shape, dtype=BF16, device=DEV).copy_(flat)
+        assert torch.equal(op.router(flat), op.router(copy))
+        assert torch.equal(op(x), op(copy).reshape(x.shape))
+
+
+@gpu_test
 def test_experts_from_bf16(gpu):
     from fastforward_amd.moe import Experts
     e, h, i = 3, 136, 200
