@@ -52,14 +52,14 @@ class Tensors:
     def __contains__(self, name):
         return name in self.where
 
-    def raw(self, name, device="cuda"):
-        """The tensor in its own type."""
+    def raw(self, name, device="cuda", dtype=None):
+        """The tensor in its own type, or in ``dtype`` (converted before it is moved)."""
         if name not in self.where:
             raise KeyError(f"checkpoint has no tensor {name!r}")
         fn = self.where[name]
         if fn not in self._files:
             self._files[fn] = self._open(fn, "pt")
-        return self._files[fn].get_tensor(name).to(device=device).contiguous()
+        return self._files[fn].get_tensor(name).to(device=device, dtype=dtype).contiguous()
 
     def blocks(self, name, device="cuda"):
         """(codes, block scales fp32) of a block-scaled FP8 weight, None for another."""
@@ -74,7 +74,7 @@ class Tensors:
     def get(self, name, device="cuda"):
         block = self.blocks(name, device)
         if block is None:
-            return self.raw(name, device).to(BF16)
+            return self.raw(name, device, BF16)
         codes, scales = block
         n, k = codes.shape
         return (codes.float() * scales.repeat_interleave(BLOCK, 0)[:n].repeat_interleave(BLOCK, 1)[:, :k]).to(BF16)

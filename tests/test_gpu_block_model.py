@@ -132,6 +132,22 @@ def test_block_checkpoint_tensors(tmp_path):
 
 
 @pytest.mark.gpu
+def test_tensors_reach_the_gpu_in_bf16(gpu, tmp_path):
+    """A tensor of another type is converted on its way: the GPU holds its bf16 copy only."""
+    from safetensors.torch import save_file
+    from fastforward_amd.checkpoint import Tensors
+    w = torch.randn(2048, 1024, generator=torch.Generator().manual_seed(4))
+    save_file({"w": w}, os.path.join(tmp_path, "model.safetensors"))
+    ts = Tensors(str(tmp_path))
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = ts.get("w", DEV)
+    assert torch.cuda.max_memory_allocated() - before <= 2 * w.numel() + 512
+    assert torch.equal(got.cpu(), w.to(BF16))
+
+
+@pytest.mark.gpu
 def test_block_checkpoint_loads(gpu, tmp_path):
     """fp8_block takes the checkpoint's codes and scales as they are, fp8 the dequantised weight."""
     from fastforward_amd.checkpoint import load_pretrained
