@@ -558,6 +558,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ 
 struct Shape {
   int64_t t, h, i;
   int top_k, experts;
+  int tune = ff_tuning(FF_TUNE_MOE_TILE);  // read once: the workspace's layout and the launches go by the same value
   int64_t pairs() const { return t * top_k; }
   int kth() const { return (int)((h + kBlock - 1) / kBlock); }
   int kti() const { return (int)((i + kBlock - 1) / kBlock); }
@@ -565,7 +566,6 @@ struct Shape {
   // 36.9 against 40.0 on tiles, 8 tokens 68.8 against 54.0).
   // The row has to fit in LDS and either grid's threads in 32 bits.
   bool by_pair() const {
-    const int tune = ff_tuning(FF_TUNE_MOE_TILE);
     return (tune ? tune == 1 : pairs() <= 32) && (int64_t)kth() * kBlock <= kInlineCodes &&
            pairs() * 8 * (kth() > kti() ? kth() : kti()) < (1 << 22);
   }
@@ -725,8 +725,7 @@ extern "C" int ff_moe_experts(const void* x, int64_t ldx, const float* weights, 
   // Rows of an expert on average: with few, tiles of 32 rows (us on 32- and 64-row tiles, 128
   // experts, 8 a token, h 2048, i 768: 8 tokens 54.0 and 61.7, 32 tokens 101 and 111, 128 tokens
   // 122 and 121, 512 tokens 163 and 155, 4096 tokens 581 and 429).
-  const int tune = ff_tuning(FF_TUNE_MOE_TILE);
-  if (tune ? tune == 2 : s.pairs() / experts < 8)
+  if (s.tune ? s.tune == 2 : s.pairs() / experts < 8)
     launch_tiles<32, 32, 3, 32, 2>(s, w, l, gate_up, gate_up_scales, down, down_scales, st);
   else
     launch_tiles<64, 64, 3, 64, 1>(s, w, l, gate_up, gate_up_scales, down, down_scales, st);

@@ -311,6 +311,51 @@ def test_experts_two_streams(gpu):
 
 
 @gpu_test
+def test_path_and_workspace_agree(gpu):
+    """The path is chosen once a call, so a knob set from another thread meanwhile moves the
+    next call: every result is one path's or the other's."""
+    import threading
+    from fastforward_amd._lib import call, entry, stream
+    t, k, e, h, i = 4, 2, 6, 136, 200
+    op = _experts(_weights(e, h, i))
+    x, w, ids = (v.to(DEV) for v in _tokens(t, k, e, h))
+    need = ctypes.c_int64(0)
+
+    def run(y, ws):
+        entry("ff_moe_experts")(x.data_ptr(), h, w.data_ptr(), ids.data_ptr(), op.gate_up._packed.data_ptr(),
+                                op.gate_up_scale.data_ptr(), op.down._packed.data_ptr(), op.down_scale.data_ptr(),
+                                y.data_ptr(), h, t, k, e, h, i, ws.data_ptr(), ws.numel(), stream())
+
+    stop, want, sizes = threading.Event(), [], []
+
+    def flip():
+        while not stop.is_set():
+            call("ff_set_tuning", 13, 1)
+            call("ff_set_tuning", 13, 2)
+    thread = threading.Thread(target=flip)
+    try:
+        for tile in (1, 2):
+            call("ff_set_tuning", 13, tile)
+            call("ff_moe_experts_workspace", t, k, e, h, i, ctypes.byref(need))
+            sizes.append(need.value)
+            ws, y = torch.empty(need.value, dtype=torch.uint8, device=DEV), torch.empty(t, h, dtype=BF16, device=DEV)
+            run(y, ws)
+            want.append(y)
+        assert sizes[0] < sizes[1]
+        ws, ys = torch.empty(sizes[1], dtype=torch.uint8, device=DEV), torch.empty(300, t, h, dtype=BF16, device=DEV)
+        thread.start()
+        for y in ys:
+            run(y, ws)
+    finally:
+        stop.set()
+        if thread.ident is not None:
+            thread.join()
+        call("ff_set_tuning", 13, 0)
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[0]) or torch.equal(y, want[1]) for y in ys)
+
+
+@gpu_test
 def test_moe_strides(gpu):
     """The whole MLP, its router's product included, on rows of any stride and alignment."""
     from fastforward_amd.moe import MoE, Router
