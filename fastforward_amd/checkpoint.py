@@ -146,9 +146,14 @@ def load_lm(path, cfg, option_ids, mode="fp8", device="cuda", static_bound=8.0, 
     ``mode`` "int4_half" / "int4_ffn" mixes the int4 bank (the reference's
     asymmetric group-32 Int4) into the interior layers (``bank_of``) and
     takes the other linears in the ``fp8_bank`` format ("fp8" or
-    "fp8_static")."""
+    "fp8_static"). Layers have one dense MLP each: ValueError, before anything is
+    loaded, for a mixture of experts (``moe.Experts`` takes such weights one by one)."""
     ts = tensors or Tensors(path)
     p = "model.language_model."
+    for j in range(cfg.layers):
+        q = f"{p}layers.{j}.mlp."
+        if q + "gate_proj.weight" not in ts and any(name.startswith(q + "experts.") for name in ts.where):
+            raise ValueError(f"layer {j} of the checkpoint is a mixture of experts, which load_lm does not read")
     embed = ts.get(p + "embed_tokens.weight", device)
     layers = []
 

@@ -131,6 +131,20 @@ def test_block_checkpoint_tensors(tmp_path):
         Tensors(path).get(name, "cpu")
 
 
+def test_expert_checkpoint_is_refused(tmp_path):
+    """By name, and before any tensor is read."""
+    from safetensors.torch import save_file
+    from fastforward_amd.checkpoint import Tensors, load_lm
+    from fastforward_amd.runtime import LMConfig
+    q = "model.language_model.layers."
+    save_file({q + "0.mlp.gate_proj.weight": torch.zeros(8, 4), q + "1.mlp.gate.weight": torch.zeros(2, 4),
+               q + "1.mlp.experts.down_proj": torch.zeros(2, 8, 4)}, os.path.join(tmp_path, "model.safetensors"))
+    cfg = LMConfig("experts", 2, 4, 1, 1, 128, 8, 10)
+    for ts in (None, Tensors(str(tmp_path))):
+        with pytest.raises(ValueError, match="layer 1 .* mixture of experts"):
+            load_lm(str(tmp_path), cfg, [0, 1], mode="fp8_block", device="cpu", tensors=ts)
+
+
 @pytest.mark.gpu
 def test_tensors_reach_the_gpu_in_bf16(gpu, tmp_path):
     """A tensor of another type is converted on its way: the GPU holds its bf16 copy only."""
