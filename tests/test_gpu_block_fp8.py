@@ -95,6 +95,42 @@ def test_linear_at_model_sizes(gpu, m, n, k):
     assert bool(((y - want).abs() <= 2.0 ** -8 * want.abs() + want.square().mean(1, keepdim=True).sqrt() / 64).all())
 
 
+# A wave of the tile kernels holds the block scales of 63 or 64 k steps at once, of its k group where
+# there are two: these k blocks come after them.
+LATE_BLOCKS = (63, 64, 128, 129)
+
+
+def late_scales(shape, seed):
+    """Block scales over a factor of 256, those of LATE_BLOCKS 16 times larger: a scale taken
+    from another block shows in the whole sum."""
+    s = torch.exp2(torch.randint(-8, 1, shape, generator=_g(seed)).float()) * 1e-3
+    for b in LATE_BLOCKS:
+        s[..., b:b + 1] *= 16
+    return s
+
+
+@gpu_test
+@pytest.mark.parametrize("k", [8264, 16584])
+def test_more_block_scales_than_lanes(gpu, k):
+    """Every kernel past the first scales that its waves load. Beside the oracle's bound (for
+    every 32 products 2^-9 of the largest) there are 130 fp32 additions, each off by 2^-24
+    of at most 32 times the same sum: 2^-12 of it, an eighth more."""
+    from fastforward_amd._lib import call
+    m, n = 33, 136
+    x, codes, scale = _case(m, n, k)
+    scale = late_scales(scale.shape, 7)
+    op = _op(codes, scale)
+    q, s = op.quantize(x.to(DEV))
+    want, bound = M.linear(x, codes, scale)
+    for tile in range(6):
+        call("ff_set_tuning", 12, tile)
+        try:
+            y = op.gemm(q, s).cpu().double()
+        finally:
+            call("ff_set_tuning", 12, 0)
+        assert ((y - want).abs() <= 1.125 * bound).all(), f"tile {tile}"
+
+
 @gpu_test
 def test_weight_quantisation(gpu):
     from fastforward_amd.linear import BlockFP8Linear

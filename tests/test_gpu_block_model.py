@@ -98,6 +98,116 @@ def test_block_step(gpu):
         torch.cuda.synchronize()
 
 
+class Observe:
+    """An op that keeps what it was given and what it returned."""
+
+    def __init__(self, op, seen, name):
+        self.op, self.seen, self.name = op, seen, name
+
+    def __getattr__(self, name):
+        return getattr(self.op, name)
+
+    def __call__(self, x):
+        y = self.op(x)
+        self.seen[self.name] = (x.clone(), y.clone())
+        return y
+
+
+def _check_moe(moe, x, y, top_k, what):
+    x, y = x.reshape(-1, x.shape[-1]), y.reshape(-1, y.shape[-1])
+    weights, chosen = M.route(moe.router(x).cpu(), top_k)
+    e = moe.experts
+    want, bound = M.experts(x.cpu(), weights, chosen, e.gate_up.cpu(), e.gate_up_scale.cpu(), e.down.cpu(),
+                            e.down_scale.cpu())
+    assert ((y.cpu().double() - want).abs() <= bound + 1e-9).all(), what
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("experts", [0, 12])
+@pytest.mark.parametrize("pick", [69, 31])
+def test_last_layer_row(gpu, experts, pick):
+    """The last layer runs one row: every op of it, dense and with experts, is given what the
+    residual stream before it and the op before it make, and the logits are the readout of
+    its result."""
+    from oracle import ops as O
+    from fastforward_amd import ops
+    from fastforward_amd.runtime import LMConfig, Runtime
+    from fastforward_amd.synthetic import make_model
+    from tests.helpers import assert_bf16_close
+    cfg = LMConfig("tail", 2, 512, 4, 2, 128, 136 if experts else 1024, 1000, experts=experts,
+                   top_k=3 if experts else 0)
+    w = make_model(cfg, mode="fp8_block", seed=6, norm_jitter=0.2, n_options=4)
+    ids, pos, _ = _request(cfg)
+    rt = Runtime(cfg, w, 70)
+    rt.set_inputs(ids, pos, pick)
+    eager = rt.step().clone()
+    lw, seen, trace = w.layers[-1], {}, []
+    plain = {name: op for name, op in vars(lw).items() if name in ("qkv", "o", "gateup", "down", "moe") and op}
+    try:
+        for name, op in plain.items():
+            setattr(lw, name, Observe(op, seen, name))
+        logits = rt.step(trace=trace).clone()
+    finally:
+        for name, op in plain.items():
+            setattr(lw, name, op)
+    assert torch.equal(logits, eager)
+
+    def linear(name):
+        x, y = seen[name]
+        op = plain[name]
+        want, bound = M.linear(x.reshape(-1, x.shape[-1]).cpu(), op.weight.cpu(), op.scale.cpu())
+        assert ((y.reshape(want.shape).cpu().double() - want).abs() <= bound).all(), name
+
+    h = trace[-1][None]
+    x = ops.fast_norm(h, lw.input_norm)
+    assert torch.equal(seen["qkv"][0], x)
+    linear("qkv")
+    # the attention of every row: the same row twice, each within a rounding of its weights and of its result
+    attn = rt._attention_generic(lw, x, rt.cos[None], rt.sin[None])[0, pick].double()
+    assert float((seen["o"][0].reshape(-1).double() - attn).norm() / attn.norm()) <= 2.0 ** -6
+    linear("o")
+    residual, post = ops.add_rms(h[:, pick:pick + 1].contiguous(), seen["o"][1].reshape(1, 1, -1), None, lw.post_norm)
+    if experts:
+        x, mlp = seen["moe"]
+        _check_moe(plain["moe"], x, mlp, 3, "experts")
+    else:
+        x, gate_up = seen["gateup"]
+        linear("gateup")
+        mid, mlp = seen["down"]
+        assert torch.equal(mid.reshape(-1), ops.swiglu(*gate_up.chunk(2, -1)).reshape(-1))
+        linear("down")
+    assert torch.equal(x.reshape(-1), post.reshape(-1))
+    last = (residual.reshape(1, -1) + mlp.reshape(1, -1)).cpu()
+    z = O.lm_readout(last, w.norm.weight.cpu(), cfg.eps, w.head.cpu())[0]
+    assert_bf16_close(logits.cpu().to(BF16), z.to(BF16), 1, 0.25, "logits")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", ["fp8", "fp8_static", "w4a16", "int4"])
+def test_experts_beside_other_linears(gpu, mode):
+    """The experts' format does not depend on the linears'."""
+    from fastforward_amd.runtime import LMConfig, Runtime
+    from fastforward_amd.synthetic import make_model
+    cfg = LMConfig("modes", 3, 512, 4, 2, 128, 136, 1000, experts=12, top_k=3)
+    w = make_model(cfg, mode=mode, seed=5, norm_jitter=0.2, n_options=4)
+    rt = Runtime(cfg, w, 70)
+    assert rt.path == "generic"
+    rt.set_inputs(*_request(cfg))
+    seen, moes = {}, [lw.moe for lw in w.layers]
+    for j, lw in enumerate(w.layers):
+        lw.moe = Observe(lw.moe, seen, j)
+    eager = rt.step().clone()
+    for lw, moe in zip(w.layers, moes):
+        lw.moe = moe
+    assert eager.isfinite().all()
+    for j, moe in enumerate(moes):
+        assert seen[j][0].numel() == 512 * (1 if j == 2 else 70)
+        _check_moe(moe, *seen[j], 3, f"layer {j}")
+    for _ in range(3):
+        assert torch.equal(rt.replay(), eager)
+        torch.cuda.synchronize()
+
+
 def _save_block_checkpoint(tmp_path):
     """The tiny transformers checkpoint with its LM linears block-scaled FP8."""
     from safetensors import safe_open

@@ -192,6 +192,46 @@ def test_every_path(gpu, t, k, e, h, i, tile):
     _check(y, x, w, ids, codes)
 
 
+def _check_rounded_twice(y, x, w, ids, codes):
+    """Within the oracle's bound and, by norm, two bf16 roundings of at most 2^-8 each."""
+    want, bound = M.experts(x, w, ids, *codes)
+    y = y.cpu().double()
+    assert ((y - want).abs() <= bound).all()
+    assert float((y - want).norm()) <= 2.0 ** -7 * float(want.norm())
+
+
+@gpu_test
+@pytest.mark.parametrize("tile", [2, 3])
+@pytest.mark.parametrize("h,i", [(8264, 40), (40, 8264)])
+def test_more_block_scales_than_lanes(gpu, h, i, tile):
+    """Both row tiles past the first scales that a wave loads, of gate and up (h) and in the down
+    products (i)."""
+    from fastforward_amd import moe
+    from fastforward_amd._lib import call
+    from tests.test_gpu_block_fp8 import late_scales
+    codes = list(_weights(2, h, i))
+    codes[1], codes[3] = late_scales(codes[1].shape, 8), late_scales(codes[3].shape, 9)
+    x, w, ids = _tokens(40, 1, 2, h)
+    op = _experts(codes)
+    call("ff_set_tuning", 13, tile)
+    moe.experts_workspace.cache_clear()
+    try:
+        y = op(x.to(DEV), w.to(DEV), ids.to(DEV))
+    finally:
+        call("ff_set_tuning", 13, 0)
+        moe.experts_workspace.cache_clear()
+    _check_rounded_twice(y, x, w, ids, codes)
+
+
+@gpu_test
+@pytest.mark.parametrize("t", [1, 3])
+def test_rows_longer_than_a_workgroup_keeps(gpu, t):
+    """Few pairs of a row whose codes do not fit in the pair kernel's LDS take the row tiles."""
+    codes = _weights(3, 49160, 16)
+    x, w, ids = _tokens(t, 2, 3, 49160)
+    _check_rounded_twice(_experts(codes)(x.to(DEV), w.to(DEV), ids.to(DEV)), x, w, ids, codes)
+
+
 @gpu_test
 @pytest.mark.parametrize("t,k,e,h,i", [(1, 8, 128, 2048, 768), (48, 4, 64, 2560, 1024), (300, 5, 12, 2120, 1000),
                                        (1024, 8, 16, 2048, 768)])
