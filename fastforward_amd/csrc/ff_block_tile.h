@@ -167,8 +167,10 @@ __device__ __forceinline__ void tile_mainloop(f32x4 (&acc)[BM / 16][CW / 16], ui
     for (int v = 0; v < NS; ++v) ws[v] = __uint_as_float(__builtin_amdgcn_readlane(wsc[v], at));
     // Instruction n = i TJ + j is followed by the adds of instruction n - LAG, the first LAG
     // of a step by those of the last step's last. A result is there some 40 clocks after its
-    // instruction's start: with LAG 3 the matrix unit is busy 83 % of the time (one wave; 89 %
-    // with two), with 2 69 and 86 %, with 1 44 and 76 %.
+    // instruction's start. In a bare loop of these instructions and adds, without loads, LDS
+    // or barriers, the matrix unit is busy 83 % of the time with LAG 3 (one wave a SIMD; 89 %
+    // with two), 69 and 86 % with 2, 44 and 76 % with 1. In the whole loop it is 22 % with one
+    // wave (576 x 6144 x 4096) and 52 % with two (4096 x 5120 x 25600): the rest waits.
     float s[RA][NS];
     static_for<0, ALL>([&](auto N_) {
       constexpr int n = decltype(N_)::value, i = n / TJ, j = n % TJ;

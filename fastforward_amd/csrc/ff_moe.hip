@@ -4,10 +4,13 @@
 //
 // y[t] = sum_j w[t, j] D_e (silu(G_e x[t]) * (U_e x[t])), e = ids[t, j]. The rows x
 // are quantised per 128 channels as the linear's rows are; the SwiGLU's values go
-// into the down products as bf16 (relative error 2^-9 each, below the output's own
-// rounding): quantised again, a value next to a border between two e4m3 codes
-// would move by 1/16 with the last bit of a sum. Sums stay fp32 throughout, and
-// their order depends on the shapes alone.
+// into the down products as bf16: each is off by at most 2^-8 of itself, as large a
+// rounding as the output's own, so an output is off by 2.3e-3 to 2.5e-3 RMS where the
+// output's rounding alone is 1.7e-3. It buys the matrix instructions' bf16 rate: fp32
+// values would need two bf16 parts, twice the down products. Quantised a second time, as
+// a dense layer of BlockFP8Linear's quantises them, a value next to a border between
+// two e4m3 codes would move by 1/16 with the last bit of a sum. Sums stay fp32
+// throughout, and their order depends on the shapes alone.
 //
 // Few (token, expert) pairs: two launches. gate_up: a workgroup per pair and 16
 // channels, the row quantised in the workgroup; down: a workgroup per token and 16
@@ -79,13 +82,15 @@ __device__ __forceinline__ T reduce(T v, F&& f) {
 }
 
 // exp(x) to about 1e-14 of its value: 2^k exp(r), k = rint(x / ln 2), |r| <= ln 2 / 2, and
-// the Taylor polynomial of degree 11 (its next term is below 7e-15).
+// the Taylor polynomial of degree 11 (its next term is below 7e-15). r = x - k ln 2 with
+// ln 2 = 0x0.b17217f7d1cf79ab.. in two parts, its leading 32 bits and the double nearest
+// to the rest: the product with the first is exact, the second's error is below 2^-85.
 __device__ __forceinline__ double exp64(double x) {
   if (x < -746.0) return 0.0;
   if (x > 710.0) return __builtin_inf();
   const double k = __builtin_rint(x * 1.4426950408889634);
-  double r = __builtin_fma(-k, 6.93147180369123816490e-01, x);  // ln 2: the leading 33 bits, then the rest
-  r = __builtin_fma(-k, 1.90821492927058770002e-10, r);
+  double r = __builtin_fma(-k, 0x0.b17217f7p0, x);
+  r = __builtin_fma(-k, 0x1.a39ef35793c76p-33, r);
   double p = 1.0 / 39916800;
   constexpr double kInv[11] = {1.0, 1.0, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320,
                                1.0 / 362880, 1.0 / 3628800};
@@ -222,9 +227,10 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(
 
 // The first `experts` workgroups order the pairs, one expert each: its pairs p = token *
 // top_k + slot in rising order to list[off[e] ..), off[e] = pairs of lower experts. Every
-// workgroup reads all ids (a few hundred KB from L2 at most) and needs nothing from the
-// others: no counters in memory, no order of arrival. ids outside [0, experts) are in no
-// list. The other workgroups quantise the rows.
+// workgroup reads all ids, twice where its expert has pairs, and needs nothing from the
+// others: no counters in memory, no order of arrival. That is experts x pairs x 8 bytes at
+// most, from L2: 33 MB at 4096 tokens x 8 of 128, and it grows with the tokens alone. ids
+// outside [0, experts) are in no list. The other workgroups quantise the rows.
 // 4.8 us to 577 tokens, about the shortest a launch takes, 12 us at 4096 tokens x 8.
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64, kPlanBatch = 8;
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* __restrict__ ids, int pairs, int experts,
@@ -297,7 +303,9 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int* __restric
 // g / (1 + exp(-g)) to a few units in the last place of fp32 (its bf16 rounding follows):
 // exp(-g) = 2^(-g log2 e), the product's rounding error added back to first order, and the
 // hardware's exponential and reciprocal (1 ulp each) in place of the library's (some 50
-// instructions a value, a fifth of the gate/up tiles' time).
+// instructions a value, a fifth of the gate/up tiles' time). Below g = -87.3 exp(-g)
+// passes 2^126, its reciprocal is subnormal and comes out as 0: so does the value, whose
+// magnitude is under 1.1e-36 there.
 __device__ __forceinline__ float silu_fast(float g) {
   constexpr float kLog2e = 1.44269504f, kLog2eLow = 1.92596299e-8f, kLn2 = 0.693147181f;
   const float p = -g * kLog2e;
