@@ -69,8 +69,9 @@ def experts_workspace(t, top_k, experts, h, i):
 
 class Experts:
     """The experts' MLPs in block-scaled FP8: y[t] = bf16(sum_j w[t, j] D_e (silu(G_e x)
-    * (U_e x))), e = ids[t, j]. x is quantised per row and 128 channels, the SwiGLU's
-    values stay bf16, sums are fp32.
+    * (U_e x))), e = ids[t, j]. x is quantised per row and 128 channels, sums are fp32. The
+    SwiGLU's values are rounded to bf16 (as large a rounding as the output's) and not
+    quantised, unlike the rows of a dense layer's ``BlockFP8Linear``.
 
     ``Experts(gate_up, down)`` quantises bf16 weights, gate_up (E, 2, I, H) with the
     gate first and down (E, H, I); ``Experts.from_codes`` takes e4m3 codes of those

@@ -490,8 +490,11 @@ int ff_quant_rows_fp8_block(const void* x, int64_t ldx, void* q, float* scales, 
 int ff_gemm_fp8_block(const void* q, const float* scales, const void* packed, const float* wscales, void* y,
                       int64_t ldy, int64_t m, int64_t n, int64_t k, ff_stream_t stream);
 /* The whole linear from bf16 rows x (row stride ldx): quantisation and product. A few
- * short rows (a row of up to 16384 channels, four of 4096) run in one launch. workspace: ff_linear_fp8_block_workspace bytes
- * (0: may be NULL), 16-byte aligned. */
+ * short rows run in one launch without a workspace: at most 16, and rows x blocks of 128
+ * channels x blocks of 8192 columns (both rounded up) at most 128, as a row of 16384
+ * channels or four of 4096 on up to 8192 columns, one of 8192 on 16384. Which calls those
+ * are is an implementation's choice: ask for the workspace of every size.
+ * workspace: ff_linear_fp8_block_workspace bytes (0: may be NULL), 16-byte aligned. */
 int ff_linear_fp8_block_workspace(int64_t m, int64_t n, int64_t k, int64_t* bytes);
 int ff_linear_fp8_block(const void* x, int64_t ldx, const void* packed, const float* wscales, void* y, int64_t ldy,
                         int64_t m, int64_t n, int64_t k, void* workspace, int64_t workspace_bytes,
@@ -518,7 +521,9 @@ int ff_moe_route(const void* logits, int logits_f32, int64_t ld, const float* bi
                  int renormalize, double scale, ff_stream_t stream);
 
 /* y[t] = bf16(sum_j weights[t, j] D_e bf16(silu(G_e x[t]) * (U_e x[t]))), e = ids[t, j],
- * with x quantised as by ff_quant_rows_fp8_block, sums in fp32. gate_up: the codes
+ * with x quantised as by ff_quant_rows_fp8_block, sums in fp32. SwiGLU's values are rounded
+ * to bf16 and not quantised (the rows of a down projection on ff_linear_fp8_block are). A
+ * value's bf16 rounding is as large as the output's. gate_up: the codes
  * (experts, 2, i, h) of G and U packed with n_pad = i rounded up to 128 and their
  * scales (experts, 2, ceil(i / 128), ceil(h / 128)); down: the codes (experts, h, i)
  * of D packed with n_pad = h rounded up to 16, scales (experts, ceil(h / 128),
