@@ -1,0 +1,620 @@
+// Causal grouped-query attention of each sequence's last tokens over a paged cache.
+//
+// Query i of a sequence's n new tokens has position L - n + i of its L and sees the
+// positions up to its own: o = sum_j p_j v_j, p = softmax_j(scale q . k_j), exact
+// softmax statistics in fp32 over 64-key blocks with a running maximum.
+//
+// Rows. A tile holds rows (query, head of the group) of one sequence and one key head,
+// query-major, so that a group of any size fills tiles and a decode token is the tile of
+// its group's heads. Products run as S^T = K Q^T and O^T = V^T P^T on
+// v_mfma_f32_16x16x32_bf16: a lane's accumulators belong to one row, and P^T leaves the
+// scores in the operand layout of the second product (lane group g of 16 lanes holds
+// keys 8 g .. 8 g + 7 of a 32-key chunk in both). V is stored as tokens are, and comes
+// out of LDS transposed (ds_read_b64_tr_b16 / _b8).
+//
+// FP8 pages: codes become bf16 in registers, exactly (a power of two scales a row): a
+// key's scale is the conversion's own operand, a value's is multiplied into its P before
+// that is rounded to bf16. P in bf16 is a rounding of 2^-9 relative at most half a step,
+// as large as the output's own; its sum is kept unrounded.
+#include <limits.h>
+
+#include "ff_block.h"
+#include "ff_cache.h"
+
+using namespace ff;
+
+namespace {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+struct Args {
+  Rows a;
+  const bf16_t* q;
+  int64_t q_ts, q_hs;
+  const uint8_t *k, *v, *ks, *vs;
+  bf16_t* y;
+  float* part_o;   // (items, BM, D) unnormalised sums of split tiles
+  float2* part_s;  // (items, BM) their maximum (of q . k) and denominator
+  int hk, group;
+  int budget;  // 64-key blocks are dealt so that about so many items per head come out; 0: no tile is split
+  int items;   // items per head that the grid holds
+  float c2;    // scale * log2(e)
+};
+
+__device__ __forceinline__ f32x4 mfma_bf16(const bf16x8& a, const u32x4& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// ------------------------------------------------------------------ the work list
+//
+// Every sequence's rows make ceil(rows / BM) tiles, and every tile is split into as many
+// key ranges as its sequence's blocks take chunks. A chunk is the share of all blocks
+// that gives `budget` items, `least` blocks at least. All workgroups compute the
+// same list from the lengths. Rows behind the last sequence are a sequence without keys.
+
+struct Seq {
+  int row0, n;    // first row (token) and rows
+  int len;        // its positions
+  int keys;       // of which the table reaches so many
+  int tiles, blocks;
+};
+
+template <int BM>
+__device__ __forceinline__ Seq seq_of(const Args& p, int b) {
+  Seq s = {0, 0, 0, 0, 0, 0};
+  const int batch = p.a.starts ? p.a.batch : p.a.t;
+  if (b > batch || (b == batch && !p.a.starts)) return s;
+  if (b == batch) {
+    s.row0 = p.a.begin(b);
+    s.n = p.a.t - s.row0;
+  } else {
+    s.row0 = p.a.begin(b);
+    s.n = max(p.a.end(b) - s.row0, 0);
+    s.len = p.a.lengths[b];
+    s.keys = max(0, (int)min((int64_t)s.len, p.a.capacity()));
+  }
+  s.tiles = (int)(((int64_t)s.n * p.group + BM - 1) / BM);
+  s.blocks = s.n ? (s.keys + 63) >> 6 : 0;
+  return s;
+}
+
+// Blocks of a chunk.
+template <int BM>
+__device__ __forceinline__ int chunk_of(const Args& p, int lane, int least) {
+  if (!p.budget) return INT_MAX;
+  int total = 0;
+  for (int b0 = 0; b0 <= p.a.batch; b0 += 64) {
+    const Seq s = seq_of<BM>(p, b0 + lane);
+    total += s.tiles * s.blocks;
+  }
+  total = __builtin_amdgcn_readlane(wave_scan(total), 63);
+  return max(least, (total + p.budget - 1) / p.budget);
+}
+
+__device__ __forceinline__ int splits_of(int blocks, int chunk) {
+  return max(1, blocks / chunk + (blocks % chunk != 0));
+}
+
+struct Item {
+  Seq s;
+  int seq, tile, split, splits;
+};
+
+// Item `id` of the list.
+template <int BM>
+__device__ __forceinline__ bool find_item(const Args& p, int lane, int chunk, int id, Item* out) {
+  int base = 0;
+  for (int b0 = 0; b0 <= p.a.batch; b0 += 64) {
+    const Seq s = seq_of<BM>(p, b0 + lane);
+    const int splits = splits_of(s.blocks, chunk), n = s.tiles * splits;
+    const int sum = wave_scan(n), first = base + sum - n;
+    const uint64_t hit = __ballot(id >= first && id < first + n);
+    if (hit) {
+      const int src = __builtin_ctzll(hit);
+      out->s = {__builtin_amdgcn_readlane(s.row0, src), __builtin_amdgcn_readlane(s.n, src),
+                __builtin_amdgcn_readlane(s.len, src),  __builtin_amdgcn_readlane(s.keys, src),
+                __builtin_amdgcn_readlane(s.tiles, src), __builtin_amdgcn_readlane(s.blocks, src)};
+      out->seq = b0 + src;
+      out->splits = __builtin_amdgcn_readlane(splits, src);
+      const int in = id - __builtin_amdgcn_readlane(first, src);
+      out->tile = in / out->splits;
+      out->split = in % out->splits;
+      return true;
+    }
+    base += __builtin_amdgcn_readlane(sum, 63);
+  }
+  return false;
+}
+
+// ------------------------------------------------------------------ pieces of a block
+
+// 16-byte chunk at which chunk c of a value row of RB bytes is kept in LDS: the rows that
+// a transposed read takes together (see below) fall on different banks.
+template <int RB, bool FP8>
+__device__ __forceinline__ int v_swizzle(int row) {
+  if (FP8) return RB == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
+  return RB == 256 ? 2 * ((row & 3) | ((row >> 1) & 4)) : 2 * (((row >> 1) & 1) | ((row >> 2) & 2));
+}
+
+__device__ __forceinline__ s16x4 read_tr16(uint32_t lds) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)lds);
+}
+__device__ __forceinline__ i32x2v read_tr8(uint32_t lds) {
+  return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2v*)(uintptr_t)lds);
+}
+
+// V^T fragment of chunk c, dims 16 dt ..: lane (r16, g) gets keys 32 c + 8 g .. + 7 of dim
+// 16 dt + r16. 16 lanes read 4 keys x 32 bytes (bf16) or 8 keys x 16 bytes (codes) and
+// receive them transposed.
+template <int D, bool FP8>
+__device__ __forceinline__ bf16x8 v_fragment(uint32_t lds, int c, int dt, int r16, int g) {
+  constexpr int RB = FP8 ? D : 2 * D;
+  if constexpr (FP8) {
+    const int row = 32 * c + 8 * g + (r16 >> 1);
+    const i32x2v q = read_tr8(lds + row * RB + 16 * (dt ^ v_swizzle<RB, FP8>(row)) + 8 * (r16 & 1));
+    return e4m3_to_bf16x8((uint32_t)q.x, (uint32_t)q.y);
+  } else {
+    s16x4 h[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = 32 * c + 8 * g + 4 * i + (r16 >> 2);
+      const int chunk = (2 * dt + ((r16 >> 1) & 1)) ^ v_swizzle<RB, FP8>(row);
+      h[i] = read_tr16(lds + row * RB + 16 * chunk + 8 * (r16 & 1));
+    }
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    return __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+}
+
+// The dims that k step st of q . k takes for lane group g: where 16 bytes of a key row
+// are 16 codes they serve two steps.
+template <bool FP8>
+__device__ __forceinline__ int step_dim(int st, int g) {
+  return FP8 ? 64 * (st >> 1) + 16 * g + 8 * (st & 1) : 32 * st + 8 * g;
+}
+
+__device__ __forceinline__ bf16x8 e4m3_to_bf16x8(uint32_t a, uint32_t b, float s) {
+  const bf16x2_t p0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, s, false);
+  const bf16x2_t p1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, s, true);
+  const bf16x2_t p2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, s, false);
+  const bf16x2_t p3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, s, true);
+  return bf16x8{p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
+}
+
+// This wave's LDS reads and writes are done (no other wave uses the memory).
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
+
+// One block of the running softmax. s[2 c + tt][r] is q . k of key 32 c + 8 g + 4 tt + r;
+// vis: the block's keys that this lane's row sees (`masked`: not all of them, in some
+// lane). P^T of chunk c goes to pf[c], times the keys' value scales (FP8).
+template <bool FP8>
+__device__ __forceinline__ float softmax_block(f32x4 (&s)[4], bool masked, uint64_t vis, int g, float c2,
+                                               const u32x2 (&vsc)[2], float& m, float& den, u32x4 (&pf)[2]) {
+  if (masked) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t bits = (uint32_t)(vis >> (32 * (i >> 1) + 8 * g)) >> (4 * (i & 1));
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[i][r] = bits >> r & 1 ? s[i][r] : -INFINITY;
+    }
+  }
+  float top = s[0][0];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) top = __builtin_elementwise_maximum(top, s[i][r]);
+  const float mnew = fmaxf(m, max_rows(top));
+  const float mref = mnew == -INFINITY ? 0.f : mnew;
+  const float alpha = __builtin_amdgcn_exp2f((m - mref) * c2);
+  float psum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      s[i][r] = __builtin_amdgcn_exp2f((s[i][r] - mref) * c2);
+      psum += s[i][r];
+    }
+  den = den * alpha + psum;
+  m = mnew;
+  if constexpr (FP8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[i][r] *= scale_of((i & 1 ? vsc[i >> 1].y : vsc[i >> 1].x) >> (8 * r) & 0xFF);
+  }
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    pf[c].x = pack_bf16x2(s[2 * c][0], s[2 * c][1]);
+    pf[c].y = pack_bf16x2(s[2 * c][2], s[2 * c][3]);
+    pf[c].z = pack_bf16x2(s[2 * c + 1][0], s[2 * c + 1][1]);
+    pf[c].w = pack_bf16x2(s[2 * c + 1][2], s[2 * c + 1][3]);
+  }
+  return alpha;
+}
+
+// Whether a block's values (all of them in LDS, those that are not there as zeros) hold an
+// infinity or a NaN: their sum by the matrix unit says so.
+template <int D, bool FP8>
+__device__ __forceinline__ bool values_odd(uint32_t lds, int r16, int g) {
+  const u32x4 ones = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+  f32x4 t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) t = mfma_bf16(v_fragment<D, FP8>(lds, c, dt, r16, g), ones, t);
+  bool odd = false;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) odd |= !(fabsf(t[r]) < INFINITY);
+  return __ballot(odd) != 0;
+}
+
+// o += V^T P^T where a row may not see a key whose values are odd: 0 times them would be NaN.
+// The product runs on the finite values; a second one counts, for each (row, dim), the
+// infinities and NaN among the values that the row does see.
+template <int D, bool FP8>
+__device__ __forceinline__ void add_odd_values(uint32_t lds, const u32x4 (&pf)[2], int r16, int g, f32x4 (&o)[D / 16]) {
+  for (int dt = 0; dt < D / 16; ++dt) {
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f}, up = sum, down = sum, nan = sum;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      typedef short s16x8 __attribute__((ext_vector_type(8)));
+      const s16x8 v = __builtin_bit_cast(s16x8, v_fragment<D, FP8>(lds, c, dt, r16, g));
+      s16x8 fine, u, d, n;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t b = (uint16_t)v[e];
+        fine[e] = (b & 0x7F80) == 0x7F80 ? 0 : v[e];
+        u[e] = b == 0x7F80 ? 0x3F80 : 0;
+        d[e] = b == 0xFF80 ? 0x3F80 : 0;
+        n[e] = (b & 0x7FFF) > 0x7F80 ? 0x3F80 : 0;
+      }
+      sum = mfma_bf16(__builtin_bit_cast(bf16x8, fine), pf[c], sum);
+      up = mfma_bf16(__builtin_bit_cast(bf16x8, u), pf[c], up);
+      down = mfma_bf16(__builtin_bit_cast(bf16x8, d), pf[c], down);
+      nan = mfma_bf16(__builtin_bit_cast(bf16x8, n), pf[c], nan);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float x = sum[r];
+      x = up[r] > 0.f ? x + INFINITY : x;
+      x = down[r] > 0.f ? x - INFINITY : x;
+      sum[r] = nan[r] > 0.f ? __builtin_nanf("") : x;
+    }
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)  // (registers cannot be indexed)
+      if (i == dt) o[i] = o[i] + sum;
+  }
+}
+
+// Bits 0 .. last of a block's 64 keys (none where last < 0).
+__device__ __forceinline__ uint64_t keys_to(int last) {
+  return last < 0 ? 0 : last >= 63 ? ~0ull : (2ull << last) - 1;
+}
+
+// ------------------------------------------------------------------ few rows
+//
+// One workgroup per item: a 16-row tile, its key blocks dealt to the waves, each with a
+// running softmax of its own; the waves are joined in LDS. Keys go from memory straight
+// into the operand registers, values by DMA into the wave's own LDS: no barrier until
+// the end. Bound by the cache's bytes.
+constexpr int kFewWaves = 4;
+
+template <int D, bool FP8>
+__global__ __launch_bounds__(64 * kFewWaves, 2) void few_rows_kernel(Args p) {
+  constexpr int RB = FP8 ? D : 2 * D, KST = D / 32, DTN = D / 16, KL = RB / 64;  // KL: 16-byte loads of a key row
+  constexpr int VI = RB / 16;                                                   // value DMAs of a block
+  constexpr int SLAB = 64 * RB, LDO = D + 4;
+  constexpr int JOIN = kFewWaves * 16 * (LDO + 2) * 4;
+  __shared__ __align__(1024) uint8_t smem[kFewWaves * SLAB > JOIN ? kFewWaves * SLAB : JOIN];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r16 = lane & 15, g = lane >> 4;
+  const int head = (int)blockIdx.x % p.hk, id = (int)blockIdx.x / p.hk;
+  const int chunk = chunk_of<16>(p, lane, kFewWaves);
+  Item it;
+  if (!find_item<16>(p, lane, chunk, id, &it)) return;
+  const int row = it.tile * 16 + r16, rows = it.s.n * p.group;
+  const bool real = row < rows;
+  const int query = (real ? row : rows - 1) / p.group, hq = head * p.group + (real ? row : rows - 1) % p.group;
+  const int token = it.s.row0 + query;
+  const int pos = real ? it.s.len - it.s.n + query : -1;
+  const int last = it.s.len - it.s.n + min(rows - 1, it.tile * 16 + 15) / p.group;  // the tile's last position
+  const int kend = min(it.s.keys, last + 1);
+  const int nb = max(0, kend + 63) >> 6, per = (nb + it.splits - 1) / it.splits;
+  const int b_end = min(nb, (it.split + 1) * per);
+
+  u32x4 qf[KST];
+  const bf16_t* qp = p.q + token * p.q_ts + hq * p.q_hs;
+#pragma unroll
+  for (int st = 0; st < KST; ++st) {
+    const bf16_t* src = qp + step_dim<FP8>(st, g);
+    if (((uintptr_t)p.q & 15) == 0 && ((p.q_ts | p.q_hs) & 7) == 0) {
+      qf[st] = *reinterpret_cast<const u32x4*>(src);
+    } else {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = bf16_to_f32(src[i]);
+      qf[st] = pack8(x);
+    }
+  }
+  f32x4 o[DTN];
+#pragma unroll
+  for (int dt = 0; dt < DTN; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, den = 0.f;
+
+  const int64_t page_rows = (int64_t)p.hk << p.a.lps, head_rows = (int64_t)head << p.a.lps;
+  const int in_page = (1 << p.a.lps) - 1;
+  const int* table = p.a.table + (int64_t)min(it.seq, p.a.batch - 1) * p.a.width;
+  const uint32_t lds = lds_addr(smem) + wave * SLAB;
+
+  for (int b = it.split * per + wave; b < b_end; b += kFewWaves) {
+    const int kb = 64 * b;
+    // the lane's key of the block: its page, and whether there is one
+    const int entry = table[min((int64_t)((kb + lane) >> p.a.lps), p.a.width - 1)];
+    const bool there = kb + lane < kend && (unsigned)entry < (unsigned)p.a.pages;
+    const uint64_t ok = __ballot(there);
+    const int page = there ? entry : 0;
+    auto row_of = [&](int key) {  // row of the pages' (page, head, slot) that holds key kb + key
+      return (int64_t)__shfl(page, key, 64) * page_rows + head_rows + ((kb + key) & in_page);
+    };
+    u32x4 kf[4][KL];
+    float ksc[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t at = row_of(32 * (i >> 1) + 8 * (r16 >> 2) + 4 * (i & 1) + (r16 & 3));
+#pragma unroll
+      for (int j = 0; j < KL; ++j) kf[i][j] = *reinterpret_cast<const u32x4*>(p.k + at * RB + 64 * j + 16 * g);
+      if (FP8) ksc[i] = scale_of(p.ks[at]);
+    }
+    u32x2 vsc[2];
+    if (FP8) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) vsc[c] = *reinterpret_cast<const u32x2*>(p.vs + row_of(32 * c + 8 * g));
+    }
+    wait_lds();
+#pragma unroll
+    for (int j = 0; j < VI; ++j) {
+      const int key = j * (64 / VI) + lane / VI;
+      lds_dma16(p.v + row_of(key) * RB + 16 * ((lane % VI) ^ v_swizzle<RB, FP8>(key)), lds + 1024 * j);
+    }
+    f32x4 s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int st = 0; st < KST; ++st) {
+        bf16x8 k;
+        if constexpr (FP8) {
+          const u32x4 c = kf[i][st >> 1];
+          k = st & 1 ? e4m3_to_bf16x8(c.z, c.w, ksc[i]) : e4m3_to_bf16x8(c.x, c.y, ksc[i]);
+        } else {
+          k = __builtin_bit_cast(bf16x8, kf[i][st]);
+        }
+        s[i] = mfma_bf16(k, qf[st], s[i]);
+      }
+    }
+    const uint64_t vis = ok & keys_to(pos - kb);
+    const bool masked = __ballot(vis != ~0ull) != 0;
+    if (FP8 && ok != ~0ull) {  // a scale byte of a key that is not there may be anything
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const uint32_t bits = (uint32_t)(ok >> (32 * c + 8 * g));
+        vsc[c].x &= ((bits & 15) * 0x204081u & 0x01010101u) * 255u;
+        vsc[c].y &= ((bits >> 4 & 15) * 0x204081u & 0x01010101u) * 255u;
+      }
+    }
+    u32x4 pf[2];
+    const float alpha = softmax_block<FP8>(s, masked, vis, g, p.c2, vsc, m, den, pf);
+#pragma unroll
+    for (int dt = 0; dt < DTN; ++dt) o[dt] = o[dt] * alpha;
+    wait_vmcnt<0>();
+    wait_lds();
+    if (ok != ~0ull) {  // values that are not there may be anything, and 0 times it not 0
+      if (!(ok >> lane & 1)) {
+#pragma unroll
+        for (int j = 0; j < RB / 16; ++j)
+          *reinterpret_cast<u32x4*>(smem + wave * SLAB + lane * RB + 16 * j) = u32x4{0, 0, 0, 0};
+      }
+      wait_lds();
+    }
+    // where the tile's rows see different keys, one that a row does not see may be odd
+    if (__ballot(real && vis != ok) && values_odd<D, FP8>(lds, r16, g)) {
+      add_odd_values<D, FP8>(lds, pf, r16, g, o);
+      continue;
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int dt = 0; dt < DTN; ++dt) o[dt] = mfma_bf16(v_fragment<D, FP8>(lds, c, dt, r16, g), pf[c], o[dt]);
+  }
+  den = sum_rows(den);
+
+  // join the waves
+  float* so = reinterpret_cast<float*>(smem);
+  float* sm = so + kFewWaves * 16 * LDO;
+  float* sd = sm + kFewWaves * 16;
+  __syncthreads();
+#pragma unroll
+  for (int dt = 0; dt < DTN; ++dt) *reinterpret_cast<f32x4*>(so + (wave * 16 + r16) * LDO + 16 * dt + 4 * g) = o[dt];
+  if (g == 0) {
+    sm[wave * 16 + r16] = m;
+    sd[wave * 16 + r16] = den;
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < 16 * (D / 4); e += 64 * kFewWaves) {
+    const int r = e / (D / 4), d0 = e % (D / 4) * 4;
+    if (it.tile * 16 + r >= rows) continue;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) mx = fmaxf(mx, sm[w * 16 + r]);
+    const float mref = mx == -INFINITY ? 0.f : mx;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) {
+      const float wt = __builtin_amdgcn_exp2f((sm[w * 16 + r] - mref) * p.c2);
+      sum += sd[w * 16 + r] * wt;
+      fma4(acc, *reinterpret_cast<const f32x4*>(so + (w * 16 + r) * LDO + d0), wt);
+    }
+    if (it.splits == 1) {
+      const int rr = it.tile * 16 + r;
+      const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+      bf16_t* to = p.y + ((int64_t)(it.s.row0 + rr / p.group) * (p.hk * p.group) + head * p.group + rr % p.group) * D;
+      *reinterpret_cast<u32x2*>(to + d0) = pack4_bf16(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+    } else {
+      const int64_t at = ((int64_t)id * p.hk + head) * 16 + r;
+      *reinterpret_cast<f32x4*>(p.part_o + at * D + d0) = acc;
+      if (d0 == 0) p.part_s[at] = float2{mx, sum};
+    }
+  }
+}
+
+// ------------------------------------------------------------------ joining split tiles
+
+// A wave per row (token, head); rows of unsplit tiles are there already.
+template <int D, int BM>
+__global__ __launch_bounds__(256) void join_kernel(Args p, int least) {
+  const int lane = threadIdx.x & 63;
+  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int heads = p.hk * p.group;
+  if (r >= (int64_t)p.a.t * heads) return;
+  const int token = __builtin_amdgcn_readfirstlane((int)(r / heads)), hq = (int)(r % heads);
+  const int head = hq / p.group;
+  const int chunk = chunk_of<BM>(p, lane, least);
+  int base = 0, first = 0, splits = 1;
+  for (int b0 = 0; b0 <= p.a.batch; b0 += 64) {
+    const Seq s = seq_of<BM>(p, b0 + lane);
+    const int sp = splits_of(s.blocks, chunk), n = s.tiles * sp;
+    const int sum = wave_scan(n);
+    const uint64_t hit = __ballot(token >= s.row0 && token < s.row0 + s.n);
+    if (hit) {
+      const int src = __builtin_ctzll(hit);
+      const int in = (token - __builtin_amdgcn_readlane(s.row0, src)) * p.group + hq % p.group;
+      splits = __builtin_amdgcn_readlane(sp, src);
+      first = base + __builtin_amdgcn_readlane(sum - n, src) + in / BM * splits;
+      base = in % BM;
+      break;
+    }
+    base += __builtin_amdgcn_readlane(sum, 63);
+  }
+  if (splits == 1 || first + splits > p.items) return;
+  const int row = base;
+  float mx = -INFINITY;
+  for (int i = lane; i < splits; i += 64) mx = fmaxf(mx, p.part_s[((int64_t)(first + i) * p.hk + head) * BM + row].x);
+  mx = wave_max(mx);
+  const float mref = mx == -INFINITY ? 0.f : mx;
+  constexpr int PER = D / 64;
+  float acc[PER] = {}, sum = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < splits; ++i) {
+    const int64_t at = ((int64_t)(first + i) * p.hk + head) * BM + row;
+    const float2 st = p.part_s[at];
+    const float wt = __builtin_amdgcn_exp2f((st.x - mref) * p.c2);
+    sum += st.y * wt;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) acc[e] = __builtin_fmaf(p.part_o[at * D + PER * lane + e], wt, acc[e]);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  bf16_t* to = p.y + r * D + PER * lane;
+  if constexpr (PER == 2) *reinterpret_cast<uint32_t*>(to) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+  else *to = (bf16_t)f32_to_bf16(acc[0] * inv);
+}
+
+// ------------------------------------------------------------------ host
+
+struct Plan {
+  int bm, least, budget;
+  int64_t items;  // per key head
+};
+
+constexpr int kWorkgroups = 512;  // two a CU
+
+Plan plan_of(int64_t t, int64_t batch, int64_t hk, int64_t group, int64_t capacity) {
+  Plan p = {16, kFewWaves, 0, 0};
+  const int64_t tiles = t * group / p.bm + batch + 1;
+  // a sequence of `least` blocks at most is one chunk whatever the lengths are
+  if ((capacity + 63) / 64 > p.least) p.budget = (int)((kWorkgroups + hk - 1) / hk);
+  p.items = tiles + p.budget;
+  return p;
+}
+
+int check(const char* what, int64_t hq, int64_t hk, int64_t d, int64_t ps, int64_t width, int64_t batch, int64_t t) {
+  FF_REQUIRE(d == 64 || d == 128, "%s: head_dim %lld unsupported (64, 128)", what, (long long)d);
+  FF_REQUIRE(ps >= 16 && ps <= 4096 && (ps & (ps - 1)) == 0, "%s: page_size %lld (a power of two, 16 .. 4096)", what,
+             (long long)ps);
+  FF_REQUIRE(hk > 0 && hq > 0 && hq <= 65535 && hq % hk == 0 && width > 0 && width <= INT32_MAX / ps && batch > 0 &&
+                 batch <= 65536 && t > 0 && t <= (1 << 24),
+             "%s: bad sizes hq=%lld hk=%lld width=%lld batch=%lld t=%lld", what, (long long)hq, (long long)hk,
+             (long long)width, (long long)batch, (long long)t);
+  const int64_t tiles = t * (hq / hk) / 16 + batch + 1;
+  FF_REQUIRE(tiles * ((width * ps + 63) / 64) <= INT32_MAX && (tiles + kWorkgroups) * hk <= INT32_MAX,
+             "%s: too large a call (rows x positions)", what);
+  return FF_OK;
+}
+
+int64_t workspace_of(const Plan& p, int64_t hk, int64_t d) {
+  return p.budget ? p.items * hk * p.bm * (d * 4 + 8) : 0;
+}
+
+}  // namespace
+
+extern "C" int ff_attention_paged_workspace(int64_t hq, int64_t hk, int64_t d, int64_t page_size, int64_t width,
+                                            int64_t batch, int64_t t, int64_t* bytes) {
+  FF_REQUIRE(bytes, "ff_attention_paged_workspace: null pointer");
+  *bytes = 0;
+  if (t == 0) return FF_OK;
+  const int st = check("ff_attention_paged_workspace", hq, hk, d, page_size, width, batch, t);
+  if (st != FF_OK) return st;
+  *bytes = workspace_of(plan_of(t, batch, hk, hq / hk, width * page_size), hk, d);
+  return FF_OK;
+}
+
+extern "C" int ff_attention_paged(const void* q, int64_t q_ts, int64_t q_hs, const void* k_pages, const void* v_pages,
+                                  const void* k_scale, const void* v_scale, int64_t pages, int64_t page_size,
+                                  int64_t hq, int64_t hk, int64_t d, int fp8, const int32_t* table, int64_t width,
+                                  const int32_t* lengths, const int32_t* starts, int64_t batch, void* y, int64_t t,
+                                  float scale, void* workspace, int64_t workspace_bytes, ff_stream_t stream) {
+  if (t == 0) return FF_OK;
+  const int st = check("ff_attention_paged", hq, hk, d, page_size, width, batch, t);
+  if (st != FF_OK) return st;
+  FF_REQUIRE(q && k_pages && v_pages && (!fp8 || (k_scale && v_scale)) && table && lengths && y,
+             "ff_attention_paged: null pointer");
+  FF_REQUIRE(pages > 0 && pages <= INT32_MAX, "ff_attention_paged: %lld pages", (long long)pages);
+  FF_REQUIRE(starts || batch == t, "ff_attention_paged: without starts every sequence has one row");
+  FF_REQUIRE(scale > 0.f && scale < __builtin_inff(), "ff_attention_paged: scale %g", (double)scale);
+  FF_REQUIRE(ff_aligned(k_pages, 16) && ff_aligned(v_pages, 16) && ff_aligned(k_scale, 8) && ff_aligned(v_scale, 8) &&
+                 ff_aligned(y, 16),
+             "ff_attention_paged: alignment");
+  const Plan plan = plan_of(t, batch, hk, hq / hk, width * page_size);
+  const int64_t need = workspace_of(plan, hk, d);
+  FF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ff_aligned(workspace, 16)),
+             "ff_attention_paged: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+  Args p;
+  p.a = Rows{table, lengths, starts, width, (int)batch, (int)t, (int)pages, __builtin_ctzll((uint64_t)page_size)};
+  p.q = (const bf16_t*)q;
+  p.q_ts = q_ts;
+  p.q_hs = q_hs;
+  p.k = (const uint8_t*)k_pages;
+  p.v = (const uint8_t*)v_pages;
+  p.ks = (const uint8_t*)k_scale;
+  p.vs = (const uint8_t*)v_scale;
+  p.y = (bf16_t*)y;
+  p.part_o = (float*)workspace;
+  p.part_s = (float2*)((char*)workspace + plan.items * hk * plan.bm * d * 4);
+  p.hk = (int)hk;
+  p.group = (int)(hq / hk);
+  p.budget = plan.budget;
+  p.items = (int)plan.items;
+  p.c2 = (float)((double)scale * 1.4426950408889634);
+  const dim3 grid((unsigned)(plan.items * hk)), block(64 * kFewWaves);
+  const dim3 join((unsigned)((t * hq + 3) / 4));
+  hipStream_t s = (hipStream_t)stream;
+#define FF_PAGED(DIM, F8)                                                                            \
+  if (d == DIM && (fp8 != 0) == F8) {                                                                \
+    hipLaunchKernelGGL((few_rows_kernel<DIM, F8>), grid, block, 0, s, p);                            \
+    if (plan.budget) hipLaunchKernelGGL((join_kernel<DIM, 16>), join, dim3(256), 0, s, p, plan.least); \
+  }
+  FF_PAGED(64, false) FF_PAGED(64, true) FF_PAGED(128, false) FF_PAGED(128, true)
+#undef FF_PAGED
+  FF_LAUNCH_CHECK("ff_attention_paged");
+  return FF_OK;
+}

@@ -1,0 +1,60 @@
+// Pieces shared by the paged cache's kernels: where a sequence's positions lie, which
+// sequence a row belongs to, and the attention's work list.
+//
+// A cache has `pages` pages of `ps` tokens (a power of two) of `hk` heads: k and v
+// (pages, hk, ps, d), bf16 or e4m3 codes, and for codes a byte per (page, head, token):
+// the biased exponent of the row's power-of-two scale, value = code * 2^(byte - 127).
+// Position p of sequence b is slot p % ps of page table[b][p / ps]. A position that the
+// table does not reach and an entry outside [0, pages) hold nothing: not written, read
+// as zeros, not attended to.
+#pragma once
+
+#include "ff_common.h"
+
+namespace ff {
+
+// The rows of a call: sequence b has rows [starts[b], starts[b + 1]) of the t rows (one
+// row each without starts), its last positions of lengths[b].
+struct Rows {
+  const int* table;
+  const int* lengths;
+  const int* starts;  // batch + 1, or null
+  int64_t width;      // entries of a table row
+  int batch, t, pages, lps;
+
+  __device__ __forceinline__ int begin(int b) const { return !starts ? b : b ? min(max(starts[b], 0), t) : 0; }
+  __device__ __forceinline__ int end(int b) const {
+    return !starts ? b + 1 : b < batch ? min(max(starts[b + 1], 0), t) : t;
+  }
+  __device__ __forceinline__ int64_t capacity() const { return width << lps; }
+};
+
+// Sequences of the N rows row0 .. row0 + N - 1 (a wave's; uniform row0): of[i] = how many
+// sequences end at or before row0 + i. batch where the row lies behind the last one.
+template <int N>
+__device__ __forceinline__ void find_sequences(const Rows& a, int row0, int lane, int (&of)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) of[i] = a.starts ? 0 : row0 + i;
+  if (!a.starts) return;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    const int end = b0 + lane < a.batch ? a.starts[b0 + lane + 1] : 0x7FFFFFFF;
+#pragma unroll
+    for (int i = 0; i < N; ++i) of[i] += __popcll(__ballot(end <= row0 + i));
+  }
+}
+
+// Page and slot of row `row` of sequence b; false where there is none.
+__device__ __forceinline__ bool find_slot(const Rows& a, int row, int b, int64_t* page, int* slot) {
+  if (row >= a.t || b >= a.batch) return false;
+  const int64_t pos = (int64_t)a.lengths[b] - a.end(b) + row;
+  if (pos < 0 || pos >= a.capacity()) return false;
+  const int p = a.table[b * a.width + (pos >> a.lps)];
+  *page = p;
+  *slot = (int)(pos & ((1 << a.lps) - 1));
+  return (unsigned)p < (unsigned)a.pages;
+}
+
+// The float of a scale byte.
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+}  // namespace ff
