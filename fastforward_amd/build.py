@@ -25,7 +25,9 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-ffp-contract=o
 # registers; left to itself the compiler writes the result to accumulation registers
 # where a wave may use more than 256, and reads every value back for its add.
 _VGPR_RESULTS = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
-EXTRA_FLAGS = {"ff_gemm_fp8_block.hip": _VGPR_RESULTS, "ff_moe.hip": _VGPR_RESULTS}
+# Paged attention: the scores go through the softmax, which reads ordinary registers.
+EXTRA_FLAGS = {"ff_gemm_fp8_block.hip": _VGPR_RESULTS, "ff_moe.hip": _VGPR_RESULTS,
+               "ff_attention_paged.hip": _VGPR_RESULTS}
 
 
 def sources():

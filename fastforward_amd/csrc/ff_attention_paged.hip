@@ -34,9 +34,9 @@ struct Args {
   const uint8_t *k, *v, *ks, *vs;
   bf16_t* y;
   float* part_o;   // (items, BM, D) unnormalised sums of split tiles
-  float2* part_s;  // (items, BM) their maximum (of q . k) and denominator
-  int hk, group;
-  int budget;  // 64-key blocks are dealt so that about so many items per head come out; 0: no tile is split
+  float2* part_s;  // (items, BM) their reference (log2) and denominator
+  int hk, group, lbm;  // BM = 1 << lbm rows a tile
+  int least, budget;  // 64-key blocks are dealt so that about so many items per head come out; 0: no tile is split
   int items;   // items per head that the grid holds
   float c2;    // scale * log2(e)
 };
@@ -50,7 +50,7 @@ __device__ __forceinline__ f32x4 mfma_bf16(const bf16x8& a, const u32x4& b, cons
 // Every sequence's rows make ceil(rows / BM) tiles, and every tile is split into as many
 // key ranges as its sequence's blocks take chunks. A chunk is the share of all blocks
 // that gives `budget` items, `least` blocks at least. All workgroups compute the
-// same list from the lengths. Rows behind the last sequence are a sequence without keys.
+// same list from the lengths; a sequence's last tiles, which see the most keys, come first. Rows behind the last sequence are a sequence without keys.
 
 struct Seq {
   int row0, n;    // first row (token) and rows
@@ -59,7 +59,6 @@ struct Seq {
   int tiles, blocks;
 };
 
-template <int BM>
 __device__ __forceinline__ Seq seq_of(const Args& p, int b) {
   Seq s = {0, 0, 0, 0, 0, 0};
   const int batch = p.a.starts ? p.a.batch : p.a.t;
@@ -73,22 +72,21 @@ __device__ __forceinline__ Seq seq_of(const Args& p, int b) {
     s.len = p.a.lengths[b];
     s.keys = max(0, (int)min((int64_t)s.len, p.a.capacity()));
   }
-  s.tiles = (int)(((int64_t)s.n * p.group + BM - 1) / BM);
+  s.tiles = (int)(((int64_t)s.n * p.group + (1 << p.lbm) - 1) >> p.lbm);
   s.blocks = s.n ? (s.keys + 63) >> 6 : 0;
   return s;
 }
 
 // Blocks of a chunk.
-template <int BM>
-__device__ __forceinline__ int chunk_of(const Args& p, int lane, int least) {
+__device__ __forceinline__ int chunk_of(const Args& p, int lane) {
   if (!p.budget) return INT_MAX;
   int total = 0;
   for (int b0 = 0; b0 <= p.a.batch; b0 += 64) {
-    const Seq s = seq_of<BM>(p, b0 + lane);
+    const Seq s = seq_of(p, b0 + lane);
     total += s.tiles * s.blocks;
   }
   total = __builtin_amdgcn_readlane(wave_scan(total), 63);
-  return max(least, (total + p.budget - 1) / p.budget);
+  return max(p.least, (total + p.budget - 1) / p.budget);
 }
 
 __device__ __forceinline__ int splits_of(int blocks, int chunk) {
@@ -101,11 +99,10 @@ struct Item {
 };
 
 // Item `id` of the list.
-template <int BM>
 __device__ __forceinline__ bool find_item(const Args& p, int lane, int chunk, int id, Item* out) {
   int base = 0;
   for (int b0 = 0; b0 <= p.a.batch; b0 += 64) {
-    const Seq s = seq_of<BM>(p, b0 + lane);
+    const Seq s = seq_of(p, b0 + lane);
     const int splits = splits_of(s.blocks, chunk), n = s.tiles * splits;
     const int sum = wave_scan(n), first = base + sum - n;
     const uint64_t hit = __ballot(id >= first && id < first + n);
@@ -117,7 +114,7 @@ __device__ __forceinline__ bool find_item(const Args& p, int lane, int chunk, in
       out->seq = b0 + src;
       out->splits = __builtin_amdgcn_readlane(splits, src);
       const int in = id - __builtin_amdgcn_readlane(first, src);
-      out->tile = in / out->splits;
+      out->tile = out->s.tiles - 1 - in / out->splits;
       out->split = in % out->splits;
       return true;
     }
@@ -134,6 +131,13 @@ template <int RB, bool FP8>
 __device__ __forceinline__ int v_swizzle(int row) {
   if (FP8) return RB == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
   return RB == 256 ? 2 * ((row & 3) | ((row >> 1) & 4)) : 2 * (((row >> 1) & 1) | ((row >> 2) & 2));
+}
+
+// The same address, of which the compiler does not know that it is: fragments read at one and
+// at the other are not kept in registers between the two.
+__device__ __forceinline__ uint32_t another(uint32_t lds) {
+  asm volatile("" : "+s"(lds));
+  return lds;
 }
 
 __device__ __forceinline__ s16x4 read_tr16(uint32_t lds) {
@@ -186,7 +190,9 @@ __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)"
 
 // One block of the running softmax. s[2 c + tt][r] is q . k of key 32 c + 8 g + 4 tt + r;
 // vis: the block's keys that this lane's row sees (`masked`: not all of them, in some
-// lane). P^T of chunk c goes to pf[c], times the keys' value scales (FP8).
+// lane). m is the reference, the maximum of q . k times c2 = scale log2 e, rounded: all
+// weights are relative to that very number. P^T of chunk c goes to pf[c], times the keys'
+// value scales (FP8).
 template <bool FP8>
 __device__ __forceinline__ float softmax_block(f32x4 (&s)[4], bool masked, uint64_t vis, int g, float c2,
                                                const u32x2 (&vsc)[2], float& m, float& den, u32x4 (&pf)[2]) {
@@ -203,15 +209,15 @@ __device__ __forceinline__ float softmax_block(f32x4 (&s)[4], bool masked, uint6
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r) top = __builtin_elementwise_maximum(top, s[i][r]);
-  const float mnew = fmaxf(m, max_rows(top));
+  const float mnew = fmaxf(m, max_rows(top) * c2);
   const float mref = mnew == -INFINITY ? 0.f : mnew;
-  const float alpha = __builtin_amdgcn_exp2f((m - mref) * c2);
+  const float alpha = __builtin_amdgcn_exp2f(m - mref);
   float psum = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      s[i][r] = __builtin_amdgcn_exp2f((s[i][r] - mref) * c2);
+      s[i][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], c2, -mref));
       psum += s[i][r];
     }
   den = den * alpha + psum;
@@ -248,42 +254,26 @@ __device__ __forceinline__ bool values_odd(uint32_t lds, int r16, int g) {
   return __ballot(odd) != 0;
 }
 
-// o += V^T P^T where a row may not see a key whose values are odd: 0 times them would be NaN.
-// The product runs on the finite values; a second one counts, for each (row, dim), the
-// infinities and NaN among the values that the row does see.
-template <int D, bool FP8>
-__device__ __forceinline__ void add_odd_values(uint32_t lds, const u32x4 (&pf)[2], int r16, int g, f32x4 (&o)[D / 16]) {
-  for (int dt = 0; dt < D / 16; ++dt) {
-    f32x4 sum = {0.f, 0.f, 0.f, 0.f}, up = sum, down = sum, nan = sum;
+// A fragment with zeros in place of infinities and NaN.
+__device__ __forceinline__ bf16x8 finite_only(const bf16x8& v) {
+  u32x4 w = __builtin_bit_cast(u32x4, v);
+  uint32_t* x = &w.x;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      typedef short s16x8 __attribute__((ext_vector_type(8)));
-      const s16x8 v = __builtin_bit_cast(s16x8, v_fragment<D, FP8>(lds, c, dt, r16, g));
-      s16x8 fine, u, d, n;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t b = (uint16_t)v[e];
-        fine[e] = (b & 0x7F80) == 0x7F80 ? 0 : v[e];
-        u[e] = b == 0x7F80 ? 0x3F80 : 0;
-        d[e] = b == 0xFF80 ? 0x3F80 : 0;
-        n[e] = (b & 0x7FFF) > 0x7F80 ? 0x3F80 : 0;
-      }
-      sum = mfma_bf16(__builtin_bit_cast(bf16x8, fine), pf[c], sum);
-      up = mfma_bf16(__builtin_bit_cast(bf16x8, u), pf[c], up);
-      down = mfma_bf16(__builtin_bit_cast(bf16x8, d), pf[c], down);
-      nan = mfma_bf16(__builtin_bit_cast(bf16x8, n), pf[c], nan);
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      float x = sum[r];
-      x = up[r] > 0.f ? x + INFINITY : x;
-      x = down[r] > 0.f ? x - INFINITY : x;
-      sum[r] = nan[r] > 0.f ? __builtin_nanf("") : x;
-    }
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i)  // (registers cannot be indexed)
-      if (i == dt) o[i] = o[i] + sum;
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = (x[i] & 0x7F80u) == 0x7F80u ? 0u : 0xFFFFu, hi = (x[i] & 0x7F800000u) == 0x7F800000u ? 0u : 0xFFFF0000u;
+    x[i] &= lo | hi;
   }
+  return __builtin_bit_cast(bf16x8, w);
+}
+
+// 4 values of a bf16 row, what is finite as 0.
+__device__ __forceinline__ f32x4 odd_only(const u32x2& w) {
+  const f32x4 v = {bf16_to_f32(w.x & 0xFFFF), __uint_as_float(w.x & 0xFFFF0000u), bf16_to_f32(w.y & 0xFFFF),
+                   __uint_as_float(w.y & 0xFFFF0000u)};
+  f32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = fabsf(v[i]) < INFINITY ? 0.f : v[i];
+  return r;
 }
 
 // Bits 0 .. last of a block's 64 keys (none where last < 0).
@@ -309,9 +299,9 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_rows_kernel(Args p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, g = lane >> 4;
   const int head = (int)blockIdx.x % p.hk, id = (int)blockIdx.x / p.hk;
-  const int chunk = chunk_of<16>(p, lane, kFewWaves);
+  const int chunk = chunk_of(p, lane);
   Item it;
-  if (!find_item<16>(p, lane, chunk, id, &it)) return;
+  if (!find_item(p, lane, chunk, id, &it)) return;
   const int row = it.tile * 16 + r16, rows = it.s.n * p.group;
   const bool real = row < rows;
   const int query = (real ? row : rows - 1) / p.group, hq = head * p.group + (real ? row : rows - 1) % p.group;
@@ -416,9 +406,32 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_rows_kernel(Args p) {
       }
       wait_lds();
     }
-    // where the tile's rows see different keys, one that a row does not see may be odd
-    if (__ballot(real && vis != ok) && values_odd<D, FP8>(lds, r16, g)) {
-      add_odd_values<D, FP8>(lds, pf, r16, g, o);
+    // Where the tile's rows see different keys, one that a row does not see may be odd, and 0 times
+    // its value not 0: the product takes the finite values, and a row adds the odd ones it sees.
+    if (__ballot(real && vis != ok) && values_odd<D, FP8>(another(lds), r16, g)) {
+      const uint32_t lds1 = another(lds);
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int dt = 0; dt < DTN; ++dt)
+          o[dt] = mfma_bf16(finite_only(v_fragment<D, FP8>(lds1, c, dt, r16, g)), pf[c], o[dt]);
+#pragma unroll 1
+      for (int key = 0; key < 64; ++key) {
+        const uint8_t* at = smem + wave * SLAB + key * RB;
+#pragma unroll
+        for (int dt = 0; dt < DTN; ++dt) {
+          f32x4 x;
+          const int place = v_swizzle<RB, FP8>(key);
+          if constexpr (FP8) {  // the only odd code is NaN
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(at + 16 * (dt ^ place) + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = (w >> (8 * r) & 0x7F) == 0x7F ? __builtin_nanf("") : 0.f;
+          } else {
+            x = odd_only(*reinterpret_cast<const u32x2*>(at + 16 * ((2 * dt + (g >> 1)) ^ place) + 8 * (g & 1)));
+          }
+          if (vis >> key & 1) o[dt] = o[dt] + x;
+        }
+      }
       continue;
     }
 #pragma unroll
@@ -451,7 +464,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_rows_kernel(Args p) {
     float sum = 0.f;
 #pragma unroll
     for (int w = 0; w < kFewWaves; ++w) {
-      const float wt = __builtin_amdgcn_exp2f((sm[w * 16 + r] - mref) * p.c2);
+      const float wt = __builtin_amdgcn_exp2f(sm[w * 16 + r] - mref);
       sum += sd[w * 16 + r] * wt;
       fma4(acc, *reinterpret_cast<const f32x4*>(so + (w * 16 + r) * LDO + d0), wt);
     }
@@ -468,21 +481,398 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_rows_kernel(Args p) {
   }
 }
 
+// ------------------------------------------------------------------ many rows
+//
+// One workgroup per item: NW waves of 32 NT rows each share the item's 64-key blocks, which
+// pass through LDS in three stages (bf16 pages by DMA; codes through registers, where they
+// become scaled bf16, in two). v_mfma_f32_32x32x16_bf16: a lane's scores and sums
+// belong to one row, and 16 of a 32-key tile's scores are the two operand
+// registers of the second product. The reference moves only where a score passes it by
+// 2^8: P then is at most 2^8, which costs nothing in a floating-point format, and
+// the sums are rescaled in few blocks only.
+// (DMA in two stages where 32 rows a wave leave room for two workgroups a CU.)
+//
+// LDS rows are bf16 (RB = 2 D bytes); 16-byte chunk c of key k is kept at chunk
+// c ^ k_place(k) (keys: the 16 keys that a fragment read takes together fall on different
+// banks), c ^ v_place(k) (values: 4 keys x 64 bytes do).
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <int D>
+__device__ __forceinline__ int k_place(int key) {
+  return D == 128 ? key & 15 : (key >> 1) & 7;
+}
+template <int D>
+__device__ __forceinline__ int v_place(int key) {
+  return D == 128 ? 4 * (key & 3) : 4 * ((key >> 1) & 1);
+}
+
+__device__ __forceinline__ f32x16 mfma32(const bf16x8& a, const u32x4& b, const f32x16& c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// V^T fragment of 16 keys from 16 c, dims 32 dt ..: lane 32 h + r gets keys 16 c + 8 h .. + 7 of
+// dim 32 dt + r.
+template <int D>
+__device__ __forceinline__ bf16x8 v_fragment32(uint32_t lds, int c, int dt, int lane) {
+  s16x4 v[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int key = 16 * c + 8 * (lane >> 5) + 4 * i + ((lane >> 2) & 3);
+    const int chunk = (4 * dt + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ v_place<D>(key);
+    v[i] = read_tr16(lds + key * 2 * D + 16 * chunk + 8 * (lane & 1));
+  }
+  typedef short s16x8 __attribute__((ext_vector_type(8)));
+  return __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+__device__ __forceinline__ float max_halves(float x) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float sum_halves(float x) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+// values_odd on this kernel's fragments.
+template <int D>
+__device__ __forceinline__ bool values_odd32(uint32_t lds, int lane) {
+  const u32x4 ones = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+  f32x16 t = {};
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) {
+      t = mfma32(v_fragment32<D>(lds, c, dt, lane), ones, t);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  bool odd = false;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) odd |= !(fabsf(t[r]) < INFINITY);
+  return __ballot(odd) != 0;
+}
+
+template <int D, bool FP8, int NW, int NT>
+__global__ __launch_bounds__(64 * NW, NT == 1 ? 2 : 1) void many_rows_kernel(Args p) {
+  constexpr int RB = 2 * D, KST = D / 16, DTN = D / 32;
+  constexpr int NS = FP8 || NT == 1 ? 2 : 3, HALF = 64 * RB, STAGE = 2 * HALF;
+  constexpr int TASKS = 8 / NW;      // of the 8 16-key groups of a block's keys and values, a wave's
+  constexpr int PI = 16 * RB / 1024; // DMAs of a group
+  __shared__ __align__(1024) uint8_t smem[NS * STAGE];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r32 = lane & 31, h = lane >> 5;
+  const int head = (int)blockIdx.x % p.hk, id = (int)blockIdx.x / p.hk;
+  Item it;
+  if (!find_item(p, lane, chunk_of(p, lane), id, &it)) return;
+  const int rows = it.s.n * p.group, row0 = (it.tile << p.lbm) + wave * 32 * NT;
+  const int shift = it.s.len - it.s.n;  // position of query 0
+  const int kend = min(it.s.keys, shift + min(rows - 1, ((it.tile + 1) << p.lbm) - 1) / p.group + 1);
+  const int nb = max(0, kend + 63) >> 6, per = (nb + it.splits - 1) / it.splits;
+  const int b0 = it.split * per, b1 = min(nb, b0 + per);
+
+  // keys that some row of the wave sees, and that all the tile's rows see
+  const int some = row0 < rows ? shift + min(rows - 1, row0 + 32 * NT - 1) / p.group + 1 : 0;
+  const int all = shift + (it.tile << p.lbm) / p.group + 1;
+
+  int pos[NT];
+  u32x4 qf[NT][KST];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int row = row0 + 32 * t + r32, real = min(row, rows - 1);
+    pos[t] = row < rows ? shift + row / p.group : -1;
+    const bf16_t* qp = p.q + (it.s.row0 + real / p.group) * p.q_ts + (head * p.group + real % p.group) * p.q_hs + 8 * h;
+    const bool vec = ((uintptr_t)p.q & 15) == 0 && ((p.q_ts | p.q_hs) & 7) == 0;
+#pragma unroll
+    for (int st = 0; st < KST; ++st) {
+      if (vec) {
+        qf[t][st] = *reinterpret_cast<const u32x4*>(qp + 16 * st);
+      } else {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = bf16_to_f32(qp[16 * st + i]);
+        qf[t][st] = pack8(x);
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t)  // waited for here, not behind the first blocks' loads
+#pragma unroll
+    for (int st = 0; st < KST; ++st)
+      asm volatile("" : : "v"(qf[t][st].x), "v"(qf[t][st].y), "v"(qf[t][st].z), "v"(qf[t][st].w));
+
+  f32x16 o[NT][DTN];
+  float m[NT], den[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    m[t] = -INFINITY;
+    den[t] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DTN; ++dt) o[t][dt] = f32x16{};
+  }
+
+  // The table is read through the scalar cache: a vector load would be waited for together
+  // with the blocks' DMAs.
+  typedef const __attribute__((address_space(4))) int* ConstInts;
+  const ConstInts table =
+      (ConstInts)(uintptr_t)(p.a.table + (int64_t)min(it.seq, p.a.batch - 1) * p.a.width);
+  const uint32_t lds0 = lds_addr(smem);
+  const int in_page = (1 << p.a.lps) - 1;
+  // A block's table entries, one for each 16 keys; read a block ahead of their use.
+  struct Entries {
+    int e[4];
+  };
+  auto entries = [&](int b) {
+    Entries n;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) n.e[j] = table[min((int64_t)((64 * b + 16 * j) >> p.a.lps), p.a.width - 1)];
+    return n;
+  };
+  auto page_there = [&](int e) { return (unsigned)e < (unsigned)p.a.pages; };
+  auto keys_there = [&](int b, const Entries& n) {
+    uint64_t ok = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ok |= page_there(n.e[j]) ? 0xFFFFull << (16 * j) : 0;
+    return ok & keys_to(kend - 1 - 64 * b);
+  };
+  // Row of the pages' (page, head, slot) of the first of 16 keys (uniform).
+  auto first_row = [&](int b, int grp, const Entries& n) {
+    const int e = grp == 0 ? n.e[0] : grp == 1 ? n.e[1] : grp == 2 ? n.e[2] : n.e[3];
+    return (((int64_t)(page_there(e) ? e : 0) * p.hk + head) << p.a.lps) + ((64 * b + 16 * grp) & in_page);
+  };
+
+  // One block into LDS. bf16: DMA of this wave's groups. Codes: into registers (load), and later
+  // scaled to LDS (store).
+  constexpr int CK = D / 16, CH = FP8 ? 2 * CK / NW : 1;  // 16-code chunks of a key, of a thread
+  u32x4 code[CH];
+  uint32_t byte[CH];
+  auto issue = [&](int b, int buf, const Entries& n) {
+#pragma unroll
+    for (int j = 0; j < TASKS; ++j) {
+      const int task = wave + j * NW, grp = task & 3;
+      const bool values = task >> 2;
+      const uint8_t* src = (values ? p.v : p.k) + first_row(b, grp, n) * RB;
+      const uint32_t dst = lds0 + buf * STAGE + values * HALF + grp * 16 * RB;
+#pragma unroll
+      for (int i = 0; i < PI; ++i) {
+        const int off = i * 1024 + lane * 16, key = off / RB, chunk = off % RB / 16;
+        lds_dma16(src + key * RB + 16 * (chunk ^ (values ? v_place<D>(key) : k_place<D>(key))), dst + i * 1024);
+      }
+    }
+  };
+  auto load = [&](int b, const Entries& n) {
+    const uint64_t ok = keys_there(b, n);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int c0 = (i * NW + wave) * 64;  // the wave's first chunk; all of them are of one 16-key group
+      const int key0 = c0 / CK & 63, key = key0 + lane / CK;
+      const bool values = c0 >= 64 * CK, there = ok >> key & 1;
+      const int64_t at = first_row(b, key0 >> 4, n) + (key & 15);
+      code[i] = *reinterpret_cast<const u32x4*>((values ? p.v : p.k) + at * D + 16 * (lane % CK));
+      byte[i] = (values ? p.vs : p.ks)[at];
+      if (!there) code[i] = u32x4{0, 0, 0, 0}, byte[i] = 0;
+    }
+  };
+  auto store = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int c0 = (i * NW + wave) * 64, key = (c0 / CK & 63) + lane / CK, chunk = 2 * (lane % CK);
+      const bool values = c0 >= 64 * CK;
+      const int place = values ? v_place<D>(key) : k_place<D>(key);
+      uint8_t* to = smem + buf * STAGE + values * HALF + key * RB;
+      const float s = scale_of(byte[i]);
+      *reinterpret_cast<bf16x8*>(to + 16 * (chunk ^ place)) = e4m3_to_bf16x8(code[i].x, code[i].y, s);
+      *reinterpret_cast<bf16x8*>(to + 16 * ((chunk + 1) ^ place)) = e4m3_to_bf16x8(code[i].z, code[i].w, s);
+    }
+  };
+
+  // Zeros in place of a block's infinite values and NaN.
+  auto scrub = [&](int buf) {
+    barrier_lds();
+    for (int e = threadIdx.x; e < HALF / 16; e += 64 * NW) {
+      bf16x8* at = reinterpret_cast<bf16x8*>(smem + buf * STAGE + HALF + 16 * e);
+      *at = finite_only(*at);
+    }
+    barrier_lds();
+  };
+
+  // The keys of blocks b, b + 1 (and b + 2) that are there, and the entries of the one after.
+  uint64_t ok = 0, ok1 = 0, ok2 = 0;
+  Entries ahead = entries(b0);
+  if (b0 < b1) {
+    ok = keys_there(b0, ahead);
+    if constexpr (FP8) {
+      load(b0, ahead);
+      store(0);
+    } else {
+      issue(b0, 0, ahead);
+    }
+    ahead = entries(b0 + 1);
+  }
+  if (b0 + 1 < b1) {
+    ok1 = keys_there(b0 + 1, ahead);
+    if constexpr (FP8) load(b0 + 1, ahead);
+    else if (NS == 3) issue(b0 + 1, 1, ahead);
+    if (FP8 || NS == 3) ahead = entries(b0 + 2);
+  }
+  for (int b = b0; b < b1; ++b, ok = ok1, ok1 = ok2) {
+    const int kb = 64 * b, buf = (b - b0) % NS;
+    if constexpr (FP8) {
+      barrier_lds();  // block b is there for every wave, block b - 1 no longer read
+      if (b + 1 < b1) store(buf ^ 1);
+    } else {
+      if (NS == 3 && b + 1 < b1) wait_vmcnt<TASKS * PI>();
+      else wait_vmcnt<0>();
+      barrier_lds();
+    }
+    constexpr int AHEAD = FP8 || NS == 3 ? 2 : 1;
+    if (b + AHEAD < b1) {
+      if constexpr (FP8) load(b + 2, ahead);
+      else issue(b + AHEAD, (b - b0 + AHEAD) % NS, ahead);
+      (AHEAD == 2 ? ok2 : ok1) = keys_there(b + AHEAD, ahead);
+      ahead = entries(b + AHEAD + 1);
+    }
+    const uint32_t lds = lds0 + buf * STAGE;
+    if (!FP8 && ok != ~0ull) {  // values that are not there may be anything, and 0 times it not 0
+      for (int e = threadIdx.x; e < HALF / 16; e += 64 * NW)
+        if (!(ok >> (e * 16 / RB) & 1)) *reinterpret_cast<u32x4*>(smem + buf * STAGE + HALF + 16 * e) = u32x4{0, 0, 0, 0};
+      barrier_lds();
+    }
+    // Where the tile's rows see different keys, one that a row does not see may have odd values, and
+    // 0 times them is not 0: a row adds the odd ones that it sees, and the product takes the
+    // finite ones. The same for all waves.
+    const bool odd = !(ok == ~0ull && kb + 64 <= all) && values_odd32<D>(another(lds + HALF), lane);
+    if (kb >= some) {
+      if (odd) scrub(buf);
+      continue;
+    }
+
+    f32x16 s[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = f32x16{};
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      // matrix row r32 of the tile is key 16 (r32 / 16) + 8 (r32 / 4 % 2) + 4 (r32 / 8 % 2) + r32 % 4
+      const int key = 32 * kt + (r32 & 16) + ((r32 & 4) << 1) + ((r32 & 8) >> 1) + (r32 & 3);
+#pragma unroll
+      for (int st = 0; st < KST; ++st) {
+        const bf16x8 k = *reinterpret_cast<const bf16x8*>(smem + buf * STAGE + key * RB +
+                                                          16 * ((2 * st + h) ^ k_place<D>(key)));
+#pragma unroll
+        for (int t = 0; t < NT; ++t) s[t][kt] = mfma32(k, qf[t][st], s[t][kt]);
+      }
+    }
+    u32x4 pf[NT][4];
+    const bool full = ok == ~0ull && kb + 64 <= all;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      if (!full) {
+        const uint64_t vis = ok & keys_to(pos[t] - kb);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t bits = (uint32_t)(vis >> (16 * c + 8 * h));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int i = 8 * (c & 1) + e;
+            s[t][c >> 1][i] = bits >> e & 1 ? s[t][c >> 1][i] : -INFINITY;
+          }
+        }
+      }
+      float top = s[t][0][0];
+#pragma unroll
+      for (int i = 1; i < 32; ++i) top = __builtin_elementwise_maximum(top, s[t][i >> 4][i & 15]);
+      top = max_halves(top) * p.c2;
+      if (__ballot(top > m[t] + 8.f)) {
+        const float mnew = fmaxf(m[t], top), mref = mnew == -INFINITY ? 0.f : mnew;
+        const float alpha = __builtin_amdgcn_exp2f(m[t] - mref);
+        m[t] = mnew;
+        den[t] *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DTN; ++dt) o[t][dt] = o[t][dt] * alpha;
+      }
+      const float mref = m[t] == -INFINITY ? 0.f : m[t];
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][c >> 1][8 * (c & 1) + e], p.c2, -mref));
+          sum[e & 3] += x[e];
+        }
+        pf[t][c] = pack8(x);
+      }
+      den[t] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    }
+    if (odd) {
+#pragma unroll 1
+      for (int key = 0; key < 64; ++key) {
+        const uint8_t* at = smem + buf * STAGE + HALF + key * RB + 8 * h;
+#pragma unroll
+        for (int i = 0; i < 4 * DTN; ++i) {
+          const f32x4 x = odd_only(*reinterpret_cast<const u32x2*>(at + 16 * (i ^ v_place<D>(key))));
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              o[t][i >> 2][4 * (i & 3) + e] += (ok & keys_to(pos[t] - kb)) >> key & 1 ? x[e] : 0.f;
+        }
+      }
+      scrub(buf);
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int dt = 0; dt < DTN; ++dt) {
+        const bf16x8 v = v_fragment32<D>(lds + HALF, c, dt, lane);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) o[t][dt] = mfma32(v, pf[t][c], o[t][dt]);
+      }
+  }
+
+  // lane (h, r32) holds dims 32 dt + 8 a + 4 h .. + 3 of its row
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const float sum = sum_halves(den[t]);
+    const int row = row0 + 32 * t + r32;
+    if (row >= rows) continue;
+    if (it.splits == 1) {
+      const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+      bf16_t* to = p.y + ((int64_t)(it.s.row0 + row / p.group) * (p.hk * p.group) + head * p.group + row % p.group) * D;
+#pragma unroll
+      for (int i = 0; i < 4 * DTN; ++i) {
+        const f32x16& x = o[t][i >> 2];
+        const int a = 4 * (i & 3);
+        *reinterpret_cast<u32x2*>(to + 8 * i + 4 * h) =
+            pack4_bf16(x[a] * inv, x[a + 1] * inv, x[a + 2] * inv, x[a + 3] * inv);
+      }
+    } else {
+      const int64_t at = (((int64_t)id * p.hk + head) << p.lbm) + (row - (it.tile << p.lbm));
+#pragma unroll
+      for (int i = 0; i < 4 * DTN; ++i) {
+        const f32x16& x = o[t][i >> 2];
+        const int a = 4 * (i & 3);
+        *reinterpret_cast<f32x4*>(p.part_o + at * D + 8 * i + 4 * h) = f32x4{x[a], x[a + 1], x[a + 2], x[a + 3]};
+      }
+      if (h == 0) p.part_s[at] = float2{m[t], sum};
+    }
+  }
+}
+
 // ------------------------------------------------------------------ joining split tiles
 
 // A wave per row (token, head); rows of unsplit tiles are there already.
-template <int D, int BM>
-__global__ __launch_bounds__(256) void join_kernel(Args p, int least) {
+template <int D>
+__global__ __launch_bounds__(256) void join_kernel(Args p) {
   const int lane = threadIdx.x & 63;
   const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int heads = p.hk * p.group;
   if (r >= (int64_t)p.a.t * heads) return;
   const int token = __builtin_amdgcn_readfirstlane((int)(r / heads)), hq = (int)(r % heads);
   const int head = hq / p.group;
-  const int chunk = chunk_of<BM>(p, lane, least);
+  const int chunk = chunk_of(p, lane);
   int base = 0, first = 0, splits = 1;
   for (int b0 = 0; b0 <= p.a.batch; b0 += 64) {
-    const Seq s = seq_of<BM>(p, b0 + lane);
+    const Seq s = seq_of(p, b0 + lane);
     const int sp = splits_of(s.blocks, chunk), n = s.tiles * sp;
     const int sum = wave_scan(n);
     const uint64_t hit = __ballot(token >= s.row0 && token < s.row0 + s.n);
@@ -490,8 +880,9 @@ __global__ __launch_bounds__(256) void join_kernel(Args p, int least) {
       const int src = __builtin_ctzll(hit);
       const int in = (token - __builtin_amdgcn_readlane(s.row0, src)) * p.group + hq % p.group;
       splits = __builtin_amdgcn_readlane(sp, src);
-      first = base + __builtin_amdgcn_readlane(sum - n, src) + in / BM * splits;
-      base = in % BM;
+      first = base + __builtin_amdgcn_readlane(sum - n, src) +
+              (__builtin_amdgcn_readlane(s.tiles, src) - 1 - (in >> p.lbm)) * splits;
+      base = in & ((1 << p.lbm) - 1);
       break;
     }
     base += __builtin_amdgcn_readlane(sum, 63);
@@ -499,16 +890,16 @@ __global__ __launch_bounds__(256) void join_kernel(Args p, int least) {
   if (splits == 1 || first + splits > p.items) return;
   const int row = base;
   float mx = -INFINITY;
-  for (int i = lane; i < splits; i += 64) mx = fmaxf(mx, p.part_s[((int64_t)(first + i) * p.hk + head) * BM + row].x);
+  for (int i = lane; i < splits; i += 64) mx = fmaxf(mx, p.part_s[(((int64_t)(first + i) * p.hk + head) << p.lbm) + row].x);
   mx = wave_max(mx);
   const float mref = mx == -INFINITY ? 0.f : mx;
   constexpr int PER = D / 64;
   float acc[PER] = {}, sum = 0.f;
 #pragma unroll 4
   for (int i = 0; i < splits; ++i) {
-    const int64_t at = ((int64_t)(first + i) * p.hk + head) * BM + row;
+    const int64_t at = (((int64_t)(first + i) * p.hk + head) << p.lbm) + row;
     const float2 st = p.part_s[at];
-    const float wt = __builtin_amdgcn_exp2f((st.x - mref) * p.c2);
+    const float wt = __builtin_amdgcn_exp2f(st.x - mref);
     sum += st.y * wt;
 #pragma unroll
     for (int e = 0; e < PER; ++e) acc[e] = __builtin_fmaf(p.part_o[at * D + PER * lane + e], wt, acc[e]);
@@ -522,17 +913,24 @@ __global__ __launch_bounds__(256) void join_kernel(Args p, int least) {
 // ------------------------------------------------------------------ host
 
 struct Plan {
-  int bm, least, budget;
+  int kind;  // 0: few rows; 1, 2: many rows, 32 and 64 a wave
+  int lbm, least, budget;
   int64_t items;  // per key head
 };
 
-constexpr int kWorkgroups = 512;  // two a CU
-
 Plan plan_of(int64_t t, int64_t batch, int64_t hk, int64_t group, int64_t capacity) {
-  Plan p = {16, kFewWaves, 0, 0};
-  const int64_t tiles = t * group / p.bm + batch + 1;
-  // a sequence of `least` blocks at most is one chunk whatever the lengths are
-  if ((capacity + 63) / 64 > p.least) p.budget = (int)((kWorkgroups + hk - 1) / hk);
+  const int64_t rows = t * group;
+  const int force = ff_tuning(FF_TUNE_PAGED_ROWS);
+  Plan p = {};
+  p.kind = force ? force - 1 : rows <= 32 * batch ? 0 : rows <= 256 * batch ? 1 : 2;
+  p.lbm = p.kind == 0 ? 4 : p.kind == 1 ? 7 : 8;
+  p.least = p.kind == 0 ? kFewWaves : 8;
+  const int64_t workgroups = p.kind == 2 ? 256 : 512;  // the GPU's, at one and two a CU
+  const int64_t tiles = (rows >> p.lbm) + batch + 1;
+  // No splits where a sequence's keys are one chunk whatever its length is, nor where there
+  // are tiles enough.
+  if ((capacity + 63) / 64 > p.least && (rows >> p.lbm) * hk < 2 * workgroups)
+    p.budget = (int)((workgroups + hk - 1) / hk);
   p.items = tiles + p.budget;
   return p;
 }
@@ -546,13 +944,13 @@ int check(const char* what, int64_t hq, int64_t hk, int64_t d, int64_t ps, int64
              "%s: bad sizes hq=%lld hk=%lld width=%lld batch=%lld t=%lld", what, (long long)hq, (long long)hk,
              (long long)width, (long long)batch, (long long)t);
   const int64_t tiles = t * (hq / hk) / 16 + batch + 1;
-  FF_REQUIRE(tiles * ((width * ps + 63) / 64) <= INT32_MAX && (tiles + kWorkgroups) * hk <= INT32_MAX,
+  FF_REQUIRE(tiles * ((width * ps + 63) / 64) <= INT32_MAX && (tiles + 512) * hk <= INT32_MAX,
              "%s: too large a call (rows x positions)", what);
   return FF_OK;
 }
 
 int64_t workspace_of(const Plan& p, int64_t hk, int64_t d) {
-  return p.budget ? p.items * hk * p.bm * (d * 4 + 8) : 0;
+  return p.budget ? ((p.items * hk) << p.lbm) * (d * 4 + 8) : 0;
 }
 
 }  // namespace
@@ -599,19 +997,23 @@ extern "C" int ff_attention_paged(const void* q, int64_t q_ts, int64_t q_hs, con
   p.vs = (const uint8_t*)v_scale;
   p.y = (bf16_t*)y;
   p.part_o = (float*)workspace;
-  p.part_s = (float2*)((char*)workspace + plan.items * hk * plan.bm * d * 4);
+  p.part_s = (float2*)((char*)workspace + ((plan.items * hk) << plan.lbm) * d * 4);
   p.hk = (int)hk;
   p.group = (int)(hq / hk);
+  p.lbm = plan.lbm;
+  p.least = plan.least;
   p.budget = plan.budget;
   p.items = (int)plan.items;
   p.c2 = (float)((double)scale * 1.4426950408889634);
-  const dim3 grid((unsigned)(plan.items * hk)), block(64 * kFewWaves);
+  const dim3 grid((unsigned)(plan.items * hk));
   const dim3 join((unsigned)((t * hq + 3) / 4));
   hipStream_t s = (hipStream_t)stream;
-#define FF_PAGED(DIM, F8)                                                                            \
-  if (d == DIM && (fp8 != 0) == F8) {                                                                \
-    hipLaunchKernelGGL((few_rows_kernel<DIM, F8>), grid, block, 0, s, p);                            \
-    if (plan.budget) hipLaunchKernelGGL((join_kernel<DIM, 16>), join, dim3(256), 0, s, p, plan.least); \
+#define FF_PAGED(DIM, F8)                                                                                          \
+  if (d == DIM && (fp8 != 0) == F8) {                                                                              \
+    if (plan.kind == 0) hipLaunchKernelGGL((few_rows_kernel<DIM, F8>), grid, dim3(64 * kFewWaves), 0, s, p);       \
+    else if (plan.kind == 1) hipLaunchKernelGGL((many_rows_kernel<DIM, F8, 4, 1>), grid, dim3(256), 0, s, p);      \
+    else hipLaunchKernelGGL((many_rows_kernel<DIM, F8, 4, 2>), grid, dim3(256), 0, s, p);                          \
+    if (plan.budget) hipLaunchKernelGGL((join_kernel<DIM>), join, dim3(256), 0, s, p);                             \
   }
   FF_PAGED(64, false) FF_PAGED(64, true) FF_PAGED(128, false) FF_PAGED(128, true)
 #undef FF_PAGED

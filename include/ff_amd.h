@@ -58,6 +58,8 @@ int ff_device_check(void);
                                  on two k groups */
 #define FF_TUNE_MOE_TILE 13   /* ff_moe_experts: 1 pair by pair, 2 32-row, 3 64-row tiles (set it before the
                                  workspace is asked for) */
+#define FF_TUNE_PAGED_ROWS 14 /* ff_attention_paged: 1 16-row tiles, 2 128-row, 3 256-row tiles (set it before the
+                                 workspace is asked for) */
 int ff_set_tuning(int knob, int value);
 
 /* fast_norm(x, module): out = bf16(bf16(x*rsqrt(sum(x^2)/h + eps)) * w), one row

@@ -136,7 +136,7 @@ def test_write_codes(gpu, d):
 
 @gpu_test
 @pytest.mark.parametrize("dtype", [BF16, E4M3])
-def test_rows_without_a_place(gpu, dtype):
+def test_rows_without_a_place(gpu, tile, dtype):
     """Lengths under the rows' count, past the table, of nothing; page ids of none; rows behind the
     last sequence; starts and lengths that are nonsense."""
     c = Case([10, 5, 100, 40, 0], [6, 9, 60, 40, 2], 2, 64, 16, dtype, width=4, spare=7)
@@ -163,6 +163,17 @@ def test_rows_without_a_place(gpu, dtype):
 
 # ---------------------------------------------------------------- attention
 
+@pytest.fixture(params=[0, 1, 2, 3])
+def tile(request):
+    """The library's own choice of tiles, then each of them for every call."""
+    from fastforward_amd import _lib, cache
+    _lib.call("ff_set_tuning", 14, request.param)
+    cache.attend_workspace.cache_clear()
+    yield request.param
+    _lib.call("ff_set_tuning", 14, 0)
+    cache.attend_workspace.cache_clear()
+
+
 @gpu_test
 @pytest.mark.parametrize("dtype", [BF16, E4M3])
 @pytest.mark.parametrize("hk,group,d,ps,lengths,new", [
@@ -170,7 +181,7 @@ def test_rows_without_a_place(gpu, dtype):
     (2, 16, 128, 32, [129, 128], None), (1, 17, 64, 16, [90], None), (2, 3, 128, 16, [31, 90, 4], [31, 1, 4]),
     (2, 4, 64, 64, [150, 300], [150, 61]), (1, 7, 128, 256, [333], [57]), (4, 1, 128, 32, [70, 0, 66], [70, 0, 3]),
     (2, 2, 128, 16, [257, 40, 1], [129, 40, 1]), (1, 4, 64, 16, [40] * 67, [2] * 67)])
-def test_attend(gpu, dtype, hk, group, d, ps, lengths, new):
+def test_attend(gpu, tile, dtype, hk, group, d, ps, lengths, new):
     c = Case(lengths, new, hk, d, ps, dtype, seed=len(lengths) + d)
     c.check_attend(_rows(6, c.t, hk * group, d, gain=1.5))
 
@@ -178,7 +189,7 @@ def test_attend(gpu, dtype, hk, group, d, ps, lengths, new):
 @gpu_test
 @pytest.mark.parametrize("dtype,d", [(BF16, 128), (BF16, 64), (E4M3, 128), (E4M3, 64)])
 @pytest.mark.parametrize("n,heads", [(1, 4), (5, 4), (70, 2), (200, 4)])
-def test_attend_every_key_counts(gpu, dtype, d, n, heads):
+def test_attend_every_key_counts(gpu, tile, dtype, d, n, heads):
     """Long sequences: each row looks for one key, far ahead of the others, all over the range it sees,
     borders of blocks, pages and splits among them; and all the others share the rest evenly."""
     length = 5000
@@ -207,7 +218,7 @@ def test_attend_every_key_counts(gpu, dtype, d, n, heads):
 
 @gpu_test
 @pytest.mark.parametrize("dtype", [BF16, E4M3])
-def test_attend_counts(gpu, dtype):
+def test_attend_counts(gpu, tile, dtype):
     """q = 0 and one-hot values by position: output j is the share of visible positions p with
     p % d == j, so that each position's being there is seen."""
     for d, n, length in ((64, 1, 1500), (128, 1, 700), (64, 90, 1100), (128, 33, 300)):
@@ -229,7 +240,7 @@ def test_attend_counts(gpu, dtype):
 
 @gpu_test
 @pytest.mark.parametrize("dtype", [BF16, E4M3])
-def test_attend_garbage_behind_the_mask(gpu, dtype):
+def test_attend_garbage_behind_the_mask(gpu, tile, dtype):
     """NaN and infinities in slots past the length, in pages of no sequence and, for earlier rows, in
     later rows of the same chunk; scores that overflow the exponential's range."""
     for d, new in ((128, [1, 1]), (64, [20, 37]), (128, [70, 9]), (64, [130, 140])):
