@@ -102,7 +102,7 @@ SIGNATURES = {
     "ff_moe_experts": [P, I64, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, P, I64, P],
     "ff_cache_write": [P, I64, I64, P, I64, I64, P, P, P, P, I64, I64, I64, I64, I32, P, I64, P, P, I64, I64, P],
     "ff_cache_read": [P, P, P, P, I64, I64, I64, I64, I32, P, I64, P, P, I64, P, P, I64, P],
-    "ff_attention_paged_workspace": [I64, I64, I64, I64, I64, I64, I64, PI64],
+    "ff_attention_paged_workspace": [I64, I64, I64, I32, I64, I64, I64, I64, PI64],
     "ff_attention_paged": [P, I64, I64, P, P, P, P, I64, I64, I64, I64, I64, I32, P, I64, P, P, I64, P, I64, F32, P, I64,
                            P],
     "ff_token_scores_workspace": [I64, I64, I64, PI64],

@@ -31,10 +31,10 @@ _ROWS = 1 << 24
 
 
 @functools.lru_cache(maxsize=1024)
-def attend_workspace(heads, kv_heads, head_dim, page_size, width, batch, t):
+def attend_workspace(heads, kv_heads, head_dim, fp8, page_size, width, batch, t):
     """Bytes of workspace ff_attention_paged needs (0: none)."""
     need = ctypes.c_int64(0)
-    call("ff_attention_paged_workspace", heads, kv_heads, head_dim, page_size, width, batch, t, ctypes.byref(need))
+    call("ff_attention_paged_workspace", heads, kv_heads, head_dim, fp8, page_size, width, batch, t, ctypes.byref(need))
     return need.value
 
 
@@ -134,7 +134,7 @@ class PagedCache:
         if q.stride(2) != 1:
             q = q.contiguous()
         y = q.new_empty((t, heads, d))
-        need = attend_workspace(heads, hk, d, self.page_size, rows[1], rows[4], t)
+        need = attend_workspace(heads, hk, d, self.dtype == E4M3, self.page_size, rows[1], rows[4], t)
         ws = q.new_empty((need,), dtype=torch.uint8) if need else None
         entry("ff_attention_paged")(q.data_ptr(), q.stride(0), q.stride(1), *self._held(), heads, hk, d,
                                     self.dtype == E4M3, *rows, y.data_ptr(), t, scale, 0 if ws is None else ws.data_ptr(),

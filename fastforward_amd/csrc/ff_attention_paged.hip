@@ -77,7 +77,12 @@ __device__ __forceinline__ Seq seq_of(const Args& p, int b) {
   return s;
 }
 
-// Blocks of a chunk.
+__device__ __forceinline__ int splits_of(int blocks, int chunk) {
+  return max(1, blocks / chunk + (blocks % chunk != 0));
+}
+
+// Blocks of a chunk: the share of all blocks that gives `budget` items, or as many more as keep the
+// items within it (one round of the GPU's workgroups; a few of a second would take as long).
 __device__ __forceinline__ int chunk_of(const Args& p, int lane) {
   if (!p.budget) return INT_MAX;
   int total = 0;
@@ -86,11 +91,18 @@ __device__ __forceinline__ int chunk_of(const Args& p, int lane) {
     total += s.tiles * s.blocks;
   }
   total = __builtin_amdgcn_readlane(wave_scan(total), 63);
-  return max(p.least, (total + p.budget - 1) / p.budget);
-}
-
-__device__ __forceinline__ int splits_of(int blocks, int chunk) {
-  return max(1, blocks / chunk + (blocks % chunk != 0));
+  int chunk = max(p.least, (total + p.budget - 1) / p.budget);
+  for (int i = 0; i < 3; ++i) {
+    int items = 0;
+    for (int b0 = 0; b0 <= p.a.batch; b0 += 64) {
+      const Seq s = seq_of(p, b0 + lane);
+      items += s.tiles * splits_of(s.blocks, chunk);
+    }
+    items = __builtin_amdgcn_readlane(wave_scan(items), 63);
+    if (items <= p.budget) break;
+    chunk = (int)min((int64_t)INT_MAX, ((int64_t)chunk * items + p.budget - 1) / p.budget);
+  }
+  return chunk;
 }
 
 struct Item {
@@ -140,8 +152,9 @@ __device__ __forceinline__ uint32_t another(uint32_t lds) {
   return lds;
 }
 
-__device__ __forceinline__ s16x4 read_tr16(uint32_t lds) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)lds);
+__device__ __forceinline__ s16x4 read_tr16(uint32_t lds, int offset = 0) {
+  typedef __attribute__((address_space(3))) uint8_t* Bytes;
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)((Bytes)(uintptr_t)lds + offset));
 }
 __device__ __forceinline__ i32x2v read_tr8(uint32_t lds) {
   return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2v*)(uintptr_t)lds);
@@ -483,7 +496,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_rows_kernel(Args p) {
 
 // ------------------------------------------------------------------ many rows
 //
-// One workgroup per item: NW waves of 32 NT rows each share the item's 64-key blocks, which
+// One workgroup per item: NW waves of 32 rows each share the item's 64-key blocks, which
 // pass through LDS in three stages (bf16 pages by DMA; codes through registers, where they
 // become scaled bf16, in two). v_mfma_f32_32x32x16_bf16: a lane's scores and sums
 // belong to one row, and 16 of a 32-key tile's scores are the two operand
@@ -510,17 +523,23 @@ __device__ __forceinline__ f32x16 mfma32(const bf16x8& a, const u32x4& b, const 
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+// lds_dma16 from a uniform base: lane l's 16 bytes at base + offset.
+__device__ __forceinline__ void lds_dma16_at(const uint8_t* base, uint32_t offset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds)
+               : "memory", "m0");
+}
+
 // V^T fragment of 16 keys from 16 c, dims 32 dt ..: lane 32 h + r gets keys 16 c + 8 h .. + 7 of
 // dim 32 dt + r.
 template <int D>
 __device__ __forceinline__ bf16x8 v_fragment32(uint32_t lds, int c, int dt, int lane) {
+  // the lane's address for dims 32 dt .., to which keys add a constant
+  const int key = 8 * (lane >> 5) + ((lane >> 2) & 3);
+  const int chunk = (4 * dt + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ v_place<D>(key);
+  const uint32_t at = lds + key * 2 * D + 16 * chunk + 8 * (lane & 1);
   s16x4 v[2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int key = 16 * c + 8 * (lane >> 5) + 4 * i + ((lane >> 2) & 3);
-    const int chunk = (4 * dt + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ v_place<D>(key);
-    v[i] = read_tr16(lds + key * 2 * D + 16 * chunk + 8 * (lane & 1));
-  }
+  for (int i = 0; i < 2; ++i) v[i] = read_tr16(at, (16 * c + 4 * i) * 2 * D);
   typedef short s16x8 __attribute__((ext_vector_type(8)));
   return __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
 }
@@ -552,10 +571,10 @@ __device__ __forceinline__ bool values_odd32(uint32_t lds, int lane) {
   return __ballot(odd) != 0;
 }
 
-template <int D, bool FP8, int NW, int NT>
-__global__ __launch_bounds__(64 * NW, NT == 1 ? 2 : 1) void many_rows_kernel(Args p) {
+template <int D, bool FP8, int NW>
+__global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void many_rows_kernel(Args p) {
   constexpr int RB = 2 * D, KST = D / 16, DTN = D / 32;
-  constexpr int NS = FP8 || NT == 1 ? 2 : 3, HALF = 64 * RB, STAGE = 2 * HALF;
+  constexpr int NS = FP8 || NW == 4 ? 2 : 3, HALF = 64 * RB, STAGE = 2 * HALF;
   constexpr int TASKS = 8 / NW;      // of the 8 16-key groups of a block's keys and values, a wave's
   constexpr int PI = 16 * RB / 1024; // DMAs of a group
   __shared__ __align__(1024) uint8_t smem[NS * STAGE];
@@ -564,51 +583,41 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? 2 : 1) void many_rows_kernel(Arg
   const int head = (int)blockIdx.x % p.hk, id = (int)blockIdx.x / p.hk;
   Item it;
   if (!find_item(p, lane, chunk_of(p, lane), id, &it)) return;
-  const int rows = it.s.n * p.group, row0 = (it.tile << p.lbm) + wave * 32 * NT;
+  const int rows = it.s.n * p.group, row0 = (it.tile << p.lbm) + wave * 32;
   const int shift = it.s.len - it.s.n;  // position of query 0
   const int kend = min(it.s.keys, shift + min(rows - 1, ((it.tile + 1) << p.lbm) - 1) / p.group + 1);
   const int nb = max(0, kend + 63) >> 6, per = (nb + it.splits - 1) / it.splits;
   const int b0 = it.split * per, b1 = min(nb, b0 + per);
 
   // keys that some row of the wave sees, and that all the tile's rows see
-  const int some = row0 < rows ? shift + min(rows - 1, row0 + 32 * NT - 1) / p.group + 1 : 0;
+  const int some = row0 < rows ? shift + min(rows - 1, row0 + 31) / p.group + 1 : 0;
   const int all = shift + (it.tile << p.lbm) / p.group + 1;
 
-  int pos[NT];
-  u32x4 qf[NT][KST];
+  u32x4 qf[KST];
+  const int row = row0 + r32, real = min(row, rows - 1);
+  const int pos = row < rows ? shift + row / p.group : -1;
+  const bf16_t* qp = p.q + (it.s.row0 + real / p.group) * p.q_ts + (head * p.group + real % p.group) * p.q_hs + 8 * h;
+  const bool vec = ((uintptr_t)p.q & 15) == 0 && ((p.q_ts | p.q_hs) & 7) == 0;
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int row = row0 + 32 * t + r32, real = min(row, rows - 1);
-    pos[t] = row < rows ? shift + row / p.group : -1;
-    const bf16_t* qp = p.q + (it.s.row0 + real / p.group) * p.q_ts + (head * p.group + real % p.group) * p.q_hs + 8 * h;
-    const bool vec = ((uintptr_t)p.q & 15) == 0 && ((p.q_ts | p.q_hs) & 7) == 0;
+  for (int st = 0; st < KST; ++st) {
+    if (vec) {
+      qf[st] = *reinterpret_cast<const u32x4*>(qp + 16 * st);
+    } else {
+      float x[8];
 #pragma unroll
-    for (int st = 0; st < KST; ++st) {
-      if (vec) {
-        qf[t][st] = *reinterpret_cast<const u32x4*>(qp + 16 * st);
-      } else {
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = bf16_to_f32(qp[16 * st + i]);
-        qf[t][st] = pack8(x);
-      }
+      for (int i = 0; i < 8; ++i) x[i] = bf16_to_f32(qp[16 * st + i]);
+      qf[st] = pack8(x);
     }
   }
+  // waited for here, not behind the first blocks' loads
 #pragma unroll
-  for (int t = 0; t < NT; ++t)  // waited for here, not behind the first blocks' loads
-#pragma unroll
-    for (int st = 0; st < KST; ++st)
-      asm volatile("" : : "v"(qf[t][st].x), "v"(qf[t][st].y), "v"(qf[t][st].z), "v"(qf[t][st].w));
+  for (int st = 0; st < KST; ++st)
+    asm volatile("" : : "v"(qf[st].x), "v"(qf[st].y), "v"(qf[st].z), "v"(qf[st].w));
 
-  f32x16 o[NT][DTN];
-  float m[NT], den[NT];
+  f32x16 o[DTN];
+  float m = -INFINITY, den = 0.f;
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    m[t] = -INFINITY;
-    den[t] = 0.f;
-#pragma unroll
-    for (int dt = 0; dt < DTN; ++dt) o[t][dt] = f32x16{};
-  }
+  for (int dt = 0; dt < DTN; ++dt) o[dt] = f32x16{};
 
   // The table is read through the scalar cache: a vector load would be waited for together
   // with the blocks' DMAs.
@@ -645,6 +654,15 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? 2 : 1) void many_rows_kernel(Arg
   constexpr int CK = D / 16, CH = FP8 ? 2 * CK / NW : 1;  // 16-code chunks of a key, of a thread
   u32x4 code[CH];
   uint32_t byte[CH];
+  uint32_t k_from[FP8 ? 1 : PI], v_from;  // where a lane's 16 bytes lie among a group's keys (i-th DMA), values (first)
+  if constexpr (!FP8) {
+#pragma unroll
+    for (int i = 0; i < PI; ++i) {
+      const int off = i * 1024 + lane * 16, key = off / RB, chunk = off % RB / 16;
+      k_from[i] = key * RB + 16 * (chunk ^ k_place<D>(key)) - i * 1024;
+      if (i == 0) v_from = key * RB + 16 * (chunk ^ v_place<D>(key));  // v_place repeats every 1024 bytes
+    }
+  }
   auto issue = [&](int b, int buf, const Entries& n) {
 #pragma unroll
     for (int j = 0; j < TASKS; ++j) {
@@ -653,10 +671,8 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? 2 : 1) void many_rows_kernel(Arg
       const uint8_t* src = (values ? p.v : p.k) + first_row(b, grp, n) * RB;
       const uint32_t dst = lds0 + buf * STAGE + values * HALF + grp * 16 * RB;
 #pragma unroll
-      for (int i = 0; i < PI; ++i) {
-        const int off = i * 1024 + lane * 16, key = off / RB, chunk = off % RB / 16;
-        lds_dma16(src + key * RB + 16 * (chunk ^ (values ? v_place<D>(key) : k_place<D>(key))), dst + i * 1024);
-      }
+      for (int i = 0; i < PI; ++i)
+        lds_dma16_at(src + i * 1024, values ? v_from : k_from[i], dst + i * 1024);
     }
   };
   auto load = [&](int b, const Entries& n) {
@@ -746,63 +762,57 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? 2 : 1) void many_rows_kernel(Arg
       continue;
     }
 
-    f32x16 s[NT][2];
+    // matrix row r32 of key tile kt is key 32 kt + 16 (r32 / 16) + 8 (r32 / 4 % 2) + 4 (r32 / 8 % 2) + r32 % 4
+    const int key = (r32 & 16) + ((r32 & 4) << 1) + ((r32 & 8) >> 1) + (r32 & 3);
+    auto k_fragment = [&](int kt, int st) {
+      return *reinterpret_cast<const bf16x8*>(smem + buf * STAGE + (32 * kt + key) * RB +
+                                              16 * ((2 * st + h) ^ k_place<D>(key)));
+    };
+    f32x16 s[2] = {};
 #pragma unroll
-    for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = f32x16{};
+    for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      // matrix row r32 of the tile is key 16 (r32 / 16) + 8 (r32 / 4 % 2) + 4 (r32 / 8 % 2) + r32 % 4
-      const int key = 32 * kt + (r32 & 16) + ((r32 & 4) << 1) + ((r32 & 8) >> 1) + (r32 & 3);
-#pragma unroll
-      for (int st = 0; st < KST; ++st) {
-        const bf16x8 k = *reinterpret_cast<const bf16x8*>(smem + buf * STAGE + key * RB +
-                                                          16 * ((2 * st + h) ^ k_place<D>(key)));
-#pragma unroll
-        for (int t = 0; t < NT; ++t) s[t][kt] = mfma32(k, qf[t][st], s[t][kt]);
-      }
-    }
-    u32x4 pf[NT][4];
+      for (int st = 0; st < KST; ++st) s[kt] = mfma32(k_fragment(kt, st), qf[st], s[kt]);
+    u32x4 pf[4];
     const bool full = ok == ~0ull && kb + 64 <= all;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      if (!full) {
-        const uint64_t vis = ok & keys_to(pos[t] - kb);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const uint32_t bits = (uint32_t)(vis >> (16 * c + 8 * h));
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int i = 8 * (c & 1) + e;
-            s[t][c >> 1][i] = bits >> e & 1 ? s[t][c >> 1][i] : -INFINITY;
-          }
-        }
-      }
-      float top = s[t][0][0];
-#pragma unroll
-      for (int i = 1; i < 32; ++i) top = __builtin_elementwise_maximum(top, s[t][i >> 4][i & 15]);
-      top = max_halves(top) * p.c2;
-      if (__ballot(top > m[t] + 8.f)) {
-        const float mnew = fmaxf(m[t], top), mref = mnew == -INFINITY ? 0.f : mnew;
-        const float alpha = __builtin_amdgcn_exp2f(m[t] - mref);
-        m[t] = mnew;
-        den[t] *= alpha;
-#pragma unroll
-        for (int dt = 0; dt < DTN; ++dt) o[t][dt] = o[t][dt] * alpha;
-      }
-      const float mref = m[t] == -INFINITY ? 0.f : m[t];
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    if (!full) {
+      asm volatile("");  // a branch: as selects the masks would be computed for every block
+      const uint64_t vis = ok & keys_to(pos - kb);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        float x[8];
+        const uint32_t bits = (uint32_t)(vis >> (16 * c + 8 * h));
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][c >> 1][8 * (c & 1) + e], p.c2, -mref));
-          sum[e & 3] += x[e];
+          const int i = 8 * (c & 1) + e;
+          s[c >> 1][i] = bits >> e & 1 ? s[c >> 1][i] : -INFINITY;
         }
-        pf[t][c] = pack8(x);
       }
-      den[t] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
+    float top = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 32; ++i) top = __builtin_elementwise_maximum(top, s[i >> 4][i & 15]);
+    top = max_halves(top) * p.c2;
+    if (__ballot(top > m + 8.f)) {
+      const float mnew = fmaxf(m, top), mref = mnew == -INFINITY ? 0.f : mnew;
+      const float alpha = __builtin_amdgcn_exp2f(m - mref);
+      m = mnew;
+      den *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DTN; ++dt) o[dt] = o[dt] * alpha;
+    }
+    const float mref = m == -INFINITY ? 0.f : m;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c >> 1][8 * (c & 1) + e], p.c2, -mref));
+        sum[e & 3] += x[e];
+      }
+      pf[c] = pack8(x);
+    }
+    den += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     if (odd) {
 #pragma unroll 1
       for (int key = 0; key < 64; ++key) {
@@ -811,10 +821,8 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? 2 : 1) void many_rows_kernel(Arg
         for (int i = 0; i < 4 * DTN; ++i) {
           const f32x4 x = odd_only(*reinterpret_cast<const u32x2*>(at + 16 * (i ^ v_place<D>(key))));
 #pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              o[t][i >> 2][4 * (i & 3) + e] += (ok & keys_to(pos[t] - kb)) >> key & 1 ? x[e] : 0.f;
+          for (int e = 0; e < 4; ++e)
+            o[i >> 2][4 * (i & 3) + e] += (ok & keys_to(pos - kb)) >> key & 1 ? x[e] : 0.f;
         }
       }
       scrub(buf);
@@ -822,115 +830,121 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? 2 : 1) void many_rows_kernel(Arg
 #pragma unroll
     for (int c = 0; c < 4; ++c)
 #pragma unroll
-      for (int dt = 0; dt < DTN; ++dt) {
-        const bf16x8 v = v_fragment32<D>(lds + HALF, c, dt, lane);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) o[t][dt] = mfma32(v, pf[t][c], o[t][dt]);
-      }
+      for (int dt = 0; dt < DTN; ++dt) o[dt] = mfma32(v_fragment32<D>(lds + HALF, c, dt, lane), pf[c], o[dt]);
   }
 
   // lane (h, r32) holds dims 32 dt + 8 a + 4 h .. + 3 of its row
+  const float sum = sum_halves(den);
+  if (row >= rows) return;
+  if (it.splits == 1) {
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    bf16_t* to = p.y + ((int64_t)(it.s.row0 + row / p.group) * (p.hk * p.group) + head * p.group + row % p.group) * D;
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const float sum = sum_halves(den[t]);
-    const int row = row0 + 32 * t + r32;
-    if (row >= rows) continue;
-    if (it.splits == 1) {
-      const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-      bf16_t* to = p.y + ((int64_t)(it.s.row0 + row / p.group) * (p.hk * p.group) + head * p.group + row % p.group) * D;
-#pragma unroll
-      for (int i = 0; i < 4 * DTN; ++i) {
-        const f32x16& x = o[t][i >> 2];
-        const int a = 4 * (i & 3);
-        *reinterpret_cast<u32x2*>(to + 8 * i + 4 * h) =
-            pack4_bf16(x[a] * inv, x[a + 1] * inv, x[a + 2] * inv, x[a + 3] * inv);
-      }
-    } else {
-      const int64_t at = (((int64_t)id * p.hk + head) << p.lbm) + (row - (it.tile << p.lbm));
-#pragma unroll
-      for (int i = 0; i < 4 * DTN; ++i) {
-        const f32x16& x = o[t][i >> 2];
-        const int a = 4 * (i & 3);
-        *reinterpret_cast<f32x4*>(p.part_o + at * D + 8 * i + 4 * h) = f32x4{x[a], x[a + 1], x[a + 2], x[a + 3]};
-      }
-      if (h == 0) p.part_s[at] = float2{m[t], sum};
+    for (int i = 0; i < 4 * DTN; ++i) {
+      const f32x16& x = o[i >> 2];
+      const int a = 4 * (i & 3);
+      *reinterpret_cast<u32x2*>(to + 8 * i + 4 * h) =
+          pack4_bf16(x[a] * inv, x[a + 1] * inv, x[a + 2] * inv, x[a + 3] * inv);
     }
+  } else {
+    const int64_t at = (((int64_t)id * p.hk + head) << p.lbm) + (row - (it.tile << p.lbm));
+#pragma unroll
+    for (int i = 0; i < 4 * DTN; ++i) {
+      const f32x16& x = o[i >> 2];
+      const int a = 4 * (i & 3);
+      *reinterpret_cast<f32x4*>(p.part_o + at * D + 8 * i + 4 * h) = f32x4{x[a], x[a + 1], x[a + 2], x[a + 3]};
+    }
+    if (h == 0) p.part_s[at] = float2{m, sum};
   }
 }
 
 // ------------------------------------------------------------------ joining split tiles
 
-// A wave per row (token, head); rows of unsplit tiles are there already.
+// A wave joins `each` neighbouring rows (token, head); rows of unsplit tiles are there already.
 template <int D>
-__global__ __launch_bounds__(256) void join_kernel(Args p) {
+__global__ __launch_bounds__(256) void join_kernel(Args p, int each) {
   const int lane = threadIdx.x & 63;
-  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int heads = p.hk * p.group;
-  if (r >= (int64_t)p.a.t * heads) return;
-  const int token = __builtin_amdgcn_readfirstlane((int)(r / heads)), hq = (int)(r % heads);
-  const int head = hq / p.group;
+  const int64_t r0 = ((int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * each;
+  const int64_t r1 = min(r0 + each, (int64_t)p.a.t * heads);
+  if (r0 >= r1) return;
   const int chunk = chunk_of(p, lane);
-  int base = 0, first = 0, splits = 1;
-  for (int b0 = 0; b0 <= p.a.batch; b0 += 64) {
-    const Seq s = seq_of(p, b0 + lane);
-    const int sp = splits_of(s.blocks, chunk), n = s.tiles * sp;
-    const int sum = wave_scan(n);
-    const uint64_t hit = __ballot(token >= s.row0 && token < s.row0 + s.n);
-    if (hit) {
-      const int src = __builtin_ctzll(hit);
-      const int in = (token - __builtin_amdgcn_readlane(s.row0, src)) * p.group + hq % p.group;
-      splits = __builtin_amdgcn_readlane(sp, src);
-      first = base + __builtin_amdgcn_readlane(sum - n, src) +
-              (__builtin_amdgcn_readlane(s.tiles, src) - 1 - (in >> p.lbm)) * splits;
-      base = in & ((1 << p.lbm) - 1);
-      break;
+  int from = 0, to = 0, splits = 1, first = 0, tiles = 0;  // the sequence of tokens from .. to - 1, its list's start
+  for (int64_t r = r0; r < r1; ++r) {
+    const int token = (int)(r / heads), hq = (int)(r % heads), head = hq / p.group;
+    if (token >= to) {
+      int base = 0;
+      for (int b0 = 0; b0 <= p.a.batch; b0 += 64) {
+        const Seq s = seq_of(p, b0 + lane);
+        const int sp = splits_of(s.blocks, chunk), n = s.tiles * sp;
+        const int sum = wave_scan(n);
+        const uint64_t hit = __ballot(token >= s.row0 && token < s.row0 + s.n);
+        if (hit) {
+          const int src = __builtin_ctzll(hit);
+          from = __builtin_amdgcn_readlane(s.row0, src);
+          to = from + __builtin_amdgcn_readlane(s.n, src);
+          splits = __builtin_amdgcn_readlane(sp, src);
+          tiles = __builtin_amdgcn_readlane(s.tiles, src);
+          first = base + __builtin_amdgcn_readlane(sum - n, src);
+          break;
+        }
+        base += __builtin_amdgcn_readlane(sum, 63);
+      }
+      if (token >= to) to = token + 1, splits = 1;  // (starts that do not rise: a row of no sequence)
     }
-    base += __builtin_amdgcn_readlane(sum, 63);
-  }
-  if (splits == 1 || first + splits > p.items) return;
-  const int row = base;
-  float mx = -INFINITY;
-  for (int i = lane; i < splits; i += 64) mx = fmaxf(mx, p.part_s[(((int64_t)(first + i) * p.hk + head) << p.lbm) + row].x);
-  mx = wave_max(mx);
-  const float mref = mx == -INFINITY ? 0.f : mx;
-  constexpr int PER = D / 64;
-  float acc[PER] = {}, sum = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < splits; ++i) {
-    const int64_t at = (((int64_t)(first + i) * p.hk + head) << p.lbm) + row;
-    const float2 st = p.part_s[at];
-    const float wt = __builtin_amdgcn_exp2f(st.x - mref);
-    sum += st.y * wt;
+    if (splits == 1) {  // on to the next sequence
+      r = min(r1, (int64_t)to * heads) - 1;
+      continue;
+    }
+    const int in = (token - from) * p.group + hq % p.group;
+    const int at0 = first + (tiles - 1 - (in >> p.lbm)) * splits, row = in & ((1 << p.lbm) - 1);
+    if (at0 < 0 || at0 + splits > p.items) continue;
+    auto at = [&](int i) { return (((int64_t)(at0 + i) * p.hk + head) << p.lbm) + row; };
+    float mx = -INFINITY;
+    for (int i = lane; i < splits; i += 64) mx = fmaxf(mx, p.part_s[at(i)].x);
+    mx = wave_max(mx);
+    const float mref = mx == -INFINITY ? 0.f : mx;
+    constexpr int PER = D / 64;
+    float acc[PER] = {}, sum = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < splits; ++i) {
+      const float2 st = p.part_s[at(i)];
+      const float wt = __builtin_amdgcn_exp2f(st.x - mref);
+      sum += st.y * wt;
 #pragma unroll
-    for (int e = 0; e < PER; ++e) acc[e] = __builtin_fmaf(p.part_o[at * D + PER * lane + e], wt, acc[e]);
+      for (int e = 0; e < PER; ++e) acc[e] = __builtin_fmaf(p.part_o[at(i) * D + PER * lane + e], wt, acc[e]);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    bf16_t* y = p.y + r * D + PER * lane;
+    if constexpr (PER == 2) *reinterpret_cast<uint32_t*>(y) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+    else *y = (bf16_t)f32_to_bf16(acc[0] * inv);
   }
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  bf16_t* to = p.y + r * D + PER * lane;
-  if constexpr (PER == 2) *reinterpret_cast<uint32_t*>(to) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
-  else *to = (bf16_t)f32_to_bf16(acc[0] * inv);
 }
 
 // ------------------------------------------------------------------ host
 
 struct Plan {
-  int kind;  // 0: few rows; 1, 2: many rows, 32 and 64 a wave
+  int kind;  // 0: few rows; 1, 2: many rows on 4 and 8 waves
   int lbm, least, budget;
   int64_t items;  // per key head
 };
 
-Plan plan_of(int64_t t, int64_t batch, int64_t hk, int64_t group, int64_t capacity) {
+Plan plan_of(int64_t t, int64_t batch, int64_t hk, int64_t group, int64_t d, int fp8, int64_t capacity) {
   const int64_t rows = t * group;
   const int force = ff_tuning(FF_TUNE_PAGED_ROWS);
   Plan p = {};
-  p.kind = force ? force - 1 : rows <= 32 * batch ? 0 : rows <= 256 * batch ? 1 : 2;
+  if (force) p.kind = force - 1;
+  else if (rows <= 64 * batch || (rows * hk <= 8192 && capacity <= 512)) p.kind = 0;
+  else p.kind = rows * hk < 256 * 256 ? 1 : 2;
   p.lbm = p.kind == 0 ? 4 : p.kind == 1 ? 7 : 8;
   p.least = p.kind == 0 ? kFewWaves : 8;
-  const int64_t workgroups = p.kind == 2 ? 256 : 512;  // the GPU's, at one and two a CU
+  // workgroups that the GPU holds at once: 256 CUs, by registers and LDS
+  const int64_t workgroups = 256 * (p.kind == 0 ? 2 : p.kind == 1 ? (d == 64 ? 3 : 2) : (d == 64 && !fp8 ? 2 : 1));
   const int64_t tiles = (rows >> p.lbm) + batch + 1;
+  const int64_t budget = workgroups / hk > 0 ? workgroups / hk : 1;
   // No splits where a sequence's keys are one chunk whatever its length is, nor where there
-  // are tiles enough.
-  if ((capacity + 63) / 64 > p.least && (rows >> p.lbm) * hk < 2 * workgroups)
-    p.budget = (int)((workgroups + hk - 1) / hk);
+  // are tiles enough whatever the starts are (one sequence: as many as workgroups).
+  if ((capacity + 63) / 64 > p.least && (rows >> p.lbm) < (batch == 1 ? 1 : 2) * budget) p.budget = (int)budget;
   p.items = tiles + p.budget;
   return p;
 }
@@ -944,7 +958,7 @@ int check(const char* what, int64_t hq, int64_t hk, int64_t d, int64_t ps, int64
              "%s: bad sizes hq=%lld hk=%lld width=%lld batch=%lld t=%lld", what, (long long)hq, (long long)hk,
              (long long)width, (long long)batch, (long long)t);
   const int64_t tiles = t * (hq / hk) / 16 + batch + 1;
-  FF_REQUIRE(tiles * ((width * ps + 63) / 64) <= INT32_MAX && (tiles + 512) * hk <= INT32_MAX,
+  FF_REQUIRE(tiles * ((width * ps + 63) / 64) <= INT32_MAX && (tiles + 768) * hk <= INT32_MAX,
              "%s: too large a call (rows x positions)", what);
   return FF_OK;
 }
@@ -955,14 +969,14 @@ int64_t workspace_of(const Plan& p, int64_t hk, int64_t d) {
 
 }  // namespace
 
-extern "C" int ff_attention_paged_workspace(int64_t hq, int64_t hk, int64_t d, int64_t page_size, int64_t width,
-                                            int64_t batch, int64_t t, int64_t* bytes) {
+extern "C" int ff_attention_paged_workspace(int64_t hq, int64_t hk, int64_t d, int fp8, int64_t page_size,
+                                            int64_t width, int64_t batch, int64_t t, int64_t* bytes) {
   FF_REQUIRE(bytes, "ff_attention_paged_workspace: null pointer");
   *bytes = 0;
   if (t == 0) return FF_OK;
   const int st = check("ff_attention_paged_workspace", hq, hk, d, page_size, width, batch, t);
   if (st != FF_OK) return st;
-  *bytes = workspace_of(plan_of(t, batch, hk, hq / hk, width * page_size), hk, d);
+  *bytes = workspace_of(plan_of(t, batch, hk, hq / hk, d, fp8, width * page_size), hk, d);
   return FF_OK;
 }
 
@@ -982,7 +996,7 @@ extern "C" int ff_attention_paged(const void* q, int64_t q_ts, int64_t q_hs, con
   FF_REQUIRE(ff_aligned(k_pages, 16) && ff_aligned(v_pages, 16) && ff_aligned(k_scale, 8) && ff_aligned(v_scale, 8) &&
                  ff_aligned(y, 16),
              "ff_attention_paged: alignment");
-  const Plan plan = plan_of(t, batch, hk, hq / hk, width * page_size);
+  const Plan plan = plan_of(t, batch, hk, hq / hk, d, fp8, width * page_size);
   const int64_t need = workspace_of(plan, hk, d);
   FF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ff_aligned(workspace, 16)),
              "ff_attention_paged: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
@@ -1006,14 +1020,16 @@ extern "C" int ff_attention_paged(const void* q, int64_t q_ts, int64_t q_hs, con
   p.items = (int)plan.items;
   p.c2 = (float)((double)scale * 1.4426950408889634);
   const dim3 grid((unsigned)(plan.items * hk));
-  const dim3 join((unsigned)((t * hq + 3) / 4));
+  // a row a wave up to 8192 waves (one round), then several
+  const int each = (int)((t * hq + 8191) / 8192);
+  const dim3 join((unsigned)((t * hq + 4 * each - 1) / (4 * each)));
   hipStream_t s = (hipStream_t)stream;
 #define FF_PAGED(DIM, F8)                                                                                          \
   if (d == DIM && (fp8 != 0) == F8) {                                                                              \
     if (plan.kind == 0) hipLaunchKernelGGL((few_rows_kernel<DIM, F8>), grid, dim3(64 * kFewWaves), 0, s, p);       \
-    else if (plan.kind == 1) hipLaunchKernelGGL((many_rows_kernel<DIM, F8, 4, 1>), grid, dim3(256), 0, s, p);      \
-    else hipLaunchKernelGGL((many_rows_kernel<DIM, F8, 4, 2>), grid, dim3(256), 0, s, p);                          \
-    if (plan.budget) hipLaunchKernelGGL((join_kernel<DIM>), join, dim3(256), 0, s, p);                             \
+    else if (plan.kind == 1) hipLaunchKernelGGL((many_rows_kernel<DIM, F8, 4>), grid, dim3(256), 0, s, p);      \
+    else hipLaunchKernelGGL((many_rows_kernel<DIM, F8, 8>), grid, dim3(512), 0, s, p);                          \
+    if (plan.budget) hipLaunchKernelGGL((join_kernel<DIM>), join, dim3(256), 0, s, p, each);                             \
   }
   FF_PAGED(64, false) FF_PAGED(64, true) FF_PAGED(128, false) FF_PAGED(128, true)
 #undef FF_PAGED

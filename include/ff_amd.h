@@ -575,8 +575,8 @@ int ff_cache_read(const void* k_pages, const void* v_pages, const void* k_scale,
  * that sees nothing is zero. workspace: ff_attention_paged_workspace bytes (host-only, 0:
  * none), 16-byte aligned, one per stream and per captured graph that may run beside another.
  * The sums' order depends on the sizes, lengths and starts alone. */
-int ff_attention_paged_workspace(int64_t hq, int64_t hk, int64_t d, int64_t page_size, int64_t width, int64_t batch,
-                                 int64_t t, int64_t* bytes);
+int ff_attention_paged_workspace(int64_t hq, int64_t hk, int64_t d, int fp8, int64_t page_size, int64_t width,
+                                 int64_t batch, int64_t t, int64_t* bytes);
 int ff_attention_paged(const void* q, int64_t q_ts, int64_t q_hs, const void* k_pages, const void* v_pages,
                        const void* k_scale, const void* v_scale, int64_t pages, int64_t page_size, int64_t hq,
                        int64_t hk, int64_t d, int fp8, const int32_t* table, int64_t width, const int32_t* lengths,

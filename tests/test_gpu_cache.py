@@ -457,5 +457,5 @@ def test_refusals_c():
                 f(**kw)
         f(k=None, t=0)
     need = ctypes.c_int64(-1)
-    _lib.call("ff_attention_paged_workspace", 32, 8, 128, 64, 2, 1, 1, ctypes.byref(need))
+    _lib.call("ff_attention_paged_workspace", 32, 8, 128, 0, 64, 2, 1, 1, ctypes.byref(need))
     assert need.value == 0                              # 128 positions are never split
