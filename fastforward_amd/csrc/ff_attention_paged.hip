@@ -860,65 +860,108 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void many_rows_kernel(Arg
 
 // ------------------------------------------------------------------ joining split tiles
 
-// A wave joins `each` neighbouring rows (token, head); rows of unsplit tiles are there already.
-template <int D>
-__global__ __launch_bounds__(256) void join_kernel(Args p, int each) {
-  const int lane = threadIdx.x & 63;
-  const int heads = p.hk * p.group;
-  const int64_t r0 = ((int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * each;
-  const int64_t r1 = min(r0 + each, (int64_t)p.a.t * heads);
-  if (r0 >= r1) return;
+// A row (token, head) is joined by GROUPS groups of D / 4 lanes, 4 dims a lane, each group taking
+// every GROUPS-th split with a running reference of its own. Few rows: 256 threads a row, so
+// that a long list of splits is short for each; many rows: a group a row. Rows of unsplit
+// tiles are there already.
+template <int D, bool WIDE>
+__global__ __launch_bounds__(256) void join_kernel(Args p) {
+  constexpr int LPR = D / 4, PER = 64 / LPR, GROUPS = WIDE ? 4 * PER : 1;
+  __shared__ f32x4 parts[WIDE ? 256 : 1];
+  __shared__ float2 stats[WIDE ? GROUPS : 1];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int heads = p.hk * p.group, rows = p.a.t * heads;
+  const int group = threadIdx.x / LPR, dim = threadIdx.x % LPR * 4;
+  const int r0 = WIDE ? blockIdx.x : ((int)blockIdx.x * 4 + wave) * PER;  // the wave's first row
+  const int row = WIDE ? r0 : r0 + lane / LPR;
   const int chunk = chunk_of(p, lane);
-  int from = 0, to = 0, splits = 1, first = 0, tiles = 0;  // the sequence of tokens from .. to - 1, its list's start
-  for (int64_t r = r0; r < r1; ++r) {
-    const int token = (int)(r / heads), hq = (int)(r % heads), head = hq / p.group;
+  // this lane's row: its first partial row, and its splits
+  int64_t at0 = 0;
+  int splits = 1, from = 0, to = 0, first = 0, tiles = 0, sp = 1;  // (of the sequence with tokens from .. to - 1)
+#pragma unroll
+  for (int i = 0; i < (WIDE ? 1 : PER); ++i) {
+    const int r = r0 + i, token = r / heads, hq = r % heads;
+    if (r >= rows) break;
     if (token >= to) {
       int base = 0;
+      to = token + 1, sp = 1;  // (starts that do not rise: a row of no sequence)
       for (int b0 = 0; b0 <= p.a.batch; b0 += 64) {
         const Seq s = seq_of(p, b0 + lane);
-        const int sp = splits_of(s.blocks, chunk), n = s.tiles * sp;
-        const int sum = wave_scan(n);
+        const int each = splits_of(s.blocks, chunk), n = s.tiles * each, sum = wave_scan(n);
         const uint64_t hit = __ballot(token >= s.row0 && token < s.row0 + s.n);
         if (hit) {
           const int src = __builtin_ctzll(hit);
           from = __builtin_amdgcn_readlane(s.row0, src);
           to = from + __builtin_amdgcn_readlane(s.n, src);
-          splits = __builtin_amdgcn_readlane(sp, src);
+          sp = __builtin_amdgcn_readlane(each, src);
           tiles = __builtin_amdgcn_readlane(s.tiles, src);
           first = base + __builtin_amdgcn_readlane(sum - n, src);
           break;
         }
         base += __builtin_amdgcn_readlane(sum, 63);
       }
-      if (token >= to) to = token + 1, splits = 1;  // (starts that do not rise: a row of no sequence)
-    }
-    if (splits == 1) {  // on to the next sequence
-      r = min(r1, (int64_t)to * heads) - 1;
-      continue;
     }
     const int in = (token - from) * p.group + hq % p.group;
-    const int at0 = first + (tiles - 1 - (in >> p.lbm)) * splits, row = in & ((1 << p.lbm) - 1);
-    if (at0 < 0 || at0 + splits > p.items) continue;
-    auto at = [&](int i) { return (((int64_t)(at0 + i) * p.hk + head) << p.lbm) + row; };
-    float mx = -INFINITY;
-    for (int i = lane; i < splits; i += 64) mx = fmaxf(mx, p.part_s[at(i)].x);
-    mx = wave_max(mx);
-    const float mref = mx == -INFINITY ? 0.f : mx;
-    constexpr int PER = D / 64;
-    float acc[PER] = {}, sum = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < splits; ++i) {
-      const float2 st = p.part_s[at(i)];
-      const float wt = __builtin_amdgcn_exp2f(st.x - mref);
-      sum += st.y * wt;
-#pragma unroll
-      for (int e = 0; e < PER; ++e) acc[e] = __builtin_fmaf(p.part_o[at(i) * D + PER * lane + e], wt, acc[e]);
-    }
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-    bf16_t* y = p.y + r * D + PER * lane;
-    if constexpr (PER == 2) *reinterpret_cast<uint32_t*>(y) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
-    else *y = (bf16_t)f32_to_bf16(acc[0] * inv);
+    const int item = first + (tiles - 1 - (in >> p.lbm)) * sp;
+    const bool mine = sp > 1 && item >= 0 && item + sp <= p.items && row == r;
+    at0 = mine ? (((int64_t)item * p.hk + hq / p.group) << p.lbm) + (in & ((1 << p.lbm) - 1)) : at0;
+    splits = mine ? sp : splits;
   }
+  if (WIDE ? splits == 1 : !__ballot(splits > 1)) return;
+  const int64_t step = (int64_t)p.hk << p.lbm;  // from a split's row to the next one's
+  float m = -INFINITY, sum = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  if (splits > 1) {
+    for (int i0 = WIDE ? group : 0; i0 < splits; i0 += 4 * GROUPS) {
+      float2 st[4];
+      f32x4 o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool there = i0 + i * GROUPS < splits;
+        const int64_t at = at0 + (there ? i0 + i * GROUPS : i0) * step;
+        st[i] = p.part_s[at];
+        o[i] = *reinterpret_cast<const f32x4*>(p.part_o + at * D + dim);
+        if (!there) st[i] = float2{-INFINITY, 0.f};
+      }
+      const float mnew = fmaxf(fmaxf(m, fmaxf(st[0].x, st[1].x)), fmaxf(st[2].x, st[3].x));
+      const float mref = mnew == -INFINITY ? 0.f : mnew;
+      const float alpha = __builtin_amdgcn_exp2f(m - mref);
+      sum *= alpha;
+      acc = acc * alpha;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // (a split without keys, and one read twice in place of none, count for nothing)
+        const float w = __builtin_amdgcn_exp2f(st[i].x - mref);
+        if (st[i].x != -INFINITY) {
+          sum = __builtin_fmaf(st[i].y, w, sum);
+          fma4(acc, o[i], w);
+        }
+      }
+      m = mnew;
+    }
+  }
+  if (WIDE) {
+    parts[threadIdx.x] = acc;
+    if (dim == 0) stats[group] = float2{m, sum};
+    __syncthreads();
+    if (group) return;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) mx = fmaxf(mx, stats[i].x);
+    const float mref = mx == -INFINITY ? 0.f : mx;
+    acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) {
+      const float w = __builtin_amdgcn_exp2f(stats[i].x - mref);
+      sum = __builtin_fmaf(stats[i].y, w, sum);
+      fma4(acc, parts[i * LPR + threadIdx.x], w);
+    }
+  }
+  if (splits == 1) return;
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  *reinterpret_cast<u32x2*>(p.y + (int64_t)row * D + dim) =
+      pack4_bf16(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
 }
 
 // ------------------------------------------------------------------ host
@@ -958,7 +1001,7 @@ int check(const char* what, int64_t hq, int64_t hk, int64_t d, int64_t ps, int64
              "%s: bad sizes hq=%lld hk=%lld width=%lld batch=%lld t=%lld", what, (long long)hq, (long long)hk,
              (long long)width, (long long)batch, (long long)t);
   const int64_t tiles = t * (hq / hk) / 16 + batch + 1;
-  FF_REQUIRE(tiles * ((width * ps + 63) / 64) <= INT32_MAX && (tiles + 768) * hk <= INT32_MAX,
+  FF_REQUIRE(tiles * ((width * ps + 63) / 64) <= INT32_MAX && (tiles + 768) * hk <= INT32_MAX && t * hq <= INT32_MAX,
              "%s: too large a call (rows x positions)", what);
   return FF_OK;
 }
@@ -1020,16 +1063,17 @@ extern "C" int ff_attention_paged(const void* q, int64_t q_ts, int64_t q_hs, con
   p.items = (int)plan.items;
   p.c2 = (float)((double)scale * 1.4426950408889634);
   const dim3 grid((unsigned)(plan.items * hk));
-  // a row a wave up to 8192 waves (one round), then several
-  const int each = (int)((t * hq + 8191) / 8192);
-  const dim3 join((unsigned)((t * hq + 4 * each - 1) / (4 * each)));
+  const bool wide = t * hq <= 2048;
+  const int64_t per = wide ? 1 : 1024 / d;  // rows of a join workgroup
+  const dim3 join((unsigned)((t * hq + per - 1) / per));
   hipStream_t s = (hipStream_t)stream;
 #define FF_PAGED(DIM, F8)                                                                                          \
   if (d == DIM && (fp8 != 0) == F8) {                                                                              \
     if (plan.kind == 0) hipLaunchKernelGGL((few_rows_kernel<DIM, F8>), grid, dim3(64 * kFewWaves), 0, s, p);       \
     else if (plan.kind == 1) hipLaunchKernelGGL((many_rows_kernel<DIM, F8, 4>), grid, dim3(256), 0, s, p);      \
     else hipLaunchKernelGGL((many_rows_kernel<DIM, F8, 8>), grid, dim3(512), 0, s, p);                          \
-    if (plan.budget) hipLaunchKernelGGL((join_kernel<DIM>), join, dim3(256), 0, s, p, each);                             \
+    if (plan.budget && wide) hipLaunchKernelGGL((join_kernel<DIM, true>), join, dim3(256), 0, s, p);               \
+    else if (plan.budget) hipLaunchKernelGGL((join_kernel<DIM, false>), join, dim3(256), 0, s, p);                 \
   }
   FF_PAGED(64, false) FF_PAGED(64, true) FF_PAGED(128, false) FF_PAGED(128, true)
 #undef FF_PAGED
