@@ -100,14 +100,21 @@ SIGNATURES = {
     "ff_moe_route": [P, I32, I64, P, P, P, I64, I64, I64, I32, I64, I64, I32, F64, P],
     "ff_moe_experts_workspace": [I64, I64, I64, I64, I64, PI64],
     "ff_moe_experts": [P, I64, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, P, I64, P],
-    "ff_cache_write": [P, I64, I64, P, I64, I64, P, P, P, P, I64, I64, I64, I64, I32, P, I64, P, P, I64, I64, P],
-    "ff_cache_read": [P, P, P, P, I64, I64, I64, I64, I32, P, I64, P, P, I64, P, P, I64, P],
-    "ff_attention_paged_workspace": [I64, I64, I64, I32, I64, I64, I64, I64, PI64],
-    "ff_attention_paged": [P, I64, I64, P, P, P, P, I64, I64, I64, I64, I64, I32, P, I64, P, P, I64, P, I64, F32, P, I64,
-                           P],
+    "ff_cache_write": [P, I64, I64, P, I64, I64, P, P, I64, P, P, I64, I64, P],
+    "ff_cache_read": [P, P, I64, P, P, I64, P, P, I64, P],
+    "ff_attention_paged_workspace": [P, I64, I64, I64, I32, I64, PI64],
+    "ff_attention_paged": [P, I64, I64, P, I64, P, I64, P, P, I64, P, I64, F32, P, I64, P],
     "ff_token_scores_workspace": [I64, I64, I64, PI64],
     "ff_token_scores": [P, I32, I64, P, I64, I64, P, P, P, P, I64, I64, I64, I64, P, I64, P],
 }
+
+
+
+class PagedCacheStruct(ctypes.Structure):
+    """ff_paged_cache."""
+    _fields_ = [(name, P) for name in ("k", "v", "k_scale", "v_scale")] + \
+        [(name, I64) for name in ("pages", "page_size", "hk", "d", "fp8")]
+
 
 _lib = None
 

@@ -19,23 +19,13 @@ launch, outputs are fresh tensors, launches go to the current stream and can be 
 (no host sync, no device-dependent grid).
 """
 import ctypes
-import functools
 
 import torch
 
-from ._lib import call, entry, stream
-from .linear import check_here
+from ._lib import PagedCacheStruct, call, entry, stream
 
 BF16, E4M3, I32 = torch.bfloat16, torch.float8_e4m3fn, torch.int32
 _ROWS = 1 << 24
-
-
-@functools.lru_cache(maxsize=1024)
-def attend_workspace(heads, kv_heads, head_dim, fp8, page_size, width, batch, t):
-    """Bytes of workspace ff_attention_paged needs (0: none)."""
-    need = ctypes.c_int64(0)
-    call("ff_attention_paged_workspace", heads, kv_heads, head_dim, fp8, page_size, width, batch, t, ctypes.byref(need))
-    return need.value
 
 
 class PagedCache:
@@ -58,63 +48,86 @@ class PagedCache:
         assert device.type == "cuda", device
         self.pages, self.page_size, self.kv_heads, self.head_dim, self.dtype = pages, page_size, kv_heads, head_dim, dtype
         shape = (pages, kv_heads, page_size, head_dim)
-        self.k, self.v = (torch.zeros(shape, device=device, dtype=torch.uint8 if dtype == E4M3 else BF16).view(dtype)
-                          for _ in range(2))
-        self.k_scale = self.v_scale = None
+        k, v = (torch.zeros(shape, device=device, dtype=torch.uint8 if dtype == E4M3 else BF16).view(dtype) for _ in range(2))
+        scales = (None, None)
         if dtype == E4M3:
-            self.k_scale, self.v_scale = (torch.zeros(shape[:3], device=device, dtype=torch.uint8) for _ in range(2))
+            scales = tuple(torch.zeros(shape[:3], device=device, dtype=torch.uint8) for _ in range(2))
+        self._hold(k, v, *scales)
 
-    def _held(self):
-        """The pages as the C entry points take them."""
-        ks = vs = 0
-        if self.k_scale is not None:
-            ks, vs = self.k_scale.data_ptr(), self.v_scale.data_ptr()
-        return (self.k.data_ptr(), self.v.data_ptr(), ks, vs, self.pages, self.page_size)
+    def _hold(self, k, v, k_scale, v_scale):
+        self._tensors = (k, v, k_scale, v_scale)
+        self._device = k.get_device()
+        self._struct = PagedCacheStruct(*(0 if x is None else x.data_ptr() for x in self._tensors), self.pages,
+                                        self.page_size, self.kv_heads, self.head_dim, k_scale is not None)
+        self._c = ctypes.addressof(self._struct)
+        self._workspace = {}               # bytes by the sizes of a call
 
-    def _rows(self, t, table, lengths, starts):
-        assert table.dim() == 2 and table.dtype == I32 and table.is_contiguous() and table.shape[1] > 0, table.shape
+    # the pages are filled in place; the tensors stay the same
+    k = property(lambda self: self._tensors[0])
+    v = property(lambda self: self._tensors[1])
+    k_scale = property(lambda self: self._tensors[2])
+    v_scale = property(lambda self: self._tensors[3])
+
+    def _rows(self, t, table, lengths, starts, *rows):
+        """Checks what the calls share (and that ``rows`` are on the cache's device, the current
+        one); the arguments as the C entry points take them."""
+        assert table.dim() == 2 and table.dtype == I32 and table.is_contiguous(), (table.shape, table.dtype)
         batch, width = table.shape
-        assert 0 < batch <= 65536 and width * self.page_size < 1 << 31 and t <= _ROWS, (batch, width, t)
+        assert 0 < batch <= 65536 and 0 < width and width * self.page_size < 1 << 31 and t <= _ROWS, (batch, width, t)
         assert lengths.shape == (batch,) and lengths.dtype == I32 and lengths.is_contiguous(), lengths.shape
         if starts is None:
             assert t == batch, f"{t} rows for {batch} sequences of one row: starts is missing"
-            check_here(self.k, table, lengths)
-            return (table.data_ptr(), width, lengths.data_ptr(), 0, batch)
-        assert starts.shape == (batch + 1,) and starts.dtype == I32 and starts.is_contiguous(), starts.shape
-        check_here(self.k, table, lengths, starts)
-        return (table.data_ptr(), width, lengths.data_ptr(), starts.data_ptr(), batch)
+            rows += (table, lengths)
+            first = 0
+        else:
+            assert starts.shape == (batch + 1,) and starts.dtype == I32 and starts.is_contiguous(), starts.shape
+            rows += (table, lengths, starts)
+            first = starts.data_ptr()
+        here = self._device
+        for x in rows:
+            assert x.get_device() == here >= 0, f"tensor on {x.device}, the cache on {self.k.device}"
+        assert torch._C._cuda_getDevice() == here, f"the cache is on GPU {here}, which is not the current one"
+        return table.data_ptr(), width, lengths.data_ptr(), first, batch
 
     def write(self, k, v, table, lengths, starts=None):
         """Put k, v (T, kv_heads, head_dim) bf16 (any strides) at their sequences' last
         positions. bf16 pages keep the values; FP8 pages e4m3(x / 2^e), 2^e the smallest power of two, e in
-        [-100, 120], for which the largest finite magnitude of the token's row in its head
-        is at most 448 * 2^e. NaN and infinities become NaN and leave the rest
-        of their row as it is. Rows behind the last sequence are not written. The positions of
-        one call are different ones: where two rows name one place, either may end there."""
-        shape = (k.shape[0], self.kv_heads, self.head_dim)
-        assert k.shape == v.shape == shape and k.dtype == v.dtype == BF16, (k.shape, v.shape, k.dtype, v.dtype)
-        rows = self._rows(shape[0], table, lengths, starts)
-        check_here(k, v)
-        if k.stride(2) != 1:
+        [-100, 120], for which the largest finite magnitude of the token's row in its head is
+        at most 448 * 2^e (and nothing past 240 * 2^120, which bf16 does not hold). NaN and
+        infinities become NaN and leave the rest of their row as it is. Rows behind the last sequence
+        are not written. The positions of one call are different ones: where two rows name
+        one place, either may end there."""
+        assert k.dim() == 3 and k.shape == v.shape and k.dtype == v.dtype == BF16, (k.shape, v.shape, k.dtype, v.dtype)
+        t, hk, d = k.shape
+        assert hk == self.kv_heads and d == self.head_dim, (k.shape, self.kv_heads, self.head_dim)
+        rows = self._rows(t, table, lengths, starts, k, v)
+        ks, vs = k.stride(), v.stride()
+        if ks[2] != 1:
             k = k.contiguous()
-        if v.stride(2) != 1:
+            ks = k.stride()
+        if vs[2] != 1:
             v = v.contiguous()
-        entry("ff_cache_write")(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                                *self._held(), self.kv_heads, self.head_dim, self.dtype == E4M3, *rows, shape[0],
-                                stream())
+            vs = v.stride()
+        entry("ff_cache_write")(k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], self._c, *rows, t, stream())
 
     def read(self, table, lengths, starts=None, rows=None):
         """(k, v), each (rows, kv_heads, head_dim) bf16, of the sequences' last positions; an FP8
         cache's values are exact in bf16. ``rows`` (default: one per sequence) is T, a host
         number. Rows behind the last sequence, and positions that hold nothing, are zero."""
         t = table.shape[0] if rows is None else rows
-        assert t >= 0 and (rows is None) <= (starts is None), "rows is missing"
+        assert t >= 0 and (rows is not None or starts is None), "rows is missing"
         args = self._rows(t, table, lengths, starts)
-        k = torch.empty((t, self.kv_heads, self.head_dim), device=table.device, dtype=BF16)
+        k = table.new_empty((t, self.kv_heads, self.head_dim), dtype=BF16)
         v = torch.empty_like(k)
-        entry("ff_cache_read")(*self._held(), self.kv_heads, self.head_dim, self.dtype == E4M3, *args, k.data_ptr(),
-                               v.data_ptr(), t, stream())
+        entry("ff_cache_read")(self._c, *args, k.data_ptr(), v.data_ptr(), t, stream())
         return k, v
+
+    def attend_workspace(self, t, heads, width, batch, starts):
+        """Bytes of workspace ff_attention_paged needs (0: none) for a table (batch, width) and,
+        where ``starts`` is true, rows by starts."""
+        need = ctypes.c_int64(0)
+        call("ff_attention_paged_workspace", self._c, heads, width, batch, starts, t, ctypes.byref(need))
+        return need.value
 
     def attend(self, q, table, lengths, starts=None, scale=None):
         """Causal attention of q (T, heads, head_dim) bf16, any strides, heads a multiple of
@@ -123,23 +136,25 @@ class PagedCache:
         1 / sqrt(head_dim)) with fp32 statistics, weights rounded to bf16 for the product
         with the values, fp32 sums. (T, heads, head_dim) bf16. A row that sees nothing, and
         rows behind the last sequence, are zero."""
-        assert q.dim() == 3 and q.dtype == BF16 and q.shape[2] == self.head_dim, (q.shape, q.dtype)
+        assert q.dim() == 3 and q.dtype == BF16, (q.shape, q.dtype)
         t, heads, d = q.shape
-        hk = self.kv_heads
-        assert heads > 0 and heads % hk == 0 and heads <= 65535, (heads, hk)
+        assert d == self.head_dim and 0 < heads <= 65535 and heads % self.kv_heads == 0, (q.shape, self.kv_heads)
         scale = d ** -0.5 if scale is None else float(scale)
         assert 0 < scale < float("inf"), scale
-        rows = self._rows(t, table, lengths, starts)
-        check_here(q)
-        if q.stride(2) != 1:
+        rows = self._rows(t, table, lengths, starts, q)
+        qs = q.stride()
+        if qs[2] != 1:
             q = q.contiguous()
+            qs = q.stride()
         y = q.new_empty((t, heads, d))
-        need = attend_workspace(heads, hk, d, self.dtype == E4M3, self.page_size, rows[1], rows[4], t)
+        sizes = (t, heads, rows[1], rows[4], starts is not None)
+        need = self._workspace.get(sizes)
+        if need is None:
+            need = self._workspace[sizes] = self.attend_workspace(*sizes)
         ws = q.new_empty((need,), dtype=torch.uint8) if need else None
-        entry("ff_attention_paged")(q.data_ptr(), q.stride(0), q.stride(1), *self._held(), heads, hk, d,
-                                    self.dtype == E4M3, *rows, y.data_ptr(), t, scale, 0 if ws is None else ws.data_ptr(),
-                                    need, stream())
+        entry("ff_attention_paged")(q.data_ptr(), qs[0], qs[1], self._c, heads, *rows, y.data_ptr(), t, scale,
+                                    0 if ws is None else ws.data_ptr(), need, stream())
         return y
 
 
-__all__ = ["PagedCache", "attend_workspace"]
+__all__ = ["PagedCache"]

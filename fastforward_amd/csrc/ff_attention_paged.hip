@@ -198,6 +198,12 @@ __device__ __forceinline__ bf16x8 e4m3_to_bf16x8(uint32_t a, uint32_t b, float s
   return bf16x8{p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
 }
 
+// lds_dma16 from a uniform base: lane l's 16 bytes at base + offset.
+__device__ __forceinline__ void lds_dma16_at(const uint8_t* base, uint32_t offset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds)
+               : "memory", "m0");
+}
+
 // This wave's LDS reads and writes are done (no other wave uses the memory).
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
 
@@ -300,33 +306,44 @@ __device__ __forceinline__ uint64_t keys_to(int last) {
 // running softmax of its own; the waves are joined in LDS. Keys go from memory straight
 // into the operand registers, values by DMA into the wave's own LDS: no barrier until
 // the end. Bound by the cache's bytes.
-constexpr int kFewWaves = 4;
+constexpr int kFewWaves = 4;     // two workgroups a CU
+constexpr int kDecodeWaves = 8;  // a workgroup a CU, no splits
 
-template <int D, bool FP8>
-__global__ __launch_bounds__(64 * kFewWaves, 2) void few_rows_kernel(Args p) {
+template <int D, bool FP8, int NW, bool DECODE>
+__global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void few_rows_kernel(Args p) {
   constexpr int RB = FP8 ? D : 2 * D, KST = D / 32, DTN = D / 16, KL = RB / 64;  // KL: 16-byte loads of a key row
-  constexpr int VI = RB / 16;                                                   // value DMAs of a block
+  constexpr int PI = 16 * RB / 1024;                                            // value DMAs of 16 keys
   constexpr int SLAB = 64 * RB, LDO = D + 4;
-  constexpr int JOIN = kFewWaves * 16 * (LDO + 2) * 4;
-  __shared__ __align__(1024) uint8_t smem[kFewWaves * SLAB > JOIN ? kFewWaves * SLAB : JOIN];
+  constexpr int JOIN = NW * 16 * (LDO + 2) * 4;
+  __shared__ __align__(1024) uint8_t smem[NW * SLAB > JOIN ? NW * SLAB : JOIN];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, g = lane >> 4;
   const int head = (int)blockIdx.x % p.hk, id = (int)blockIdx.x / p.hk;
-  const int chunk = chunk_of(p, lane);
   Item it;
-  if (!find_item(p, lane, chunk, id, &it)) return;
+  if constexpr (DECODE) {  // one row a sequence and no splits: the list is known without the lengths
+    const int tiles = (p.group + 15) >> 4;
+    it.seq = id / tiles;
+    it.tile = id % tiles;
+    it.split = 0;
+    it.splits = 1;
+    if (it.seq >= p.a.t) return;
+    it.s = seq_of(p, it.seq);
+  } else {
+    if (!find_item(p, lane, chunk_of(p, lane), id, &it)) return;
+  }
+  const int64_t page_rows = (int64_t)p.hk << p.a.lps, head_rows = (int64_t)head << p.a.lps;
+  const int in_page = (1 << p.a.lps) - 1;
+  const int* table = p.a.table + (int64_t)min(it.seq, p.a.batch - 1) * p.a.width;
+  // table entry of the lane's key of block b
+  auto entry_of = [&](int b) { return table[min((int64_t)((64 * b + lane) >> p.a.lps), p.a.width - 1)]; };
+  int ahead = DECODE ? entry_of(wave) : 0;
+
   const int row = it.tile * 16 + r16, rows = it.s.n * p.group;
   const bool real = row < rows;
-  const int query = (real ? row : rows - 1) / p.group, hq = head * p.group + (real ? row : rows - 1) % p.group;
-  const int token = it.s.row0 + query;
-  const int pos = real ? it.s.len - it.s.n + query : -1;
-  const int last = it.s.len - it.s.n + min(rows - 1, it.tile * 16 + 15) / p.group;  // the tile's last position
-  const int kend = min(it.s.keys, last + 1);
-  const int nb = max(0, kend + 63) >> 6, per = (nb + it.splits - 1) / it.splits;
-  const int b_end = min(nb, (it.split + 1) * per);
-
+  const int query = DECODE ? 0 : (real ? row : rows - 1) / p.group;
+  const int hq = head * p.group + (real ? row : rows - 1) - query * p.group;
   u32x4 qf[KST];
-  const bf16_t* qp = p.q + token * p.q_ts + hq * p.q_hs;
+  const bf16_t* qp = p.q + (it.s.row0 + query) * p.q_ts + hq * p.q_hs;
 #pragma unroll
   for (int st = 0; st < KST; ++st) {
     const bf16_t* src = qp + step_dim<FP8>(st, g);
@@ -339,46 +356,59 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_rows_kernel(Args p) {
       qf[st] = pack8(x);
     }
   }
+  const int pos = real ? it.s.len - it.s.n + query : -1;
+  // one past the tile's last position
+  const int kend = min(it.s.keys, DECODE ? it.s.len : it.s.len - it.s.n + min(rows - 1, it.tile * 16 + 15) / p.group + 1);
+  const int nb = max(0, kend + 63) >> 6, per = DECODE ? nb : (nb + it.splits - 1) / it.splits;
+  const int b_end = min(nb, (it.split + 1) * per), b_first = it.split * per + wave;
+  if (!DECODE) ahead = entry_of(b_first);
+
   f32x4 o[DTN];
 #pragma unroll
   for (int dt = 0; dt < DTN; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, den = 0.f;
-
-  const int64_t page_rows = (int64_t)p.hk << p.a.lps, head_rows = (int64_t)head << p.a.lps;
-  const int in_page = (1 << p.a.lps) - 1;
-  const int* table = p.a.table + (int64_t)min(it.seq, p.a.batch - 1) * p.a.width;
   const uint32_t lds = lds_addr(smem) + wave * SLAB;
+  uint32_t v_from[PI];  // where a lane's 16 bytes lie among 16 keys' values, for the i-th DMA of them
+#pragma unroll
+  for (int i = 0; i < PI; ++i) {
+    const int key = i * (1024 / RB) + lane / (RB / 16);
+    v_from[i] = key * RB + 16 * (lane % (RB / 16) ^ v_swizzle<RB, FP8>(key)) - i * 1024;
+  }
 
-  for (int b = it.split * per + wave; b < b_end; b += kFewWaves) {
+  for (int b = b_first; b < b_end; b += NW) {
     const int kb = 64 * b;
     // the lane's key of the block: its page, and whether there is one
-    const int entry = table[min((int64_t)((kb + lane) >> p.a.lps), p.a.width - 1)];
+    const int entry = ahead;
+    ahead = entry_of(b + NW);
     const bool there = kb + lane < kend && (unsigned)entry < (unsigned)p.a.pages;
     const uint64_t ok = __ballot(there);
-    const int page = there ? entry : 0;
-    auto row_of = [&](int key) {  // row of the pages' (page, head, slot) that holds key kb + key
-      return (int64_t)__shfl(page, key, 64) * page_rows + head_rows + ((kb + key) & in_page);
+    // row of the pages' (page, head, slot) that holds the first of 16 keys: a uniform one
+    auto first = [&](int j) {
+      return __builtin_amdgcn_readlane(there ? entry : 0, 16 * j) * page_rows + head_rows + ((kb + 16 * j) & in_page);
     };
+    const int64_t f0 = first(0), f1 = first(1), f2 = first(2), f3 = first(3);
     u32x4 kf[4][KL];
     float ksc[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t at = row_of(32 * (i >> 1) + 8 * (r16 >> 2) + 4 * (i & 1) + (r16 & 3));
+    for (int i = 0; i < 4; ++i) {  // key 32 (i / 2) + 8 (r16 / 4) + 4 (i % 2) + r16 % 4
+      const int64_t at = (r16 & 8 ? (i < 2 ? f1 : f3) : (i < 2 ? f0 : f2)) + 2 * (r16 & 4) + 4 * (i & 1) + (r16 & 3);
 #pragma unroll
       for (int j = 0; j < KL; ++j) kf[i][j] = *reinterpret_cast<const u32x4*>(p.k + at * RB + 64 * j + 16 * g);
       if (FP8) ksc[i] = scale_of(p.ks[at]);
     }
     u32x2 vsc[2];
     if (FP8) {
-#pragma unroll
-      for (int c = 0; c < 2; ++c) vsc[c] = *reinterpret_cast<const u32x2*>(p.vs + row_of(32 * c + 8 * g));
+      vsc[0] = *reinterpret_cast<const u32x2*>(p.vs + (g & 2 ? f1 : f0) + 8 * (g & 1));
+      vsc[1] = *reinterpret_cast<const u32x2*>(p.vs + (g & 2 ? f3 : f2) + 8 * (g & 1));
     }
     wait_lds();
 #pragma unroll
-    for (int j = 0; j < VI; ++j) {
-      const int key = j * (64 / VI) + lane / VI;
-      lds_dma16(p.v + row_of(key) * RB + 16 * ((lane % VI) ^ v_swizzle<RB, FP8>(key)), lds + 1024 * j);
-    }
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < PI; ++i)
+        lds_dma16_at(p.v + (j == 0 ? f0 : j == 1 ? f1 : j == 2 ? f2 : f3) * RB + i * 1024, v_from[i],
+                     lds + (j * PI + i) * 1024);
+    __builtin_amdgcn_sched_barrier(0);  // all of the block's loads before the first wait for one
     f32x4 s[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -456,35 +486,37 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_rows_kernel(Args p) {
 
   // join the waves
   float* so = reinterpret_cast<float*>(smem);
-  float* sm = so + kFewWaves * 16 * LDO;
-  float* sd = sm + kFewWaves * 16;
+  float* sm = so + NW * 16 * LDO;
+  float* sd = sm + NW * 16;
   __syncthreads();
+  if (real) {
 #pragma unroll
-  for (int dt = 0; dt < DTN; ++dt) *reinterpret_cast<f32x4*>(so + (wave * 16 + r16) * LDO + 16 * dt + 4 * g) = o[dt];
+    for (int dt = 0; dt < DTN; ++dt) *reinterpret_cast<f32x4*>(so + (wave * 16 + r16) * LDO + 16 * dt + 4 * g) = o[dt];
+  }
   if (g == 0) {
     sm[wave * 16 + r16] = m;
     sd[wave * 16 + r16] = den;
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < 16 * (D / 4); e += 64 * kFewWaves) {
+  const int here = min(rows - it.tile * 16, 16);  // rows of the tile
+  for (int e = threadIdx.x; e < here * (D / 4); e += 64 * NW) {
     const int r = e / (D / 4), d0 = e % (D / 4) * 4;
-    if (it.tile * 16 + r >= rows) continue;
     float mx = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kFewWaves; ++w) mx = fmaxf(mx, sm[w * 16 + r]);
+    for (int w = 0; w < NW; ++w) mx = fmaxf(mx, sm[w * 16 + r]);
     const float mref = mx == -INFINITY ? 0.f : mx;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     float sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kFewWaves; ++w) {
+    for (int w = 0; w < NW; ++w) {
       const float wt = __builtin_amdgcn_exp2f(sm[w * 16 + r] - mref);
       sum += sd[w * 16 + r] * wt;
       fma4(acc, *reinterpret_cast<const f32x4*>(so + (w * 16 + r) * LDO + d0), wt);
     }
     if (it.splits == 1) {
-      const int rr = it.tile * 16 + r;
+      const int rr = it.tile * 16 + r, query = DECODE ? 0 : rr / p.group;
       const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-      bf16_t* to = p.y + ((int64_t)(it.s.row0 + rr / p.group) * (p.hk * p.group) + head * p.group + rr % p.group) * D;
+      bf16_t* to = p.y + ((int64_t)(it.s.row0 + query) * (p.hk * p.group) + head * p.group + rr - query * p.group) * D;
       *reinterpret_cast<u32x2*>(to + d0) = pack4_bf16(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
     } else {
       const int64_t at = ((int64_t)id * p.hk + head) * 16 + r;
@@ -521,12 +553,6 @@ __device__ __forceinline__ int v_place(int key) {
 
 __device__ __forceinline__ f32x16 mfma32(const bf16x8& a, const u32x4& b, const f32x16& c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
-// lds_dma16 from a uniform base: lane l's 16 bytes at base + offset.
-__device__ __forceinline__ void lds_dma16_at(const uint8_t* base, uint32_t offset, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds)
-               : "memory", "m0");
 }
 
 // V^T fragment of 16 keys from 16 c, dims 32 dt ..: lane 32 h + r gets keys 16 c + 8 h .. + 7 of
@@ -968,17 +994,27 @@ __global__ __launch_bounds__(256) void join_kernel(Args p) {
 
 struct Plan {
   int kind;  // 0: few rows; 1, 2: many rows on 4 and 8 waves
+  bool decode;
   int lbm, least, budget;
   int64_t items;  // per key head
 };
 
-Plan plan_of(int64_t t, int64_t batch, int64_t hk, int64_t group, int64_t d, int fp8, int64_t capacity) {
+Plan plan_of(int64_t t, int64_t batch, bool starts, int64_t hk, int64_t group, int64_t d, int fp8, int64_t capacity) {
   const int64_t rows = t * group;
   const int force = ff_tuning(FF_TUNE_PAGED_ROWS);
   Plan p = {};
   if (force) p.kind = force - 1;
   else if (rows <= 64 * batch || (rows * hk <= 8192 && capacity <= 512)) p.kind = 0;
   else p.kind = rows * hk < 256 * 256 ? 1 : 2;
+  // One row a sequence, up to 768 positions, a CU for each tile: one launch. A CU takes in 64 bytes a
+  // clock at most, so that longer caches are better shared by several and joined.
+  const int64_t decode = (group + 15) / 16 * t;
+  if (p.kind == 0 && !starts && capacity <= 768 && decode * hk <= 256) {
+    p.decode = true;
+    p.lbm = 4;
+    p.items = decode;
+    return p;
+  }
   p.lbm = p.kind == 0 ? 4 : p.kind == 1 ? 7 : 8;
   p.least = p.kind == 0 ? kFewWaves : 8;
   // workgroups that the GPU holds at once: 256 CUs, by registers and LDS
@@ -992,16 +1028,13 @@ Plan plan_of(int64_t t, int64_t batch, int64_t hk, int64_t group, int64_t d, int
   return p;
 }
 
-int check(const char* what, int64_t hq, int64_t hk, int64_t d, int64_t ps, int64_t width, int64_t batch, int64_t t) {
-  FF_REQUIRE(d == 64 || d == 128, "%s: head_dim %lld unsupported (64, 128)", what, (long long)d);
-  FF_REQUIRE(ps >= 16 && ps <= 4096 && (ps & (ps - 1)) == 0, "%s: page_size %lld (a power of two, 16 .. 4096)", what,
-             (long long)ps);
-  FF_REQUIRE(hk > 0 && hq > 0 && hq <= 65535 && hq % hk == 0 && width > 0 && width <= INT32_MAX / ps && batch > 0 &&
-                 batch <= 65536 && t > 0 && t <= (1 << 24),
-             "%s: bad sizes hq=%lld hk=%lld width=%lld batch=%lld t=%lld", what, (long long)hq, (long long)hk,
-             (long long)width, (long long)batch, (long long)t);
-  const int64_t tiles = t * (hq / hk) / 16 + batch + 1;
-  FF_REQUIRE(tiles * ((width * ps + 63) / 64) <= INT32_MAX && (tiles + 768) * hk <= INT32_MAX && t * hq <= INT32_MAX,
+// (sizes of the cache and the rows are checked already)
+int check_sizes(const char* what, const ff_paged_cache* c, int64_t hq, int64_t width, int64_t batch, int64_t t) {
+  FF_REQUIRE(hq > 0 && hq <= 65535 && hq % c->hk == 0, "%s: bad sizes hq=%lld hk=%lld", what, (long long)hq,
+             (long long)c->hk);
+  const int64_t tiles = t * (hq / c->hk) / 16 + batch + 1;
+  FF_REQUIRE(tiles * ((width * c->page_size + 63) / 64) <= INT32_MAX && (tiles + 768) * c->hk <= INT32_MAX &&
+                 t * hq <= INT32_MAX,
              "%s: too large a call (rows x positions)", what);
   return FF_OK;
 }
@@ -1012,46 +1045,50 @@ int64_t workspace_of(const Plan& p, int64_t hk, int64_t d) {
 
 }  // namespace
 
-extern "C" int ff_attention_paged_workspace(int64_t hq, int64_t hk, int64_t d, int fp8, int64_t page_size,
-                                            int64_t width, int64_t batch, int64_t t, int64_t* bytes) {
+extern "C" int ff_attention_paged_workspace(const ff_paged_cache* cache, int64_t hq, int64_t width, int64_t batch,
+                                            int starts, int64_t t, int64_t* bytes) {
   FF_REQUIRE(bytes, "ff_attention_paged_workspace: null pointer");
   *bytes = 0;
   if (t == 0) return FF_OK;
-  const int st = check("ff_attention_paged_workspace", hq, hk, d, page_size, width, batch, t);
+  int st = check_cache("ff_attention_paged_workspace", cache);
   if (st != FF_OK) return st;
-  *bytes = workspace_of(plan_of(t, batch, hk, hq / hk, d, fp8, width * page_size), hk, d);
+  FF_REQUIRE(width > 0 && width <= INT32_MAX / cache->page_size && batch > 0 && batch <= 65536 && t > 0 && t <= (1 << 24),
+             "ff_attention_paged_workspace: bad sizes width=%lld batch=%lld t=%lld", (long long)width, (long long)batch,
+             (long long)t);
+  st = check_sizes("ff_attention_paged_workspace", cache, hq, width, batch, t);
+  if (st != FF_OK) return st;
+  *bytes = workspace_of(plan_of(t, batch, starts, cache->hk, hq / cache->hk, cache->d, cache->fp8 != 0,
+                                width * cache->page_size), cache->hk, cache->d);
   return FF_OK;
 }
 
-extern "C" int ff_attention_paged(const void* q, int64_t q_ts, int64_t q_hs, const void* k_pages, const void* v_pages,
-                                  const void* k_scale, const void* v_scale, int64_t pages, int64_t page_size,
-                                  int64_t hq, int64_t hk, int64_t d, int fp8, const int32_t* table, int64_t width,
-                                  const int32_t* lengths, const int32_t* starts, int64_t batch, void* y, int64_t t,
-                                  float scale, void* workspace, int64_t workspace_bytes, ff_stream_t stream) {
+extern "C" int ff_attention_paged(const void* q, int64_t q_ts, int64_t q_hs, const ff_paged_cache* cache, int64_t hq,
+                                  const int32_t* table, int64_t width, const int32_t* lengths, const int32_t* starts,
+                                  int64_t batch, void* y, int64_t t, float scale, void* workspace,
+                                  int64_t workspace_bytes, ff_stream_t stream) {
   if (t == 0) return FF_OK;
-  const int st = check("ff_attention_paged", hq, hk, d, page_size, width, batch, t);
+  int st = check_rows("ff_attention_paged", cache, table, width, lengths, starts, batch, t);
   if (st != FF_OK) return st;
-  FF_REQUIRE(q && k_pages && v_pages && (!fp8 || (k_scale && v_scale)) && table && lengths && y,
-             "ff_attention_paged: null pointer");
-  FF_REQUIRE(pages > 0 && pages <= INT32_MAX, "ff_attention_paged: %lld pages", (long long)pages);
-  FF_REQUIRE(starts || batch == t, "ff_attention_paged: without starts every sequence has one row");
+  st = check_sizes("ff_attention_paged", cache, hq, width, batch, t);
+  if (st != FF_OK) return st;
+  FF_REQUIRE(q && y, "ff_attention_paged: null pointer");
   FF_REQUIRE(scale > 0.f && scale < __builtin_inff(), "ff_attention_paged: scale %g", (double)scale);
-  FF_REQUIRE(ff_aligned(k_pages, 16) && ff_aligned(v_pages, 16) && ff_aligned(k_scale, 8) && ff_aligned(v_scale, 8) &&
-                 ff_aligned(y, 16),
-             "ff_attention_paged: alignment");
-  const Plan plan = plan_of(t, batch, hk, hq / hk, d, fp8, width * page_size);
+  FF_REQUIRE(ff_aligned(y, 16), "ff_attention_paged: alignment");
+  const int64_t hk = cache->hk, d = cache->d;
+  const bool fp8 = cache->fp8 != 0;
+  const Plan plan = plan_of(t, batch, starts != nullptr, hk, hq / hk, d, fp8, width * cache->page_size);
   const int64_t need = workspace_of(plan, hk, d);
   FF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ff_aligned(workspace, 16)),
              "ff_attention_paged: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
   Args p;
-  p.a = Rows{table, lengths, starts, width, (int)batch, (int)t, (int)pages, __builtin_ctzll((uint64_t)page_size)};
+  p.a = rows_of(cache, table, width, lengths, starts, batch, t);
   p.q = (const bf16_t*)q;
   p.q_ts = q_ts;
   p.q_hs = q_hs;
-  p.k = (const uint8_t*)k_pages;
-  p.v = (const uint8_t*)v_pages;
-  p.ks = (const uint8_t*)k_scale;
-  p.vs = (const uint8_t*)v_scale;
+  p.k = (const uint8_t*)cache->k;
+  p.v = (const uint8_t*)cache->v;
+  p.ks = (const uint8_t*)cache->k_scale;
+  p.vs = (const uint8_t*)cache->v_scale;
   p.y = (bf16_t*)y;
   p.part_o = (float*)workspace;
   p.part_s = (float2*)((char*)workspace + ((plan.items * hk) << plan.lbm) * d * 4);
@@ -1068,8 +1105,11 @@ extern "C" int ff_attention_paged(const void* q, int64_t q_ts, int64_t q_hs, con
   const dim3 join((unsigned)((t * hq + per - 1) / per));
   hipStream_t s = (hipStream_t)stream;
 #define FF_PAGED(DIM, F8)                                                                                          \
-  if (d == DIM && (fp8 != 0) == F8) {                                                                              \
-    if (plan.kind == 0) hipLaunchKernelGGL((few_rows_kernel<DIM, F8>), grid, dim3(64 * kFewWaves), 0, s, p);       \
+  if (d == DIM && fp8 == F8) {                                                                              \
+    if (plan.decode)                                                                                               \
+      hipLaunchKernelGGL((few_rows_kernel<DIM, F8, kDecodeWaves, true>), grid, dim3(64 * kDecodeWaves), 0, s, p);  \
+    else if (plan.kind == 0)                                                                                       \
+      hipLaunchKernelGGL((few_rows_kernel<DIM, F8, kFewWaves, false>), grid, dim3(64 * kFewWaves), 0, s, p);       \
     else if (plan.kind == 1) hipLaunchKernelGGL((many_rows_kernel<DIM, F8, 4>), grid, dim3(256), 0, s, p);      \
     else hipLaunchKernelGGL((many_rows_kernel<DIM, F8, 8>), grid, dim3(512), 0, s, p);                          \
     if (plan.budget && wide) hipLaunchKernelGGL((join_kernel<DIM, true>), join, dim3(256), 0, s, p);               \

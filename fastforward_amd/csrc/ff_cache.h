@@ -54,6 +54,33 @@ __device__ __forceinline__ bool find_slot(const Rows& a, int row, int b, int64_t
   return (unsigned)p < (unsigned)a.pages;
 }
 
+// Host checks that the entry points share.
+inline int check_cache(const char* what, const ff_paged_cache* c) {
+  FF_REQUIRE(c, "%s: null pointer", what);
+  FF_REQUIRE(c->d == 64 || c->d == 128, "%s: head_dim %lld unsupported (64, 128)", what, (long long)c->d);
+  FF_REQUIRE(c->page_size >= 16 && c->page_size <= 4096 && (c->page_size & (c->page_size - 1)) == 0,
+             "%s: page_size %lld (a power of two, 16 .. 4096)", what, (long long)c->page_size);
+  FF_REQUIRE(c->pages > 0 && c->pages <= INT32_MAX && c->hk > 0 && c->hk <= 65535, "%s: bad sizes pages=%lld hk=%lld",
+             what, (long long)c->pages, (long long)c->hk);
+  return FF_OK;
+}
+inline int check_rows(const char* what, const ff_paged_cache* c, const int32_t* table, int64_t width,
+                      const int32_t* lengths, const int32_t* starts, int64_t batch, int64_t t) {
+  const int st = check_cache(what, c);
+  if (st != FF_OK) return st;
+  FF_REQUIRE(c->k && c->v && (!c->fp8 || (c->k_scale && c->v_scale)) && table && lengths, "%s: null pointer", what);
+  FF_REQUIRE(width > 0 && width <= INT32_MAX / c->page_size && batch > 0 && batch <= 65536 && t > 0 && t <= (1 << 24),
+             "%s: bad sizes width=%lld batch=%lld t=%lld", what, (long long)width, (long long)batch, (long long)t);
+  FF_REQUIRE(starts || batch == t, "%s: without starts every sequence has one row", what);
+  FF_REQUIRE(ff_aligned(c->k, 16) && ff_aligned(c->v, 16) && ff_aligned(c->k_scale, 8) && ff_aligned(c->v_scale, 8),
+             "%s: alignment", what);
+  return FF_OK;
+}
+inline Rows rows_of(const ff_paged_cache* c, const int32_t* table, int64_t width, const int32_t* lengths,
+                    const int32_t* starts, int64_t batch, int64_t t) {
+  return Rows{table, lengths, starts, width, (int)batch, (int)t, (int)c->pages, __builtin_ctzll((uint64_t)c->page_size)};
+}
+
 // The float of a scale byte.
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
 

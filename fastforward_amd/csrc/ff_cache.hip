@@ -133,72 +133,47 @@ __global__ __launch_bounds__(256) void cache_read_kernel(Rows a, Pages c, bf16_t
   *reinterpret_cast<u32x4*>(v + to) = y;
 }
 
-int check(const char* what, const void* kc, const void* vc, const void* ks, const void* vs, int64_t pages, int64_t ps,
-          int64_t hk, int64_t d, int fp8, const int32_t* table, int64_t width, const int32_t* lengths, int64_t batch,
-          int64_t t) {
-  FF_REQUIRE(kc && vc && (!fp8 || (ks && vs)) && table && lengths, "%s: null pointer", what);
-  FF_REQUIRE(d == 64 || d == 128, "%s: head_dim %lld unsupported (64, 128)", what, (long long)d);
-  FF_REQUIRE(ps >= 16 && ps <= 4096 && (ps & (ps - 1)) == 0, "%s: page_size %lld (a power of two, 16 .. 4096)", what,
-             (long long)ps);
-  FF_REQUIRE(pages > 0 && pages <= INT32_MAX && hk > 0 && hk <= 65535 && width > 0 && width <= INT32_MAX / ps &&
-                 batch > 0 && batch <= 65536 && t > 0 && t <= (1 << 24),
-             "%s: bad sizes pages=%lld hk=%lld width=%lld batch=%lld t=%lld", what, (long long)pages, (long long)hk,
-             (long long)width, (long long)batch, (long long)t);
-  FF_REQUIRE(ff_aligned(kc, 16) && ff_aligned(vc, 16), "%s: alignment", what);
-  return FF_OK;
-}
-
-Rows rows_of(const int32_t* table, int64_t width, const int32_t* lengths, const int32_t* starts, int64_t batch,
-             int64_t t, int64_t pages, int64_t ps) {
-  return Rows{table, lengths, starts, width, (int)batch, (int)t, (int)pages, __builtin_ctzll((uint64_t)ps)};
+Pages pages_of(const ff_paged_cache* c) {
+  return Pages{(uint8_t*)c->k, (uint8_t*)c->v, (uint8_t*)c->k_scale, (uint8_t*)c->v_scale};
 }
 
 }  // namespace
 
 extern "C" int ff_cache_write(const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs,
-                              void* k_pages, void* v_pages, void* k_scale, void* v_scale, int64_t pages,
-                              int64_t page_size, int64_t hk, int64_t d, int fp8, const int32_t* table, int64_t width,
-                              const int32_t* lengths, const int32_t* starts, int64_t batch, int64_t t,
-                              ff_stream_t stream) {
+                              const ff_paged_cache* cache, const int32_t* table, int64_t width, const int32_t* lengths,
+                              const int32_t* starts, int64_t batch, int64_t t, ff_stream_t stream) {
   if (t == 0) return FF_OK;
-  const int st = check("ff_cache_write", k_pages, v_pages, k_scale, v_scale, pages, page_size, hk, d, fp8, table, width,
-                       lengths, batch, t);
+  const int st = check_rows("ff_cache_write", cache, table, width, lengths, starts, batch, t);
   if (st != FF_OK) return st;
   FF_REQUIRE(k && v, "ff_cache_write: null pointer");
-  FF_REQUIRE(starts || batch == t, "ff_cache_write: without starts every sequence has one row");
-  const Rows a = rows_of(table, width, lengths, starts, batch, t, pages, page_size);
-  const Pages c = {(uint8_t*)k_pages, (uint8_t*)v_pages, (uint8_t*)k_scale, (uint8_t*)v_scale};
-  const int vec = (ff_aligned(k, 16) && k_ts % 8 == 0 && k_hs % 8 == 0) | (ff_aligned(v, 16) && v_ts % 8 == 0 && v_hs % 8 == 0) << 1;
-  const int64_t per = 4 * 512 / d;  // tokens of a workgroup
-  const dim3 grid((unsigned)((t + per - 1) / per), (unsigned)hk);
-#define FF_WRITE(DIM, F8)                                                                                           \
-  if (d == DIM && (fp8 != 0) == F8)                                                                                 \
-    hipLaunchKernelGGL((cache_write_kernel<DIM, F8>), grid, dim3(256), 0, (hipStream_t)stream, a, c, (const bf16_t*)k, \
-                       k_ts, k_hs, (const bf16_t*)v, v_ts, v_hs, (int)hk, vec);
+  const Rows a = rows_of(cache, table, width, lengths, starts, batch, t);
+  const int vec = (ff_aligned(k, 16) && k_ts % 8 == 0 && k_hs % 8 == 0) |
+                  (ff_aligned(v, 16) && v_ts % 8 == 0 && v_hs % 8 == 0) << 1;
+  const int64_t per = 4 * 512 / cache->d;  // tokens of a workgroup
+  const dim3 grid((unsigned)((t + per - 1) / per), (unsigned)cache->hk);
+#define FF_WRITE(DIM, F8)                                                                                    \
+  if (cache->d == DIM && (cache->fp8 != 0) == F8)                                                            \
+    hipLaunchKernelGGL((cache_write_kernel<DIM, F8>), grid, dim3(256), 0, (hipStream_t)stream, a,            \
+                       pages_of(cache), (const bf16_t*)k, k_ts, k_hs, (const bf16_t*)v, v_ts, v_hs, (int)cache->hk, vec);
   FF_WRITE(64, false) FF_WRITE(64, true) FF_WRITE(128, false) FF_WRITE(128, true)
 #undef FF_WRITE
   FF_LAUNCH_CHECK("ff_cache_write");
   return FF_OK;
 }
 
-extern "C" int ff_cache_read(const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale,
-                             int64_t pages, int64_t page_size, int64_t hk, int64_t d, int fp8, const int32_t* table,
-                             int64_t width, const int32_t* lengths, const int32_t* starts, int64_t batch, void* k,
-                             void* v, int64_t t, ff_stream_t stream) {
+extern "C" int ff_cache_read(const ff_paged_cache* cache, const int32_t* table, int64_t width, const int32_t* lengths,
+                             const int32_t* starts, int64_t batch, void* k, void* v, int64_t t, ff_stream_t stream) {
   if (t == 0) return FF_OK;
-  const int st = check("ff_cache_read", k_pages, v_pages, k_scale, v_scale, pages, page_size, hk, d, fp8, table, width,
-                       lengths, batch, t);
+  const int st = check_rows("ff_cache_read", cache, table, width, lengths, starts, batch, t);
   if (st != FF_OK) return st;
   FF_REQUIRE(k && v && ff_aligned(k, 16) && ff_aligned(v, 16), "ff_cache_read: output");
-  FF_REQUIRE(starts || batch == t, "ff_cache_read: without starts every sequence has one row");
-  const Rows a = rows_of(table, width, lengths, starts, batch, t, pages, page_size);
-  const Pages c = {(uint8_t*)k_pages, (uint8_t*)v_pages, (uint8_t*)k_scale, (uint8_t*)v_scale};
-  const int64_t per = 4 * 512 / d;
-  const dim3 grid((unsigned)((t + per - 1) / per), (unsigned)hk);
-#define FF_READ(DIM, F8)                                                                                          \
-  if (d == DIM && (fp8 != 0) == F8)                                                                               \
-    hipLaunchKernelGGL((cache_read_kernel<DIM, F8>), grid, dim3(256), 0, (hipStream_t)stream, a, c, (bf16_t*)k,   \
-                       (bf16_t*)v, (int)hk);
+  const Rows a = rows_of(cache, table, width, lengths, starts, batch, t);
+  const int64_t per = 4 * 512 / cache->d;
+  const dim3 grid((unsigned)((t + per - 1) / per), (unsigned)cache->hk);
+#define FF_READ(DIM, F8)                                                                          \
+  if (cache->d == DIM && (cache->fp8 != 0) == F8)                                                 \
+    hipLaunchKernelGGL((cache_read_kernel<DIM, F8>), grid, dim3(256), 0, (hipStream_t)stream, a,  \
+                       pages_of(cache), (bf16_t*)k, (bf16_t*)v, (int)cache->hk);
   FF_READ(64, false) FF_READ(64, true) FF_READ(128, false) FF_READ(128, true)
 #undef FF_READ
   FF_LAUNCH_CHECK("ff_cache_read");

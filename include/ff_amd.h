@@ -542,15 +542,19 @@ int ff_moe_experts(const void* x, int64_t ldx, const float* weights, const int* 
 /* ---------------------------------------------------------------- kept prompts
  * No reference counterpart: its step runs a prompt once and keeps nothing. */
 
-/* A paged cache: k_pages, v_pages (pages, hk, page_size, d), bf16 or (fp8) e4m3 codes with
+/* A paged cache: k, v (pages, hk, page_size, d), bf16 or (fp8) e4m3 codes with
  * k_scale, v_scale (pages, hk, page_size) bytes, value = code * 2^(byte - 127). page_size is
- * a power of two, 16 .. 4096, d 64 or 128. Position p of sequence b is slot p % page_size of
+ * a power of two, 16 .. 4096, d 64 or 128; k, v 16-byte, the scales 8-byte aligned. Position p of sequence b is slot p % page_size of
  * page table[b, p / page_size], table (batch, width); lengths (batch): the positions of
  * each sequence. starts (batch + 1), rising from 0 to at most t: sequence b has rows
  * starts[b] .. starts[b + 1] - 1 of the call's t, its last positions; NULL: one row each,
  * t == batch. Rows behind the last sequence belong to none. A position past the table's
  * reach and a page outside [0, pages) hold nothing. table, lengths and starts are read by the
  * kernels alone, and whatever they hold no access leaves the buffers. */
+typedef struct {
+  void *k, *v, *k_scale, *v_scale;
+  int64_t pages, page_size, hk, d, fp8;
+} ff_paged_cache;
 
 /* k, v rows (t, hk, d) bf16 with token strides k_ts, v_ts and head strides k_hs, v_hs
  * (elements) -> the pages. fp8: e = the smallest integer in [-100, 120] with amax <= 448 * 2^e,
@@ -558,30 +562,26 @@ int ff_moe_experts(const void* x, int64_t ldx, const float* weights, const int* 
  * (240 at most where e is 120), byte = e + 127; NaN and infinities become NaN. Where two rows name one place either may
  * end there. */
 int ff_cache_write(const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs,
-                   void* k_pages, void* v_pages, void* k_scale, void* v_scale, int64_t pages, int64_t page_size,
-                   int64_t hk, int64_t d, int fp8, const int32_t* table, int64_t width, const int32_t* lengths,
+                   const ff_paged_cache* cache, const int32_t* table, int64_t width, const int32_t* lengths,
                    const int32_t* starts, int64_t batch, int64_t t, ff_stream_t stream);
 
 /* The inverse: k, v (t, hk, d) bf16 contiguous, 16-byte aligned; zeros for what holds nothing. */
-int ff_cache_read(const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale, int64_t pages,
-                  int64_t page_size, int64_t hk, int64_t d, int fp8, const int32_t* table, int64_t width,
-                  const int32_t* lengths, const int32_t* starts, int64_t batch, void* k, void* v, int64_t t,
-                  ff_stream_t stream);
+int ff_cache_read(const ff_paged_cache* cache, const int32_t* table, int64_t width, const int32_t* lengths,
+                  const int32_t* starts, int64_t batch, void* k, void* v, int64_t t, ff_stream_t stream);
 
 /* Causal grouped-query attention of the rows over their sequences' pages: y (t, hq, d) bf16
  * contiguous, y[row] = sum_j p_j v_j over the positions j up to the row's own, p = softmax of
  * scale * q . k_j. Statistics and sums fp32, p rounded to bf16 before it meets v. Query head h
  * reads key head h / (hq / hk). q (t, hq, d) bf16 with strides q_ts, q_hs. scale > 0. A row
  * that sees nothing is zero. workspace: ff_attention_paged_workspace bytes (host-only, 0:
- * none), 16-byte aligned, one per stream and per captured graph that may run beside another.
+ * none; its `starts`: whether there are any), 16-byte aligned, one per stream and per captured graph that may run beside another.
  * The sums' order depends on the sizes, lengths and starts alone. */
-int ff_attention_paged_workspace(int64_t hq, int64_t hk, int64_t d, int fp8, int64_t page_size, int64_t width,
-                                 int64_t batch, int64_t t, int64_t* bytes);
-int ff_attention_paged(const void* q, int64_t q_ts, int64_t q_hs, const void* k_pages, const void* v_pages,
-                       const void* k_scale, const void* v_scale, int64_t pages, int64_t page_size, int64_t hq,
-                       int64_t hk, int64_t d, int fp8, const int32_t* table, int64_t width, const int32_t* lengths,
-                       const int32_t* starts, int64_t batch, void* y, int64_t t, float scale, void* workspace,
-                       int64_t workspace_bytes, ff_stream_t stream);
+int ff_attention_paged_workspace(const ff_paged_cache* cache, int64_t hq, int64_t width, int64_t batch, int starts,
+                                 int64_t t, int64_t* bytes);
+int ff_attention_paged(const void* q, int64_t q_ts, int64_t q_hs, const ff_paged_cache* cache, int64_t hq,
+                       const int32_t* table, int64_t width, const int32_t* lengths, const int32_t* starts,
+                       int64_t batch, void* y, int64_t t, float scale, void* workspace, int64_t workspace_bytes,
+                       ff_stream_t stream);
 
 /* Rows of logits (t, v), row stride ld, bf16 or (f32) fp32: logprobs (t, n) of tokens (t, n) int64
  * with strides tok_ts, tok_ns (a token outside [0, v) scores 0); entropy (t) in nats; the top

@@ -166,12 +166,10 @@ def test_rows_without_a_place(gpu, tile, dtype):
 @pytest.fixture(params=[0, 1, 2, 3])
 def tile(request):
     """The library's own choice of tiles, then each of them for every call."""
-    from fastforward_amd import _lib, cache
+    from fastforward_amd import _lib
     _lib.call("ff_set_tuning", 14, request.param)
-    cache.attend_workspace.cache_clear()
     yield request.param
     _lib.call("ff_set_tuning", 14, 0)
-    cache.attend_workspace.cache_clear()
 
 
 @gpu_test
@@ -376,13 +374,12 @@ def test_far_pages(gpu):
 
 # ---------------------------------------------------------------- refusals (CPU)
 
-def _bare(dtype=BF16):
+def _bare():
     """A cache object without a GPU, for calls that are refused before any launch."""
     from fastforward_amd.cache import PagedCache
     c = PagedCache.__new__(PagedCache)
-    c.pages, c.page_size, c.kv_heads, c.head_dim, c.dtype = 4, 16, 2, 64, dtype
-    c.k = c.v = torch.zeros(4, 2, 16, 64, dtype=BF16)
-    c.k_scale = c.v_scale = None
+    c.pages, c.page_size, c.kv_heads, c.head_dim, c.dtype = 4, 16, 2, 64, BF16
+    c._hold(*(torch.zeros(4, 2, 16, 64, dtype=BF16) for _ in range(2)), None, None)
     return c
 
 
@@ -424,38 +421,41 @@ def test_refusals_c():
     buf = (ctypes.c_char * 4096)()
     p = (ctypes.addressof(buf) + 255) // 256 * 256
 
-    def attend(q=p, pages=4, ps=16, hq=4, hk=2, d=64, fp8=0, ks=None, width=2, starts=p, batch=3, t=3, scale=1.0, y=p,
-               ws=p, nbytes=1 << 30):
-        _lib.call("ff_attention_paged", q, hq * d, d, p, p, ks, ks, pages, ps, hq, hk, d, fp8, p, width, p, starts, batch,
-                  y, t, scale, ws, nbytes, None)
+    def cache(k=p, ks=None, pages=4, ps=16, hk=2, d=64, fp8=0):
+        return ctypes.byref(_lib.PagedCacheStruct(k, p, ks, ks, pages, ps, hk, d, fp8))
 
-    for kw, message in ((dict(d=96), "head_dim"), (dict(ps=24), "page_size"), (dict(ps=8), "page_size"),
-                        (dict(hq=3), "bad sizes"), (dict(hk=0), "bad sizes"), (dict(width=0), "bad sizes"),
-                        (dict(width=1 << 27), "bad sizes"), (dict(batch=0), "bad sizes"), (dict(t=-1), "bad sizes"),
-                        (dict(t=1 << 25), "bad sizes"), (dict(t=1 << 24, width=1 << 20), "too large"),
-                        (dict(q=None), "null"), (dict(y=None), "null"), (dict(fp8=1), "null"), (dict(pages=0), "pages"),
-                        (dict(starts=None, t=2), "starts"), (dict(scale=0.0), "scale"), (dict(scale=math.nan), "scale"),
-                        (dict(y=p + 2), "alignment"), (dict(ks=p + 4, fp8=1), "alignment"),
+    def attend(q=p, hq=4, width=2, lengths=p, starts=p, batch=3, t=3, scale=1.0, y=p, ws=p, nbytes=1 << 30, **kw):
+        _lib.call("ff_attention_paged", q, 256, 64, cache(**kw), hq, p, width, lengths, starts, batch, y, t, scale, ws,
+                  nbytes, None)
+
+    def write(k_rows=p, width=2, lengths=p, starts=p, batch=3, t=3, **kw):
+        _lib.call("ff_cache_write", k_rows, 128, 64, p, 128, 64, cache(**kw), p, width, lengths, starts, batch, t, None)
+
+    def read(k_rows=p, width=2, lengths=p, starts=p, batch=3, t=3, **kw):
+        _lib.call("ff_cache_read", cache(**kw), p, width, lengths, starts, batch, k_rows, p, t, None)
+
+    shared = ((dict(d=96), "head_dim"), (dict(ps=24), "page_size"), (dict(ps=8), "page_size"), (dict(ps=8192), "page_size"),
+              (dict(hk=0), "bad sizes"), (dict(width=0), "bad sizes"), (dict(width=1 << 27), "bad sizes"),
+              (dict(batch=0), "bad sizes"), (dict(t=-1), "bad sizes"), (dict(t=1 << 25), "bad sizes"),
+              (dict(pages=0), "bad sizes"), (dict(pages=1 << 31), "bad sizes"), (dict(k=None), "null"),
+              (dict(lengths=None), "null"), (dict(fp8=1), "null"), (dict(starts=None, t=2), "starts"),
+              (dict(k=p + 8), "alignment"), (dict(ks=p + 4, fp8=1), "alignment"))
+    for f in (attend, write, read):
+        for kw, message in shared:
+            with pytest.raises(RuntimeError, match=message):
+                f(**kw)
+    for kw, message in ((dict(hq=3), "bad sizes"), (dict(hq=0), "bad sizes"), (dict(t=1 << 24, width=1 << 20), "too large"),
+                        (dict(q=None), "null"), (dict(y=None), "null"), (dict(scale=0.0), "scale"),
+                        (dict(scale=math.nan), "scale"), (dict(y=p + 2), "alignment"),
                         (dict(width=100, nbytes=64), "workspace"), (dict(width=100, ws=None), "workspace")):
         with pytest.raises(RuntimeError, match=message):
             attend(**kw)
-    attend(q=None, t=0)
-
-    def write(k=p, pages=4, ps=16, hk=2, d=64, fp8=0, width=2, starts=p, batch=3, t=3):
-        _lib.call("ff_cache_write", k, 128, 64, p, 128, 64, p, p, None, None, pages, ps, hk, d, fp8, p, width, p, starts,
-                  batch, t, None)
-
-    def read(k=p, pages=4, ps=16, hk=2, d=64, fp8=0, width=2, starts=p, batch=3, t=3):
-        _lib.call("ff_cache_read", p, p, None, None, pages, ps, hk, d, fp8, p, width, p, starts, batch, k, p, t, None)
-
     for f in (write, read):
-        for kw, message in ((dict(d=32), "head_dim"), (dict(ps=48), "page_size"), (dict(hk=0), "bad sizes"),
-                            (dict(pages=0), "bad sizes"), (dict(width=0), "bad sizes"), (dict(batch=0), "bad sizes"),
-                            (dict(t=-1), "bad sizes"), (dict(k=None), "null|output"), (dict(fp8=1), "null"),
-                            (dict(starts=None, t=2), "starts")):
-            with pytest.raises(RuntimeError, match=message):
-                f(**kw)
-        f(k=None, t=0)
+        with pytest.raises(RuntimeError, match="null|output"):
+            f(k_rows=None)
+    attend(q=None, t=0)
+    write(k_rows=None, t=0)
+    read(k_rows=None, t=0)
     need = ctypes.c_int64(-1)
-    _lib.call("ff_attention_paged_workspace", 32, 8, 128, 0, 64, 2, 1, 1, ctypes.byref(need))
+    _lib.call("ff_attention_paged_workspace", cache(hk=8, d=128, ps=64), 32, 2, 1, 0, 1, ctypes.byref(need))
     assert need.value == 0                              # 128 positions are never split
