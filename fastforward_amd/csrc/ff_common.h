@@ -312,6 +312,7 @@ __device__ __forceinline__ float dpp(float x) {
 }
 constexpr int kDppXor1 = 0xB1;        // quad_perm [1,0,3,2]
 constexpr int kDppXor2 = 0x4E;        // quad_perm [2,3,0,1]
+constexpr int kDppQuadReverse = 0x1B; // quad_perm [3,2,1,0]
 constexpr int kDppRowMirror = 0x140;  // lane i <- 15 - i
 constexpr int kDppHalfMirror = 0x141; // lane i <- 7 - i within each 8
 constexpr int kDppRowRor8 = 0x128;    // lane i <- lane (i + 8) mod 16 of its row

@@ -1,20 +1,23 @@
 // Log probabilities of given tokens, entropy and the most likely tokens of rows of
 // logits, in one pass over them.
 //
-// Every lane keeps a running maximum m and, of its values x, the sums over all but one
-// occurrence of the maximum: r = sum e^(x - m) and t = sum (x - m) e^(x - m). With M, R
-// and T of the whole row, log sum e^x = M + log1p(R), so
-//   log p(x) = (x - M) - log1p(R),   entropy = log1p(R) - T / (1 + R):
-// what is left of a near-certain token's probability keeps its relative precision in 32
-// bits, since 1 is never added to it. The exponents are of base 2 until the end.
+// A wave sums relative to a reference c that is one of its logits: over all the others,
+// r = sum e^(x - c) and t = sum (x - c) e^(x - c), so that a row's are
+//   log p(x) = (x - c) - log1p(r),   entropy = log1p(r) - t / (1 + r).
+// c moves to the largest logit where that passes it by 4 ln 2. A token that is all but
+// certain is then the reference, the 1 is never added, and what is left of the
+// probability keeps its relative precision in 32 bits; a token above c by less
+// has a probability of 16 / 17 at most, where there is nothing to lose. Exponents are of base
+// 2 until the end.
 //
-// The most likely tokens: a wave's best 64 so far lie sorted in its lanes, as one
-// 64-bit key of (value, lowest index first). A vector of logits enters only where one of
-// its values beats the wave's k-th best, which soon is rare. Waves, then parts of a row,
-// are joined by taking the best of their lists' heads k times.
+// The most likely tokens: a wave's best 64 so far lie sorted in its lanes, as 64-bit keys of
+// (value, lowest index first). A vector of logits is looked at only where one of
+// them is above the wave's k-th best, or c's limit: one comparison with the smaller of the
+// two. Waves, then parts of a row, are joined by taking the best of their lists' heads
+// k times.
 //
-// Bound by the logits' bytes: a row is read once, 16 bytes a lane and load. Few rows are
-// split over workgroups, and a second launch joins their parts.
+// Bound by the logits' bytes: a row is read once, 16 bytes a lane and load, four loads in
+// flight while the four before are taken. Few rows are split over workgroups, and a second launch joins their parts.
 #include "ff_common.h"
 
 using namespace ff;
@@ -32,7 +35,7 @@ struct Args {
   int64_t tok_ts, tok_ns;
   float *logprobs, *entropy, *top_logprobs;
   int* top_ids;
-  float* part;          // (rows, parts, 4): maximum, r, t, whether a NaN or +inf was seen
+  float* part;          // (rows, parts, 4): c, r, t
   uint64_t* part_keys;  // (rows, parts, top)
   int64_t v;
   int t, n, top, parts;
@@ -50,105 +53,90 @@ __device__ __forceinline__ float value_of(uint64_t key) {
   return k == 0xFFFFFFFFu ? __builtin_nanf("") : __uint_as_float(k >> 31 ? k & 0x7FFFFFFFu : ~k);
 }
 
-// A row's statistics (or a part's): m in natural units; r and t as above, t in base 2.
+// A row's statistics, or a part's: the reference (-inf: no logit yet), r and t (in base 2).
 struct Stats {
   float m, r, t;
 };
 
-// Joins b into a.
+// What s adds, its reference too, relative to one that is `down` above (in base 2; -inf or so far that
+// nothing is left: 0, or NaN where there is one).
+__device__ __forceinline__ Stats lowered(const Stats& s, float down) {
+  const float e = __builtin_amdgcn_exp2f(down);
+  if (!(e > 0.f)) return Stats{s.m, s.r * 0.f, s.t * 0.f};
+  return Stats{s.m, e * (1.f + s.r), e * (s.t + down * (1.f + s.r))};
+}
+
+// Joins b into a. (A side without a reference has r 0, or NaN where it saw one.)
 __device__ __forceinline__ void join(Stats& a, const Stats& b) {
-  if (b.m == -INFINITY) return;
-  if (a.m == -INFINITY) {
-    a = b;
+  if (a.m == -INFINITY || b.m == -INFINITY) {
+    const Stats s = b.m == -INFINITY ? a : b;
+    a = Stats{s.m, a.r + b.r, s.t};
     return;
   }
   const bool up = b.m > a.m;
-  const float d = -fabsf(a.m - b.m) * kLog2e, e = __builtin_amdgcn_exp2f(d);
-  const Stats hi = up ? b : a, lo = up ? a : b;
-  // the lower side's 1 + r and its maximum's own share move d down
-  a.m = hi.m;
-  a.r = hi.r + e * (1.f + lo.r);
-  a.t = hi.t + e * (lo.t + d * (1.f + lo.r));
+  const Stats hi = up ? b : a, lo = lowered(up ? a : b, (up ? a.m - b.m : b.m - a.m) * kLog2e);
+  a = Stats{hi.m, hi.r + lo.r, hi.t + lo.t};
 }
 
-__device__ __forceinline__ Stats shuffle_xor(const Stats& s, int mask) {
-  return Stats{__shfl_xor(s.m, mask, 64), __shfl_xor(s.r, mask, 64), __shfl_xor(s.t, mask, 64)};
-}
-
-__device__ __forceinline__ uint64_t shuffle(uint64_t v, int lane) {
-  return (uint64_t)(uint32_t)__shfl((int)(v >> 32), lane, 64) << 32 | (uint32_t)__shfl((int)(uint32_t)v, lane, 64);
+template <int CTRL>
+__device__ __forceinline__ uint64_t dpp64(uint64_t v) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_update_dpp((int)(v >> 32), (int)(v >> 32), CTRL, 0xF, 0xF, false) << 32 |
+         (uint32_t)__builtin_amdgcn_update_dpp((int)(uint32_t)v, (int)(uint32_t)v, CTRL, 0xF, 0xF, false);
 }
 __device__ __forceinline__ uint64_t read_lane(uint64_t v, int lane) {
   return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
          (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
 }
+__device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
+template <bool WIDE>
+__device__ __forceinline__ uint64_t swapped(uint64_t v) {
+  const uint32_t h = (uint32_t)(v >> 32), l = (uint32_t)v;
+  const auto a = WIDE ? __builtin_amdgcn_permlane32_swap(h, h, false, false) : __builtin_amdgcn_permlane16_swap(h, h, false, false);
+  const auto b = WIDE ? __builtin_amdgcn_permlane32_swap(l, l, false, false) : __builtin_amdgcn_permlane16_swap(l, l, false, false);
+  return larger((uint64_t)a[0] << 32 | b[0], (uint64_t)a[1] << 32 | b[1]);
+}
 
 // Puts the uniform key into the wave's falling list (one entry a lane).
-__device__ __forceinline__ void insert(uint64_t& list, uint64_t key, int lane) {
-  const uint64_t up = shuffle(list, lane - 1 < 0 ? 0 : lane - 1);
-  const bool beats = key > list;
-  list = !beats ? list : lane && key > up ? up : key;
+__device__ __forceinline__ void insert(uint64_t& list, uint64_t key) {
+  // the lane before (wave_shr:1); lane 0 has none, and gets a key above all
+  const uint64_t up = (uint64_t)(uint32_t)__builtin_amdgcn_update_dpp(-1, (int)(list >> 32), 0x138, 0xF, 0xF, false) << 32 |
+                      (uint32_t)__builtin_amdgcn_update_dpp(-1, (int)(uint32_t)list, 0x138, 0xF, 0xF, false);
+  list = key <= list ? list : key > up ? up : key;
 }
 
-template <int N>
-__device__ __forceinline__ void take(const float (&x)[N], uint32_t index0, Stats& s) {
-  float top = x[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
-  if (top > s.m) {  // a new maximum: the old one becomes an ordinary value
-    if (s.m != -INFINITY) {
-      const float d = (s.m - top) * kLog2e, e = __builtin_amdgcn_exp2f(d);
-      s.t = e * (s.t + d * (1.f + s.r));
-      s.r = e * (1.f + s.r);
-    }
-    s.m = top;
-    bool first = true;  // one occurrence of it is left out
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const bool it = first && x[i] == top;
-      first = first && !it;
-      const float d = fmaxf((x[i] - top) * kLog2e, -1e6f), e = __builtin_amdgcn_exp2f(d);
-      s.r += it ? 0.f : e;
-      s.t = __builtin_fmaf(e, d, s.t);
-    }
-  } else if (s.m != -INFINITY) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float d = fmaxf((x[i] - s.m) * kLog2e, -1e6f), e = __builtin_amdgcn_exp2f(d);
-      s.r += e;
-      s.t = __builtin_fmaf(e, d, s.t);
-    }
-  }
-}
-
-// The best `top` of `lists` falling lists of `top` keys at `keys` (LDS), by one wave: the
-// result's entry i in lane i.
+// The best `top` of the falling lists of `top` keys at `keys` (LDS), LISTS at most 8 or 64
+// of them, by one wave: entry i of the result in lane i.
+template <int LISTS>
 __device__ __forceinline__ uint64_t best_of(const uint64_t* keys, int lists, int top, int lane) {
   uint64_t out = 0;
-  // lane l holds the heads of lists l, l + 64, ...; lists <= 64
-  int at = 0;
-  uint64_t head = lane < lists ? keys[(int64_t)lane * top] : 0;
+  int at = lane * top;
+  const int end = lane < lists ? at + top : 0;
+  uint64_t head = at < end ? keys[at] : 0, next = at + 1 < end ? keys[at + 1] : 0;
   for (int i = 0; i < top; ++i) {
-    uint64_t best = head;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint64_t other = (uint64_t)(uint32_t)__shfl_xor((int)(best >> 32), o, 64) << 32 |
-                             (uint32_t)__shfl_xor((int)(uint32_t)best, o, 64);
-      best = best > other ? best : other;
+    uint64_t best = larger(head, dpp64<kDppXor1>(head));
+    best = larger(best, dpp64<kDppXor2>(best));
+    best = larger(best, dpp64<kDppHalfMirror>(best));
+    if (LISTS > 8) {
+      best = larger(best, dpp64<kDppRowMirror>(best));
+      best = swapped<false>(best);
+      best = swapped<true>(best);
     }
+    best = read_lane(best, 0);
     if (lane == i) out = best;
-    if (head == best && best) {  // keys differ, so one lane at most
+    if (head == best) {  // keys differ, so one lane (or all that have none left)
       ++at;
-      head = at < top ? keys[(int64_t)lane * top + at] : 0;
+      head = next;
+      next = at + 1 < end ? keys[at + 1] : 0;
     }
   }
   return out;
 }
 
-// Writes a row's results; the whole wave. `odd`: the row holds a NaN or +inf.
+// Writes a row's results; the whole wave.
 template <typename T>
-__device__ __forceinline__ void finish(const Args& p, int row, const Stats& s, bool odd, uint64_t list, int lane) {
+__device__ __forceinline__ void finish(const Args& p, int row, const Stats& s, uint64_t list, int lane) {
   const float nan = __builtin_nanf("");
+  const bool odd = s.r != s.r || s.t != s.t || s.m == INFINITY;  // the row holds a NaN or +inf
   const bool none = s.m == -INFINITY;  // every token is switched off
   const float l = log1pf(s.r);
   const T* x = (const T*)p.x + row * p.ld;
@@ -169,29 +157,230 @@ __device__ __forceinline__ void finish(const Args& p, int row, const Stats& s, b
   }
 }
 
+// One step of a bitonic network over the wave: the lanes whose bit `bit` is clear keep the larger
+// of their own key and `other`, the others the smaller.
+__device__ __forceinline__ uint64_t keep(uint64_t mine, uint64_t other, int lane, int bit) {
+  return (mine > other) == ((lane & bit) == 0) ? mine : other;
+}
+__device__ __forceinline__ uint64_t xor4(uint64_t v) { return dpp64<kDppQuadReverse>(dpp64<kDppHalfMirror>(v)); }
+__device__ __forceinline__ uint64_t xor8(uint64_t v) { return dpp64<kDppRowRor8>(v); }
+template <bool WIDE>
+__device__ __forceinline__ uint64_t xor_rows(uint64_t v, int lane) {  // lane ^ 16, or ^ 32
+  const uint32_t h = (uint32_t)(v >> 32), l = (uint32_t)v;
+  const auto a = WIDE ? __builtin_amdgcn_permlane32_swap(h, h, false, false) : __builtin_amdgcn_permlane16_swap(h, h, false, false);
+  const auto b = WIDE ? __builtin_amdgcn_permlane32_swap(l, l, false, false) : __builtin_amdgcn_permlane16_swap(l, l, false, false);
+  const int k = lane & (WIDE ? 32 : 16) ? 0 : 1;
+  return (uint64_t)a[k] << 32 | b[k];
+}
+
+// The lanes' keys in falling order.
+__device__ __forceinline__ uint64_t sorted(uint64_t v, int lane) {
+  v = keep(v, dpp64<kDppXor1>(v), lane, 1);
+  v = keep(v, dpp64<kDppQuadReverse>(v), lane, 2);
+  v = keep(v, dpp64<kDppXor1>(v), lane, 1);
+  v = keep(v, dpp64<kDppHalfMirror>(v), lane, 4);
+  v = keep(v, dpp64<kDppXor2>(v), lane, 2);
+  v = keep(v, dpp64<kDppXor1>(v), lane, 1);
+  v = keep(v, dpp64<kDppRowMirror>(v), lane, 8);
+#pragma unroll
+  for (int size = 16; size <= 64; size *= 2) {
+    if (size == 32) v = keep(v, xor_rows<false>(dpp64<kDppRowMirror>(v), lane), lane, 16);
+    if (size == 64) {
+      v = keep(v, xor_rows<true>(xor_rows<false>(dpp64<kDppRowMirror>(v), lane), lane), lane, 32);
+      v = keep(v, xor_rows<false>(v, lane), lane, 16);
+    }
+    if (size > 16) v = keep(v, xor8(v), lane, 8);
+    v = keep(v, xor4(v), lane, 4);
+    v = keep(v, dpp64<kDppXor2>(v), lane, 2);
+    v = keep(v, dpp64<kDppXor1>(v), lane, 1);
+  }
+  return v;
+}
+
+// A wave's pass over its logits. Exponents are y = fma(x, log2 e, -yc), yc = c log2 e rounded: one
+// instruction, and all weights are relative to 2^yc. The reference's own weight is 2^off,
+// off = fma(c, log2 e, -yc), by which the sums are divided at the end. Where c log2 e may overflow
+// (`huge`), y = (x - c) log2 e.
+template <int N>
+struct Wave {
+  float c = -INFINITY, limit = -INFINITY;  // the reference and where it moves; uniform
+  float yc = 0.f, off = 0.f;
+  bool huge = false;
+  float r = 0.f, t = 0.f;                  // this lane's part of the sums, t of y e
+  uint64_t list = 0, least = 0;            // the best keys; the k-th best (uniform)
+  float kth = __builtin_nanf("");          // its logit (NaN: there are not k, or it is one)
+  float bound = __builtin_nanf("");        // what makes a vector worth a look; NaN: every one is
+
+  template <bool HUGE_C>
+  __device__ __forceinline__ void add(float x, bool counts) {
+    const float y = fmaxf(HUGE_C ? (x - c) * kLog2e : __builtin_fmaf(x, kLog2e, -yc), -1e6f);
+    const float e = counts ? __builtin_amdgcn_exp2f(y) : 0.f;
+    r += e;
+    t = __builtin_fmaf(e, y, t);
+  }
+
+  // N logits of every lane, those of lane l at first + l N (all above the indices of earlier calls).
+  // Past the end lanes have -inf.
+  __device__ __forceinline__ void take(const float (&x)[N], int64_t first, int64_t end, int top, int lane) {
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = __builtin_elementwise_maximum(m, x[i]);  // (NaN if there is one)
+    if (!__ballot(!(m <= bound))) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) add<false>(x[i], true);
+      return;
+    }
+    if (huge || __ballot(!(m <= limit))) {
+      refer(x, lane);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) add<false>(x[i], true);
+    }
+    if (top) {
+      if (!least) seed(x, first, end, top, lane);
+      else if (__ballot(!(m <= kth))) pick(x, first, end, top);
+    }
+    // (NaN while there is no reference or there are not k)
+    bound = huge || c == -INFINITY || (top && kth != kth) ? __builtin_nanf("") : top ? fminf(limit, kth) : limit;
+  }
+
+  // Moves the reference where a logit passes its limit, and adds the logits.
+  __device__ __forceinline__ void refer(const float (&x)[N], int lane) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, x[i]);
+    const float high = wave_max(m);
+    bool skip = false;  // this lane holds the new reference
+    if (high > limit) {
+      const bool big = fabsf(high) > 1e38f;
+      const float y = big ? 0.f : high * kLog2e;
+      if (c != -INFINITY) {  // the old one becomes an ordinary logit, lane 0's
+        const float down = big || huge ? (c - high) * kLog2e : yc - y, e = __builtin_amdgcn_exp2f(down);
+        const float one = lane ? 0.f : __builtin_amdgcn_exp2f(off);
+        t = e > 0.f ? e * (t + down * (one + r) + off * one) : t * 0.f;
+        r = e > 0.f ? e * (one + r) : r * 0.f;
+      }
+      c = high;
+      huge = big;
+      yc = y;
+      off = big ? 0.f : __builtin_fmaf(high, kLog2e, -y);
+      limit = high + 2.7725887f;
+      skip = __builtin_ctzll(__ballot(m == high)) == lane;
+    }
+    if (c != -INFINITY) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const bool it = skip && x[i] == c;  // one occurrence of it is left out
+        skip = skip && !it;
+        if (huge) add<true>(x[i], !it);
+        else add<false>(x[i], !it);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) r += x[i] != x[i] ? x[i] : 0.f;  // (a NaN always comes here; add's maximum drops it)
+  }
+
+  // The first logits: the lanes' best keys at once, then the others that beat the k-th of those.
+  __device__ __forceinline__ void seed(const float (&x)[N], int64_t first, int64_t end, int top, int lane) {
+    uint64_t key[N], best = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int64_t index = first + lane * N + i;
+      key[i] = index < end ? key_of(x[i], (uint32_t)index) : 0;
+      best = larger(best, key[i]);
+    }
+    list = sorted(best, lane);
+    least = read_lane(list, top - 1);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      uint64_t hits = __ballot(key[i] > least && key[i] != best);
+      while (hits) {
+        put(read_lane(key[i], __builtin_ctzll(hits)), top);
+        hits &= hits - 1;
+      }
+    }
+    kth = value_of(least);
+  }
+
+  // Later ones: a logit equal to the k-th best comes behind it.
+  __device__ __forceinline__ void pick(const float (&x)[N], int64_t first, int64_t end, int top) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      uint64_t hits = __ballot(!(x[i] <= kth));
+      while (hits) {
+        const int src = __builtin_ctzll(hits);
+        const int64_t index = first + src * N + i;
+        const float v = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(x[i]), src));
+        if (index < end) put(key_of(v, (uint32_t)index), top);
+        hits &= hits - 1;
+      }
+    }
+    kth = value_of(least);
+  }
+
+  __device__ __forceinline__ void put(uint64_t key, int top) {
+    if (key <= least) return;
+    insert(list, key);
+    least = read_lane(list, top - 1);
+  }
+
+  __device__ __forceinline__ Stats stats() const {
+    const float rs = wave_sum(r), ts = wave_sum(t);
+    if (c == -INFINITY) return Stats{c, rs, ts};  // no logit, or NaN
+    const float w = __builtin_amdgcn_exp2f(-off);
+    return Stats{c, rs * w, (ts - off * rs) * w};
+  }
+};
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void scores_kernel(Args p, int64_t per, int vec) {
-  constexpr int N = 16 / sizeof(T);
+  constexpr int N = 16 / sizeof(T), U = 4;
   __shared__ uint64_t keys[kWaves * kMaxTop];
   __shared__ Stats stats[kWaves];
-  __shared__ int odds[kWaves];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
   const T* x = (const T*)p.x + row * p.ld;
   const int64_t begin = part * per, end = min(begin + per, p.v);
-  Stats s = {-INFINITY, 0.f, 0.f};
-  bool odd = false;
-  uint64_t list = 0, least = 0;  // least: the k-th best so far
-  for (int64_t i0 = begin + wave * 64 * N; i0 < end; i0 += kThreads * N) {
+  Wave<N> w;
+  auto unpack = [&](const u32x4& v, float (&f)[N]) {
+    if constexpr (N == 8) {
+      unpack8(v, f);
+    } else {
+      f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
+    }
+  };
+  int64_t i0 = begin + wave * 64 * N;
+  if (vec) {
+    constexpr int64_t STEP = kThreads * N;
+    const T* at = x + lane * N;
+    const int64_t whole = end - ((U - 1) * STEP + 64 * N);  // i0 up to which U vectors are whole
+    u32x4 next[U];
+    if (i0 <= whole) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) next[u] = *reinterpret_cast<const u32x4*>(at + i0 + u * STEP);
+    }
+    while (i0 <= whole) {
+      u32x4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = next[u];
+      if (i0 + U * STEP <= whole) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) next[u] = *reinterpret_cast<const u32x4*>(at + i0 + (U + u) * STEP);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float f[N];
+        unpack(v[u], f);
+        w.take(f, i0 + u * STEP, end, p.top, lane);
+      }
+      i0 += U * STEP;
+    }
+  }
+  for (; i0 < end; i0 += kThreads * N) {
     const int64_t i = i0 + lane * N;
     float f[N];
     if (vec && i + N <= end) {
-      const u32x4 w = *reinterpret_cast<const u32x4*>(x + i);
-      if constexpr (N == 8) {
-        unpack8(w, f);
-      } else {
-        f[0] = __uint_as_float(w.x), f[1] = __uint_as_float(w.y), f[2] = __uint_as_float(w.z), f[3] = __uint_as_float(w.w);
-      }
+      unpack(*reinterpret_cast<const u32x4*>(x + i), f);
     } else {
 #pragma unroll
       for (int e = 0; e < N; ++e) {
@@ -199,83 +388,46 @@ __global__ __launch_bounds__(kThreads) void scores_kernel(Args p, int64_t per, i
         if (i + e < end) f[e] = N == 8 ? bf16_to_f32(((const bf16_t*)x)[i + e]) : ((const float*)x)[i + e];
       }
     }
-#pragma unroll
-    for (int e = 0; e < N; ++e) odd |= !(f[e] < INFINITY);
-    take<N>(f, (uint32_t)i, s);
-    if (p.top) {
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const uint64_t key = i + e < end ? key_of(f[e], (uint32_t)(i + e)) : 0;
-        uint64_t hits = __ballot(key > least);
-        while (hits) {
-          const int src = __builtin_ctzll(hits);
-          hits &= hits - 1;
-          const uint64_t k = read_lane(key, src);
-          if (k > least) {
-            insert(list, k, lane);
-            least = read_lane(list, p.top - 1);
-          }
-        }
-      }
-    }
+    w.take(f, i0, end, p.top, lane);
   }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    // both partners join in the same order, so that they get the same bits
-    const Stats other = shuffle_xor(s, o);
-    Stats a = lane & o ? other : s;
-    join(a, lane & o ? s : other);
-    s = a;
-  }
-  odd = __ballot(odd) != 0;
-  if (lane < p.top) keys[wave * p.top + lane] = list;
-  if (lane == 0) {
-    stats[wave] = s;
-    odds[wave] = odd;
-  }
+  if (lane < p.top) keys[wave * p.top + lane] = w.list;
+  const Stats mine = w.stats();
+  if (lane == 0) stats[wave] = mine;
   __syncthreads();
   if (wave) return;
-  s = stats[0];
-  odd = odds[0];
-  for (int w = 1; w < kWaves; ++w) {
-    join(s, stats[w]);
-    odd |= odds[w];
-  }
-  if (p.top) list = best_of(keys, kWaves, p.top, lane);
+  Stats s = stats[0];
+  for (int i = 1; i < kWaves; ++i) join(s, stats[i]);
+  const uint64_t list = p.top ? best_of<8>(keys, kWaves, p.top, lane) : 0;
   if (p.parts == 1) {
-    finish<T>(p, row, s, odd, list, lane);
+    finish<T>(p, row, s, list, lane);
     return;
   }
   const int64_t at = (int64_t)row * p.parts + part;
-  if (lane == 0) *reinterpret_cast<f32x4*>(p.part + 4 * at) = f32x4{s.m, s.r, s.t, odd ? 1.f : 0.f};
+  if (lane == 0) *reinterpret_cast<f32x4*>(p.part + 4 * at) = f32x4{s.m, s.r, s.t, 0.f};
   if (lane < p.top) p.part_keys[at * p.top + lane] = list;
 }
 
-// A wave per row joins its parts (64 at most).
+// A workgroup per row joins its parts (64 at most).
 template <typename T>
-__global__ __launch_bounds__(64) void join_kernel(Args p) {
+__global__ __launch_bounds__(256) void join_kernel(Args p) {
   __shared__ uint64_t keys[64 * kMaxTop];
-  const int lane = threadIdx.x, row = blockIdx.x;
+  const int lane = threadIdx.x & 63, row = blockIdx.x;
   const int64_t at = (int64_t)row * p.parts;
   Stats s = {-INFINITY, 0.f, 0.f};
-  bool odd = false;
   if (lane < p.parts) {
     const f32x4 q = *reinterpret_cast<const f32x4*>(p.part + 4 * (at + lane));
     s = Stats{q[0], q[1], q[2]};
-    odd = q[3] != 0.f;
   }
-  odd = __ballot(odd) != 0;
-  for (int i = lane; i < p.parts * p.top; i += 64) keys[i] = p.part_keys[at * p.top + i];
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const Stats other = shuffle_xor(s, o);
-    Stats a = lane & o ? other : s;
-    join(a, lane & o ? s : other);
-    s = a;
-  }
+  for (int i = threadIdx.x; i < p.parts * p.top; i += 256) keys[i] = p.part_keys[at * p.top + i];
   __syncthreads();
-  const uint64_t list = p.top ? best_of(keys, p.parts, p.top, lane) : 0;
-  finish<T>(p, row, s, odd, list, lane);
+  if (threadIdx.x >= 64) return;
+  // all parts relative to the largest reference
+  const float high = wave_max(s.m);
+  const bool first = __builtin_ctzll(__ballot(s.m == high) | 1ull << 63) == lane;
+  if (!first && s.m != -INFINITY) s = lowered(s, (s.m - high) * kLog2e);
+  s = Stats{high, wave_sum(s.r), wave_sum(s.t)};
+  const uint64_t list = p.top ? best_of<64>(keys, p.parts, p.top, lane) : 0;
+  finish<T>(p, row, s, list, lane);
 }
 
 // Parts of a row: enough workgroups for the GPU, 2048 logits a part at least.
@@ -329,8 +481,8 @@ extern "C" int ff_token_scores(const void* logits, int f32, int64_t ld, const in
   if (f32) hipLaunchKernelGGL((scores_kernel<float>), grid, dim3(kThreads), 0, s, p, per, vec);
   else hipLaunchKernelGGL((scores_kernel<bf16_t>), grid, dim3(kThreads), 0, s, p, per, vec);
   if (parts > 1) {
-    if (f32) hipLaunchKernelGGL((join_kernel<float>), dim3((unsigned)t), dim3(64), 0, s, p);
-    else hipLaunchKernelGGL((join_kernel<bf16_t>), dim3((unsigned)t), dim3(64), 0, s, p);
+    if (f32) hipLaunchKernelGGL((join_kernel<float>), dim3((unsigned)t), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((join_kernel<bf16_t>), dim3((unsigned)t), dim3(256), 0, s, p);
   }
   FF_LAUNCH_CHECK("ff_token_scores");
   return FF_OK;

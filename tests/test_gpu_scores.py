@@ -34,6 +34,8 @@ def _check(logits, tokens, top):
 
     def near(a, want, tol):
         a = a.cpu().double()
+        # the difference of the type's lowest and largest values, 6.8e38, is past fp32's 3.4e38: -inf there
+        want = torch.where(want.abs() > 2.0 ** 128, want.sign() * math.inf, want)
         assert torch.equal(a.isnan(), want.isnan()) and torch.equal(a.isinf(), want.isinf())
         off = torch.where(want.abs() < math.inf, (a - want).abs() - tol, torch.zeros_like(want))
         assert float(off.max() if off.numel() else 0) <= 1e-37, float(off.max())
@@ -69,7 +71,7 @@ def test_scores_special_rows(gpu, dtype, v):
     """Rows of nothing, one token left, all equal, NaN, infinities, near-certain tokens, falling and rising
     rows (every logit enters the list of the likeliest), the type's lowest value, tokens that are none."""
     inf, low = math.inf, torch.finfo(dtype).min
-    l = torch.randn(16, v, generator=_g(4)) * 2
+    l = torch.randn(19, v, generator=_g(4)) * 2
     l[0] = -inf
     l[1], l[1, 37] = -inf, 3.0
     l[2] = 0
@@ -86,8 +88,11 @@ def test_scores_special_rows(gpu, dtype, v):
     l[13, 3], l[13, 5], l[13, 6], l[13, 8] = math.nan, -math.nan, inf, -inf
     l[14] = -inf
     l[14, 1::7] = low
+    l[16, :v // 2] = low                             # whole waves of the lowest value, then others; the reverse
+    l[17, v // 2:] = low
+    l[18, :v // 2], l[18, v // 2:] = low, -low
     l = l.to(dtype)
-    tokens = torch.tensor([0, 1, 37, v - 1, v, -1, -100, 7, 1 << 40]).repeat(16, 1)
+    tokens = torch.tensor([0, 1, 37, v - 1, v, -1, -100, 7, 1 << 40]).repeat(19, 1)
     for top in (0, 1, 20, min(v, 64)):
         _check(l, tokens, top)
 
