@@ -117,7 +117,7 @@ class PagedCache:
         t = table.shape[0] if rows is None else rows
         assert t >= 0 and (rows is not None or starts is None), "rows is missing"
         args = self._rows(t, table, lengths, starts)
-        k = table.new_empty((t, self.kv_heads, self.head_dim), dtype=BF16)
+        k = table.new_empty(t, self.kv_heads, self.head_dim, dtype=BF16)
         v = torch.empty_like(k)
         entry("ff_cache_read")(self._c, *args, k.data_ptr(), v.data_ptr(), t, stream())
         return k, v
@@ -146,12 +146,12 @@ class PagedCache:
         if qs[2] != 1:
             q = q.contiguous()
             qs = q.stride()
-        y = q.new_empty((t, heads, d))
+        y = q.new_empty(t, heads, d)
         sizes = (t, heads, rows[1], rows[4], starts is not None)
         need = self._workspace.get(sizes)
         if need is None:
             need = self._workspace[sizes] = self.attend_workspace(*sizes)
-        ws = q.new_empty((need,), dtype=torch.uint8) if need else None
+        ws = q.new_empty(need, dtype=torch.uint8) if need else None
         entry("ff_attention_paged")(q.data_ptr(), qs[0], qs[1], self._c, heads, *rows, y.data_ptr(), t, scale,
                                     0 if ws is None else ws.data_ptr(), need, stream())
         return y

@@ -16,8 +16,8 @@
 // two. Waves, then parts of a row, are joined by taking the best of their lists' heads
 // k times.
 //
-// Bound by the logits' bytes: a row is read once, 16 bytes a lane and load, four loads in
-// flight while the four before are taken. Few rows are split over workgroups, and a second launch joins their parts.
+// Bound by the logits' bytes: a row is read once, 16 bytes a lane and load, two loads
+// ahead. Few rows are split over workgroups, and a second launch joins their parts.
 #include "ff_common.h"
 
 using namespace ff;
@@ -219,27 +219,43 @@ struct Wave {
     t = __builtin_fmaf(e, y, t);
   }
 
-  // N logits of every lane, those of lane l at first + l N (all above the indices of earlier calls).
-  // Past the end lanes have -inf.
-  __device__ __forceinline__ void take(const float (&x)[N], int64_t first, int64_t end, int top, int lane) {
+  // Whether N logits of every lane need a look.
+  __device__ __forceinline__ bool hot(const float (&x)[N]) const {
     float m = x[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) m = __builtin_elementwise_maximum(m, x[i]);  // (NaN if there is one)
-    if (!__ballot(!(m <= bound))) {
+    return __ballot(!(m <= bound)) != 0;
+  }
+  __device__ __forceinline__ void add_all(const float (&x)[N]) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) add<false>(x[i], true);
-      return;
-    }
-    if (huge || __ballot(!(m <= limit))) {
-      refer(x, lane);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) add<false>(x[i], true);
-    }
+    for (int i = 0; i < N; ++i) add<false>(x[i], true);
+  }
+
+  // The wave's first logits, those of lane l at first + l N. Past the end lanes have -inf.
+  __device__ __forceinline__ void begin(const float (&x)[N], int64_t first, int64_t end, int top, int lane) {
+    refer(x, lane);
     if (top) {
-      if (!least) seed(x, first, end, top, lane);
-      else if (__ballot(!(m <= kth))) pick(x, first, end, top);
+      seed(x, first, end, top, lane);
+      kth = value_of(least);
     }
+    set_bound(top);
+  }
+
+  // Later ones that need a look, all above the indices of earlier ones.
+  __device__ __forceinline__ void look(const float (&x)[N], int64_t first, int64_t end, int top, int lane) {
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = __builtin_elementwise_maximum(m, x[i]);
+    if (huge || __ballot(!(m <= limit))) refer(x, lane);
+    else add_all(x);
+    if (top) {
+      if (__ballot(!(m <= kth))) pick(x, first, end, top);
+      kth = value_of(least);
+    }
+    set_bound(top);
+  }
+
+  __device__ __forceinline__ void set_bound(int top) {
     // (NaN while there is no reference or there are not k)
     bound = huge || c == -INFINITY || (top && kth != kth) ? __builtin_nanf("") : top ? fminf(limit, kth) : limit;
   }
@@ -282,24 +298,24 @@ struct Wave {
 
   // The first logits: the lanes' best keys at once, then the others that beat the k-th of those.
   __device__ __forceinline__ void seed(const float (&x)[N], int64_t first, int64_t end, int top, int lane) {
-    uint64_t key[N], best = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
+    auto key = [&](int i) {
       const int64_t index = first + lane * N + i;
-      key[i] = index < end ? key_of(x[i], (uint32_t)index) : 0;
-      best = larger(best, key[i]);
-    }
+      return index < end ? key_of(x[i], (uint32_t)index) : 0;
+    };
+    uint64_t best = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) best = larger(best, key(i));
     list = sorted(best, lane);
     least = read_lane(list, top - 1);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      uint64_t hits = __ballot(key[i] > least && key[i] != best);
+      const uint64_t k = key(i);
+      uint64_t hits = __ballot(k > least && k != best);
       while (hits) {
-        put(read_lane(key[i], __builtin_ctzll(hits)), top);
+        put(read_lane(k, __builtin_ctzll(hits)), top);
         hits &= hits - 1;
       }
     }
-    kth = value_of(least);
   }
 
   // Later ones: a logit equal to the k-th best comes behind it.
@@ -315,7 +331,6 @@ struct Wave {
         hits &= hits - 1;
       }
     }
-    kth = value_of(least);
   }
 
   __device__ __forceinline__ void put(uint64_t key, int top) {
@@ -332,13 +347,18 @@ struct Wave {
   }
 };
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void scores_kernel(Args p, int64_t per, int vec) {
-  constexpr int N = 16 / sizeof(T), U = 4;
-  __shared__ uint64_t keys[kWaves * kMaxTop];
-  __shared__ Stats stats[kWaves];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
+// W waves a row (or a part of one), kWaves / W rows a workgroup.
+template <typename T, int W>
+__global__ __launch_bounds__(kThreads, 6) void scores_kernel(Args p, int64_t per, int vec) {
+  constexpr int N = 16 / sizeof(T);
+  constexpr int64_t STEP = 64 * W * N;
+  __shared__ uint64_t keys[W > 1 ? W * kMaxTop : 1];
+  __shared__ Stats stats[W];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % W;
+  const int row = W == kWaves ? blockIdx.x / p.parts : blockIdx.x * (kWaves / W) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / W;
+  const int part = W == kWaves ? blockIdx.x % p.parts : 0;
+  static_assert(W == kWaves || W == 1, "a workgroup's barriers are one row's");
+  if (row >= p.t) return;
   const T* x = (const T*)p.x + row * p.ld;
   const int64_t begin = part * per, end = min(begin + per, p.v);
   Wave<N> w;
@@ -349,55 +369,82 @@ __global__ __launch_bounds__(kThreads) void scores_kernel(Args p, int64_t per, i
       f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
     }
   };
-  int64_t i0 = begin + wave * 64 * N;
-  if (vec) {
-    constexpr int64_t STEP = kThreads * N;
-    const T* at = x + lane * N;
-    const int64_t whole = end - ((U - 1) * STEP + 64 * N);  // i0 up to which U vectors are whole
-    u32x4 next[U];
-    if (i0 <= whole) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) next[u] = *reinterpret_cast<const u32x4*>(at + i0 + u * STEP);
-    }
-    while (i0 <= whole) {
-      u32x4 v[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = next[u];
-      if (i0 + U * STEP <= whole) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) next[u] = *reinterpret_cast<const u32x4*>(at + i0 + (U + u) * STEP);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float f[N];
-        unpack(v[u], f);
-        w.take(f, i0 + u * STEP, end, p.top, lane);
-      }
-      i0 += U * STEP;
-    }
-  }
-  for (; i0 < end; i0 += kThreads * N) {
-    const int64_t i = i0 + lane * N;
-    float f[N];
+  // 16 bytes of a lane's logits, -inf past the end
+  auto load = [&](int64_t i) {
+    u32x4 v;
     if (vec && i + N <= end) {
-      unpack(*reinterpret_cast<const u32x4*>(x + i), f);
+      v = *reinterpret_cast<const u32x4*>(x + i);
     } else {
+      uint32_t word[4];
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        f[e] = -INFINITY;
-        if (i + e < end) f[e] = N == 8 ? bf16_to_f32(((const bf16_t*)x)[i + e]) : ((const float*)x)[i + e];
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (N == 8) {
+          const uint32_t lo = i + 2 * e < end ? x[i + 2 * e] : 0xFF80u, hi = i + 2 * e + 1 < end ? x[i + 2 * e + 1] : 0xFF80u;
+          word[e] = lo | hi << 16;
+        } else {
+          word[e] = i + e < end ? __float_as_uint(x[i + e]) : 0xFF800000u;
+        }
+      }
+      v = u32x4{word[0], word[1], word[2], word[3]};
+    }
+    return v;
+  };
+  int64_t i0 = begin + wave * 64 * N;
+  if (i0 < end) {
+    float f[N];
+    unpack(load(i0 + lane * N), f);
+    w.begin(f, i0, end, p.top, lane);
+    i0 += STEP;
+  }
+  if (vec) {
+    const T* at = x + lane * N;
+    const int64_t whole = end - (STEP + 64 * N);  // i0 up to which two vectors are whole
+    u32x4 next[2];
+    if (i0 <= whole) {
+      next[0] = *reinterpret_cast<const u32x4*>(at + i0);
+      next[1] = *reinterpret_cast<const u32x4*>(at + i0 + STEP);
+    }
+    for (; i0 <= whole; i0 += 2 * STEP) {
+      const u32x4 v[2] = {next[0], next[1]};
+      if (i0 + 2 * STEP <= whole) {
+        next[0] = *reinterpret_cast<const u32x4*>(at + i0 + 2 * STEP);
+        next[1] = *reinterpret_cast<const u32x4*>(at + i0 + 3 * STEP);
+      }
+      float f[2][N];
+      unpack(v[0], f[0]);
+      unpack(v[1], f[1]);
+      const bool hot = w.hot(f[0]) | w.hot(f[1]);
+      if (!hot) {
+        w.add_all(f[0]);
+        w.add_all(f[1]);
+      } else {
+#pragma unroll 1
+        for (int u = 0; u < 2; ++u) {
+          float g[N];
+#pragma unroll
+          for (int e = 0; e < N; ++e) g[e] = u ? f[1][e] : f[0][e];
+          w.look(g, i0 + u * STEP, end, p.top, lane);
+        }
       }
     }
-    w.take(f, i0, end, p.top, lane);
   }
-  if (lane < p.top) keys[wave * p.top + lane] = w.list;
-  const Stats mine = w.stats();
-  if (lane == 0) stats[wave] = mine;
-  __syncthreads();
-  if (wave) return;
-  Stats s = stats[0];
-  for (int i = 1; i < kWaves; ++i) join(s, stats[i]);
-  const uint64_t list = p.top ? best_of<8>(keys, kWaves, p.top, lane) : 0;
+  for (; i0 < end; i0 += STEP) {
+    float f[N];
+    unpack(load(i0 + lane * N), f);
+    w.look(f, i0, end, p.top, lane);
+  }
+  Stats s = w.stats();
+  uint64_t list = w.list;
+  if constexpr (W > 1) {
+    if (lane < p.top) keys[wave * p.top + lane] = list;
+    if (lane == 0) stats[wave] = s;
+    __syncthreads();
+    if (wave) return;
+    s = stats[0];
+    for (int i = 1; i < W; ++i) join(s, stats[i]);
+    if (p.top > 8) list = best_of<W>(keys, W, p.top, lane);
+    else if (p.top) list = sorted(lane % 8 < p.top ? keys[lane / 8 * p.top + lane % 8] : 0, lane);
+  }
   if (p.parts == 1) {
     finish<T>(p, row, s, list, lane);
     return;
@@ -477,9 +524,17 @@ extern "C" int ff_token_scores(const void* logits, int f32, int64_t ld, const in
   const int64_t per = (chunks + parts - 1) / parts * unit;
   const int vec = ff_aligned(logits, 16) && ld % unit == 0;
   hipStream_t s = (hipStream_t)stream;
-  const dim3 grid((unsigned)(t * parts));
-  if (f32) hipLaunchKernelGGL((scores_kernel<float>), grid, dim3(kThreads), 0, s, p, per, vec);
-  else hipLaunchKernelGGL((scores_kernel<bf16_t>), grid, dim3(kThreads), 0, s, p, per, vec);
+  // A row a wave where there are rows for every SIMD twice and they are short: no lists to join, and one
+  // to begin instead of eight.
+  if (parts == 1 && t >= 2048 && v <= 32768) {
+    const dim3 grid((unsigned)((t + kWaves - 1) / kWaves));
+    if (f32) hipLaunchKernelGGL((scores_kernel<float, 1>), grid, dim3(kThreads), 0, s, p, per, vec);
+    else hipLaunchKernelGGL((scores_kernel<bf16_t, 1>), grid, dim3(kThreads), 0, s, p, per, vec);
+  } else {
+    const dim3 grid((unsigned)(t * parts));
+    if (f32) hipLaunchKernelGGL((scores_kernel<float, kWaves>), grid, dim3(kThreads), 0, s, p, per, vec);
+    else hipLaunchKernelGGL((scores_kernel<bf16_t, kWaves>), grid, dim3(kThreads), 0, s, p, per, vec);
+  }
   if (parts > 1) {
     if (f32) hipLaunchKernelGGL((join_kernel<float>), dim3((unsigned)t), dim3(256), 0, s, p);
     else hipLaunchKernelGGL((join_kernel<bf16_t>), dim3((unsigned)t), dim3(256), 0, s, p);

@@ -15,7 +15,6 @@ from typing import NamedTuple, Optional
 import torch
 
 from ._lib import call, entry, stream
-from .linear import check_here
 
 BF16, F32 = torch.bfloat16, torch.float32
 MAX_TOP = 64
@@ -54,19 +53,23 @@ def token_scores(logits, tokens, top=0):
     assert tokens.dtype == torch.int64 and tokens.dim() in (1, 2) and tokens.shape[0] == t, (tokens.shape, tokens.dtype)
     n = 1 if tokens.dim() == 1 else tokens.shape[1]
     assert n <= 65536, n
-    check_here(logits, tokens)
-    if logits.stride(1) != 1 and v > 1:
-        logits = logits.contiguous()
-    logprobs = logits.new_empty(tokens.shape, dtype=F32)
-    entropy = logits.new_empty((t,), dtype=F32)
-    top_logprobs = logits.new_empty((t, top), dtype=F32) if top else None
-    top_ids = logits.new_empty((t, top), dtype=torch.int32) if top else None
+    here = logits.get_device()
+    assert here == tokens.get_device() >= 0, f"logits on {logits.device}, tokens on {tokens.device}"
+    assert torch._C._cuda_getDevice() == here, f"tensors on GPU {here}, which is not the current one"
+    ld, step = logits.stride()
+    if step != 1 and v > 1:
+        logits, ld = logits.contiguous(), v
+    strides = tokens.stride()
+    logprobs = torch.empty_like(tokens, dtype=F32, memory_format=torch.contiguous_format)
+    entropy = logits.new_empty(t, dtype=F32)
+    top_logprobs = logits.new_empty(t, top, dtype=F32) if top else None
+    top_ids = logits.new_empty(t, top, dtype=torch.int32) if top else None
     need = scores_workspace(t, v, top)
-    ws = logits.new_empty((need,), dtype=torch.uint8) if need else None
-    entry("ff_token_scores")(logits.data_ptr(), logits.dtype == F32, logits.stride(0), tokens.data_ptr(), tokens.stride(0),
-                             tokens.stride(-1), logprobs.data_ptr(), entropy.data_ptr(),
-                             top_logprobs.data_ptr() if top else 0, top_ids.data_ptr() if top else 0, t, v, n, top,
-                             0 if ws is None else ws.data_ptr(), need, stream())
+    ws = logits.new_empty(need, dtype=torch.uint8) if need else None
+    entry("ff_token_scores")(logits.data_ptr(), logits.dtype == F32, ld, tokens.data_ptr(), strides[0], strides[-1],
+                             logprobs.data_ptr(), entropy.data_ptr(), top_logprobs.data_ptr() if top else 0,
+                             top_ids.data_ptr() if top else 0, t, v, n, top, 0 if ws is None else ws.data_ptr(), need,
+                             stream())
     return TokenScores(logprobs, entropy, top_logprobs, top_ids)
 
 

@@ -52,7 +52,7 @@ def _check(logits, tokens, top):
 @gpu_test
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("t,v,n,top", [(1, 1, 1, 1), (1, 7, 3, 7), (3, 100, 2, 64), (2, 511, 1, 0), (5, 4099, 4, 20),
-                                       (1, 20011, 1, 5), (300, 65, 2, 3), (257, 200, 1, 33), (2, 40000, 8, 1)])
+                                       (1, 20011, 1, 5), (300, 65, 2, 3), (257, 200, 1, 33), (2, 40000, 8, 1), (2049, 70, 1, 9)])
 def test_scores(gpu, dtype, t, v, n, top):
     l = (torch.randn(t, v, generator=_g(v)) * 3).to(dtype)           # bf16 logits tie often
     tokens = torch.randint(0, v, (t, n), generator=_g(n))
@@ -93,6 +93,8 @@ def test_scores_special_rows(gpu, dtype, v):
     l[18, :v // 2], l[18, v // 2:] = low, -low
     l = l.to(dtype)
     tokens = torch.tensor([0, 1, 37, v - 1, v, -1, -100, 7, 1 << 40]).repeat(19, 1)
+    if v == 60:                                      # a row a wave
+        l, tokens = l.repeat(108, 1), tokens.repeat(108, 1)
     for top in (0, 1, 20, min(v, 64)):
         _check(l, tokens, top)
 
