@@ -35,6 +35,7 @@ struct Args {
   bf16_t* y;
   float* part_o;   // (items, BM, D) unnormalised sums of split tiles
   float2* part_s;  // (items, BM) their reference (log2) and denominator
+  int2* part_of;   // (rows) where a row (token, head) begins there, and its splits (1: it is done)
   int hk, group, lbm;  // BM = 1 << lbm rows a tile
   int least, budget;  // 64-key blocks are dealt so that about so many items per head come out; 0: no tile is split
   int items;   // items per head that the grid holds
@@ -50,7 +51,8 @@ __device__ __forceinline__ f32x4 mfma_bf16(const bf16x8& a, const u32x4& b, cons
 // Every sequence's rows make ceil(rows / BM) tiles, and every tile is split into as many
 // key ranges as its sequence's blocks take chunks. A chunk is the share of all blocks
 // that gives `budget` items, `least` blocks at least. All workgroups compute the
-// same list from the lengths; a sequence's last tiles, which see the most keys, come first. Rows behind the last sequence are a sequence without keys.
+// same list from the lengths; a sequence's last tiles, which see the most keys, come first.
+// A split's rows go to the workspace, with a note for each row where its splits are. Rows behind the last sequence are a sequence without keys.
 
 struct Seq {
   int row0, n;    // first row (token) and rows
@@ -81,40 +83,41 @@ __device__ __forceinline__ int splits_of(int blocks, int chunk) {
   return max(1, blocks / chunk + (blocks % chunk != 0));
 }
 
-// Blocks of a chunk: the share of all blocks that gives `budget` items, or as many more as keep the
-// items within it (one round of the GPU's workgroups; a few of a second would take as long).
-__device__ __forceinline__ int chunk_of(const Args& p, int lane) {
-  if (!p.budget) return INT_MAX;
-  int total = 0;
-  for (int b0 = 0; b0 <= p.a.batch; b0 += 64) {
-    const Seq s = seq_of(p, b0 + lane);
-    total += s.tiles * s.blocks;
-  }
-  total = __builtin_amdgcn_readlane(wave_scan(total), 63);
-  int chunk = max(p.least, (total + p.budget - 1) / p.budget);
-  for (int i = 0; i < 3; ++i) {
-    int items = 0;
-    for (int b0 = 0; b0 <= p.a.batch; b0 += 64) {
-      const Seq s = seq_of(p, b0 + lane);
-      items += s.tiles * splits_of(s.blocks, chunk);
-    }
-    items = __builtin_amdgcn_readlane(wave_scan(items), 63);
-    if (items <= p.budget) break;
-    chunk = (int)min((int64_t)INT_MAX, ((int64_t)chunk * items + p.budget - 1) / p.budget);
-  }
-  return chunk;
-}
-
 struct Item {
   Seq s;
   int seq, tile, split, splits;
 };
 
-// Item `id` of the list.
-__device__ __forceinline__ bool find_item(const Args& p, int lane, int chunk, int id, Item* out) {
+// Item `id` of the list. The chunk is the share of all blocks that gives `budget` items, or as many
+// more as keep the items within it (one round of the GPU's workgroups; a few of a second would take as
+// long). Up to 63 sequences are read once, a lane each.
+__device__ __forceinline__ bool find_item(const Args& p, int lane, int id, Item* out) {
+  const Seq mine = seq_of(p, lane);
+  const bool once = p.a.batch < 64;
+  auto seq = [&](int b0) { return once ? mine : seq_of(p, b0 + lane); };
+  int chunk = INT_MAX;
+  if (p.budget) {
+    int total = 0;
+    for (int b0 = 0; b0 <= p.a.batch; b0 += 64) {
+      const Seq s = seq(b0);
+      total += s.tiles * s.blocks;
+    }
+    total = __builtin_amdgcn_readlane(wave_scan(total), 63);
+    chunk = max(p.least, (total + p.budget - 1) / p.budget);
+    for (int i = 0; i < 3; ++i) {
+      int items = 0;
+      for (int b0 = 0; b0 <= p.a.batch; b0 += 64) {
+        const Seq s = seq(b0);
+        items += s.tiles * splits_of(s.blocks, chunk);
+      }
+      items = __builtin_amdgcn_readlane(wave_scan(items), 63);
+      if (items <= p.budget) break;
+      chunk = (int)min((int64_t)INT_MAX, ((int64_t)chunk * items + p.budget - 1) / p.budget);
+    }
+  }
   int base = 0;
   for (int b0 = 0; b0 <= p.a.batch; b0 += 64) {
-    const Seq s = seq_of(p, b0 + lane);
+    const Seq s = seq(b0);
     const int splits = splits_of(s.blocks, chunk), n = s.tiles * splits;
     const int sum = wave_scan(n), first = base + sum - n;
     const uint64_t hit = __ballot(id >= first && id < first + n);
@@ -329,7 +332,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void few_rows_kernel(Args
     if (it.seq >= p.a.t) return;
     it.s = seq_of(p, it.seq);
   } else {
-    if (!find_item(p, lane, chunk_of(p, lane), id, &it)) return;
+    if (!find_item(p, lane, id, &it)) return;
   }
   const int64_t page_rows = (int64_t)p.hk << p.a.lps, head_rows = (int64_t)head << p.a.lps;
   const int in_page = (1 << p.a.lps) - 1;
@@ -513,15 +516,17 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void few_rows_kernel(Args
       sum += sd[w * 16 + r] * wt;
       fma4(acc, *reinterpret_cast<const f32x4*>(so + (w * 16 + r) * LDO + d0), wt);
     }
+    const int rr = it.tile * 16 + r, query = DECODE ? 0 : rr / p.group;
+    const int64_t to = (int64_t)(it.s.row0 + query) * (p.hk * p.group) + head * p.group + rr - query * p.group;
     if (it.splits == 1) {
-      const int rr = it.tile * 16 + r, query = DECODE ? 0 : rr / p.group;
       const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-      bf16_t* to = p.y + ((int64_t)(it.s.row0 + query) * (p.hk * p.group) + head * p.group + rr - query * p.group) * D;
-      *reinterpret_cast<u32x2*>(to + d0) = pack4_bf16(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+      *reinterpret_cast<u32x2*>(p.y + to * D + d0) = pack4_bf16(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+      if (!DECODE && p.budget && d0 == 0) p.part_of[to] = int2{0, 1};
     } else {
       const int64_t at = ((int64_t)id * p.hk + head) * 16 + r;
       *reinterpret_cast<f32x4*>(p.part_o + at * D + d0) = acc;
       if (d0 == 0) p.part_s[at] = float2{mx, sum};
+      if (d0 == 0 && it.split == 0) p.part_of[to] = int2{(int)at, it.splits};
     }
   }
 }
@@ -608,7 +613,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void many_rows_kernel(Arg
   const int r32 = lane & 31, h = lane >> 5;
   const int head = (int)blockIdx.x % p.hk, id = (int)blockIdx.x / p.hk;
   Item it;
-  if (!find_item(p, lane, chunk_of(p, lane), id, &it)) return;
+  if (!find_item(p, lane, id, &it)) return;
   const int rows = it.s.n * p.group, row0 = (it.tile << p.lbm) + wave * 32;
   const int shift = it.s.len - it.s.n;  // position of query 0
   const int kend = min(it.s.keys, shift + min(rows - 1, ((it.tile + 1) << p.lbm) - 1) / p.group + 1);
@@ -862,16 +867,17 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void many_rows_kernel(Arg
   // lane (h, r32) holds dims 32 dt + 8 a + 4 h .. + 3 of its row
   const float sum = sum_halves(den);
   if (row >= rows) return;
+  const int64_t to = (int64_t)(it.s.row0 + row / p.group) * (p.hk * p.group) + head * p.group + row % p.group;
   if (it.splits == 1) {
     const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-    bf16_t* to = p.y + ((int64_t)(it.s.row0 + row / p.group) * (p.hk * p.group) + head * p.group + row % p.group) * D;
 #pragma unroll
     for (int i = 0; i < 4 * DTN; ++i) {
       const f32x16& x = o[i >> 2];
       const int a = 4 * (i & 3);
-      *reinterpret_cast<u32x2*>(to + 8 * i + 4 * h) =
+      *reinterpret_cast<u32x2*>(p.y + to * D + 8 * i + 4 * h) =
           pack4_bf16(x[a] * inv, x[a + 1] * inv, x[a + 2] * inv, x[a + 3] * inv);
     }
+    if (p.budget && h == 0) p.part_of[to] = int2{0, 1};
   } else {
     const int64_t at = (((int64_t)id * p.hk + head) << p.lbm) + (row - (it.tile << p.lbm));
 #pragma unroll
@@ -881,6 +887,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void many_rows_kernel(Arg
       *reinterpret_cast<f32x4*>(p.part_o + at * D + 8 * i + 4 * h) = f32x4{x[a], x[a + 1], x[a + 2], x[a + 3]};
     }
     if (h == 0) p.part_s[at] = float2{m, sum};
+    if (h == 0 && it.split == 0) p.part_of[to] = int2{(int)at, it.splits};
   }
 }
 
@@ -895,76 +902,43 @@ __global__ __launch_bounds__(256) void join_kernel(Args p) {
   constexpr int LPR = D / 4, PER = 64 / LPR, GROUPS = WIDE ? 4 * PER : 1;
   __shared__ f32x4 parts[WIDE ? 256 : 1];
   __shared__ float2 stats[WIDE ? GROUPS : 1];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int heads = p.hk * p.group, rows = p.a.t * heads;
   const int group = threadIdx.x / LPR, dim = threadIdx.x % LPR * 4;
-  const int r0 = WIDE ? blockIdx.x : ((int)blockIdx.x * 4 + wave) * PER;  // the wave's first row
-  const int row = WIDE ? r0 : r0 + lane / LPR;
-  const int chunk = chunk_of(p, lane);
-  // this lane's row: its first partial row, and its splits
-  int64_t at0 = 0;
-  int splits = 1, from = 0, to = 0, first = 0, tiles = 0, sp = 1;  // (of the sequence with tokens from .. to - 1)
-#pragma unroll
-  for (int i = 0; i < (WIDE ? 1 : PER); ++i) {
-    const int r = r0 + i, token = r / heads, hq = r % heads;
-    if (r >= rows) break;
-    if (token >= to) {
-      int base = 0;
-      to = token + 1, sp = 1;  // (starts that do not rise: a row of no sequence)
-      for (int b0 = 0; b0 <= p.a.batch; b0 += 64) {
-        const Seq s = seq_of(p, b0 + lane);
-        const int each = splits_of(s.blocks, chunk), n = s.tiles * each, sum = wave_scan(n);
-        const uint64_t hit = __ballot(token >= s.row0 && token < s.row0 + s.n);
-        if (hit) {
-          const int src = __builtin_ctzll(hit);
-          from = __builtin_amdgcn_readlane(s.row0, src);
-          to = from + __builtin_amdgcn_readlane(s.n, src);
-          sp = __builtin_amdgcn_readlane(each, src);
-          tiles = __builtin_amdgcn_readlane(s.tiles, src);
-          first = base + __builtin_amdgcn_readlane(sum - n, src);
-          break;
-        }
-        base += __builtin_amdgcn_readlane(sum, 63);
-      }
-    }
-    const int in = (token - from) * p.group + hq % p.group;
-    const int item = first + (tiles - 1 - (in >> p.lbm)) * sp;
-    const bool mine = sp > 1 && item >= 0 && item + sp <= p.items && row == r;
-    at0 = mine ? (((int64_t)item * p.hk + hq / p.group) << p.lbm) + (in & ((1 << p.lbm) - 1)) : at0;
-    splits = mine ? sp : splits;
-  }
-  if (WIDE ? splits == 1 : !__ballot(splits > 1)) return;
+  const int row = WIDE ? blockIdx.x : (int)blockIdx.x * 4 * PER + group;
+  if (row >= p.a.t * p.hk * p.group) return;
+  const int2 of = p.part_of[row];
+  const int64_t at0 = of.x;
+  const int splits = of.y;
   const int64_t step = (int64_t)p.hk << p.lbm;  // from a split's row to the next one's
+  // (starts that do not rise leave rows that no tile has)
+  if (splits <= 1 || at0 < 0 || at0 + (splits - 1) * step >= ((int64_t)p.items * p.hk) << p.lbm) return;
   float m = -INFINITY, sum = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  if (splits > 1) {
-    for (int i0 = WIDE ? group : 0; i0 < splits; i0 += 4 * GROUPS) {
-      float2 st[4];
-      f32x4 o[4];
+  for (int i0 = WIDE ? group : 0; i0 < splits; i0 += 4 * GROUPS) {
+    float2 st[4];
+    f32x4 o[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool there = i0 + i * GROUPS < splits;
-        const int64_t at = at0 + (there ? i0 + i * GROUPS : i0) * step;
-        st[i] = p.part_s[at];
-        o[i] = *reinterpret_cast<const f32x4*>(p.part_o + at * D + dim);
-        if (!there) st[i] = float2{-INFINITY, 0.f};
-      }
-      const float mnew = fmaxf(fmaxf(m, fmaxf(st[0].x, st[1].x)), fmaxf(st[2].x, st[3].x));
-      const float mref = mnew == -INFINITY ? 0.f : mnew;
-      const float alpha = __builtin_amdgcn_exp2f(m - mref);
-      sum *= alpha;
-      acc = acc * alpha;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // (a split without keys, and one read twice in place of none, count for nothing)
-        const float w = __builtin_amdgcn_exp2f(st[i].x - mref);
-        if (st[i].x != -INFINITY) {
-          sum = __builtin_fmaf(st[i].y, w, sum);
-          fma4(acc, o[i], w);
-        }
-      }
-      m = mnew;
+    for (int i = 0; i < 4; ++i) {
+      const bool there = i0 + i * GROUPS < splits;
+      const int64_t at = at0 + (there ? i0 + i * GROUPS : i0) * step;
+      st[i] = p.part_s[at];
+      o[i] = *reinterpret_cast<const f32x4*>(p.part_o + at * D + dim);
+      if (!there) st[i] = float2{-INFINITY, 0.f};
     }
+    const float mnew = fmaxf(fmaxf(m, fmaxf(st[0].x, st[1].x)), fmaxf(st[2].x, st[3].x));
+    const float mref = mnew == -INFINITY ? 0.f : mnew;
+    const float alpha = __builtin_amdgcn_exp2f(m - mref);
+    sum *= alpha;
+    acc = acc * alpha;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // (a split without keys, and one read twice in place of none, count for nothing)
+      const float w = __builtin_amdgcn_exp2f(st[i].x - mref);
+      if (st[i].x != -INFINITY) {
+        sum = __builtin_fmaf(st[i].y, w, sum);
+        fma4(acc, o[i], w);
+      }
+    }
+    m = mnew;
   }
   if (WIDE) {
     parts[threadIdx.x] = acc;
@@ -984,7 +958,6 @@ __global__ __launch_bounds__(256) void join_kernel(Args p) {
       fma4(acc, parts[i * LPR + threadIdx.x], w);
     }
   }
-  if (splits == 1) return;
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   *reinterpret_cast<u32x2*>(p.y + (int64_t)row * D + dim) =
       pack4_bf16(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
@@ -1024,6 +997,7 @@ Plan plan_of(int64_t t, int64_t batch, bool starts, int64_t hk, int64_t group, i
   // No splits where a sequence's keys are one chunk whatever its length is, nor where there
   // are tiles enough whatever the starts are (one sequence: as many as workgroups).
   if ((capacity + 63) / 64 > p.least && (rows >> p.lbm) < (batch == 1 ? 1 : 2) * budget) p.budget = (int)budget;
+  if (((tiles + budget) * hk << p.lbm) > INT32_MAX) p.budget = 0;  // (rows of the splits are counted in 32 bits)
   p.items = tiles + p.budget;
   return p;
 }
@@ -1039,8 +1013,8 @@ int check_sizes(const char* what, const ff_paged_cache* c, int64_t hq, int64_t w
   return FF_OK;
 }
 
-int64_t workspace_of(const Plan& p, int64_t hk, int64_t d) {
-  return p.budget ? ((p.items * hk) << p.lbm) * (d * 4 + 8) : 0;
+int64_t workspace_of(const Plan& p, int64_t t, int64_t hq, int64_t hk, int64_t d) {
+  return p.budget ? ((p.items * hk) << p.lbm) * (d * 4 + 8) + t * hq * 8 : 0;
 }
 
 }  // namespace
@@ -1058,7 +1032,7 @@ extern "C" int ff_attention_paged_workspace(const ff_paged_cache* cache, int64_t
   st = check_sizes("ff_attention_paged_workspace", cache, hq, width, batch, t);
   if (st != FF_OK) return st;
   *bytes = workspace_of(plan_of(t, batch, starts, cache->hk, hq / cache->hk, cache->d, cache->fp8 != 0,
-                                width * cache->page_size), cache->hk, cache->d);
+                                width * cache->page_size), t, hq, cache->hk, cache->d);
   return FF_OK;
 }
 
@@ -1077,7 +1051,7 @@ extern "C" int ff_attention_paged(const void* q, int64_t q_ts, int64_t q_hs, con
   const int64_t hk = cache->hk, d = cache->d;
   const bool fp8 = cache->fp8 != 0;
   const Plan plan = plan_of(t, batch, starts != nullptr, hk, hq / hk, d, fp8, width * cache->page_size);
-  const int64_t need = workspace_of(plan, hk, d);
+  const int64_t need = workspace_of(plan, t, hq, hk, d);
   FF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ff_aligned(workspace, 16)),
              "ff_attention_paged: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
   Args p;
@@ -1092,6 +1066,7 @@ extern "C" int ff_attention_paged(const void* q, int64_t q_ts, int64_t q_hs, con
   p.y = (bf16_t*)y;
   p.part_o = (float*)workspace;
   p.part_s = (float2*)((char*)workspace + ((plan.items * hk) << plan.lbm) * d * 4);
+  p.part_of = (int2*)(p.part_s + ((plan.items * hk) << plan.lbm));
   p.hk = (int)hk;
   p.group = (int)(hq / hk);
   p.lbm = plan.lbm;

@@ -132,7 +132,7 @@ def token_scores(logits, tokens, top=0):
     inside = (tok >= 0) & (tok < v)
     logprobs = torch.where(inside, lp.gather(1, tok.clamp(0, v - 1)), torch.zeros(1, dtype=F64))
     entropy = -torch.where(lp == -math.inf, torch.zeros_like(lp), lp.exp() * lp).sum(1)
-    ids = torch.where(x.isnan(), torch.full_like(x, math.inf), x)
-    order = [sorted(range(v), key=lambda j: (not bool(x[i, j].isnan()), -float(ids[i, j]), j))[:top] for i in range(t)]
-    ids = torch.tensor(order, dtype=torch.int64).reshape(t, top)
+    # falling values, NaN above them, the lowest index first among equals (both sorts keep the order of equals)
+    ids = torch.where(x.isnan(), torch.full_like(x, math.inf), x).sort(dim=1, descending=True, stable=True).indices
+    ids = ids.gather(1, x.gather(1, ids).isnan().int().sort(dim=1, descending=True, stable=True).indices)[:, :top]
     return logprobs.reshape(tokens.shape), entropy, lp.gather(1, ids), ids.to(torch.int32)
