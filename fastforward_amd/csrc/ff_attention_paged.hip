@@ -972,13 +972,35 @@ struct Plan {
   int64_t items;  // per key head
 };
 
+// 256-row tiles (one workgroup of 8 waves a CU) against 128-row ones (two or three of 4): half the loads
+// of keys and values, coarser work. Ahead where there is a tile for every CU and the table may hold
+// eight times the new tokens or more, so that tiles are equally long; at 128 dims also where there are two
+// tiles a CU; for codes at 128 dims (two workgroups a CU leave them short of registers) where the
+// table may hold four times the new tokens. us, 256 against 128 rows, 32 / 8 heads: 2048 tokens over 30700
+// positions 1021 and 1060 (64 dims 636 and 705), over 4000 194 and 181, 4096 over none 153 and 157 (64
+// dims 107 and 93); codes: 512 over 4000 59 and 64, 4096 over none 159 and 186, 2048 over none 76 and 72.
+bool wide_tiles(int64_t rows, int64_t t, int64_t batch, int64_t hk, int64_t d, int fp8, int64_t capacity) {
+  const int64_t all = rows * hk, depth = capacity * batch;
+  if (all >= 65536 && depth >= 8 * t) return true;
+  if (d == 64) return false;
+  return all >= 131072 || (fp8 && all >= 16384 && depth >= 4 * t);
+}
+
 Plan plan_of(int64_t t, int64_t batch, bool starts, int64_t hk, int64_t group, int64_t d, int fp8, int64_t capacity) {
   const int64_t rows = t * group;
   const int force = ff_tuning(FF_TUNE_PAGED_ROWS);
   Plan p = {};
+  // 16-row tiles read the cache once a tile, and a wave has a block of its own: ahead where every
+  // sequence is one tile, and while the (tile, block) pairs that the table can hold are about as many as
+  // the GPU's waves (2048; twice that for codes, whose way through registers to LDS makes the large tiles slower
+  // to begin). us, 16-row against 128-row tiles, 32 / 8 heads: 40 tokens over 1000 positions (1360 pairs) 17.3 and
+  // 19.3, 100 over 1000 (3600) 23.4 and 22.3, 100 over 4000 (13000) 54.1 and 29.5, 8 sequences of 16 over 500 (2304)
+  // 23.1 and 23.1, over 1000 (4352) 32.7 and 23.2; codes: 100 over 1000 18.6 and 24.8, 8 of 40 over 500 (5760)
+  // 33.6 and 29.5, 100 over 4000 33.5 and 34.4.
+  const int64_t pairs = (rows / 16 + batch) * hk * ((capacity + 63) / 64);
   if (force) p.kind = force - 1;
-  else if (rows <= 64 * batch || (rows * hk <= 8192 && capacity <= 512)) p.kind = 0;
-  else p.kind = rows * hk < 256 * 256 ? 1 : 2;
+  else if (rows <= 16 * batch || pairs <= (fp8 ? 5120 : 2560)) p.kind = 0;
+  else p.kind = wide_tiles(rows, t, batch, hk, d, fp8, capacity) ? 2 : 1;
   // One row a sequence, up to 768 positions, a CU for each tile: one launch. A CU takes in 64 bytes a
   // clock at most, so that longer caches are better shared by several and joined.
   const int64_t decode = (group + 15) / 16 * t;
