@@ -13,8 +13,7 @@
 // The most likely tokens: a wave's best 64 so far lie sorted in its lanes, as 64-bit keys of
 // (value, lowest index first). A vector of logits is looked at only where one of
 // them is above the wave's k-th best, or c's limit: one comparison with the smaller of the
-// two. Waves, then parts of a row, are joined by taking the best of their lists' heads
-// k times.
+// two. The lists of waves, then of a row's parts, are joined by sorts over the lanes.
 //
 // Bound by the logits' bytes: a row is read once, 16 bytes a lane and load, two loads
 // ahead. Few rows are split over workgroups, and a second launch joins their parts.
@@ -26,6 +25,10 @@ namespace {
 
 constexpr int kWaves = 8, kThreads = 64 * kWaves;
 constexpr int kMaxTop = 64;
+// Lists past this length are joined list after list by four waves, shorter ones by two sorts (one row's 64
+// parts, the whole call: 20 keys 16 us against 19 list after list, 32 keys 18.5 against 21.5; of 64 keys all
+// but the first sort would overflow: 34 us, and 49 by taking the best head 64 times).
+constexpr int kLongTop = 32;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 struct Args {
@@ -183,37 +186,30 @@ __device__ __forceinline__ uint64_t sorted(uint64_t v, int lane) {
   return v;
 }
 
-// The best `top` of the falling lists of `top` keys at `keys` (LDS), LISTS at most 8 or 64
-// of them, by one wave: entry i of the result in lane i. The best of the lists' heads `top` times.
-template <int LISTS>
-__device__ __forceinline__ uint64_t best_heads(const uint64_t* keys, int lists, int top, int lane) {
-  uint64_t out = 0;
-  int at = lane * top;
-  const int end = lane < lists ? at + top : 0;
-  uint64_t head = at < end ? keys[at] : 0, next = at + 1 < end ? keys[at + 1] : 0;
-  for (int i = 0; i < top; ++i) {
-    uint64_t best = larger(head, dpp64<kDppXor1>(head));
-    best = larger(best, dpp64<kDppXor2>(best));
-    best = larger(best, dpp64<kDppHalfMirror>(best));
-    if (LISTS > 8) {
-      best = larger(best, dpp64<kDppRowMirror>(best));
-      best = swapped<false>(best);
-      best = swapped<true>(best);
-    }
-    best = read_lane(best, 0);
-    if (lane == i) out = best;
-    if (head == best) {  // keys differ, so one lane (or all that have none left)
-      ++at;
-      head = next;
-      next = at + 1 < end ? keys[at + 1] : 0;
-    }
-  }
-  return out;
+// The best 64 of a falling list and of keys in rising order: the larger of each two is a bitonic sequence.
+__device__ __forceinline__ uint64_t merged(uint64_t falling, uint64_t rising, int lane) {
+  uint64_t v = larger(falling, rising);
+  v = keep(v, xor_rows<true>(v, lane), lane, 32);
+  v = keep(v, xor_rows<false>(v, lane), lane, 16);
+  v = keep(v, xor8(v), lane, 8);
+  v = keep(v, xor4(v), lane, 4);
+  v = keep(v, dpp64<kDppXor2>(v), lane, 2);
+  return keep(v, dpp64<kDppXor1>(v), lane, 1);
 }
 
-// The same: the lists' first keys, 64 in all, are sorted at once, and the others that beat the top-th of
-// those (2 or 3 for 20 of 64 lists) are sorted in; heads one by one only where there are more than 64 of
-// both. 64 lists of 20: the join of one row's parts 4.6 us against 7.3.
+// The best of the falling lists [from, to) of `top` keys at `keys` (LDS), by one wave: entry i in lane i.
+__device__ __forceinline__ uint64_t best_merged(const uint64_t* keys, int from, int to, int top, int lane) {
+  uint64_t v = 0;
+  for (int i = from; i < to; ++i) {
+    const uint64_t key = 63 - lane < top ? keys[i * top + 63 - lane] : 0;
+    if (read_lane(key, 63) > read_lane(v, top - 1)) v = merged(v, key, lane);
+  }
+  return v;
+}
+
+// The best of up to LISTS (8 or 64) lists: their first keys, 64 in all, are sorted at once, and the others
+// that beat the top-th of those (2 or 3 for 20 of 64 lists) are sorted in; list after list only where there
+// are more than 64 of both. 64 lists of 20: the join of one row's parts 4.6 us against 7.3.
 template <int LISTS>
 __device__ __forceinline__ uint64_t best_of(const uint64_t* keys, int lists, int top, int lane, uint64_t* pool) {
   constexpr int M = 64 / LISTS;
@@ -226,7 +222,7 @@ __device__ __forceinline__ uint64_t best_of(const uint64_t* keys, int lists, int
   int count = __popcll(__ballot(v != 0 && lane < top));
   if (lane < count) pool[lane] = v;
   for (int j = M + 1; hits; ++j) {
-    if (count + __popcll(hits) > 64) return best_heads<LISTS>(keys, lists, top, lane);
+    if (count + __popcll(hits) > 64) return best_merged(keys, 0, lists, top, lane);
     if (key > least) pool[count + __popcll(hits & ((1ull << lane) - 1))] = key;
     count += __popcll(hits);
     key = entry(j);
@@ -522,10 +518,26 @@ __global__ __launch_bounds__(256) void join_kernel(Args p) {
   }
   for (int i = threadIdx.x; i < p.parts * p.top; i += 256) keys[i] = p.part_keys[at * p.top + i];
   __syncthreads();
+  const bool all = p.top > kLongTop;  // every wave merges a quarter of the lists
+  if (all) {
+    const int from = p.parts * wave / 4, to = p.parts * (wave + 1) / 4;
+    const uint64_t list = best_merged(keys, from, to, p.top, lane);
+    if (lane < p.top && from < to) keys[from * p.top + lane] = list;  // read by this wave alone so far
+    __syncthreads();
+  }
   if (wave > 1) return;
   s = joined(s, lane);
-  if (wave) finish_tokens<T>(p, row, s, token, lane);
-  else if (p.top) finish_top(p, row, s, best_of<64>(keys, p.parts, p.top, lane, pool), lane);
+  if (wave) {
+    finish_tokens<T>(p, row, s, token, lane);
+  } else if (all) {
+    uint64_t list = 0;
+    for (int w = 0; w < 4; ++w)
+      if (p.parts * w / 4 < p.parts * (w + 1) / 4)
+        list = merged(list, 63 - lane < p.top ? keys[p.parts * w / 4 * p.top + 63 - lane] : 0, lane);
+    finish_top(p, row, s, list, lane);
+  } else if (p.top) {
+    finish_top(p, row, s, best_of<64>(keys, p.parts, p.top, lane, pool), lane);
+  }
 }
 
 // Parts of a row: enough workgroups for the GPU, 2048 logits a part at least.

@@ -100,6 +100,25 @@ def test_scores_special_rows(gpu, dtype, v):
 
 
 @gpu_test
+@pytest.mark.parametrize("top", [1, 8, 9, 20, 32, 33, 64])
+def test_scores_lists_of_many_parts(gpu, top):
+    """The likeliest tokens of rows in 64 parts: spread out, all in one part, in one wave of a part, one in
+    each part, far apart, the same few values everywhere."""
+    v = 140003
+    l = torch.randn(8, v, generator=_g(9))
+    l[1] = torch.linspace(4, -4, v)
+    l[2] = torch.linspace(-4, 4, v)
+    l[3, 70000:70300] += 9
+    l[4, ::2189] += 9
+    l[5] = -torch.arange(v) % 37 * 0.25
+    for at in range(0, 80):
+        l[6, 1024 * at] += 20 + 0.01 * at
+    l[7, 100000:100064] += 9 + torch.randperm(64, generator=_g(1)) * 0.125
+    for dtype in (F32, BF16):
+        _check(l.to(dtype), torch.arange(8)[:, None], top)
+
+
+@gpu_test
 def test_scores_near_certain(gpu):
     """log p of a token that is all but certain, to 32-bit precision: -log1p of a small sum."""
     from fastforward_amd.scores import token_scores
