@@ -707,19 +707,25 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void many_rows_kernel(Arg
     }
   };
   auto load = [&](int b, const Entries& n) {
-    const uint64_t ok = keys_there(b, n);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int c0 = (i * NW + wave) * 64;  // the wave's first chunk; all of them are of one 16-key group
       const int key0 = c0 / CK & 63, key = key0 + lane / CK;
-      const bool values = c0 >= 64 * CK, there = ok >> key & 1;
+      const bool values = c0 >= 64 * CK;
       const int64_t at = first_row(b, key0 >> 4, n) + (key & 15);
       code[i] = *reinterpret_cast<const u32x4*>((values ? p.v : p.k) + at * D + 16 * (lane % CK));
       byte[i] = (values ? p.vs : p.ks)[at];
-      if (!there) code[i] = u32x4{0, 0, 0, 0}, byte[i] = 0;
     }
   };
-  auto store = [&](int buf) {
+  auto store = [&](int buf, uint64_t there) {
+    if (there != ~0ull) {  // nothing is read as zero (waits for the loads here alone)
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const bool it = there >> (((i * NW + wave) * 64 / CK & 63) + lane / CK) & 1;
+        code[i] = it ? code[i] : u32x4{0, 0, 0, 0};
+        byte[i] = it ? byte[i] : 0;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int c0 = (i * NW + wave) * 64, key = (c0 / CK & 63) + lane / CK, chunk = 2 * (lane % CK);
@@ -749,7 +755,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void many_rows_kernel(Arg
     ok = keys_there(b0, ahead);
     if constexpr (FP8) {
       load(b0, ahead);
-      store(0);
+      store(0, ok);
     } else {
       issue(b0, 0, ahead);
     }
@@ -765,7 +771,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void many_rows_kernel(Arg
     const int kb = 64 * b, buf = (b - b0) % NS;
     if constexpr (FP8) {
       barrier_lds();  // block b is there for every wave, block b - 1 no longer read
-      if (b + 1 < b1) store(buf ^ 1);
+      if (b + 1 < b1) store(buf ^ 1, ok1);
     } else {
       if (NS == 3 && b + 1 < b1) wait_vmcnt<TASKS * PI>();
       else wait_vmcnt<0>();
