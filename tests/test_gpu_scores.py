@@ -18,9 +18,14 @@ def _g(seed):
     return torch.Generator().manual_seed(seed)
 
 
-def _check(logits, tokens, top):
+def _check(logits, tokens, top, times=1):
+    """With ``times``, the rows that many times over in the call."""
     from fastforward_amd.scores import token_scores
-    got = token_scores(logits.to(DEV), tokens.to(DEV), top=top)
+    got = token_scores(logits.to(DEV).repeat(times, 1), tokens.to(DEV).repeat(times, *[1] * (tokens.dim() - 1)), top=top)
+    if times > 1:
+        for x in got[:4 if top else 2]:
+            assert torch.equal(x.view(torch.int32).reshape(times, -1), x.view(torch.int32).reshape(times, -1)[:1].expand(times, -1))
+    got = type(got)(*(x if x is None else x[:logits.shape[0]] for x in got))
     logprobs, entropy, top_logprobs, top_ids = S.token_scores(logits, tokens, top)
     assert got.logprobs.shape == tokens.shape and got.entropy.shape == (logits.shape[0],)
     # log p = (x - m) - log1p(r): the difference's rounding 2^-24 of it; r is a sum of at most v / 512
@@ -116,6 +121,42 @@ def test_scores_lists_of_many_parts(gpu, top):
     l[7, 100000:100064] += 9 + torch.randperm(64, generator=_g(1)) * 0.125
     for dtype in (F32, BF16):
         _check(l.to(dtype), torch.arange(8)[:, None], top)
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("v,times", [(26003, 13), (26000, 13), (4003, 103)])
+def test_scores_long_rows(gpu, dtype, v, times):
+    """Rows that one workgroup, or one wave, reads in many steps: the likeliest early, late, in one wave's share,
+    equal ones and both zeros across waves, NaN and infinities late, rising and falling rows, nothing at first."""
+    inf, low = math.inf, torch.finfo(dtype).min
+    l = torch.randn(20, v, generator=_g(v)) * 2
+    l[1] = torch.linspace(-30, 30, v)
+    l[2] = torch.linspace(30, -30, v)
+    l[3] = 0
+    l[4] = torch.where(torch.arange(v) % 3 == 0, 0.0, -0.0)
+    l[5] = -torch.arange(v) % 11 * 0.5
+    l[6, v - 70:] += 20
+    l[7, 512 * 3:512 * 3 + 64] += 12
+    l[8, ::1024] = 9.0                                # a lane's vectors of a wave, all equal
+    l[9, :v - 100] = -inf
+    l[10, :v // 2] = low
+    l[11, v - 2] = math.nan
+    l[12, v - 300] = inf
+    l[13] = -40.0
+    l[13, v - 1] = 0.0
+    l[14, v // 2:] = -inf
+    l[15] = -inf
+    l[16] = torch.where(torch.arange(v) % 2 == 0, -0.0, -1e-3)
+    l[16, v // 3] = 0.0
+    l[17, torch.arange(0, v, 97)] = 3.0 + torch.arange(0, v, 97) / v
+    l[18] = l[18] * 1e37
+    l[19] = torch.finfo(dtype).max
+    l[19, ::5] = low
+    l = l.to(dtype)
+    tokens = torch.stack([torch.zeros(20, dtype=torch.int64), l.float().nan_to_num(0).argmax(1), torch.full((20,), v - 1)], 1)
+    for top in (0, 1, 5, 20, 64):
+        _check(l, tokens, top, times)
 
 
 @gpu_test
