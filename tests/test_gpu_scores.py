@@ -160,6 +160,19 @@ def test_scores_long_rows(gpu, dtype, v, times):
 
 
 @gpu_test
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_scores_of_any_size(gpu, dtype):
+    """Logits of every magnitude and offset, the largest of a wave's first ones and later ones of another size."""
+    sizes = torch.tensor([10.0 ** i for i in range(-3, 38)])
+    l = torch.randn(41, 3001, generator=_g(8)) * sizes[:, None]
+    l = torch.cat([l, l[:30] + sizes[:30, None] * 4, l[:30] - sizes[:30, None] * 9, l.clone(), -l.abs()])
+    l[101:142, 2500:] = torch.randn(41, 501, generator=_g(7)) * sizes.flip(0)[:, None]
+    l = l.to(dtype)
+    for times in (1, 15):                             # split rows, and a row a wave
+        _check(l, torch.tensor([0, 1, 2600]).repeat(183, 1), 8, times)
+
+
+@gpu_test
 def test_scores_near_certain(gpu):
     """log p of a token that is all but certain, to 32-bit precision: -log1p of a small sum."""
     from fastforward_amd.scores import token_scores
