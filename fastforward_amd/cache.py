@@ -25,7 +25,7 @@ import torch
 from ._lib import PagedCacheStruct, call, entry, stream
 
 BF16, E4M3, I32 = torch.bfloat16, torch.float8_e4m3fn, torch.int32
-_ROWS = 1 << 24
+_ROWS, _POSITIONS = 1 << 24, (1 << 31) - (1 << 16)
 
 
 class PagedCache:
@@ -73,7 +73,7 @@ class PagedCache:
         one); the arguments as the C entry points take them."""
         assert table.dim() == 2 and table.dtype == I32 and table.is_contiguous(), (table.shape, table.dtype)
         batch, width = table.shape
-        assert 0 < batch <= 65536 and 0 < width and width * self.page_size < 1 << 31 and t <= _ROWS, (batch, width, t)
+        assert 0 < batch <= 65536 and 0 < width and width * self.page_size <= _POSITIONS and t <= _ROWS, (batch, width, t)
         assert lengths.shape == (batch,) and lengths.dtype == I32 and lengths.is_contiguous(), lengths.shape
         if starts is None:
             assert t == batch, f"{t} rows for {batch} sequences of one row: starts is missing"
@@ -135,7 +135,8 @@ class PagedCache:
         own (written before, its own among them). Softmax of q . k * ``scale`` (default
         1 / sqrt(head_dim)) with fp32 statistics, weights rounded to bf16 for the product
         with the values, fp32 sums. (T, heads, head_dim) bf16. A row that sees nothing, and
-        rows behind the last sequence, are zero."""
+        rows behind the last sequence, are zero. Scores are up to 2^30 in size (past it they
+        may become NaN); an infinite value that a row sees makes it infinite or NaN."""
         assert q.dim() == 3 and q.dtype == BF16, (q.shape, q.dtype)
         t, heads, d = q.shape
         assert d == self.head_dim and 0 < heads <= 65535 and heads % self.kv_heads == 0, (q.shape, self.kv_heads)

@@ -1054,7 +1054,7 @@ extern "C" int ff_attention_paged_workspace(const ff_paged_cache* cache, int64_t
   if (t == 0) return FF_OK;
   int st = check_cache("ff_attention_paged_workspace", cache);
   if (st != FF_OK) return st;
-  FF_REQUIRE(width > 0 && width <= INT32_MAX / cache->page_size && batch > 0 && batch <= 65536 && t > 0 && t <= (1 << 24),
+  FF_REQUIRE(width > 0 && width <= kMaxPositions / cache->page_size && batch > 0 && batch <= 65536 && t > 0 && t <= (1 << 24),
              "ff_attention_paged_workspace: bad sizes width=%lld batch=%lld t=%lld", (long long)width, (long long)batch,
              (long long)t);
   st = check_sizes("ff_attention_paged_workspace", cache, hq, width, batch, t);

@@ -54,6 +54,9 @@ __device__ __forceinline__ bool find_slot(const Rows& a, int row, int b, int64_t
   return (unsigned)p < (unsigned)a.pages;
 }
 
+// Positions that a table may reach: those of the blocks behind the last one, too, are counted in 32 bits.
+constexpr int64_t kMaxPositions = INT32_MAX - 65535;
+
 // Host checks that the entry points share.
 inline int check_cache(const char* what, const ff_paged_cache* c) {
   FF_REQUIRE(c, "%s: null pointer", what);
@@ -69,7 +72,7 @@ inline int check_rows(const char* what, const ff_paged_cache* c, const int32_t* 
   const int st = check_cache(what, c);
   if (st != FF_OK) return st;
   FF_REQUIRE(c->k && c->v && (!c->fp8 || (c->k_scale && c->v_scale)) && table && lengths, "%s: null pointer", what);
-  FF_REQUIRE(width > 0 && width <= INT32_MAX / c->page_size && batch > 0 && batch <= 65536 && t > 0 && t <= (1 << 24),
+  FF_REQUIRE(width > 0 && width <= kMaxPositions / c->page_size && batch > 0 && batch <= 65536 && t > 0 && t <= (1 << 24),
              "%s: bad sizes width=%lld batch=%lld t=%lld", what, (long long)width, (long long)batch, (long long)t);
   FF_REQUIRE(starts || batch == t, "%s: without starts every sequence has one row", what);
   FF_REQUIRE(ff_aligned(c->k, 16) && ff_aligned(c->v, 16) && ff_aligned(c->k_scale, 8) && ff_aligned(c->v_scale, 8),

@@ -544,13 +544,14 @@ int ff_moe_experts(const void* x, int64_t ldx, const float* weights, const int* 
 
 /* A paged cache: k, v (pages, hk, page_size, d), bf16 or (fp8) e4m3 codes with
  * k_scale, v_scale (pages, hk, page_size) bytes, value = code * 2^(byte - 127). page_size is
- * a power of two, 16 .. 4096, d 64 or 128; k, v 16-byte, the scales 8-byte aligned. Position p of sequence b is slot p % page_size of
- * page table[b, p / page_size], table (batch, width); lengths (batch): the positions of
- * each sequence. starts (batch + 1), rising from 0 to at most t: sequence b has rows
- * starts[b] .. starts[b + 1] - 1 of the call's t, its last positions; NULL: one row each,
- * t == batch. Rows behind the last sequence belong to none. A position past the table's
- * reach and a page outside [0, pages) hold nothing. table, lengths and starts are read by the
- * kernels alone, and whatever they hold no access leaves the buffers. */
+ * a power of two, 16 .. 4096, d 64 or 128; k, v 16-byte, the scales 8-byte aligned. Position p of
+ * sequence b is slot p % page_size of page table[b, p / page_size], table (batch, width), width *
+ * page_size at most 2^31 - 2^16; lengths (batch): the positions of each sequence. starts
+ * (batch + 1), rising from 0 to at most t: sequence b has rows starts[b] .. starts[b + 1] - 1 of
+ * the call's t, its last positions; NULL: one row each, t == batch. Rows behind the last sequence
+ * belong to none. A position past the table's reach and a page outside [0, pages) hold nothing.
+ * table, lengths and starts are read by the kernels alone, and whatever they hold no access
+ * leaves the buffers. */
 typedef struct {
   void *k, *v, *k_scale, *v_scale;
   int64_t pages, page_size, hk, d, fp8;
@@ -575,7 +576,8 @@ int ff_cache_read(const ff_paged_cache* cache, const int32_t* table, int64_t wid
  * reads key head h / (hq / hk). q (t, hq, d) bf16 with strides q_ts, q_hs. scale > 0. A row
  * that sees nothing is zero. workspace: ff_attention_paged_workspace bytes (host-only, 0:
  * none; its `starts`: whether there are any), 16-byte aligned, one per stream and per captured graph that may run beside another.
- * The sums' order depends on the sizes, lengths and starts alone. */
+ * The sums' order depends on the sizes, lengths and starts alone. Scores up to 2^30 in size (past it they may
+ * become NaN); an infinite value that a row sees makes it infinite or NaN. */
 int ff_attention_paged_workspace(const ff_paged_cache* cache, int64_t hq, int64_t width, int64_t batch, int starts,
                                  int64_t t, int64_t* bytes);
 int ff_attention_paged(const void* q, int64_t q_ts, int64_t q_hs, const ff_paged_cache* cache, int64_t hq,

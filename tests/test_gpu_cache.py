@@ -396,6 +396,7 @@ def test_refusals():
            (table.T.contiguous().T, lengths, starts), (table, lengths[:2], starts), (table, lengths.long(), starts),
            (table, lengths, starts[:3]), (table, lengths, starts.long()), (table[:2], lengths[:2], None),
            (torch.zeros(3, 1 << 27, dtype=I32, device="meta"), lengths, starts),
+           (torch.zeros(3, (1 << 27) - 4095, dtype=I32, device="meta"), lengths, starts),
            (table, lengths, starts)]                                  # the last: not on the GPU
     for args in bad:
         for call in (lambda *a: c.write(rows, rows, *a), lambda *a: c.attend(q, *a), lambda *a: c.read(*a, rows=3)):
@@ -436,6 +437,7 @@ def test_refusals_c():
 
     shared = ((dict(d=96), "head_dim"), (dict(ps=24), "page_size"), (dict(ps=8), "page_size"), (dict(ps=8192), "page_size"),
               (dict(hk=0), "bad sizes"), (dict(width=0), "bad sizes"), (dict(width=1 << 27), "bad sizes"),
+              (dict(width=(1 << 27) - 4095), "bad sizes"),
               (dict(batch=0), "bad sizes"), (dict(t=-1), "bad sizes"), (dict(t=1 << 25), "bad sizes"),
               (dict(pages=0), "bad sizes"), (dict(pages=1 << 31), "bad sizes"), (dict(k=None), "null"),
               (dict(lengths=None), "null"), (dict(fp8=1), "null"), (dict(starts=None, t=2), "starts"),
