@@ -32,6 +32,10 @@ constexpr int kMaxTop = 64;
 // parts, the whole call: 20 keys 16 us against 19 list after list, 32 keys 18.5 against 21.5; of 64 keys all
 // but the first sort would overflow: 34 us, and 49 by taking the best head 64 times).
 constexpr int kLongTop = 32;
+// Up to so many alternatives a workgroup begins with the bound that the maxima of its 32 rows of 16 lanes
+// give, longer lists with a sort of each wave's lanes (us, maxima and sort, rows of 151936: 577 rows of 20 keys 60 and 65, 64 rows
+// of 28 28.5 and 33.6, of 32 36 and 36; one row of 28 16.9 and 17.7, of 32 21.4 and 18.9).
+constexpr int kSeedTop = 28;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 struct Args {
@@ -189,6 +193,38 @@ __device__ __forceinline__ uint64_t sorted(uint64_t v, int lane) {
   return v;
 }
 
+// The same of 32-bit keys, for each half of the wave.
+__device__ __forceinline__ uint32_t keep32(uint32_t mine, uint32_t other, int lane, int bit) {
+  return lane & bit ? min(mine, other) : max(mine, other);
+}
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp32(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xF, 0xF, false);
+}
+template <bool WIDE>
+__device__ __forceinline__ uint32_t xor_rows32(uint32_t v, int lane) {
+  const auto a = WIDE ? __builtin_amdgcn_permlane32_swap(v, v, false, false) : __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  return a[lane & (WIDE ? 32 : 16) ? 0 : 1];
+}
+__device__ __forceinline__ uint32_t sorted32(uint32_t v, int lane) {
+  v = keep32(v, dpp32<kDppXor1>(v), lane, 1);
+  v = keep32(v, dpp32<kDppQuadReverse>(v), lane, 2);
+  v = keep32(v, dpp32<kDppXor1>(v), lane, 1);
+  v = keep32(v, dpp32<kDppHalfMirror>(v), lane, 4);
+  v = keep32(v, dpp32<kDppXor2>(v), lane, 2);
+  v = keep32(v, dpp32<kDppXor1>(v), lane, 1);
+  v = keep32(v, dpp32<kDppRowMirror>(v), lane, 8);
+  v = keep32(v, dpp32<kDppQuadReverse>(dpp32<kDppHalfMirror>(v)), lane, 4);
+  v = keep32(v, dpp32<kDppXor2>(v), lane, 2);
+  v = keep32(v, dpp32<kDppXor1>(v), lane, 1);
+  v = keep32(v, xor_rows32<false>(dpp32<kDppRowMirror>(v), lane), lane, 16);
+  v = keep32(v, dpp32<kDppRowRor8>(v), lane, 8);
+  v = keep32(v, dpp32<kDppQuadReverse>(dpp32<kDppHalfMirror>(v)), lane, 4);
+  v = keep32(v, dpp32<kDppXor2>(v), lane, 2);
+  v = keep32(v, dpp32<kDppXor1>(v), lane, 1);
+  return v;
+}
+
 // The best 64 of a falling list and of keys in rising order: the larger of each two is a bitonic sequence.
 __device__ __forceinline__ uint64_t merged(uint64_t falling, uint64_t rising, int lane) {
   uint64_t v = larger(falling, rising);
@@ -270,12 +306,19 @@ struct Wave {
     for (int i = 0; i < N; ++i) add<false>(x[i], true);
   }
 
-  // The wave's first logits, those of lane l at first + l N. Past the end lanes have -inf.
-  __device__ __forceinline__ void begin(const float (&x)[N], int64_t first, int64_t end, int top, int lane) {
+  // The wave's first logits, those of lane l at first + l N. Past the end lanes have -inf. `row`: upper half of
+  // a key that at least `top` of the row's (or part's) reach, 0 if there is none.
+  __device__ __forceinline__ void begin(const float (&x)[N], int64_t first, int64_t end, int top, int lane, uint32_t row) {
     refer(x, lane);
     if (top) {
-      seed(x, first, end, top, lane);
-      kth = value_of(least);
+      if (row > 0x00800000u && row < 0xFF800000u) {  // a finite one
+        raise(row, 0);
+        pick(x, first, end, top);
+        kth = fmaxf(kth, value_of(least));
+      } else {
+        seed(x, first, end, top, lane);
+        kth = value_of(least);
+      }
     }
     set_bound(top);
   }
@@ -296,7 +339,6 @@ struct Wave {
 
   // Takes over the row's bound: 2 below a key's upper half, so that equal values and both zeros stay above it.
   __device__ __forceinline__ void raise(uint32_t bound_key, int top) {
-    if (!top) return;
     const uint32_t k = bound_key - 2;
     const float v = bound_key > 2 ? __uint_as_float(k >> 31 ? k & 0x7FFFFFFFu : ~k) : __builtin_nanf("");
     kth = fmaxf(kth, v);
@@ -418,7 +460,7 @@ __global__ __launch_bounds__(kThreads, 6) void scores_kernel(Args p, int64_t per
   __shared__ uint64_t keys[W > 1 ? W * kMaxTop : 1];
   __shared__ uint64_t pool[W > 1 ? 64 : 1];
   __shared__ Stats stats[W];
-  __shared__ uint32_t row_kth, shown[kWaves];
+  __shared__ uint32_t row_kth, shown[kWaves], maxima[32];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % W;
   const int row = W == kWaves ? blockIdx.x / p.parts : blockIdx.x * (kWaves / W) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / W;
   const int part = W == kWaves ? blockIdx.x % p.parts : 0;
@@ -485,12 +527,31 @@ __global__ __launch_bounds__(kThreads, 6) void scores_kernel(Args p, int64_t per
   const bool whole_row = W == 1 || p.parts == 1;
   Token token = {0.f, false};
   if (whole_row && wave == (W > 1)) token = token_at<T>(p, row, lane);
+  float f0[N];
   if (i0 < end) {
     const u32x4 v = load(i0 + lane * N);
     load_next(i0 + STEP);
-    float f[N];
-    unpack(v, f);
-    w.begin(f, i0, end, p.top, lane);
+    unpack(v, f0);
+  }
+  uint32_t bound0 = 0;
+  if (W > 1 && p.top && p.top <= kSeedTop) {
+    uint32_t k = 0;
+    if (i0 < end) {
+      float m = f0[0];
+#pragma unroll
+      for (int i = 1; i < N; ++i) m = __builtin_elementwise_maximum(m, f0[i]);
+      k = (uint32_t)(key_of(m, 0) >> 32);
+      k = max(k, dpp32<kDppXor1>(k));
+      k = max(k, dpp32<kDppXor2>(k));
+      k = max(k, dpp32<kDppHalfMirror>(k));
+      k = max(k, dpp32<kDppRowMirror>(k));
+    }
+    if ((lane & 15) == 0) maxima[wave * 4 + lane / 16] = k;
+    __syncthreads();
+    bound0 = (uint32_t)__builtin_amdgcn_readlane((int)sorted32(maxima[lane & 31], lane), p.top - 1);
+  }
+  if (i0 < end) {
+    w.begin(f0, i0, end, p.top, lane, bound0);
     share(w);
     i0 += STEP;
   }
@@ -502,7 +563,7 @@ __global__ __launch_bounds__(kThreads, 6) void scores_kernel(Args p, int64_t per
     float f[2][N];
     unpack(v[0], f[0]);
     unpack(v[1], f[1]);
-    if (W > 1) w.raise(seen, p.top);
+    if (W > 1 && p.top) w.raise(seen, p.top);
     const bool hot = w.hot(f[0]) | w.hot(f[1]);
     if (!hot) {
       w.add_all(f[0]);
