@@ -185,6 +185,23 @@ def test_attend(gpu, tile, dtype, hk, group, d, ps, lengths, new):
 
 
 @gpu_test
+@pytest.mark.parametrize("batch,most,hk,dtype,d", [
+    (63, 1, 1, BF16, 64), (64, 1, 1, E4M3, 64), (65, 3, 2, BF16, 64), (256, 1, 1, BF16, 64), (300, 1, 2, E4M3, 128),
+    (700, 1, 1, BF16, 64), (260, 2, 1, E4M3, 64), (257, 1, 8, BF16, 64)])
+def test_attend_many_sequences(gpu, batch, most, hk, dtype, d):
+    """More sequences than a wave's lanes, short ones, none, and one that is far past the others."""
+    lengths = torch.randint(0, 60, (batch,), generator=_g(batch))
+    lengths[batch // 3] = 1500
+    lengths[batch - 1] = 130
+    new = None if most == 1 else torch.randint(0, most + 1, (batch,), generator=_g(3)).minimum(lengths).tolist()
+    c = Case(lengths.tolist(), new, hk, d, 16, dtype, seed=batch)
+    c.check_attend(_rows(7, c.t, 2 * hk, d))
+    if most == 1:                                     # the same rows by starts
+        c.starts = torch.arange(batch + 1, dtype=I32)
+        c.check_attend(_rows(7, c.t, 2 * hk, d))
+
+
+@gpu_test
 @pytest.mark.parametrize("dtype,d", [(BF16, 128), (BF16, 64), (E4M3, 128), (E4M3, 64)])
 @pytest.mark.parametrize("n,heads", [(1, 4), (5, 4), (70, 2), (200, 4)])
 def test_attend_every_key_counts(gpu, tile, dtype, d, n, heads):
