@@ -14,8 +14,8 @@
 //
 // FP8 pages: codes become bf16 in registers, exactly (a power of two scales a row): a
 // key's scale is the conversion's own operand, a value's is multiplied into its P before
-// that is rounded to bf16. P in bf16 is a rounding of 2^-9 relative at most half a step,
-// as large as the output's own; its sum is kept unrounded.
+// that is rounded to bf16. P in bf16 is off by half a step at most, 2^-8 of it, as the
+// output's own rounding; its sum is kept unrounded.
 #include <limits.h>
 
 #include "ff_block.h"
@@ -52,7 +52,8 @@ __device__ __forceinline__ f32x4 mfma_bf16(const bf16x8& a, const u32x4& b, cons
 // key ranges as its sequence's blocks take chunks. A chunk is the share of all blocks
 // that gives `budget` items, `least` blocks at least. All workgroups compute the
 // same list from the lengths; a sequence's last tiles, which see the most keys, come first.
-// A split's rows go to the workspace, with a note for each row where its splits are. Rows behind the last sequence are a sequence without keys.
+// A split's rows go to the workspace, with a note for each row where its splits are. Rows
+// behind the last sequence are a sequence without keys.
 
 struct Seq {
   int row0, n;    // first row (token) and rows
@@ -327,7 +328,9 @@ __device__ __forceinline__ uint64_t keys_to(int last) {
 // One workgroup per item: a 16-row tile, its key blocks dealt to the waves, each with a
 // running softmax of its own; the waves are joined in LDS. Keys go from memory straight
 // into the operand registers, values by DMA into the wave's own LDS: no barrier until
-// the end. Bound by the cache's bytes.
+// the end. Bound by the cache's bytes: 131072 FP8 positions of 8 heads of 128 (271 MB) 52 us, 48
+// sequences of about 3000 in bf16 (597 MB) 122 us, 5.2 and 4.9 TB/s. Blocks of 64 keys keep 32 KB of
+// a wave in flight; a CU takes in 64 bytes a clock, so that one row's cache is dealt to all of them.
 constexpr int kFewWaves = 4;     // two workgroups a CU
 constexpr int kDecodeWaves = 8;  // a workgroup a CU, no splits
 
@@ -560,7 +563,10 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void few_rows_kernel(Args
 // belong to one row, and 16 of a 32-key tile's scores are the two operand
 // registers of the second product. The reference moves only where a score passes it by
 // 2^8: P then is at most 2^8, which costs nothing in a floating-point format, and
-// the sums are rescaled in few blocks only.
+// the sums are rescaled in few blocks only. Bound by the matrix instructions with the softmax beside
+// them: 2048 tokens over 32748 positions, 32 / 8 heads of 128, 1.03 ms (1.03 PFLOP/s; the products alone 1.13
+// in a copy of the kernel; 16 x 16 x 32 tiles a wave 5.35 ms, four waves of 32 rows 1.06, of 64 1.48). 64 dims
+// have half the products for the same exponentials: 0.60 ms, 0.88 PFLOP/s.
 // (DMA in two stages where 32 rows a wave leave room for two workgroups a CU.)
 //
 // LDS rows are bf16 (RB = 2 D bytes); 16-byte chunk c of key k is kept at chunk
@@ -1004,7 +1010,7 @@ struct Plan {
 // eight times the new tokens or more, so that tiles are equally long; at 128 dims also where there are two
 // tiles a CU; for codes at 128 dims (two workgroups a CU leave them short of registers) where the
 // table may hold four times the new tokens. us, 256 against 128 rows, 32 / 8 heads: 2048 tokens over 30700
-// positions 1021 and 1060 (64 dims 636 and 705), over 4000 194 and 181, 4096 over none 153 and 157 (64
+// positions 1021 and 1060 (64 dims 636 and 705), over 4000 196 and 181, 4096 over none 153 and 157 (64
 // dims 107 and 93); codes: 512 over 4000 59 and 64, 4096 over none 159 and 186, 2048 over none 76 and 72.
 bool wide_tiles(int64_t rows, int64_t t, int64_t batch, int64_t hk, int64_t d, int fp8, int64_t capacity) {
   const int64_t all = rows * hk, depth = capacity * batch;

@@ -18,8 +18,9 @@
 // fp32 rows 73 -> 66, 5 of 577 60 -> 56; with the best of the waves' own k-th bests 137, 71, 57).
 // The lists of waves, then of a row's parts, are joined by sorts over the lanes.
 //
-// Bound by the logits' bytes: a row is read once, 16 bytes a lane and load, two loads
-// ahead. Few rows are split over workgroups, and a second launch joins their parts.
+// Bound by the logits' bytes, beside ten instructions a logit: a row is read once, 16 bytes a lane
+// and load, two loads ahead. 577 rows of 151936 in bf16 39 us (4.5 TB/s), with 5 alternatives 46. Few
+// rows are split over workgroups, and a second launch joins their parts (one row 10 and 5 us).
 #include "ff_common.h"
 
 using namespace ff;
