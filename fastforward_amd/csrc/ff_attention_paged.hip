@@ -35,6 +35,7 @@ struct Args {
   bf16_t* y;
   float* part_o;   // (items, BM, D) unnormalised sums of split tiles
   float2* part_s;  // (items, BM) their reference (log2) and denominator
+  int* plan;       // the list of many sequences, or null
   int2* part_of;   // (rows) where a row (token, head) begins there, and its splits (1: it is done)
   int hk, group, lbm;  // BM = 1 << lbm rows a tile
   int least, budget;  // 64-key blocks are dealt so that about so many items per head come out; 0: no tile is split
@@ -51,7 +52,7 @@ __device__ __forceinline__ f32x4 mfma_bf16(const bf16x8& a, const u32x4& b, cons
 // Every sequence's rows make ceil(rows / BM) tiles, and every tile is split into as many
 // key ranges as its sequence's blocks take chunks. A chunk is the share of all blocks
 // that gives `budget` items, `least` blocks at least. All workgroups compute the
-// same list from the lengths; a sequence's last tiles, which see the most keys, come first.
+// same list from the lengths (of more than 64 sequences a launch writes it); a sequence's last tiles, which see the most keys, come first.
 // A split's rows go to the workspace, with a note for each row where its splits are. Rows
 // behind the last sequence are a sequence without keys.
 
@@ -87,75 +88,108 @@ struct Item {
   int seq, tile, split, splits;
 };
 
-// Calls f(first sequence, this lane's) for 64 sequences at a time until it returns true; four loads of them are
-// in flight together. Up to 63 sequences are read once (`mine`), a lane each.
-template <class F>
-__device__ __forceinline__ void each_64(const Args& p, int lane, const Seq& mine, F f) {
-  if (p.a.batch < 64) {
-    f(0, mine);
-    return;
+// The chunk: the share of all blocks that gives `budget` items, or as many more as keep the items within it
+// (one round of the GPU's workgroups; a few of a second would take as long). Where the tiles alone are more
+// than that, only sequences past their share are split. sum(f): f over all sequences.
+template <class Sum>
+__device__ __forceinline__ int chunk_of(const Args& p, Sum sum) {
+  if (!p.budget) return INT_MAX;
+  const int total = sum([](const Seq& s) { return s.tiles * s.blocks; });
+  const int tiles = sum([](const Seq& s) { return s.tiles; });
+  int chunk = max(p.least, (total + p.budget - 1) / p.budget);
+  for (int i = 0; i < 3 && tiles < p.budget; ++i) {
+    const int items = sum([=](const Seq& s) { return s.tiles * splits_of(s.blocks, chunk); });
+    if (items <= p.budget) break;
+    chunk = (int)min((int64_t)INT_MAX, ((int64_t)chunk * items + p.budget - 1) / p.budget);
   }
-  for (int b0 = 0; b0 <= p.a.batch; b0 += 256) {
-    Seq s[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = seq_of(p, b0 + 64 * i + lane);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (f(b0 + 64 * i, s[i])) return;
-  }
+  return chunk;
 }
 
-// Item `id` of the list. The chunk is the share of all blocks that gives `budget` items, or as many
-// more as keep the items within it (one round of the GPU's workgroups; a few of a second would take as
-// long). Where the tiles alone are more than that, only sequences past their share are split. (Decode
-// of 256 sequences of 500 positions 134 -> 110 us, with one of 60000 among 255 of 100 766 -> 93.)
-__device__ __forceinline__ bool find_item(const Args& p, int lane, int id, Item* out) {
-  const Seq mine = seq_of(p, lane);
-  int chunk = INT_MAX;
-  if (p.budget) {
-    int total = 0, tiles = 0;
-    each_64(p, lane, mine, [&](int, const Seq& s) {
-      total += s.tiles * s.blocks;
-      tiles += s.tiles;
-      return false;
-    });
-    total = __builtin_amdgcn_readlane(wave_scan(total), 63);
-    tiles = __builtin_amdgcn_readlane(wave_scan(tiles), 63);
-    chunk = max(p.least, (total + p.budget - 1) / p.budget);
-    for (int i = 0; i < 3 && tiles < p.budget; ++i) {
-      int items = 0;
-      each_64(p, lane, mine, [&](int, const Seq& s) {
-        items += s.tiles * splits_of(s.blocks, chunk);
-        return false;
-      });
-      items = __builtin_amdgcn_readlane(wave_scan(items), 63);
-      if (items <= p.budget) break;
-      chunk = (int)min((int64_t)INT_MAX, ((int64_t)chunk * items + p.budget - 1) / p.budget);
-    }
-  }
-  int base = 0;
-  bool found = false;
-  each_64(p, lane, mine, [&](int b0, const Seq& s) {
-    const int splits = splits_of(s.blocks, chunk), n = s.tiles * splits;
-    const int sum = wave_scan(n), first = base + sum - n;
-    const uint64_t hit = __ballot(id >= first && id < first + n);
-    if (hit) {
-      const int src = __builtin_ctzll(hit);
-      out->s = {__builtin_amdgcn_readlane(s.row0, src), __builtin_amdgcn_readlane(s.n, src),
-                __builtin_amdgcn_readlane(s.len, src),  __builtin_amdgcn_readlane(s.keys, src),
-                __builtin_amdgcn_readlane(s.tiles, src), __builtin_amdgcn_readlane(s.blocks, src)};
-      out->seq = b0 + src;
-      out->splits = __builtin_amdgcn_readlane(splits, src);
-      const int in = id - __builtin_amdgcn_readlane(first, src);
-      out->tile = out->s.tiles - 1 - in / out->splits;
-      out->split = in % out->splits;
-      found = true;
-      return true;
-    }
-    base += __builtin_amdgcn_readlane(sum, 63);
-    return false;
+// Sequences for a lane each, the rows behind the last one among them.
+__host__ __device__ inline bool fit_lanes(int64_t batch, bool starts) { return batch + starts <= 64; }
+
+// The list of more sequences than a wave has lanes, by one workgroup in a launch of its own: plan[0] the chunk,
+// plan[1 + b] the first item of sequence b (b = batch: of the rows behind the last; batch + 1: all items). With
+// every workgroup reading all lengths instead, decode of 256 sequences of 500 positions took 134 us (102 so), 1024
+// sequences of 3 tokens over 200 positions 427 (208).
+__global__ __launch_bounds__(1024) void plan_kernel(Args p) {
+  __shared__ int part[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  auto all = [&](int v) {  // the workgroup's sum
+    v = __builtin_amdgcn_readlane(wave_scan(v), 63);
+    __syncthreads();
+    if (lane == 0) part[wave] = v;
+    __syncthreads();
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) sum += part[w];
+    return sum;
+  };
+  const int chunk = chunk_of(p, [&](auto f) {
+    int v = 0;
+    for (int b = threadIdx.x; b <= p.a.batch; b += 1024) v += f(seq_of(p, b));
+    return all(v);
   });
-  return found;
+  if (threadIdx.x == 0) p.plan[0] = chunk;
+  int base = 0;
+  for (int b0 = 0; b0 <= p.a.batch; b0 += 1024) {
+    const int b = b0 + threadIdx.x;
+    const Seq s = seq_of(p, b);
+    const int n = b <= p.a.batch ? s.tiles * splits_of(s.blocks, chunk) : 0, upto = wave_scan(n);
+    __syncthreads();
+    if (lane == 63) part[wave] = upto;
+    __syncthreads();
+    int before = 0, sum = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+      before += w < wave ? part[w] : 0;
+      sum += part[w];
+    }
+    if (b <= p.a.batch) p.plan[1 + b] = base + before + upto - n;
+    base += sum;
+  }
+  if (threadIdx.x == 0) p.plan[2 + p.a.batch] = base;
+}
+
+// Item `id` of the list.
+__device__ __forceinline__ bool find_item(const Args& p, int lane, int id, Item* out) {
+  Seq s;
+  int chunk, first;
+  if (p.plan) {
+    const int* starts = p.plan + 1;
+    int lo = 0;
+    for (int n = p.a.batch + 2; n > 1;) {  // the last one that begins at or before the item, among n from lo
+      const int step = (n + 63) >> 6, at = lane * step;
+      const int c = max(__popcll(__ballot((at < n ? starts[lo + at] : INT_MAX) <= id)) - 1, 0);
+      lo += c * step;
+      n = min(step, n - c * step);
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    if (lo > p.a.batch) return false;
+    chunk = __builtin_amdgcn_readfirstlane(p.plan[0]);
+    first = __builtin_amdgcn_readfirstlane(starts[lo]);
+    s = seq_of(p, lo);
+    out->seq = lo;
+    lane = 0;
+  } else {
+    s = seq_of(p, lane);
+    chunk = chunk_of(p, [&](auto f) { return __builtin_amdgcn_readlane(wave_scan(f(s)), 63); });
+    const int n = s.tiles * splits_of(s.blocks, chunk), upto = wave_scan(n);
+    const uint64_t hit = __ballot(id >= upto - n && id < upto);
+    if (!hit) return false;
+    lane = __builtin_ctzll(hit);
+    first = __builtin_amdgcn_readlane(upto - n, lane);
+    out->seq = lane;
+  }
+  out->s = {__builtin_amdgcn_readlane(s.row0, lane), __builtin_amdgcn_readlane(s.n, lane),
+            __builtin_amdgcn_readlane(s.len, lane),  __builtin_amdgcn_readlane(s.keys, lane),
+            __builtin_amdgcn_readlane(s.tiles, lane), __builtin_amdgcn_readlane(s.blocks, lane)};
+  out->splits = splits_of(out->s.blocks, chunk);
+  const int in = id - first;
+  if (in < 0 || in >= out->s.tiles * out->splits) return false;  // (counts of starts that do not rise may pass 32 bits)
+  out->tile = out->s.tiles - 1 - in / out->splits;
+  out->split = in % out->splits;
+  return true;
 }
 
 // ------------------------------------------------------------------ pieces of a block
@@ -1003,6 +1037,7 @@ struct Plan {
   bool decode;
   int lbm, least, budget;
   int64_t items;  // per key head
+  bool listed;    // a launch writes the list
 };
 
 // 256-row tiles (one workgroup of 8 waves a CU) against 128-row ones (two or three of 4): half the loads
@@ -1052,8 +1087,13 @@ Plan plan_of(int64_t t, int64_t batch, bool starts, int64_t hk, int64_t group, i
   // No splits where a sequence's keys are one chunk whatever its length is, nor where there
   // are tiles enough whatever the starts are (one sequence: as many as workgroups).
   if ((capacity + 63) / 64 > p.least && (rows >> p.lbm) < (batch == 1 ? 1 : 2) * budget) p.budget = (int)budget;
+  // Decode of more sequences is split as well where one may be far longer than a workgroup's share: 1024
+  // sequences of 100 positions, one of 60000 among them, 794 us without splits.
+  if (p.kind == 0 && !starts && !fit_lanes(batch, starts) && capacity > 4096) p.budget = (int)budget;
   if (((tiles + budget) * hk << p.lbm) > INT32_MAX) p.budget = 0;  // (rows of the splits are counted in 32 bits)
   p.items = tiles + p.budget;
+  // (no list: 16-row tiles of one row a sequence that are not split)
+  p.listed = !fit_lanes(batch, starts) && (starts || p.budget || p.kind);
   return p;
 }
 
@@ -1068,8 +1108,12 @@ int check_sizes(const char* what, const ff_paged_cache* c, int64_t hq, int64_t w
   return FF_OK;
 }
 
-int64_t workspace_of(const Plan& p, int64_t t, int64_t hq, int64_t hk, int64_t d) {
+// Partial sums, their statistics, the rows' notes; the list.
+int64_t parts_bytes(const Plan& p, int64_t t, int64_t hq, int64_t hk, int64_t d) {
   return p.budget ? ((p.items * hk) << p.lbm) * (d * 4 + 8) + t * hq * 8 : 0;
+}
+int64_t workspace_of(const Plan& p, int64_t t, int64_t hq, int64_t hk, int64_t d, int64_t batch) {
+  return parts_bytes(p, t, hq, hk, d) + (p.listed ? (batch + 3) * 4 : 0);
 }
 
 }  // namespace
@@ -1087,7 +1131,7 @@ extern "C" int ff_attention_paged_workspace(const ff_paged_cache* cache, int64_t
   st = check_sizes("ff_attention_paged_workspace", cache, hq, width, batch, t);
   if (st != FF_OK) return st;
   *bytes = workspace_of(plan_of(t, batch, starts, cache->hk, hq / cache->hk, cache->d, cache->fp8 != 0,
-                                width * cache->page_size), t, hq, cache->hk, cache->d);
+                                width * cache->page_size), t, hq, cache->hk, cache->d, batch);
   return FF_OK;
 }
 
@@ -1106,7 +1150,7 @@ extern "C" int ff_attention_paged(const void* q, int64_t q_ts, int64_t q_hs, con
   const int64_t hk = cache->hk, d = cache->d;
   const bool fp8 = cache->fp8 != 0;
   const Plan plan = plan_of(t, batch, starts != nullptr, hk, hq / hk, d, fp8, width * cache->page_size);
-  const int64_t need = workspace_of(plan, t, hq, hk, d);
+  const int64_t need = workspace_of(plan, t, hq, hk, d, batch);
   FF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ff_aligned(workspace, 16)),
              "ff_attention_paged: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
   Args p;
@@ -1122,6 +1166,7 @@ extern "C" int ff_attention_paged(const void* q, int64_t q_ts, int64_t q_hs, con
   p.part_o = (float*)workspace;
   p.part_s = (float2*)((char*)workspace + ((plan.items * hk) << plan.lbm) * d * 4);
   p.part_of = (int2*)(p.part_s + ((plan.items * hk) << plan.lbm));
+  p.plan = plan.listed ? (int*)((char*)workspace + parts_bytes(plan, t, hq, hk, d)) : nullptr;
   p.hk = (int)hk;
   p.group = (int)(hq / hk);
   p.lbm = plan.lbm;
@@ -1134,6 +1179,7 @@ extern "C" int ff_attention_paged(const void* q, int64_t q_ts, int64_t q_hs, con
   const int64_t per = wide ? 1 : 1024 / d;  // rows of a join workgroup
   const dim3 join((unsigned)((t * hq + per - 1) / per));
   hipStream_t s = (hipStream_t)stream;
+  if (plan.listed) hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, s, p);
 #define FF_PAGED(DIM, F8)                                                                                          \
   if (d == DIM && fp8 == F8) {                                                                              \
     if (plan.decode)                                                                                               \

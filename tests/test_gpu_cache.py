@@ -196,6 +196,12 @@ def test_attend_many_sequences(gpu, batch, most, hk, dtype, d):
     new = None if most == 1 else torch.randint(0, most + 1, (batch,), generator=_g(3)).minimum(lengths).tolist()
     c = Case(lengths.tolist(), new, hk, d, 16, dtype, seed=batch)
     c.check_attend(_rows(7, c.t, 2 * hk, d))
+    if batch == 300:                                  # starts that say anything: other rows, but no fault
+        for seed in range(3):
+            odd = torch.randint(-5, 400, (batch + 1,), generator=_g(seed)).to(I32)
+            q = _rows(7, c.t, 2 * hk, d).to(DEV)
+            assert c.dev.attend(q, c.table.to(DEV), c.lengths.to(DEV), odd.to(DEV)).shape == q.shape
+        torch.cuda.synchronize()
     if most == 1:                                     # the same rows by starts
         c.starts = torch.arange(batch + 1, dtype=I32)
         c.check_attend(_rows(7, c.t, 2 * hk, d))
