@@ -109,7 +109,6 @@ SIGNATURES = {
 }
 
 
-
 class PagedCacheStruct(ctypes.Structure):
     """ff_paged_cache."""
     _fields_ = [(name, P) for name in ("k", "v", "k_scale", "v_scale")] + \

@@ -157,14 +157,7 @@ __device__ __forceinline__ bool find_item(const Args& p, int lane, int id, Item*
   int chunk, first;
   if (p.plan) {
     const int* starts = p.plan + 1;
-    int lo = 0;
-    for (int n = p.a.batch + 2; n > 1;) {  // the last one that begins at or before the item, among n from lo
-      const int step = (n + 63) >> 6, at = lane * step;
-      const int c = max(__popcll(__ballot((at < n ? starts[lo + at] : INT_MAX) <= id)) - 1, 0);
-      lo += c * step;
-      n = min(step, n - c * step);
-    }
-    lo = __builtin_amdgcn_readfirstlane(lo);
+    const int lo = last_upto(starts, p.a.batch + 2, id, lane);  // the last one that begins at or before the item
     if (lo > p.a.batch) return false;
     chunk = __builtin_amdgcn_readfirstlane(p.plan[0]);
     first = __builtin_amdgcn_readfirstlane(starts[lo]);

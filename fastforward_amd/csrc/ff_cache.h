@@ -29,17 +29,32 @@ struct Rows {
   __device__ __forceinline__ int64_t capacity() const { return width << lps; }
 };
 
+// The largest index in [0, n) with at[index] <= x, by a wave; at rises, at[0] <= x. (Some index in [0, n) whatever
+// it holds.)
+__device__ __forceinline__ int last_upto(const int* at, int n, int x, int lane) {
+  int lo = 0;
+  while (n > 1) {
+    const int step = (n + 63) >> 6, i = lane * step;
+    const int c = max(__popcll(__ballot((i < n ? at[lo + i] : 0x7FFFFFFF) <= x)) - 1, 0);
+    lo += c * step;
+    n = min(step, n - c * step);
+  }
+  return __builtin_amdgcn_readfirstlane(lo);
+}
+
 // Sequences of the N rows row0 .. row0 + N - 1 (a wave's; uniform row0): of[i] = how many
 // sequences end at or before row0 + i. batch where the row lies behind the last one.
 template <int N>
 __device__ __forceinline__ void find_sequences(const Rows& a, int row0, int lane, int (&of)[N]) {
+  int b0 = a.starts && a.batch > 64 ? last_upto(a.starts, a.batch + 1, row0, lane) : 0;
 #pragma unroll
-  for (int i = 0; i < N; ++i) of[i] = a.starts ? 0 : row0 + i;
+  for (int i = 0; i < N; ++i) of[i] = a.starts ? b0 : row0 + i;
   if (!a.starts) return;
-  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+  for (; b0 < a.batch; b0 += 64) {
     const int end = b0 + lane < a.batch ? a.starts[b0 + lane + 1] : 0x7FFFFFFF;
 #pragma unroll
     for (int i = 0; i < N; ++i) of[i] += __popcll(__ballot(end <= row0 + i));
+    if (__ballot(end > row0 + N - 1)) break;
   }
 }
 

@@ -195,6 +195,11 @@ def test_attend_many_sequences(gpu, batch, most, hk, dtype, d):
     lengths[batch - 1] = 130
     new = None if most == 1 else torch.randint(0, most + 1, (batch,), generator=_g(3)).minimum(lengths).tolist()
     c = Case(lengths.tolist(), new, hk, d, 16, dtype, seed=batch)
+    k, v = _rows(8, c.t, hk, d), _rows(9, c.t, hk, d)
+    c.dev.write(k.to(DEV), v.to(DEV), *c.args())
+    S.write(c.cpu, k, v, c.table, c.lengths, c.starts)
+    for name, want in c.cpu.items():
+        assert torch.equal(getattr(c.dev, name).cpu().view(torch.uint8), want.view(torch.uint8)), name
     c.check_attend(_rows(7, c.t, 2 * hk, d))
     if batch == 300:                                  # starts that say anything: other rows, but no fault
         for seed in range(3):
@@ -205,6 +210,8 @@ def test_attend_many_sequences(gpu, batch, most, hk, dtype, d):
     if most == 1:                                     # the same rows by starts
         c.starts = torch.arange(batch + 1, dtype=I32)
         c.check_attend(_rows(7, c.t, 2 * hk, d))
+        for x, y in zip(c.dev.read(*c.args(), rows=c.t + 5), c.dev.read(*c.args(False))):
+            assert torch.equal(x[:c.t], y) and not x[c.t:].any()
 
 
 @gpu_test
