@@ -215,6 +215,31 @@ def test_attend_many_sequences(gpu, batch, most, hk, dtype, d):
 
 
 @gpu_test
+@pytest.mark.parametrize("ragged", [False, True])
+def test_attend_many_sequences_graph(gpu, ragged):
+    """The list of many sequences is written anew on every replay."""
+    batch = 100
+    lengths = [30 + i for i in range(batch)]
+    lengths[40] = 5000
+    c = Case(lengths, [2] * batch if ragged else None, 1, 64, 16)
+    q, args = _rows(3, c.t, 4, 64).to(DEV), c.args()
+    c.dev.attend(q, *args)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = c.dev.attend(q, *args)
+    for seed in range(4):
+        now = [int(n) for n in torch.randint(2, 140, (batch,), generator=_g(seed)).minimum(c.lengths)]
+        now[40] = (5000, 700, 0, 4999)[seed]
+        args[1].copy_(torch.tensor(now, dtype=I32))
+        q.copy_(_rows(seed, c.t, 4, 64))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        assert torch.equal(got, c.dev.attend(q, *args))
+        close(got, *S.attend(c.cpu, q.cpu(), c.table, torch.tensor(now), c.starts), 64)
+
+
+@gpu_test
 @pytest.mark.parametrize("dtype,d", [(BF16, 128), (BF16, 64), (E4M3, 128), (E4M3, 64)])
 @pytest.mark.parametrize("n,heads", [(1, 4), (5, 4), (70, 2), (200, 4)])
 def test_attend_every_key_counts(gpu, tile, dtype, d, n, heads):
