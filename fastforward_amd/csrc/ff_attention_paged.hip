@@ -16,6 +16,7 @@
 // key's scale is the conversion's own operand, a value's is multiplied into its P before
 // that is rounded to bf16. P in bf16 is off by half a step at most, 2^-8 of it, as the
 // output's own rounding; its sum is kept unrounded.
+#include <float.h>
 #include <limits.h>
 
 #include "ff_block.h"
@@ -254,6 +255,11 @@ __device__ __forceinline__ void lds_dma16_at(const uint8_t* base, uint32_t offse
                : "memory", "m0");
 }
 
+// The reference of a row that sees a key is at least this, also where its scores are NaN or -inf. A reference of
+// -inf is a row that sees nothing, which alone is zero: the others divide by their sum, be it 0 or NaN.
+constexpr float kLeast = -FLT_MAX;
+__device__ __forceinline__ float inverse_sum(float m, float sum) { return m == -INFINITY ? 0.f : 1.0f / sum; }
+
 // This wave's LDS reads and writes are done (no other wave uses the memory).
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
 
@@ -278,7 +284,7 @@ __device__ __forceinline__ float softmax_block(f32x4 (&s)[4], bool masked, uint6
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r) top = __builtin_elementwise_maximum(top, s[i][r]);
-  const float mnew = fmaxf(m, max_rows(top) * c2);
+  const float mnew = fmaxf(m, fmaxf(max_rows(top) * c2, masked && !vis ? -INFINITY : kLeast));  // (drops NaN)
   const float mref = mnew == -INFINITY ? 0.f : mnew;
   const float alpha = __builtin_amdgcn_exp2f(m - mref);
   float psum = 0.f;
@@ -570,7 +576,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void few_rows_kernel(Args
     const int rr = it.tile * 16 + r, query = DECODE ? 0 : rr / p.group;
     const int64_t to = (int64_t)(it.s.row0 + query) * (p.hk * p.group) + head * p.group + rr - query * p.group;
     if (it.splits == 1) {
-      const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+      const float inv = inverse_sum(mx, sum);
       *reinterpret_cast<u32x2*>(p.y + to * D + d0) = pack4_bf16(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
       if (!DECODE && p.budget && d0 == 0) p.part_of[to] = int2{0, 1};
     } else {
@@ -865,10 +871,12 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void many_rows_kernel(Arg
 #pragma unroll
       for (int st = 0; st < KST; ++st) s[kt] = mfma32(k_fragment(kt, st), qf[st], s[kt]);
     u32x4 pf[4];
+    float least = kLeast;
     const bool full = ok == ~0ull && kb + 64 <= all;
     if (!full) {
       asm volatile("");  // a branch: as selects the masks would be computed for every block
       const uint64_t vis = ok & keys_to(pos - kb);
+      least = vis ? kLeast : -INFINITY;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const uint32_t bits = (uint32_t)(vis >> (16 * c + 8 * h));
@@ -882,7 +890,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void many_rows_kernel(Arg
     float top = s[0][0];
 #pragma unroll
     for (int i = 1; i < 32; ++i) top = __builtin_elementwise_maximum(top, s[i >> 4][i & 15]);
-    top = max_halves(top) * p.c2;
+    top = fmaxf(max_halves(top) * p.c2, least);  // (drops NaN)
     if (__ballot(top > m + 8.f)) {
       const float mnew = fmaxf(m, top), mref = mnew == -INFINITY ? 0.f : mnew;
       const float alpha = __builtin_amdgcn_exp2f(m - mref);
@@ -929,7 +937,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void many_rows_kernel(Arg
   if (row >= rows) return;
   const int64_t to = (int64_t)(it.s.row0 + row / p.group) * (p.hk * p.group) + head * p.group + row % p.group;
   if (it.splits == 1) {
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    const float inv = inverse_sum(m, sum);
 #pragma unroll
     for (int i = 0; i < 4 * DTN; ++i) {
       const f32x16& x = o[i >> 2];
@@ -1009,6 +1017,7 @@ __global__ __launch_bounds__(256) void join_kernel(Args p) {
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i) mx = fmaxf(mx, stats[i].x);
     const float mref = mx == -INFINITY ? 0.f : mx;
+    m = mx;
     acc = f32x4{0.f, 0.f, 0.f, 0.f};
     sum = 0.f;
 #pragma unroll
@@ -1018,7 +1027,7 @@ __global__ __launch_bounds__(256) void join_kernel(Args p) {
       fma4(acc, parts[i * LPR + threadIdx.x], w);
     }
   }
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  const float inv = inverse_sum(m, sum);
   *reinterpret_cast<u32x2*>(p.y + (int64_t)row * D + dim) =
       pack4_bf16(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
 }

@@ -1,0 +1,58 @@
+"""Rows of the paged attention that are not ordinary: NaN and infinities in queries and in the keys
+that a row sees, in calls that are split and calls that are not."""
+import math
+
+import pytest
+import torch
+
+from oracle import serving as S
+from tests.test_gpu_cache import BF16, DEV, E4M3, Case, _rows, close, tile  # noqa: F401 (a fixture)
+
+gpu_test = pytest.mark.gpu
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+@pytest.mark.parametrize("lengths,new,heads,width", [
+    ([90], None, 4, None), ([1500], None, 4, None), ([90], None, 4, 300), ([1500], [40], 4, None),
+    ([700, 1300], [300, 5], 8, 200), ([100] * 70, [2] * 70, 4, None)])
+def test_odd_queries(gpu, tile, dtype, lengths, new, heads, width):  # noqa: F811
+    """A NaN in a query makes its row NaN, and so do scores that are all -inf; rows that see nothing
+    are zero, and the others are as they were. Rows joined by workgroups and by groups of lanes."""
+    for d in (64, 128):
+        c = Case(lengths, new, 2, d, 16, dtype, seed=d, width=width)
+        c.cpu["k"][..., 5] = -1.0 if dtype == BF16 else torch.tensor(-1.0).to(E4M3)
+        c.upload("k")
+        if len(lengths) > 1:
+            c.lengths[-1] = 1                             # the rows of its sequence before the last see nothing
+        q = _rows(d, c.t, heads, d)
+        q[0, 0, 7] = math.nan
+        q[c.t // 2, heads - 1, 5] = math.inf              # -inf for every key
+        q[c.t // 3, 1, 5] = math.inf
+        y, o = c.check_attend(q)
+        assert y[0, 0].isnan().all() and y[c.t // 3, 1].isnan().all()
+        if lengths == [1500] and new is None:             # without any key
+            c.lengths[0] = 0
+            assert not c.dev.attend(q.to(DEV), *c.args()).any()
+
+
+@gpu_test
+@pytest.mark.parametrize("new", [None, [9], [200]])
+def test_odd_ranges_of_keys(gpu, tile, new):  # noqa: F811
+    """Long runs of keys that score -inf weigh nothing beside others; one NaN key that is seen is NaN,
+    wherever it lies and whatever the others are."""
+    for at in (0, 1000, 2499):
+        c = Case([2500], new, 1, 128, 16, BF16, seed=at)
+        keys = torch.arange(2500)
+        page, slot = c.table[0].long()[keys // 16], keys % 16
+        far = (keys - at).abs() > 40                       # all but a few score -inf
+        c.cpu["k"][page[far], 0, slot[far], 3] = -math.inf
+        c.upload("k")
+        q = _rows(1, c.t, 4, 128).abs()
+        y, o = c.check_attend(q)
+        assert not o[-1].isnan().any()
+        c.cpu["k"][page[at], 0, slot[at], 9] = math.nan
+        c.upload("k")
+        y = c.dev.attend(q.to(DEV), *c.args()).cpu()
+        o, _, _ = S.attend(c.cpu, q, c.table, c.lengths, c.starts)
+        assert torch.equal(y.isnan(), o.isnan()) and y[-1].isnan().all()
