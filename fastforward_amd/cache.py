@@ -136,8 +136,9 @@ class PagedCache:
         1 / sqrt(head_dim)) with fp32 statistics, weights rounded to bf16 for the product
         with the values, fp32 sums. (T, heads, head_dim) bf16. A row that sees nothing, and
         rows behind the last sequence, are zero; a NaN in a row's query or in a key that it
-        sees makes it NaN. Scores are up to 2^30 in size (past it they
-        may become NaN); an infinite value that a row sees makes it infinite or NaN."""
+        sees makes it NaN. Scores are up to 2^30 in size (past it they may become NaN), and
+        a row's largest value times the positions that it sees up to 2^127 (past it the sums may become
+        infinite); an infinite value that a row sees makes it infinite or NaN."""
         assert q.dim() == 3 and q.dtype == BF16, (q.shape, q.dtype)
         t, heads, d = q.shape
         assert d == self.head_dim and 0 < heads <= 65535 and heads % self.kv_heads == 0, (q.shape, self.kv_heads)

@@ -594,9 +594,9 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void few_rows_kernel(Args
 // pass through LDS in three stages (bf16 pages by DMA; codes through registers, where they
 // become scaled bf16, in two). v_mfma_f32_32x32x16_bf16: a lane's scores and sums
 // belong to one row, and 16 of a 32-key tile's scores are the two operand
-// registers of the second product. The reference moves only where a score passes it by
-// 2^8: P then is at most 2^8, which costs nothing in a floating-point format, and
-// the sums are rescaled in few blocks only. Bound by the matrix instructions with the softmax beside
+// registers of the second product. The reference moves only where a score passes it, and
+// then to 2^8 times that score: P is 1 at most and mostly near 2^-8, which costs nothing in a
+// floating-point format, and the sums are rescaled in few blocks only. Bound by the matrix instructions with the softmax beside
 // them: 2048 tokens over 32748 positions, 32 / 8 heads of 128, 1.03 ms (1.03 PFLOP/s; the products alone 1.13
 // in a copy of the kernel; 16 x 16 x 32 tiles a wave 5.35 ms, four waves of 32 rows 1.06, of 64 1.48). 64 dims
 // have half the products for the same exponentials: 0.60 ms, 0.88 PFLOP/s.
@@ -891,8 +891,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void many_rows_kernel(Arg
 #pragma unroll
     for (int i = 1; i < 32; ++i) top = __builtin_elementwise_maximum(top, s[i >> 4][i & 15]);
     top = fmaxf(max_halves(top) * p.c2, least);  // (drops NaN)
-    if (__ballot(top > m + 8.f)) {
-      const float mnew = fmaxf(m, top), mref = mnew == -INFINITY ? 0.f : mnew;
+    if (__ballot(top > m)) {
+      const float mnew = top > m ? top + 8.f : m, mref = mnew == -INFINITY ? 0.f : mnew;
       const float alpha = __builtin_amdgcn_exp2f(m - mref);
       m = mnew;
       den *= alpha;

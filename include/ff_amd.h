@@ -574,10 +574,12 @@ int ff_cache_read(const ff_paged_cache* cache, const int32_t* table, int64_t wid
  * contiguous, y[row] = sum_j p_j v_j over the positions j up to the row's own, p = softmax of
  * scale * q . k_j. Statistics and sums fp32, p rounded to bf16 before it meets v. Query head h
  * reads key head h / (hq / hk). q (t, hq, d) bf16 with strides q_ts, q_hs. scale > 0. A row
- * that sees nothing is zero; a NaN in its query or in a key that it sees makes it NaN. workspace: ff_attention_paged_workspace bytes (host-only, 0:
- * none; its `starts`: whether there are any), 16-byte aligned, one per stream and per captured graph that may run beside another.
- * The sums' order depends on the sizes, lengths and starts alone. Scores up to 2^30 in size (past it they may
- * become NaN); an infinite value that a row sees makes it infinite or NaN. */
+ * that sees nothing is zero; a NaN in its query or in a key that it sees makes it NaN. workspace:
+ * ff_attention_paged_workspace bytes (host-only, 0: none; its `starts`: whether there are any), 16-byte
+ * aligned, one per stream and per captured graph that may run beside another. The sums' order depends on
+ * the sizes, lengths and starts alone. Scores up to 2^30 in size (past it they may become NaN), a row's
+ * largest value times the positions that it sees up to 2^127 (past it the sums may become infinite); an
+ * infinite value that a row sees makes it infinite or NaN. */
 int ff_attention_paged_workspace(const ff_paged_cache* cache, int64_t hq, int64_t width, int64_t batch, int starts,
                                  int64_t t, int64_t* bytes);
 int ff_attention_paged(const void* q, int64_t q_ts, int64_t q_hs, const ff_paged_cache* cache, int64_t hq,

@@ -56,3 +56,31 @@ def test_odd_ranges_of_keys(gpu, tile, new):  # noqa: F811
         y = c.dev.attend(q.to(DEV), *c.args()).cpu()
         o, _, _ = S.attend(c.cpu, q, c.table, c.lengths, c.starts)
         assert torch.equal(y.isnan(), o.isnan()) and y[-1].isnan().all()
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (BF16, 64), (E4M3, 128), (E4M3, 64)])
+@pytest.mark.parametrize("length,n", [(128, 1), (128, 30), (2000, 3), (2000, 200)])
+def test_large_values(gpu, tile, dtype, d, length, n):  # noqa: F811
+    """Values whose size times the positions' number is below 2^127 never overflow: the first block's
+    scores are 2^7.9 times below the others', the most that a reference may lag behind."""
+    c = Case([length], [n], 1, d, 64, dtype, seed=length + d)
+    for name in ("k", "v"):
+        x = S.values(c.cpu, name)
+        if name == "k":
+            x[..., 0] = 1.0
+            page = int(c.table[0, 0])
+            x[page, :, :, 0] = 0.0
+            x[..., 1:] *= 2.0 ** -10
+        else:
+            x = (x.sign() + (x == 0)) * 2.0 ** (119 if length == 128 else 115)
+        x = x.to(BF16)
+        if dtype == BF16:
+            c.cpu[name] = x
+        else:
+            c.cpu[name], c.cpu[name + "_scale"] = S.codes(x)
+        c.upload(name)
+    q = _rows(2, n, 4, d) * 2.0 ** -10
+    q[..., 0] = 7.875                                     # in base 2, by the scale
+    y, o = c.check_attend(q.to(BF16), scale=math.log(2.0))
+    assert (o.abs() < math.inf).all() and y.isfinite().all()
