@@ -32,7 +32,8 @@ class PagedCache:
     """Keys and values of one layer: ``k``, ``v`` (pages, kv_heads, page_size, head_dim), bf16
     or, ``dtype=torch.float8_e4m3fn``, e4m3 codes with ``k_scale``, ``v_scale`` (pages,
     kv_heads, page_size) uint8, the biased exponent of a token's scale in each head:
-    value = code * 2^(byte - 127). ``head_dim`` is 64 or 128, ``page_size`` a power of
+    value = code * 2^(byte - 127), NaN where the byte is 255. ``write`` makes bytes from 27 to 247; ``attend``
+    may take values under smaller ones, below 2^-91 all of them, as zeros. ``head_dim`` is 64 or 128, ``page_size`` a power of
     two, 16 to 4096. Pages begin as zeros; which sequence a page belongs to is the
     caller's to say, and sequences may share the pages of a common prefix.
 

@@ -487,10 +487,10 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void few_rows_kernel(Args
     }
     const uint64_t vis = ok & keys_to(pos - kb);
     const bool masked = __ballot(vis != ~0ull) != 0;
-    if (FP8 && ok != ~0ull) {  // a scale byte of a key that is not there may be anything
+    if (FP8 && masked) {  // a scale byte of a key that the row does not see may be anything, and 0 times it not 0
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const uint32_t bits = (uint32_t)(ok >> (32 * c + 8 * g));
+        const uint32_t bits = (uint32_t)(vis >> (32 * c + 8 * g));
         vsc[c].x &= ((bits & 15) * 0x204081u & 0x01010101u) * 255u;
         vsc[c].y &= ((bits >> 4 & 15) * 0x204081u & 0x01010101u) * 255u;
       }

@@ -99,7 +99,7 @@ inline Rows rows_of(const ff_paged_cache* c, const int32_t* table, int64_t width
   return Rows{table, lengths, starts, width, (int)batch, (int)t, (int)c->pages, __builtin_ctzll((uint64_t)c->page_size)};
 }
 
-// The float of a scale byte.
+// The float of a scale byte (0 for byte 0, and for 255 an infinity, which is no number times any code).
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
 
 }  // namespace ff

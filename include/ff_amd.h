@@ -543,7 +543,8 @@ int ff_moe_experts(const void* x, int64_t ldx, const float* weights, const int* 
  * No reference counterpart: its step runs a prompt once and keeps nothing. */
 
 /* A paged cache: k, v (pages, hk, page_size, d), bf16 or (fp8) e4m3 codes with
- * k_scale, v_scale (pages, hk, page_size) bytes, value = code * 2^(byte - 127). page_size is
+ * k_scale, v_scale (pages, hk, page_size) bytes, value = code * 2^(byte - 127), NaN where the byte is 255
+ * (ff_cache_write makes 27 .. 247; the attention may take values under smaller bytes as zeros). page_size is
  * a power of two, 16 .. 4096, d 64 or 128; k, v 16-byte, the scales 8-byte aligned. Position p of
  * sequence b is slot p % page_size of page table[b, p / page_size], table (batch, width), width *
  * page_size at most 2^31 - 2^16; lengths (batch): the positions of each sequence. starts

@@ -84,3 +84,51 @@ def test_large_values(gpu, tile, dtype, d, length, n):  # noqa: F811
     q[..., 0] = 7.875                                     # in base 2, by the scale
     y, o = c.check_attend(q.to(BF16), scale=math.log(2.0))
     assert (o.abs() < math.inf).all() and y.isfinite().all()
+
+
+@gpu_test
+def test_every_scale_byte(gpu):
+    """read gives code * 2^(byte - 127) of all codes under all bytes, rounded to bf16 where that has fewer
+    bits (below its normal range) or no such value; NaN under byte 255."""
+    c = Case([4096], None, 1, 128, 16, E4M3, fill=False, spare=0)
+    c.table[0] = torch.arange(256)
+    byte = torch.arange(256, dtype=torch.uint8)
+    c.cpu["k"] = byte.reshape(1, 1, 2, 128).repeat(256, 1, 8, 1).view(E4M3)
+    c.cpu["v"] = c.cpu["k"].flip(2)
+    for name in ("k", "v"):
+        c.cpu[name + "_scale"] = byte[:, None, None].expand(256, 1, 16).contiguous()
+        c.upload(name)
+    starts = torch.tensor([0, 4096], dtype=torch.int32)
+    got = c.dev.read(*c.args(False), starts.to(DEV), rows=4096)
+    for x, want in zip(got, S.read(c.cpu, c.table, c.lengths, starts, 4096)):
+        want[255 * 16:] = math.nan
+        want = want.float().to(BF16)                       # exact in fp32: 2^-136 is a multiple of its smallest value
+        assert torch.equal(x.cpu().isnan(), want.isnan()) and torch.equal(x.cpu().nan_to_num(0), want.nan_to_num(0))
+
+
+@gpu_test
+@pytest.mark.parametrize("n,length", [(20, 100), (3, 700), (150, 400)])
+def test_scale_bytes(gpu, tile, n, length):  # noqa: F811
+    """A row does not depend on the scale bytes of keys that it does not see, whatever they are; bytes that write
+    never makes are read as they are."""
+    for d in (64, 128):
+        c = Case([length], [n], 1, d, 64, E4M3, seed=d)
+        page, slot = int(c.table[0, (length - 1) // 64]), (length - 1) % 64
+        q = _rows(3, n, 3, d)
+        want = c.dev.attend(q.to(DEV), *c.args())
+        for byte in (0, 1, 26, 248, 254, 255):
+            c.dev.k_scale[page, 0, slot], c.dev.v_scale[page, 0, slot] = byte, byte
+            assert torch.equal(c.dev.attend(q.to(DEV), *c.args())[:-1], want[:-1]), byte
+        small = S.codes((torch.rand(c.cpu["v"].shape, generator=torch.Generator().manual_seed(1)) * 448).to(BF16))[0]
+        small = (small.float() / 448).to(E4M3)
+        for k_byte, v_byte in ((1, 1), (26, 26), (120, 248 - 5), (133, 90)):
+            for name, x, byte in (("k", c.cpu["k"], k_byte), ("v", small, v_byte)):
+                c.cpu[name], c.cpu[name + "_scale"] = x, torch.full_like(c.cpu[name + "_scale"], byte)
+                c.upload(name)
+            c.check_attend(q)
+        c.cpu["k_scale"].fill_(120)
+        c.cpu["v_scale"].fill_(254)                        # values up to 2^127, one position
+        c.upload("k"), c.upload("v")
+        c.starts = torch.tensor([0, 1], dtype=torch.int32)
+        c.lengths[0], c.t = 1, 1
+        c.check_attend(q[:1])
