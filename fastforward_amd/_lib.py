@@ -152,6 +152,20 @@ def call(name, *args):
     st = getattr(lib, name)(*args)
     if st != 0:
         raise RuntimeError(f"{name} failed ({st}): {lib.ff_last_error().decode()}")
+    if name == "ff_set_tuning":
+        for forget in _planned:
+            forget()
+
+
+_planned = []
+
+
+def planned(fn):
+    """``fn`` of sizes remembered for the last 1024 of them, and forgotten where ``call`` sets a tile
+    choice, on which plans and their workspaces depend."""
+    fn = functools.lru_cache(maxsize=1024)(fn)
+    _planned.append(fn.cache_clear)
+    return fn
 
 
 @functools.lru_cache(maxsize=None)

@@ -22,10 +22,20 @@ import ctypes
 
 import torch
 
-from ._lib import PagedCacheStruct, call, entry, stream
+from ._lib import PagedCacheStruct, call, entry, planned, stream
 
 BF16, E4M3, I32 = torch.bfloat16, torch.float8_e4m3fn, torch.int32
 _ROWS, _POSITIONS = 1 << 24, (1 << 31) - (1 << 16)
+
+
+@planned
+def attend_workspace(page_size, kv_heads, head_dim, fp8, t, heads, width, batch, starts):
+    """Bytes of workspace ff_attention_paged needs (0: none) for a table (batch, width) and, where
+    ``starts`` is true, rows by starts."""
+    need = ctypes.c_int64(0)
+    sizes = PagedCacheStruct(0, 0, 0, 0, 1, page_size, kv_heads, head_dim, fp8)
+    call("ff_attention_paged_workspace", ctypes.byref(sizes), heads, width, batch, starts, t, ctypes.byref(need))
+    return need.value
 
 
 class PagedCache:
@@ -61,7 +71,7 @@ class PagedCache:
         self._struct = PagedCacheStruct(*(0 if x is None else x.data_ptr() for x in self._tensors), self.pages,
                                         self.page_size, self.kv_heads, self.head_dim, k_scale is not None)
         self._c = ctypes.addressof(self._struct)
-        self._workspace = {}               # bytes by the sizes of a call
+        self._sizes = (self.page_size, self.kv_heads, self.head_dim, k_scale is not None)
 
     # the pages are filled in place; the tensors stay the same
     k = property(lambda self: self._tensors[0])
@@ -124,11 +134,8 @@ class PagedCache:
         return k, v
 
     def attend_workspace(self, t, heads, width, batch, starts):
-        """Bytes of workspace ff_attention_paged needs (0: none) for a table (batch, width) and,
-        where ``starts`` is true, rows by starts."""
-        need = ctypes.c_int64(0)
-        call("ff_attention_paged_workspace", self._c, heads, width, batch, starts, t, ctypes.byref(need))
-        return need.value
+        """Bytes of workspace that a call of ``attend`` takes (0: none)."""
+        return attend_workspace(*self._sizes, t, heads, width, batch, bool(starts))
 
     def attend(self, q, table, lengths, starts=None, scale=None):
         """Causal attention of q (T, heads, head_dim) bf16, any strides, heads a multiple of
@@ -151,14 +158,11 @@ class PagedCache:
             q = q.contiguous()
             qs = q.stride()
         y = q.new_empty(t, heads, d)
-        sizes = (t, heads, rows[1], rows[4], starts is not None)
-        need = self._workspace.get(sizes)
-        if need is None:
-            need = self._workspace[sizes] = self.attend_workspace(*sizes)
+        need = attend_workspace(*self._sizes, t, heads, rows[1], rows[4], starts is not None)
         ws = q.new_empty(need, dtype=torch.uint8) if need else None
         entry("ff_attention_paged")(q.data_ptr(), qs[0], qs[1], self._c, heads, *rows, y.data_ptr(), t, scale,
                                     0 if ws is None else ws.data_ptr(), need, stream())
         return y
 
 
-__all__ = ["PagedCache"]
+__all__ = ["PagedCache", "attend_workspace"]

@@ -132,3 +132,17 @@ def test_scale_bytes(gpu, tile, n, length):  # noqa: F811
         c.starts = torch.tensor([0, 1], dtype=torch.int32)
         c.lengths[0], c.t = 1, 1
         c.check_attend(q[:1])
+
+
+@gpu_test
+def test_tile_choice_between_calls(gpu):
+    """A tile choice that is set between two calls of the same sizes."""
+    from fastforward_amd import _lib
+    c = Case([600], [200], 2, 128, 64)
+    q = _rows(1, 200, 8, 128)
+    try:
+        for choice in (0, 1, 2, 3, 1, 0):
+            _lib.call("ff_set_tuning", 14, choice)
+            c.check_attend(q)
+    finally:
+        _lib.call("ff_set_tuning", 14, 0)

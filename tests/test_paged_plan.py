@@ -1,0 +1,52 @@
+"""What a call of the paged attention takes, by its sizes: host code, no GPU."""
+import ctypes
+import gc
+
+import pytest
+
+from fastforward_amd import _lib
+from fastforward_amd import cache as C
+
+
+def _cache(page_size=64, kv_heads=8, head_dim=128):
+    """A cache object without pages, for its plans."""
+    import torch
+    c = C.PagedCache.__new__(C.PagedCache)
+    c.pages, c.page_size, c.kv_heads, c.head_dim, c.dtype = 1, page_size, kv_heads, head_dim, torch.bfloat16
+    c._hold(torch.empty(0), torch.empty(0), None, None)
+    return c
+
+
+def _asked(page_size, kv_heads, head_dim, fp8, t, heads, width, batch, starts):
+    need = ctypes.c_int64(-1)
+    sizes = _lib.PagedCacheStruct(0, 0, 0, 0, 1, page_size, kv_heads, head_dim, fp8)
+    _lib.call("ff_attention_paged_workspace", ctypes.byref(sizes), heads, width, batch, starts, t, ctypes.byref(need))
+    return need.value
+
+
+def test_sizes_are_not_kept_without_bound():
+    """A serving process sees ever new sizes: nothing of the cache grows with them."""
+    c = _cache()
+    for t in range(1, 3000):
+        assert c.attend_workspace(t, 32, 64, 1, True) >= 0
+
+    def entries(x):
+        return sum(len(v) for v in vars(x).values() if isinstance(v, (dict, list, set)))
+    gc.collect()
+    assert entries(c) == 0 and C.attend_workspace.cache_info().currsize <= 1024
+
+
+def test_tile_choice_is_followed():
+    """A tile choice that is set after a size was asked for holds for the next call of that size."""
+    args = (64, 8, 128, False, 200, 32, 64, 1, True)
+    first = C.attend_workspace(*args)
+    try:
+        seen = set()
+        for tile in (1, 2, 3):
+            _lib.call("ff_set_tuning", 14, tile)
+            assert C.attend_workspace(*args) == _asked(*args)
+            seen.add(C.attend_workspace(*args))
+        assert len(seen) == 3
+    finally:
+        _lib.call("ff_set_tuning", 14, 0)
+    assert C.attend_workspace(*args) == first == _asked(*args)
