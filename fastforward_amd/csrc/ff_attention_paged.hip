@@ -1099,6 +1099,20 @@ Plan plan_of(int64_t t, int64_t batch, bool starts, int64_t hk, int64_t group, i
   return p;
 }
 
+int threads_of(const Plan& p) { return 64 * (p.decode ? kDecodeWaves : p.kind == 2 ? 8 : 4); }
+
+// Rows (token, head) of a workgroup of the join.
+int64_t join_rows(int64_t t, int64_t hq, int64_t d) { return t * hq <= 2048 ? 1 : 1024 / d; }
+
+// A launch has fewer than 2^32 threads; past that it would fail between others that do not.
+int check_launches(const char* what, const Plan& p, int64_t t, int64_t hq, int64_t hk, int64_t d) {
+  const int64_t per = join_rows(t, hq, d);
+  FF_REQUIRE(p.items * hk <= (int64_t)UINT32_MAX / threads_of(p) &&
+                 (!p.budget || (t * hq + per - 1) / per <= (int64_t)UINT32_MAX / 256),
+             "%s: too large a call (%lld workgroups)", what, (long long)(p.items * hk));
+  return FF_OK;
+}
+
 // (sizes of the cache and the rows are checked already)
 int check_sizes(const char* what, const ff_paged_cache* c, int64_t hq, int64_t width, int64_t batch, int64_t t) {
   FF_REQUIRE(hq > 0 && hq <= 65535 && hq % c->hk == 0, "%s: bad sizes hq=%lld hk=%lld", what, (long long)hq,
@@ -1132,8 +1146,11 @@ extern "C" int ff_attention_paged_workspace(const ff_paged_cache* cache, int64_t
              (long long)t);
   st = check_sizes("ff_attention_paged_workspace", cache, hq, width, batch, t);
   if (st != FF_OK) return st;
-  *bytes = workspace_of(plan_of(t, batch, starts, cache->hk, hq / cache->hk, cache->d, cache->fp8 != 0,
-                                width * cache->page_size), t, hq, cache->hk, cache->d, batch);
+  const Plan plan =
+      plan_of(t, batch, starts, cache->hk, hq / cache->hk, cache->d, cache->fp8 != 0, width * cache->page_size);
+  st = check_launches("ff_attention_paged_workspace", plan, t, hq, cache->hk, cache->d);
+  if (st != FF_OK) return st;
+  *bytes = workspace_of(plan, t, hq, cache->hk, cache->d, batch);
   return FF_OK;
 }
 
@@ -1152,6 +1169,8 @@ extern "C" int ff_attention_paged(const void* q, int64_t q_ts, int64_t q_hs, con
   const int64_t hk = cache->hk, d = cache->d;
   const bool fp8 = cache->fp8 != 0;
   const Plan plan = plan_of(t, batch, starts != nullptr, hk, hq / hk, d, fp8, width * cache->page_size);
+  st = check_launches("ff_attention_paged", plan, t, hq, hk, d);
+  if (st != FF_OK) return st;
   const int64_t need = workspace_of(plan, t, hq, hk, d, batch);
   FF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ff_aligned(workspace, 16)),
              "ff_attention_paged: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
@@ -1177,19 +1196,18 @@ extern "C" int ff_attention_paged(const void* q, int64_t q_ts, int64_t q_hs, con
   p.items = (int)plan.items;
   p.c2 = (float)((double)scale * 1.4426950408889634);
   const dim3 grid((unsigned)(plan.items * hk));
-  const bool wide = t * hq <= 2048;
-  const int64_t per = wide ? 1 : 1024 / d;  // rows of a join workgroup
+  const int64_t per = join_rows(t, hq, d);
+  const bool wide = per == 1;
   const dim3 join((unsigned)((t * hq + per - 1) / per));
   hipStream_t s = (hipStream_t)stream;
   if (plan.listed) hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, s, p);
+  const dim3 block((unsigned)threads_of(plan));
 #define FF_PAGED(DIM, F8)                                                                                          \
   if (d == DIM && fp8 == F8) {                                                                              \
-    if (plan.decode)                                                                                               \
-      hipLaunchKernelGGL((few_rows_kernel<DIM, F8, kDecodeWaves, true>), grid, dim3(64 * kDecodeWaves), 0, s, p);  \
-    else if (plan.kind == 0)                                                                                       \
-      hipLaunchKernelGGL((few_rows_kernel<DIM, F8, kFewWaves, false>), grid, dim3(64 * kFewWaves), 0, s, p);       \
-    else if (plan.kind == 1) hipLaunchKernelGGL((many_rows_kernel<DIM, F8, 4>), grid, dim3(256), 0, s, p);      \
-    else hipLaunchKernelGGL((many_rows_kernel<DIM, F8, 8>), grid, dim3(512), 0, s, p);                          \
+    if (plan.decode) hipLaunchKernelGGL((few_rows_kernel<DIM, F8, kDecodeWaves, true>), grid, block, 0, s, p);     \
+    else if (plan.kind == 0) hipLaunchKernelGGL((few_rows_kernel<DIM, F8, kFewWaves, false>), grid, block, 0, s, p); \
+    else if (plan.kind == 1) hipLaunchKernelGGL((many_rows_kernel<DIM, F8, 4>), grid, block, 0, s, p);             \
+    else hipLaunchKernelGGL((many_rows_kernel<DIM, F8, 8>), grid, block, 0, s, p);                                 \
     if (plan.budget && wide) hipLaunchKernelGGL((join_kernel<DIM, true>), join, dim3(256), 0, s, p);               \
     else if (plan.budget) hipLaunchKernelGGL((join_kernel<DIM, false>), join, dim3(256), 0, s, p);                 \
   }

@@ -50,3 +50,13 @@ def test_tile_choice_is_followed():
     finally:
         _lib.call("ff_set_tuning", 14, 0)
     assert C.attend_workspace(*args) == first == _asked(*args)
+
+
+def test_launches_past_their_limit_are_refused():
+    """131073 tiles for each of 128 key heads are 2^32 threads, which no launch has."""
+    sizes = (16, 128, 64, False)
+    assert C.attend_workspace(*sizes, 1 << 20, 128, 1, 65000, True) >= 0
+    with pytest.raises(RuntimeError, match="too large"):
+        C.attend_workspace(*sizes, 1 << 20, 128, 1, 65536, True)
+    rows = C.attend_workspace(*sizes, 65536, 128, 1, 65536, False)      # a decode step of as many sequences
+    assert rows >= 0
