@@ -146,3 +146,37 @@ def test_tile_choice_between_calls(gpu):
             c.check_attend(q)
     finally:
         _lib.call("ff_set_tuning", 14, 0)
+
+
+def _part(c, q, y, sequences):
+    """Compares the rows of some sequences with the oracle's."""
+    starts = list(range(len(c.lengths) + 1)) if c.starts is None else c.starts.tolist()
+    rows = [i for b in sequences for i in range(starts[b], starts[b + 1])]
+    upto = torch.tensor([0] + [starts[b + 1] - starts[b] for b in sequences]).cumsum(0).to(torch.int32)
+    o, a, most = S.attend(c.cpu, q[rows], c.table[sequences], c.lengths[sequences], upto)
+    close(y[rows], o, a, most, c.d)
+
+
+@gpu_test
+@pytest.mark.parametrize("batch,hk,dtype", [(1023, 8, BF16), (1024, 8, E4M3), (1025, 8, BF16), (2100, 8, BF16), (4200, 2, E4M3)])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_thousands_of_sequences(gpu, batch, hk, dtype, ragged):
+    """The work list past one, two and four times its workgroup's threads; some sequences without rows or
+    keys, two past 4096 positions."""
+    gen = torch.Generator().manual_seed(batch)
+    lengths = torch.randint(0, 31, (batch,), generator=gen)
+    lengths[1022], lengths[batch - 2] = 5000, 4100
+    new = torch.randint(0, 4, (batch,), generator=gen).minimum(lengths).tolist() if ragged else None
+    c = Case(lengths.tolist(), new, hk, 64, 16, dtype, seed=batch)
+    k, v, q = _rows(1, c.t, hk, 64), _rows(2, c.t, hk, 64), _rows(3, c.t, 2 * hk, 64)
+    c.dev.write(k.to(DEV), v.to(DEV), *c.args())
+    S.write(c.cpu, k, v, c.table, c.lengths, c.starts)
+    for name, want in c.cpu.items():
+        assert torch.equal(getattr(c.dev, name).cpu().view(torch.uint8), want.view(torch.uint8)), name
+    y = c.dev.attend(q.to(DEV), *c.args()).cpu()
+    near = {0, 1, 63, 64, 511, 512, 1020, 1021, 1022, batch - 3, batch - 2, batch - 1}
+    near |= set(range(1000, min(batch, 1060))) | set(range(2040, min(batch, 2056))) | set(range(4090, min(batch, 4102)))
+    _part(c, q, y, sorted(near | set(range(0, batch, 37))))
+    if not ragged:                                        # the same rows by starts
+        c.starts = torch.arange(batch + 1, dtype=torch.int32)
+        _part(c, q, c.dev.attend(q.to(DEV), *c.args()).cpu(), sorted(near))
