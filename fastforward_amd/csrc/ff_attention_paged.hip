@@ -34,13 +34,13 @@ struct Args {
   int64_t q_ts, q_hs;
   const uint8_t *k, *v, *ks, *vs;
   bf16_t* y;
-  float* part_o;   // (items, BM, D) unnormalised sums of split tiles
-  float2* part_s;  // (items, BM) their reference (log2) and denominator
+  float* part_o;   // (slots, hk, BM, D) unnormalised sums of split tiles
+  float2* part_s;  // (slots, hk, BM) their reference (log2) and denominator
   int* plan;       // the list of many sequences, or null
   int2* part_of;   // (rows) where a row (token, head) begins there, and its splits (1: it is done)
   int hk, group, lbm;  // BM = 1 << lbm rows a tile
   int least, budget;  // 64-key blocks are dealt so that about so many items per head come out; 0: no tile is split
-  int items;   // items per head that the grid holds
+  int slots;   // items of split tiles, per head, that the workspace holds
   float c2;    // scale * log2(e)
 };
 
@@ -54,8 +54,8 @@ __device__ __forceinline__ f32x4 mfma_bf16(const bf16x8& a, const u32x4& b, cons
 // key ranges as its sequence's blocks take chunks. A chunk is the share of all blocks
 // that gives `budget` items, `least` blocks at least. All workgroups compute the
 // same list from the lengths (of more than 64 sequences a launch writes it); a sequence's last tiles, which see the most keys, come first.
-// A split's rows go to the workspace, with a note for each row where its splits are. Rows
-// behind the last sequence are a sequence without keys.
+// A split's rows go to the workspace, where the items of split tiles have slots in the list's order, with a
+// note for each row where its splits are. Rows behind the last sequence are a sequence without keys.
 
 struct Seq {
   int row0, n;    // first row (token) and rows
@@ -87,7 +87,12 @@ __device__ __forceinline__ int splits_of(int blocks, int chunk) {
 struct Item {
   Seq s;
   int seq, tile, split, splits;
+  int slot;  // of a split tile's item
 };
+
+// Slots of a sequence with `splits` splits a tile. A split sequence has more blocks than a chunk, so that
+// its splits are fewer than twice blocks / chunk, and all of them fewer than twice the budget.
+__device__ __forceinline__ int slots_of(const Seq& s, int splits) { return splits > 1 ? s.tiles * splits : 0; }
 
 // The chunk: the share of all blocks that gives `budget` items, or as many more as keep the items within it
 // (one round of the GPU's workgroups; a few of a second would take as long). Where the tiles alone are more
@@ -97,7 +102,7 @@ __device__ __forceinline__ int chunk_of(const Args& p, Sum sum) {
   if (!p.budget) return INT_MAX;
   const int total = sum([](const Seq& s) { return s.tiles * s.blocks; });
   const int tiles = sum([](const Seq& s) { return s.tiles; });
-  int chunk = max(p.least, (total + p.budget - 1) / p.budget);
+  int chunk = max(p.least, (int)(((int64_t)total + p.budget - 1) / p.budget));
   for (int i = 0; i < 3 && tiles < p.budget; ++i) {
     const int items = sum([=](const Seq& s) { return s.tiles * splits_of(s.blocks, chunk); });
     if (items <= p.budget) break;
@@ -110,44 +115,46 @@ __device__ __forceinline__ int chunk_of(const Args& p, Sum sum) {
 __host__ __device__ inline bool fit_lanes(int64_t batch, bool starts) { return batch + starts <= 64; }
 
 // The list of more sequences than a wave has lanes, by one workgroup in a launch of its own: plan[0] the chunk,
-// plan[1 + b] the first item of sequence b (b = batch: of the rows behind the last; batch + 1: all items). With
-// every workgroup reading all lengths instead, decode of 256 sequences of 500 positions took 134 us (102 so), 1024
+// plan[1 + b] the first item of sequence b (b = batch: of the rows behind the last; batch + 1: all items),
+// plan[3 + batch + b] its first slot. With every workgroup reading all lengths instead, decode of 256 sequences of 500 positions took 134 us (102 so), 1024
 // sequences of 3 tokens over 200 positions 427 (208).
 __global__ __launch_bounds__(1024) void plan_kernel(Args p) {
   __shared__ int part[16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  auto all = [&](int v) {  // the workgroup's sum
-    v = __builtin_amdgcn_readlane(wave_scan(v), 63);
-    __syncthreads();
-    if (lane == 0) part[wave] = v;
-    __syncthreads();
-    int sum = 0;
-#pragma unroll
-    for (int w = 0; w < 16; ++w) sum += part[w];
-    return sum;
-  };
-  const int chunk = chunk_of(p, [&](auto f) {
-    int v = 0;
-    for (int b = threadIdx.x; b <= p.a.batch; b += 1024) v += f(seq_of(p, b));
-    return all(v);
-  });
-  if (threadIdx.x == 0) p.plan[0] = chunk;
-  int base = 0;
-  for (int b0 = 0; b0 <= p.a.batch; b0 += 1024) {
-    const int b = b0 + threadIdx.x;
-    const Seq s = seq_of(p, b);
-    const int n = b <= p.a.batch ? s.tiles * splits_of(s.blocks, chunk) : 0, upto = wave_scan(n);
+  // The workgroup's sum of v, and how much of it lies before the thread's own.
+  auto scan = [&](int v, int* before) {
+    const int upto = wave_scan(v);
     __syncthreads();
     if (lane == 63) part[wave] = upto;
     __syncthreads();
-    int before = 0, sum = 0;
+    int sum = 0;
+    *before = upto - v;
 #pragma unroll
     for (int w = 0; w < 16; ++w) {
-      before += w < wave ? part[w] : 0;
+      *before += w < wave ? part[w] : 0;
       sum += part[w];
     }
-    if (b <= p.a.batch) p.plan[1 + b] = base + before + upto - n;
-    base += sum;
+    return sum;
+  };
+  int before;
+  const int chunk = chunk_of(p, [&](auto f) {
+    int v = 0;
+    for (int b = threadIdx.x; b <= p.a.batch; b += 1024) v += f(seq_of(p, b));
+    return scan(v, &before);
+  });
+  if (threadIdx.x == 0) p.plan[0] = chunk;
+  int base = 0, slots = 0;
+  for (int b0 = 0; b0 <= p.a.batch; b0 += 1024) {
+    const int b = b0 + threadIdx.x;
+    const bool in = b <= p.a.batch;
+    const Seq s = seq_of(p, b);
+    const int splits = splits_of(s.blocks, chunk);
+    const int n = scan(in ? s.tiles * splits : 0, &before);
+    if (in) p.plan[1 + b] = base + before;
+    base += n;
+    const int m = scan(in ? slots_of(s, splits) : 0, &before);
+    if (in) p.plan[3 + p.a.batch + b] = slots + before;
+    slots += m;
   }
   if (threadIdx.x == 0) p.plan[2 + p.a.batch] = base;
 }
@@ -155,24 +162,27 @@ __global__ __launch_bounds__(1024) void plan_kernel(Args p) {
 // Item `id` of the list.
 __device__ __forceinline__ bool find_item(const Args& p, int lane, int id, Item* out) {
   Seq s;
-  int chunk, first;
+  int chunk, first, slot;
   if (p.plan) {
     const int* starts = p.plan + 1;
     const int lo = last_upto(starts, p.a.batch + 2, id, lane);  // the last one that begins at or before the item
     if (lo > p.a.batch) return false;
     chunk = __builtin_amdgcn_readfirstlane(p.plan[0]);
     first = __builtin_amdgcn_readfirstlane(starts[lo]);
+    slot = __builtin_amdgcn_readfirstlane(starts[p.a.batch + 2 + lo]);
     s = seq_of(p, lo);
     out->seq = lo;
     lane = 0;
   } else {
     s = seq_of(p, lane);
     chunk = chunk_of(p, [&](auto f) { return __builtin_amdgcn_readlane(wave_scan(f(s)), 63); });
-    const int n = s.tiles * splits_of(s.blocks, chunk), upto = wave_scan(n);
+    const int splits = splits_of(s.blocks, chunk), n = s.tiles * splits, upto = wave_scan(n);
+    const int m = slots_of(s, splits), slots = wave_scan(m);
     const uint64_t hit = __ballot(id >= upto - n && id < upto);
     if (!hit) return false;
     lane = __builtin_ctzll(hit);
     first = __builtin_amdgcn_readlane(upto - n, lane);
+    slot = __builtin_amdgcn_readlane(slots - m, lane);
     out->seq = lane;
   }
   out->s = {__builtin_amdgcn_readlane(s.row0, lane), __builtin_amdgcn_readlane(s.n, lane),
@@ -183,7 +193,9 @@ __device__ __forceinline__ bool find_item(const Args& p, int lane, int id, Item*
   if (in < 0 || in >= out->s.tiles * out->splits) return false;  // (counts of starts that do not rise may pass 32 bits)
   out->tile = out->s.tiles - 1 - in / out->splits;
   out->split = in % out->splits;
-  return true;
+  out->slot = slot + in;
+  // (and so may those of slots, without which an item of a split tile does nothing)
+  return out->splits == 1 || (unsigned)out->slot < (unsigned)p.slots;
 }
 
 // ------------------------------------------------------------------ pieces of a block
@@ -580,7 +592,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void few_rows_kernel(Args
       *reinterpret_cast<u32x2*>(p.y + to * D + d0) = pack4_bf16(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
       if (!DECODE && p.budget && d0 == 0) p.part_of[to] = int2{0, 1};
     } else {
-      const int64_t at = ((int64_t)id * p.hk + head) * 16 + r;
+      const int64_t at = ((int64_t)it.slot * p.hk + head) * 16 + r;
       *reinterpret_cast<f32x4*>(p.part_o + at * D + d0) = acc;
       if (d0 == 0) p.part_s[at] = float2{mx, sum};
       if (d0 == 0 && it.split == 0) p.part_of[to] = int2{(int)at, it.splits};
@@ -947,7 +959,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void many_rows_kernel(Arg
     }
     if (p.budget && h == 0) p.part_of[to] = int2{0, 1};
   } else {
-    const int64_t at = (((int64_t)id * p.hk + head) << p.lbm) + (row - (it.tile << p.lbm));
+    const int64_t at = (((int64_t)it.slot * p.hk + head) << p.lbm) + (row - (it.tile << p.lbm));
 #pragma unroll
     for (int i = 0; i < 4 * DTN; ++i) {
       const f32x16& x = o[i >> 2];
@@ -978,7 +990,7 @@ __global__ __launch_bounds__(256) void join_kernel(Args p) {
   const int splits = of.y;
   const int64_t step = (int64_t)p.hk << p.lbm;  // from a split's row to the next one's
   // (starts that do not rise leave rows that no tile has)
-  if (splits <= 1 || at0 < 0 || at0 + (splits - 1) * step >= ((int64_t)p.items * p.hk) << p.lbm) return;
+  if (splits <= 1 || at0 < 0 || at0 + (splits - 1) * step >= ((int64_t)p.slots * p.hk) << p.lbm) return;
   float m = -INFINITY, sum = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   for (int i0 = WIDE ? group : 0; i0 < splits; i0 += 4 * GROUPS) {
@@ -1038,7 +1050,7 @@ struct Plan {
   int kind;  // 0: few rows; 1, 2: many rows on 4 and 8 waves
   bool decode;
   int lbm, least, budget;
-  int64_t items;  // per key head
+  int64_t items, slots;  // per key head
   bool listed;    // a launch writes the list
 };
 
@@ -1092,8 +1104,8 @@ Plan plan_of(int64_t t, int64_t batch, bool starts, int64_t hk, int64_t group, i
   // Decode of more sequences is split as well where one may be far longer than a workgroup's share: 1024
   // sequences of 100 positions, one of 60000 among them, 794 us without splits.
   if (p.kind == 0 && !starts && !fit_lanes(batch, starts) && capacity > 4096) p.budget = (int)budget;
-  if (((tiles + budget) * hk << p.lbm) > INT32_MAX) p.budget = 0;  // (rows of the splits are counted in 32 bits)
   p.items = tiles + p.budget;
+  p.slots = 2 * p.budget < p.items ? 2 * p.budget : p.items;  // (1536, or 2 hk, for all heads: their rows fit 32 bits)
   // (no list: 16-row tiles of one row a sequence that are not split)
   p.listed = !fit_lanes(batch, starts) && (starts || p.budget || p.kind);
   return p;
@@ -1126,10 +1138,10 @@ int check_sizes(const char* what, const ff_paged_cache* c, int64_t hq, int64_t w
 
 // Partial sums, their statistics, the rows' notes; the list.
 int64_t parts_bytes(const Plan& p, int64_t t, int64_t hq, int64_t hk, int64_t d) {
-  return p.budget ? ((p.items * hk) << p.lbm) * (d * 4 + 8) + t * hq * 8 : 0;
+  return p.budget ? ((p.slots * hk) << p.lbm) * (d * 4 + 8) + t * hq * 8 : 0;
 }
 int64_t workspace_of(const Plan& p, int64_t t, int64_t hq, int64_t hk, int64_t d, int64_t batch) {
-  return parts_bytes(p, t, hq, hk, d) + (p.listed ? (batch + 3) * 4 : 0);
+  return parts_bytes(p, t, hq, hk, d) + (p.listed ? (2 * batch + 4) * 4 : 0);
 }
 
 }  // namespace
@@ -1185,15 +1197,15 @@ extern "C" int ff_attention_paged(const void* q, int64_t q_ts, int64_t q_hs, con
   p.vs = (const uint8_t*)cache->v_scale;
   p.y = (bf16_t*)y;
   p.part_o = (float*)workspace;
-  p.part_s = (float2*)((char*)workspace + ((plan.items * hk) << plan.lbm) * d * 4);
-  p.part_of = (int2*)(p.part_s + ((plan.items * hk) << plan.lbm));
+  p.part_s = (float2*)((char*)workspace + ((plan.slots * hk) << plan.lbm) * d * 4);
+  p.part_of = (int2*)(p.part_s + ((plan.slots * hk) << plan.lbm));
   p.plan = plan.listed ? (int*)((char*)workspace + parts_bytes(plan, t, hq, hk, d)) : nullptr;
   p.hk = (int)hk;
   p.group = (int)(hq / hk);
   p.lbm = plan.lbm;
   p.least = plan.least;
   p.budget = plan.budget;
-  p.items = (int)plan.items;
+  p.slots = (int)plan.slots;
   p.c2 = (float)((double)scale * 1.4426950408889634);
   const dim3 grid((unsigned)(plan.items * hk));
   const int64_t per = join_rows(t, hq, d);

@@ -60,3 +60,12 @@ def test_launches_past_their_limit_are_refused():
         C.attend_workspace(*sizes, 1 << 20, 128, 1, 65536, True)
     rows = C.attend_workspace(*sizes, 65536, 128, 1, 65536, False)      # a decode step of as many sequences
     assert rows >= 0
+
+
+def test_workspace_of_many_sequences():
+    """Only split tiles leave partial sums, and they are about as many as workgroups, however many
+    sequences there are: what grows with them is a note of 8 bytes a row and head, and the list."""
+    for t in (64, 1024, 4096, 65536):
+        for fp8 in (False, True):
+            need = C.attend_workspace(64, 8, 128, fp8, t, 32, 128, t, False)
+            assert 0 < need <= (40 << 20) + t * (32 * 8 + 8), (t, need)
