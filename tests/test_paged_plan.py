@@ -69,3 +69,12 @@ def test_workspace_of_many_sequences():
         for fp8 in (False, True):
             need = C.attend_workspace(64, 8, 128, fp8, t, 32, 128, t, False)
             assert 0 < need <= (40 << 20) + t * (32 * 8 + 8), (t, need)
+
+
+def test_one_long_sequence_among_many():
+    """A decode step's rows are split over keys where the table reaches far, whether starts say which rows
+    are whose or not."""
+    for t in (100, 1024, 4096):
+        for width in (65, 1024):
+            plain = C.attend_workspace(64, 8, 128, False, t, 32, width, t, False)
+            assert C.attend_workspace(64, 8, 128, False, t, 32, width, t, True) >= plain > 4 << 20
