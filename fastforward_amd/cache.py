@@ -106,8 +106,9 @@ class PagedCache:
         [-100, 120], for which the largest finite magnitude of the token's row in its head is
         at most 448 * 2^e (and nothing past 240 * 2^120, which bf16 does not hold). NaN and
         infinities become NaN and leave the rest of their row as it is. Rows behind the last sequence
-        are not written. The positions of one call are different ones: where two rows name
-        one place, either may end there."""
+        are not written. The rows of one call have different places: where two name the same one (sequences
+        that share the page of a position that both write), what ends there may be pieces of both, and a
+        code under the other row's scale."""
         assert k.dim() == 3 and k.shape == v.shape and k.dtype == v.dtype == BF16, (k.shape, v.shape, k.dtype, v.dtype)
         t, hk, d = k.shape
         assert hk == self.kv_heads and d == self.head_dim, (k.shape, self.kv_heads, self.head_dim)

@@ -561,8 +561,8 @@ typedef struct {
 /* k, v rows (t, hk, d) bf16 with token strides k_ts, v_ts and head strides k_hs, v_hs
  * (elements) -> the pages. fp8: e = the smallest integer in [-100, 120] with amax <= 448 * 2^e,
  * amax the largest finite magnitude of a token's row in a head; code = e4m3(x * 2^-e)
- * (240 at most where e is 120), byte = e + 127; NaN and infinities become NaN. Where two rows name one place either may
- * end there. */
+ * (240 at most where e is 120), byte = e + 127; NaN and infinities become NaN. Rows of one call have different
+ * places; where two have the same, pieces of both may end there. */
 int ff_cache_write(const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs,
                    const ff_paged_cache* cache, const int32_t* table, int64_t width, const int32_t* lengths,
                    const int32_t* starts, int64_t batch, int64_t t, ff_stream_t stream);
