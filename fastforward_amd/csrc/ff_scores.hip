@@ -96,13 +96,6 @@ __device__ __forceinline__ uint64_t read_lane(uint64_t v, int lane) {
          (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
 }
 __device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
-template <bool WIDE>
-__device__ __forceinline__ uint64_t swapped(uint64_t v) {
-  const uint32_t h = (uint32_t)(v >> 32), l = (uint32_t)v;
-  const auto a = WIDE ? __builtin_amdgcn_permlane32_swap(h, h, false, false) : __builtin_amdgcn_permlane16_swap(h, h, false, false);
-  const auto b = WIDE ? __builtin_amdgcn_permlane32_swap(l, l, false, false) : __builtin_amdgcn_permlane16_swap(l, l, false, false);
-  return larger((uint64_t)a[0] << 32 | b[0], (uint64_t)a[1] << 32 | b[1]);
-}
 
 // Puts the uniform key into the wave's falling list (one entry a lane).
 __device__ __forceinline__ void insert(uint64_t& list, uint64_t key) {
