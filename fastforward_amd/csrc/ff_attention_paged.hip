@@ -1068,6 +1068,9 @@ bool wide_tiles(int64_t rows, int64_t t, int64_t batch, int64_t hk, int64_t d, i
   return all >= 131072 || (fp8 && all >= 16384 && depth >= 4 * t);
 }
 
+// The sizes of the call are all that the host knows: a table that reaches further than the sequences has their
+// kernel, splits and join chosen for what it may hold (one token over 577 positions 11 us, 13.6 with a table of 8192;
+// 61 tokens over 176 9.6 and 15).
 Plan plan_of(int64_t t, int64_t batch, bool starts, int64_t hk, int64_t group, int64_t d, int fp8, int64_t capacity) {
   const int64_t rows = t * group;
   const int force = ff_tuning(FF_TUNE_PAGED_ROWS);
@@ -1083,8 +1086,10 @@ Plan plan_of(int64_t t, int64_t batch, bool starts, int64_t hk, int64_t group, i
   if (force) p.kind = force - 1;
   else if (rows <= 16 * batch || pairs <= (fp8 ? 5120 : 2560)) p.kind = 0;
   else p.kind = wide_tiles(rows, t, batch, hk, d, fp8, capacity) ? 2 : 1;
-  // One row a sequence, up to 768 positions, a CU for each tile: one launch. A CU takes in 64 bytes a
-  // clock at most, so that longer caches are better shared by several and joined.
+  // One row a sequence, a table of up to 768 positions, a CU for each tile: one launch. A CU takes in 64 bytes a
+  // clock at most, so that longer caches are better shared by several and joined. us, one launch and splits, 32 / 8
+  // heads of 128: 320 positions 9.1 and 13.7, 577 11.2 and 13.9, 768 11.8 and 13.7, 1024 15.3 and 14.0, 1500 20.6 and
+  // 13.9; codes 768 9.3 and 13.5, 1024 10.3 and 13.6, 1500 12.8 and 13.5; 32 sequences of 577 16.1 and 21.2.
   const int64_t decode = (group + 15) / 16 * t;
   if (p.kind == 0 && !starts && capacity <= 768 && decode * hk <= 256) {
     p.decode = true;
@@ -1115,7 +1120,8 @@ Plan plan_of(int64_t t, int64_t batch, bool starts, int64_t hk, int64_t group, i
 
 int threads_of(const Plan& p) { return 64 * (p.decode ? kDecodeWaves : p.kind == 2 ? 8 : 4); }
 
-// Rows (token, head) of a workgroup of the join.
+// Rows (token, head) of a workgroup of the join. us, one and 8 or 16: one token over 131072 positions (32 rows, 64
+// splits) 101 and 120; from 512 rows on they are even; 6 chunks of about 300 tokens of 20 heads 78 and 56.
 int64_t join_rows(int64_t t, int64_t hq, int64_t d) { return t * hq <= 2048 ? 1 : 1024 / d; }
 
 // A launch has fewer than 2^32 threads; past that it would fail between others that do not.
